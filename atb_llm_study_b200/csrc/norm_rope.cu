@@ -12,6 +12,7 @@
 #include <cstdlib>
 
 #include "common.cuh"
+#include "quant.cuh"
 
 using namespace b200;
 
@@ -76,6 +77,69 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_kernel(const __nv_bfloat
       for (int i = 0; i < 8; ++i) o[i] = v[c][i] * inv * g[i];
       *reinterpret_cast<uint4*>(out + row * stride + idx * 8) = pack8(o);
     }
+  }
+}
+
+// rmsnorm_kernel with the normalised row quantised to 8 bits in the same pass
+// (out, optional, is the bf16 row it would write).  The integers come from the
+// row as rounded to bf16, so they and the scale are those of rmsnorm_kernel
+// followed by the row quantisation, bit for bit: a path can fuse the two or
+// not without changing a result.  Same thread / chunk mapping and sums.
+template <int CH>
+__global__ void __launch_bounds__(kNormThreads) rmsnorm_quant_kernel(const __nv_bfloat16* __restrict__ x,
+                                                                     const __nv_bfloat16* residual,
+                                                                     const __nv_bfloat16* __restrict__ w, int8_t* q,
+                                                                     int64_t ldq, float* __restrict__ scale,
+                                                                     __nv_bfloat16* out, __nv_bfloat16* residual_out,
+                                                                     int64_t dim, int64_t stride, float eps) {
+  __shared__ float red[kNormThreads / 32];
+  __shared__ uint32_t mred[kNormThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const int64_t nchunk = dim / 8;
+  const __nv_bfloat16* xr = x + row * stride;
+  float v[CH][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
+    if (idx < nchunk) {
+      unpack8(*reinterpret_cast<const uint4*>(xr + idx * 8), v[c]);
+      if (residual) {
+        float r[8];
+        unpack8(*reinterpret_cast<const uint4*>(residual + row * stride + idx * 8), r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] += r[i];
+        if (residual_out) *reinterpret_cast<uint4*>(residual_out + row * stride + idx * 8) = pack8(v[c]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
+    }
+  }
+  const float tot = block_sum<kNormThreads>(ss, red);
+  const float inv = rsqrtf(tot / (float)dim + eps);
+  uint4 o[CH];
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
+    if (idx < nchunk) {
+      float g[8], n[8];
+      unpack8(*reinterpret_cast<const uint4*>(w + idx * 8), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n[i] = v[c][i] * inv * g[i];
+      o[c] = pack8(n);
+      if (out) *reinterpret_cast<uint4*>(out + row * stride + idx * 8) = o[c];
+      m = amax_pairs(m, o[c]);
+    }
+  }
+  const RowQuant r = row_quant(block_amax<kNormThreads>(m, mred));
+  if (threadIdx.x == 0) scale[row] = r.scale;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
+    if (idx < nchunk) *reinterpret_cast<uint2*>(q + row * ldq + idx * 8) = quant8(o[c], r);
   }
 }
 
@@ -603,6 +667,33 @@ extern "C" int b200_rmsnorm(const void* x, const void* residual, const void* wei
     case 8: launch_kernel(rmsnorm_kernel<8>, g, kNormThreads, 0, stream, xb, rb, wb, ob, rob, dim, stride, eps); break;
     default: return B200_ERROR_UNSUPPORTED;
   }
+  B200_CHECK_LAUNCH();
+  return B200_OK;
+}
+
+extern "C" int b200_rmsnorm_quant_int8(const void* x, const void* residual, const void* weight, int8_t* q, int64_t ldq,
+                                       float* scale, void* out, void* residual_out, int64_t rows, int64_t dim,
+                                       int64_t stride, float eps, b200_stream_t stream) {
+  if (!x || !weight || !q || !scale || rows < 0 || dim <= 0 || dim % 16 || stride < dim || stride % 8 || ldq < dim ||
+      ldq % 16)
+    return B200_ERROR_INVALID_PARAM;
+  if (!aligned16(x) || !aligned16(q) || !aligned16(weight) || ((uintptr_t)scale & 3u) || (out && !aligned16(out)) ||
+      (residual && !aligned16(residual)) || (residual_out && !aligned16(residual_out)))
+    return B200_ERROR_INVALID_PARAM;
+  if (rows > INT32_MAX) return B200_ERROR_UNSUPPORTED;
+  if (rows == 0) return B200_OK;
+  const int64_t per = (dim / 8 + kNormThreads - 1) / kNormThreads;
+  auto xb = static_cast<const __nv_bfloat16*>(x);
+  auto rb = static_cast<const __nv_bfloat16*>(residual);
+  auto wb = static_cast<const __nv_bfloat16*>(weight);
+  auto ob = static_cast<__nv_bfloat16*>(out);
+  auto rob = static_cast<__nv_bfloat16*>(residual_out);
+  const dim3 g((unsigned)rows);
+  if (per <= 1) launch_kernel(rmsnorm_quant_kernel<1>, g, kNormThreads, 0, stream, xb, rb, wb, q, ldq, scale, ob, rob, dim, stride, eps);
+  else if (per <= 2) launch_kernel(rmsnorm_quant_kernel<2>, g, kNormThreads, 0, stream, xb, rb, wb, q, ldq, scale, ob, rob, dim, stride, eps);
+  else if (per <= 4) launch_kernel(rmsnorm_quant_kernel<4>, g, kNormThreads, 0, stream, xb, rb, wb, q, ldq, scale, ob, rob, dim, stride, eps);
+  else if (per <= 8) launch_kernel(rmsnorm_quant_kernel<8>, g, kNormThreads, 0, stream, xb, rb, wb, q, ldq, scale, ob, rob, dim, stride, eps);
+  else return B200_ERROR_UNSUPPORTED;
   B200_CHECK_LAUNCH();
   return B200_OK;
 }

@@ -69,6 +69,36 @@ B200_API int b200_device_error_read(unsigned* out_bits, int clear, b200_stream_t
 B200_API int b200_rmsnorm(const void* x, const void* residual, const void* weight, void* out, void* residual_out,
                  int64_t rows, int64_t dim, int64_t stride, float eps, b200_stream_t stream);
 
+/* Rows of bf16 values to 8-bit integers with one scale a row, for
+ * b200_gemm_int8 / b200_grouped_gemm_int8: activations (a row per token) and
+ * weights (a row per output channel) alike.  For row r of q [rows, ldq]:
+ *   s = row_src ? row_src[r] : r        (the row of x it is made from)
+ *   amax = max_j |x[s, j]|, scale[r] = fp32(amax / 127),
+ *   q[r, j] = the integer nearest to 127 x[s, j] / amax, ties to even (exact).
+ * A row of zeros gets scale 0 and zeros.  A row with a NaN or an infinity gets
+ * scale NaN and zeros, so all its products are NaN and no other row's are.
+ * x [src_rows, ldx] bf16; row_src [rows] (device, NULL: the same row,
+ * src_rows >= rows) gathers, e.g. by b200_moe_permute's perm_src; rows at or
+ * above *row_count (device int32, NULL: none) are left as they are, e.g. with
+ * expert_offsets + E.  An index outside [0, src_rows) leaves its row as it is
+ * and sets the device error word.  q must not overlap x.  dim % 16 == 0,
+ * ldx % 8 == 0, ldq % 16 == 0, x and q 16-byte aligned.  No reference
+ * counterpart: the reference runs fp16 throughout
+ * (atb_cpp_llm/src/io/weight_helpers.cpp:16-76). */
+B200_API int b200_quant_rows_int8(const void* x, int64_t ldx, int64_t src_rows, const int32_t* row_src,
+                                  const int32_t* row_count, int8_t* q, int64_t ldq, float* scale, int64_t rows,
+                                  int64_t dim, b200_stream_t stream);
+
+/* b200_rmsnorm and b200_quant_rows_int8 of its output in one pass: q, scale,
+ * residual_out (optional, may alias residual) and out (optional, the bf16 row
+ * itself) are what the two calls give, bit for bit.  x / residual / out /
+ * residual_out have row stride `stride`, q ldq.  dim % 16 == 0, dim <= 8192.
+ * Replaces RmsNormGraph::Build (atb_cpp_llm/src/components/common/rms_norm_graph.cpp:59-84)
+ * in front of 8-bit projections. */
+B200_API int b200_rmsnorm_quant_int8(const void* x, const void* residual, const void* weight, int8_t* q, int64_t ldq,
+                                     float* scale, void* out, void* residual_out, int64_t rows, int64_t dim,
+                                     int64_t stride, float eps, b200_stream_t stream);
+
 /* LayerNorm with gamma/beta over the last dim ([rows, dim], contiguous, dim % 8 == 0).
  * Replaces LayerNormOp::Create (atb_cpp_llm/src/ops/layer_norm_op.cpp:7-22). */
 B200_API int b200_layernorm(const void* x, const void* gamma, const void* beta, void* out, int64_t rows, int64_t dim,
@@ -180,6 +210,21 @@ B200_API int b200_gemm_bf16(const void* A, int64_t lda, const void* B, int64_t l
 /* Bytes of workspace b200_gemm_bf16 uses for split-K at this shape (0 = none). */
 B200_API int64_t b200_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int epilogue);
 
+/* The same product of 8-bit integers with a scale per row of A (token) and per
+ * row of B (output channel):
+ *   C[m, n] = epilogue(a_scale[m] * b_scale[n] * sum_k A[m, k] B[n, k])
+ * A [M, K], B [N, K] int8 (b200_quant_rows_int8's output; any value, -128
+ * included), the sum exact in 32 bits, scales fp32, one rounding to bf16.  The
+ * epilogues, their operands and SwiGLU's interleaved gate / up rows are
+ * b200_gemm_bf16's.  K % 16 == 0, K <= 131056; lda, ldb multiples of 16 bytes;
+ * N % 8 == 0 (SwiGLU: 16), ldc, ldr multiples of 8; every pointer 16-byte
+ * aligned.  Takes no workspace, so calls on several streams need nothing of
+ * their own.  Replaces LinearOp::Create(transB=true)
+ * (atb_cpp_llm/src/ops/linear_op.cpp:7-20) where the weights are kept in 8 bits. */
+B200_API int b200_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
+                            const float* b_scale, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int epilogue,
+                            const void* bias, const void* residual, int64_t ldr, b200_stream_t stream);
+
 /* ---------------------------------------------------------------- experts */
 
 /* Grouped expert GEMM: for each group g < groups (<= 256), the rows
@@ -194,6 +239,15 @@ B200_API int64_t b200_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int 
 B200_API int b200_grouped_gemm_bf16(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc,
                                     const int32_t* group_offsets, int groups, int64_t rows, int64_t N, int64_t K,
                                     int epilogue, b200_stream_t stream);
+
+/* b200_grouped_gemm_bf16 with 8-bit operands and b200_gemm_int8's scales:
+ * a_scale [rows] of the rows of A, b_scale [groups * N] of the rows of B.
+ * Rows outside [0, group_offsets[groups]) are left as they are; offsets that
+ * fall or leave [0, rows] are clamped and set the device error word. */
+B200_API int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
+                                    const float* b_scale, void* C, int64_t ldc, const int32_t* group_offsets,
+                                    int groups, int64_t rows, int64_t N, int64_t K, int epilogue,
+                                    b200_stream_t stream);
 
 /* Router: logits = x [T, H] (bf16, row stride ldx) . gate_weight [E, H]^T in
  * fp32, softmax over the E (<= 128) experts, the top_k (<= 8) largest logits
@@ -211,6 +265,29 @@ B200_API int b200_moe_route(const void* x, int64_t ldx, const void* gate_weight,
 /* The selection of b200_moe_route from given fp32 logits [T, E]. */
 B200_API int b200_moe_topk(const float* logits, int64_t T, int num_experts, int top_k, int renormalize, float scale,
                            int32_t* topk_ids, float* topk_weights, b200_stream_t stream);
+
+enum b200_router_score { B200_SCORE_SOFTMAX = 0, B200_SCORE_SIGMOID = 1 };
+
+/* Selection with groups and a balance bias from fp32 logits [T, ld] (the
+ * published DeepSeek-V2 / V3 gates).  Per token, with x the logits clamped to
+ * the finite range (NaN counts as the lowest value):
+ *   s = softmax(x) or sigmoid(x) over the E (<= 256) experts (`scoring`);
+ *   c = s + bias (bias [E] fp32 or NULL; it moves the choice, not the weights);
+ *   the experts form num_groups (<= 32) equal groups of consecutive ones, each
+ *   scored by the sum of its group_top (1 or 2) largest c; only the
+ *   topk_groups best groups' experts can be chosen;
+ *   topk_ids [T, top_k] (int32): the top_k (<= 8) largest c, descending;
+ *   topk_weights [T, top_k] (fp32): their s, divided by its sum over the
+ *   chosen when `renormalize` (0 where that sum is 0), times scale.
+ * Ties go to the lower index, among groups and among experts; without a bias
+ * experts are ranked by their logits.  Scores that differ by less than fp32
+ * resolves are compared in double.  num_groups = topk_groups = group_top = 1
+ * gives the ungrouped choice.  Fills MlpConfig.num_experts / top_k
+ * (atb_cpp_llm/include/atb_llm/layer_desc.h:59-60). */
+B200_API int b200_moe_topk_grouped(const float* logits, int64_t ld, const float* bias, int64_t T, int num_experts,
+                                   int top_k, int scoring, int num_groups, int topk_groups, int group_top,
+                                   int renormalize, float scale, int32_t* topk_ids, float* topk_weights,
+                                   b200_stream_t stream);
 
 /* Expert permutation of the T*top_k (token, choice) entries: entry i = t*top_k
  * + j goes to slot perm_pos[i] = expert_offsets[e] + (entries of expert e

@@ -50,6 +50,42 @@ def route_topk(logits, k, renormalize=True, scale=1.0):
     return ids, w.astype(np.float32)
 
 
+def route_grouped(logits, k, sigmoid=False, bias=None, groups=1, keep=1, best=1, renormalize=True, scale=1.0):
+    """The grouped selection (published DeepSeek-V2 / V3 gates) in float64:
+    ``logits [T, E]`` -> ``(ids [T, k] int32, weights [T, k])``.
+
+    Scores s = softmax or sigmoid of the clamped logits (NaN: lowest); c = s +
+    bias; a group's score is the sum of its ``best`` largest c; the ``keep``
+    best groups' experts compete by c (by the logits where there is no bias);
+    weights are the chosen s, renormalised or not, times ``scale``.  Ties go to
+    the lower index."""
+    top = float(np.finfo(np.float32).max)
+    x = np.asarray(logits, np.float64)
+    x = np.clip(np.where(np.isnan(x), -top, x), -top, top)
+    T, E = x.shape
+    with np.errstate(over="ignore"):
+        if sigmoid:
+            s = 1 / (1 + np.exp(-x))
+        else:
+            s = np.exp(x - x.max(1, keepdims=True))
+            s = s / s.sum(1, keepdims=True)
+    c = s if bias is None else s + np.asarray(bias, np.float64)
+    order_by = x if bias is None else c
+    if keep < groups:
+        in_group = (x if bias is None and best == 1 else c).reshape(T, groups, E // groups)
+        score = np.sort(in_group, 2)[:, :, ::-1][:, :, :best].sum(2)
+        kept = np.argsort(-score, 1, kind="stable")[:, :keep]
+        mask = np.zeros((T, groups), bool)
+        np.put_along_axis(mask, kept, True, 1)
+        order_by = np.where(np.repeat(mask, E // groups, 1), order_by, -np.inf)
+    ids = np.argsort(-order_by, 1, kind="stable")[:, :k]
+    w = np.take_along_axis(s, ids, 1)
+    if renormalize:
+        total = w.sum(1, keepdims=True)
+        w = np.where(total > 0, w / np.where(total > 0, total, 1.0), 0.0)
+    return ids.astype(np.int32), w * scale
+
+
 def permute(ids, num_experts):
     """Stable grouping of the (token, choice) entries by expert.
 

@@ -1,0 +1,462 @@
+"""GPU parity of the 8-bit linear layers through the C ABI: row quantisation
+(bit-exact), its fused RMSNorm form (bit-exact against the two calls), the
+8-bit products, plain and grouped, against float64, and a routed expert MLP
+run through all of them.
+
+Tolerances.  The integer sums are exact, so a product carries: the conversion
+of the sum to fp32, two scale products, and the bias / residual additions (at
+most 6 roundings of 2^-24 of the terms), then one rounding to bf16 (2^-8 of the
+value).  GELU adds tanhf's 2 ulp.  SwiGLU's exponential is the fast one:
+(2 + 1.2 |g|) 2^-23 relative, 1.3e-5 for |g| <= 90, below which the gate
+vanishes, and the division is within 2 ulp.  So |out - ref| <= 2^-8 |ref| +
+2e-5 (|ref| + |terms|) for all of them.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import int8, moe
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import gpu_util as G
+
+F = np.float32
+NONE, BIAS, RESIDUAL, SWIGLU, BIAS_GELU, BIAS_RESIDUAL = range(6)
+
+
+def i8(a):
+    return G._keep(torch.from_numpy(np.ascontiguousarray(np.asarray(a, np.int8))).to(G.DEV))
+
+
+def all_bf16_up_to(top_bits):
+    """Every non-negative bf16 value up to the one with these bits, as float32."""
+    return (np.arange(top_bits + 1, dtype=np.uint32) << 16).view(F)
+
+
+def quant(x, ldx=None, ldq=None, src=None, count=None, rows=None):
+    """b200_quant_rows_int8 of a bf16 device tensor's first columns."""
+    n, dim = x.shape
+    rows = rows if rows is not None else (len(src) if src is not None else n)
+    ldq = ldq or dim
+    q = torch.full((rows, ldq), 99, dtype=torch.int8, device=G.DEV)
+    s = torch.full((rows,), 77.0, dtype=torch.float32, device=G.DEV)
+    G.check(G.L().b200_quant_rows_int8(x.data_ptr(), ldx or x.stride(0), n, G.ptr(None if src is None else G.i32(src)),
+                                       G.ptr(None if count is None else G.i32([count])), q.data_ptr(), ldq, s.data_ptr(),
+                                       rows, dim, G.stream()), "quant_rows_int8")
+    torch.cuda.synchronize()
+    return q.cpu().numpy(), G.host(s)
+
+
+# ------------------------------------------------------------ quantisation
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 16), (3, 48), (777, 1408), (64, 2048), (5, 2064), (33, 4096), (2, 8208), (7, 14336),
+                                      (2, 16384), (3, 16400), (2, 131056)])
+def test_quant_rows(rows, dim):
+    rng = np.random.default_rng(dim)
+    x = G.rounded(rng.standard_normal((rows, dim)).astype(F) * np.exp2(rng.integers(-20, 20, (rows, 1))).astype(F))
+    q, s = quant(G.bf16(x))
+    rq, rs = int8.quant_rows(x)
+    np.testing.assert_array_equal(q, rq)
+    np.testing.assert_array_equal(s, rs)
+
+
+@pytest.mark.parametrize("top", [0x0001, 0x0002, 0x0003, 0x007f, 0x0080, 0x00ff, 0x0d80, 0x0dff, 0x0e00, 0x3f7f, 0x3f80,
+                                 0x3f81, 0x3faa, 0x3ffd, 0x4213, 0x7180, 0x71ff, 0x7200, 0x7f00, 0x7f7e, 0x7f7f],
+                         ids=hex)
+def test_quant_every_value_below_a_maximum(top):
+    # ties, subnormals and both ends of the range: every bf16 magnitude up to the row's largest, both signs
+    v = all_bf16_up_to(top)
+    dim = -(-len(v) // 16) * 16
+    x = np.zeros((2, dim), F)
+    x[0, :len(v)] = v
+    x[1, :len(v)] = -v
+    q, s = quant(G.bf16(x))
+    rq, rs = int8.quant_rows(x)
+    np.testing.assert_array_equal(q, rq)
+    np.testing.assert_array_equal(s, rs)
+
+
+def test_quant_empty_and_non_finite_rows():
+    x = np.ones((6, 64), F)
+    x[1] = 0
+    x[2, 5] = np.inf
+    x[3, 63] = -np.inf
+    x[4, 0] = np.nan
+    x[5, 7] = -0.0
+    q, s = quant(G.bf16(x))
+    rq, rs = int8.quant_rows(x)
+    np.testing.assert_array_equal(q, rq)
+    np.testing.assert_array_equal(s, rs)
+    assert s[1] == 0 and np.isnan(s[2:5]).all() and not q[1:5].any()
+
+
+def test_quant_strides_gather_and_count():
+    rng = np.random.default_rng(1)
+    wide = G.bf16(rng.standard_normal((40, 112)).astype(F))
+    x = wide[:, 16:80]  # 64 columns of 112-wide rows
+    rx = G.host(x)
+    q, s = quant(x, ldx=112, ldq=96)
+    rq, rs = int8.quant_rows(rx)
+    np.testing.assert_array_equal(q[:, :64], rq)
+    assert (q[:, 64:] == 99).all()  # what lies between the rows is left alone
+    np.testing.assert_array_equal(s, rs)
+    src = rng.integers(0, 40, 101)
+    q, s = quant(x, ldx=112, src=src, count=90)
+    np.testing.assert_array_equal(q[:90], rq[src[:90]])
+    np.testing.assert_array_equal(s[:90], rs[src[:90]])
+    assert (q[90:] == 99).all() and (s[90:] == 77).all()
+    assert G.device_errors() == 0
+    src[[3, 50]] = [40, -1]  # out of range: reported, their rows left alone
+    q, s = quant(x, ldx=112, src=src)
+    ok = np.ones(101, bool)
+    ok[[3, 50]] = False
+    np.testing.assert_array_equal(q[ok], rq[src[ok]])
+    assert (q[~ok] == 99).all() and (s[~ok] == 77).all()
+    assert G.device_errors() == 2
+
+
+@pytest.mark.parametrize("rows,dim,stride", [(1, 16, 16), (64, 4096, 4096), (333, 1408, 1424), (3, 2064, 2064), (5, 8192, 8192)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm_quant_is_the_two_calls(rows, dim, stride, residual):
+    rng = np.random.default_rng(rows + dim)
+    L = G.L()
+    x = G.bf16(rng.standard_normal((rows, stride)).astype(F) * 3)
+    x[rows // 2] = 0  # a row of zeros
+    r = G.bf16(rng.standard_normal((rows, stride)).astype(F)) if residual else None
+    if residual:
+        r[rows // 2] = 0
+    w = G.bf16(1 + 0.1 * rng.standard_normal(dim).astype(F))
+    out, ro, out2, ro2 = (torch.zeros(rows, stride, dtype=torch.bfloat16, device=G.DEV) for _ in range(4))
+    q = torch.zeros(rows, dim, dtype=torch.int8, device=G.DEV)
+    s = torch.zeros(rows, dtype=torch.float32, device=G.DEV)
+    G.check(L.b200_rmsnorm(x.data_ptr(), G.ptr(r), w.data_ptr(), out.data_ptr(), ro.data_ptr() if residual else None, rows,
+                           dim, stride, 1e-6, G.stream()))
+    for with_out in (True, False):
+        q.fill_(99)
+        G.check(L.b200_rmsnorm_quant_int8(x.data_ptr(), G.ptr(r), w.data_ptr(), q.data_ptr(), dim, s.data_ptr(),
+                                          out2.data_ptr() if with_out else None, ro2.data_ptr() if residual else None, rows,
+                                          dim, stride, 1e-6, G.stream()))
+        torch.cuda.synchronize()
+        rq, rs = int8.quant_rows(G.host(out)[:, :dim])
+        np.testing.assert_array_equal(q.cpu().numpy(), rq)
+        np.testing.assert_array_equal(G.host(s), rs)
+        if residual:
+            np.testing.assert_array_equal(G.host(ro2), G.host(ro))
+    np.testing.assert_array_equal(G.host(out2), G.host(out))
+    if residual:  # the sum written over the residual
+        G.check(L.b200_rmsnorm_quant_int8(x.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), dim, s.data_ptr(), None,
+                                          r.data_ptr(), rows, dim, stride, 1e-6, G.stream()))
+        torch.cuda.synchronize()
+        np.testing.assert_array_equal(G.host(r)[:, :dim], G.host(ro)[:, :dim])
+        np.testing.assert_array_equal(q.cpu().numpy(), rq)
+
+
+# ----------------------------------------------------------------- products
+
+
+def near(out, ref, terms=0.0):
+    """The bound of the module's docstring; NaN where the reference is NaN."""
+    out, ref = np.asarray(out, np.float64), np.asarray(ref, np.float64)
+    bad = np.isnan(ref)
+    assert (np.isnan(out) == bad).all()
+    err = np.abs(out - ref)
+    lim = 2.0**-8 * np.abs(ref) + 2e-5 * (np.abs(ref) + terms) + 1e-30
+    worst = np.where(bad, 0, err - lim)
+    assert (worst <= 0).all(), (float(worst.max()), np.unravel_index(worst.argmax(), worst.shape))
+
+
+def operands(rng, M, N, K, epi, full=False):
+    a = rng.integers(-128 if full else -127, 128, (M, K)).astype(np.int8)
+    b = rng.integers(-128 if full else -127, 128, (N, K)).astype(np.int8)
+    unit = 1.0 / (73 * np.sqrt(K))  # products of about one standard deviation
+    sa = (rng.uniform(0.5, 2, M) * unit).astype(F)
+    sb = (rng.uniform(0.5, 2, N) / 73 * 40).astype(F)
+    bias = G.rounded(rng.standard_normal(N)) if epi in (BIAS, BIAS_GELU, BIAS_RESIDUAL) else None
+    res = G.rounded(rng.standard_normal((M, N))) if epi in (RESIDUAL, BIAS_RESIDUAL) else None
+    return a, sa, b, sb, bias, res
+
+
+def gemm(a, sa, b, sb, epi, bias=None, res=None, pad=0, out=None, inplace=False):
+    """b200_gemm_int8 on numpy operands; pad: extra columns in every row stride."""
+    M, K = a.shape
+    N = b.shape[0]
+    outN = N // 2 if epi == SWIGLU else N
+    wide = lambda m, fill: np.concatenate([m, np.full((len(m), pad), fill, m.dtype)], 1)  # noqa: E731
+    A, B = i8(wide(a, 55)), i8(wide(b, -77))
+    R = G.bf16(wide(np.asarray(res, F), 1e30)) if res is not None else None
+    C = R if inplace else torch.full((M, outN + pad), 7.0, dtype=torch.bfloat16, device=G.DEV)
+    G.check(G.L().b200_gemm_int8(A.data_ptr(), K + pad, G.f32(sa).data_ptr(), B.data_ptr(), K + pad, G.f32(sb).data_ptr(),
+                                 C.data_ptr(), outN + pad, M, N, K, epi, G.ptr(None if bias is None else G.bf16(bias)),
+                                 G.ptr(R), N + pad, G.stream()), "gemm_int8")
+    torch.cuda.synchronize()
+    assert G.device_errors() == 0
+    h = G.host(C)
+    if pad and not inplace:
+        assert (h[:, outN:] == 7).all()
+    return h[:, :outN]
+
+
+SHAPES = [(1, 8, 16), (1, 4096, 4096), (2, 136, 144), (8, 256, 48), (15, 520, 1040), (16, 128, 128), (17, 264, 272),
+          (32, 6144, 512), (33, 1032, 2064), (64, 512, 4096), (65, 2056, 128), (96, 24, 4112), (128, 640, 1408),
+          (129, 128, 256), (130, 136, 272), (200, 1408, 2048), (257, 264, 1040), (300, 8, 16), (512, 4096, 1024),
+          (777, 520, 1040), (1025, 1288, 400), (2049, 2568, 144)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_gemm_shapes(M, N, K):
+    rng = np.random.default_rng(M * 7 + N + K)
+    a, sa, b, sb, _, _ = operands(rng, M, N, K, NONE)
+    near(gemm(a, sa, b, sb, NONE), int8.gemm(a, sa, b, sb))
+
+
+@pytest.mark.parametrize("epi", range(6))
+@pytest.mark.parametrize("M,N,K", [(1, 144, 272), (20, 528, 1040), (50, 272, 4112), (128, 1040, 512), (131, 144, 272),
+                                   (700, 1296, 528)])
+def test_gemm_epilogues(M, N, K, epi):
+    rng = np.random.default_rng(M + epi)
+    a, sa, b, sb, bias, res = operands(rng, M, N, K, epi)
+    ref = int8.gemm(a, sa, b, sb, epi, bias, res)
+    out = gemm(a, sa, b, sb, epi, bias, res, pad=16)
+    if epi == SWIGLU:
+        v = int8.gemm(a, sa, b, sb)
+        near(out, ref, 0.0 * v[:, ::2])
+    else:
+        terms = np.abs(int8.gemm(a, sa, b, sb)) + (0 if bias is None else np.abs(bias)) + (0 if res is None else np.abs(res))
+        near(out, ref, terms)
+    if epi == RESIDUAL:  # the residual stream updated in place
+        near(gemm(a, sa, b, sb, epi, bias, res, pad=16, inplace=True), ref, terms)
+
+
+@pytest.mark.parametrize("M,K", [(3, 131056), (140, 131056)])
+def test_gemm_longest_sums_of_extremes(M, K):
+    # -128 * -128 over the longest K: 2^31 - 2^18, exact in 32 bits
+    a, b = np.full((M, K), -128, np.int8), np.full((16, K), -128, np.int8)
+    b[1::2] = 127
+    sa, sb = np.full(M, 2.0**-20, F), np.full(16, 1.0, F)
+    near(gemm(a, sa, b, sb, NONE), int8.gemm(a, sa, b, sb))
+
+
+@pytest.mark.parametrize("M", [5, 64, 150])
+def test_gemm_integers_are_exact(M):
+    # sums small enough for bf16 come back as themselves, so every partial product is in its place
+    rng = np.random.default_rng(M)
+    N, K = 264, 2064
+    a, b = np.zeros((M, K), np.int8), np.zeros((N, K), np.int8)
+    a[np.arange(M), rng.permutation(K)[:M]] = rng.integers(-8, 9, M)
+    b[:] = rng.integers(-8, 9, (N, K))
+    out = gemm(a, np.ones(M, F), b, np.ones(N, F), NONE)
+    np.testing.assert_array_equal(out, a.astype(np.int64) @ b.astype(np.int64).T)
+
+
+def test_gemm_non_finite_scales_stay_in_their_rows():
+    rng = np.random.default_rng(9)
+    for M in (6, 200):
+        for epi in (NONE, SWIGLU):
+            a, sa, b, sb, _, _ = operands(rng, M, 272, 528, epi)
+            sa[3] = np.nan
+            a[3] = 0
+            sa[4] = 0
+            near(gemm(a, sa, b, sb, epi), int8.gemm(a, sa, b, sb, epi))
+
+
+def test_gemm_swiglu_of_large_gates():
+    rng = np.random.default_rng(10)
+    for M in (6, 200):
+        a, sa, b, sb, _, _ = operands(rng, M, 272, 528, SWIGLU)
+        out = gemm(a, sa * 200, b, sb, SWIGLU)
+        assert np.isfinite(out).all()
+        ref = int8.gemm(a, sa * 200, b, sb, SWIGLU)
+        gate = int8.gemm(a, sa * 200, b, sb)[:, ::2]
+        seen = gate > -80  # below, the gate's e^g leaves the fast division's range: less than 1e-30 of the up value
+        near(np.where(seen, out, 0), np.where(seen, ref, 0))
+        assert np.abs(np.where(seen, 0, out)).max() < 1e-25
+
+
+def test_gemm_same_bits_twice_and_on_two_streams():
+    rng = np.random.default_rng(11)
+    for M, N, K in [(8, 4096, 4096), (300, 1024, 2048)]:
+        a, sa, b, sb, _, _ = operands(rng, M, N, K, NONE)
+        want = gemm(a, sa, b, sb, NONE)
+        A, B, SA, SB = i8(a), i8(b), G.f32(sa), G.f32(sb)
+        outs = [torch.zeros(M, N, dtype=torch.bfloat16, device=G.DEV) for _ in range(6)]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for i, o in enumerate(outs):
+            G.check(G.L().b200_gemm_int8(A.data_ptr(), K, SA.data_ptr(), B.data_ptr(), K, SB.data_ptr(), o.data_ptr(), N, M,
+                                         N, K, NONE, None, None, 0, streams[i % 2].cuda_stream))
+        torch.cuda.synchronize()
+        for o in outs:
+            np.testing.assert_array_equal(G.host(o), want)
+
+
+# ------------------------------------------------------------ grouped product
+
+
+def grouped(a, sa, b, sb, sizes, N, epi, extra=0):
+    K = a.shape[1]
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    rows = int(off[-1]) + extra
+    outN = N // 2 if epi == SWIGLU else N
+    pad = np.zeros((rows - len(a), K), np.int8)
+    C = torch.full((rows, outN), 7.0, dtype=torch.bfloat16, device=G.DEV)
+    SA = G.f32(np.concatenate([sa, np.ones(rows - len(sa), F)]))
+    G.check(G.L().b200_grouped_gemm_int8(i8(np.concatenate([a, pad])).data_ptr(), K, SA.data_ptr(), i8(b).data_ptr(), K,
+                                         G.f32(sb).data_ptr(), C.data_ptr(), outN, G.i32(off).data_ptr(), len(sizes), rows,
+                                         N, K, epi, G.stream()), "grouped_gemm_int8")
+    torch.cuda.synchronize()
+    assert G.device_errors() == 0
+    h = G.host(C)
+    assert (h[off[-1]:] == 7).all()  # rows behind the last group stay as they were
+    return h[:off[-1]], off
+
+
+GROUPS = [
+    ([3, 0, 17, 64, 1, 0, 100, 7], 256, 512), ([3, 0, 17, 64, 1, 0, 100, 7], 208, 528), ([1], 128, 128), ([0, 1, 0], 24, 16),
+    ([2] * 64, 176, 256), ([0, 0, 0, 40], 128, 144), ([300, 0, 513, 129], 512, 256), ([300, 0, 513, 129], 144, 272),
+    ([128, 256, 1, 700], 1296, 144), ([0, 0, 900], 2816, 400), ([97] * 5, 272, 1040), ([5, 700, 3, 0, 2, 1], 544, 256),
+    ([0] * 40 + [9], 144, 272), ([1000] + [0] * 255, 48, 48)]
+
+
+@pytest.mark.parametrize("epi", [NONE, SWIGLU])
+@pytest.mark.parametrize("sizes,N,K", GROUPS, ids=[str(i) for i in range(len(GROUPS))])
+def test_grouped_gemm(sizes, N, K, epi):
+    if epi == SWIGLU:
+        N = -(-N // 16) * 16  # gate / up pairs of 8 (others are refused, tests/test_int8_cpu.py)
+    rng = np.random.default_rng(sum(sizes) + N + epi)
+    rows, n = int(sum(sizes)), len(sizes)
+    a, sa, b, sb, _, _ = operands(rng, rows, n * N, K, epi)
+    out, off = grouped(a, sa, b, sb, sizes, N, epi, extra=37)
+    for g in range(n):
+        r, w = slice(off[g], off[g + 1]), slice(g * N, (g + 1) * N)
+        near(out[r], int8.gemm(a[r], sa[r], b[w], sb[w], epi))
+
+
+def test_grouped_gemm_without_rows_and_with_bad_offsets():
+    rng = np.random.default_rng(4)
+    a, sa, b, sb, _, _ = operands(rng, 20, 3 * 128, 256, NONE)
+    L = G.L()
+
+    def call(off, rows=20):
+        C = torch.full((20, 128), 7.0, dtype=torch.bfloat16, device=G.DEV)
+        G.check(L.b200_grouped_gemm_int8(i8(a).data_ptr(), 256, G.f32(sa).data_ptr(), i8(b).data_ptr(), 256,
+                                         G.f32(sb).data_ptr(), C.data_ptr(), 128, G.i32(off).data_ptr(), 3, rows, 128, 256,
+                                         NONE, G.stream()))
+        torch.cuda.synchronize()
+        return G.host(C), G.device_errors()
+
+    out, err = call([0, 0, 0, 0])
+    assert (out == 7).all() and err == 0
+    for off in ([0, 10, 5, 20], [0, 10, 15, 30], [-3, 5, 10, 20], [4, 5, 10, 20]):
+        assert call(off)[1] == 2, off
+
+
+# ----------------------------------------------------------- used together
+
+
+@pytest.mark.parametrize("T,E,k,H,I,groups", [(1, 8, 2, 256, 272, 1), (33, 64, 6, 512, 176, 8), (700, 16, 4, 272, 144, 4)])
+def test_routed_experts(T, E, k, H, I, groups):
+    """Router selection -> permutation -> gather + quantise -> gate/up -> quantise -> down -> combine, each stage
+    against float64 on its own inputs, and the same bits from a captured graph and from two graphs replayed in turn."""
+    rng = np.random.default_rng(T)
+    L = G.L()
+    R = T * k
+    x = G.rounded(rng.standard_normal((T, H)))
+    lg = (rng.standard_normal((T, E)) * 1.5).astype(F)
+    b1, sb1 = rng.integers(-127, 128, (E * 2 * I, H)).astype(np.int8), rng.uniform(1, 3, E * 2 * I).astype(F) * 3e-4
+    b2, sb2 = rng.integers(-127, 128, (E * H, I)).astype(np.int8), rng.uniform(1, 3, E * H).astype(F) * 3e-4
+    X, LG, B1, S1, B2, S2 = G.bf16(x), G.f32(lg), i8(b1), G.f32(sb1), i8(b2), G.f32(sb2)
+    new = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=G.DEV)  # noqa: E731
+
+    def buffers():
+        return dict(ids=new(T, k, t=torch.int32), w=new(T, k, t=torch.float32), off=new(E + 1, t=torch.int32),
+                    pos=new(R, t=torch.int32), src=new(R, t=torch.int32),
+                    ws=new(max(16, L.b200_moe_permute_workspace_bytes(T, k, E)), t=torch.uint8), q1=new(R, H, t=torch.int8),
+                    s1=new(R, t=torch.float32), act=new(R, I), q2=new(R, I, t=torch.int8), s2=new(R, t=torch.float32),
+                    y=new(R, H), out=new(T, H))
+
+    def run(d, st):
+        p = {n: t.data_ptr() for n, t in d.items()}
+        G.check(L.b200_moe_topk_grouped(LG.data_ptr(), E, None, T, E, k, 1, groups, max(1, groups // 2),
+                                        2 if groups > 1 else 1, 1, 1.0, p["ids"], p["w"], st))
+        G.check(L.b200_moe_permute(p["ids"], T, k, E, None, 0, 0, None, p["off"], p["pos"], p["src"], p["ws"],
+                                   d["ws"].numel(), st))
+        total = p["off"] + 4 * E
+        G.check(L.b200_quant_rows_int8(X.data_ptr(), H, T, p["src"], total, p["q1"], H, p["s1"], R, H, st))
+        G.check(L.b200_grouped_gemm_int8(p["q1"], H, p["s1"], B1.data_ptr(), H, S1.data_ptr(), p["act"], I, p["off"], E, R,
+                                         2 * I, H, SWIGLU, st))
+        G.check(L.b200_quant_rows_int8(p["act"], I, R, None, total, p["q2"], I, p["s2"], R, I, st))
+        G.check(L.b200_grouped_gemm_int8(p["q2"], I, p["s2"], B2.data_ptr(), I, S2.data_ptr(), p["y"], H, p["off"], E, R, H,
+                                         I, NONE, st))
+        G.check(L.b200_moe_combine(p["y"], p["pos"], p["w"], T, k, H, X.data_ptr(), None, p["out"], None, None, 1e-6, st))
+
+    d = buffers()
+    run(d, G.stream())
+    torch.cuda.synchronize()
+    assert G.device_errors() == 0
+    ids, w = moe.route_grouped(lg, k, True, None, groups, max(1, groups // 2), 2 if groups > 1 else 1)
+    np.testing.assert_array_equal(d["ids"].cpu().numpy(), ids)
+    off, pos, src = moe.permute(ids, E)
+    np.testing.assert_array_equal(d["src"].cpu().numpy(), src)
+    q1, s1 = int8.quant_rows(x[src])
+    np.testing.assert_array_equal(d["q1"].cpu().numpy(), q1)
+    act, y = G.host(d["act"]), G.host(d["y"])
+    q2, s2 = int8.quant_rows(act)
+    np.testing.assert_array_equal(d["q2"].cpu().numpy(), q2)
+    np.testing.assert_array_equal(G.host(d["s2"]), s2)
+    for e in range(E):
+        r = slice(off[e], off[e + 1])
+        up, down = slice(e * 2 * I, (e + 1) * 2 * I), slice(e * H, (e + 1) * H)
+        near(act[r], int8.gemm(q1[r], s1[r], b1[up], sb1[up], SWIGLU))
+        near(y[r], int8.gemm(q2[r], s2[r], b2[down], sb2[down]))
+    routed = (y[pos].reshape(T, k, H) * w[:, :, None]).sum(1)
+    # fp32 sums of k + 1 terms and fp32 weights, one rounding to bf16
+    near(G.host(d["out"]), x + routed, 2 * np.abs(y[pos]).reshape(T, k, H).max(1))
+
+    # captured, with the weights shared and the buffers each graph's own
+    graphs = []
+    for _ in range(2):
+        g, b = torch.cuda.CUDAGraph(), buffers()
+        st = torch.cuda.Stream()
+        with torch.cuda.graph(g, stream=st):
+            run(b, torch.cuda.current_stream().cuda_stream)
+        graphs.append((g, b))
+    for _ in range(3):
+        for g, _b in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for _g, b in graphs:
+        np.testing.assert_array_equal(G.host(b["out"]), G.host(d["out"]))
+    assert G.device_errors() == 0
+
+
+def test_weights_quantised_right_before_the_product():
+    """The product's weights made by the kernels just before it, back to back on one stream, many times over."""
+    rng = np.random.default_rng(12)
+    M, N, K = 16, 2048, 4096
+    L = G.L()
+    x = G.bf16(rng.standard_normal((M, K)).astype(F))
+    q, s = torch.zeros(M, K, dtype=torch.int8, device=G.DEV), torch.zeros(M, dtype=torch.float32, device=G.DEV)
+    wq, ws = torch.zeros(N, K, dtype=torch.int8, device=G.DEV), torch.zeros(N, dtype=torch.float32, device=G.DEV)
+    weights = [G.bf16(rng.standard_normal((N, K)).astype(F)) for _ in range(3)]
+    outs = [torch.zeros(M, N, dtype=torch.bfloat16, device=G.DEV) for _ in range(30)]
+    for i, o in enumerate(outs):
+        w = weights[i % 3]
+        if i % 2:
+            G.check(L.b200_quant_rows_int8(w.data_ptr(), K, N, None, None, wq.data_ptr(), K, ws.data_ptr(), N, K, G.stream()))
+            G.check(L.b200_quant_rows_int8(x.data_ptr(), K, M, None, None, q.data_ptr(), K, s.data_ptr(), M, K, G.stream()))
+        else:
+            G.check(L.b200_quant_rows_int8(x.data_ptr(), K, M, None, None, q.data_ptr(), K, s.data_ptr(), M, K, G.stream()))
+            G.check(L.b200_quant_rows_int8(w.data_ptr(), K, N, None, None, wq.data_ptr(), K, ws.data_ptr(), N, K, G.stream()))
+        G.check(L.b200_gemm_int8(q.data_ptr(), K, s.data_ptr(), wq.data_ptr(), K, ws.data_ptr(), o.data_ptr(), N, M, N, K,
+                                 NONE, None, None, 0, G.stream()))
+    torch.cuda.synchronize()
+    qa, sa = int8.quant_rows(G.host(x))
+    for i in range(3):
+        qb, sb = int8.quant_rows(G.host(weights[i]))
+        near(G.host(outs[i]), int8.gemm(qa, sa, qb, sb))
+        for j in range(i, 30, 3):
+            np.testing.assert_array_equal(G.host(outs[j]), G.host(outs[i]))

@@ -1,0 +1,130 @@
+"""GPU parity of b200_moe_topk_grouped against the float64 restatement.
+
+Expert ids are equal, ties and near-ties included: the definition ranks scores
+in 64 bits, and the kernel decides in double whatever fp32 cannot tell apart.
+Weights: fp32 scores are within 1.8e-6 of the largest one (expf 2 ulp, at most
+21 roundings of the sum, the division), renormalising adds as much again.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import moe
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import gpu_util as G
+
+F = np.float32
+
+
+def route(lg, k, sigmoid=False, bias=None, groups=1, keep=1, best=1, renorm=True, scale=1.0, pad=0):
+    T, E = lg.shape
+    d = G.f32(np.concatenate([lg, np.full((T, pad), 1e9, F)], 1) if pad else lg)
+    ids = torch.full((T + 1, k), -5, dtype=torch.int32, device=G.DEV)
+    w = torch.full((T + 1, k), -5.0, dtype=torch.float32, device=G.DEV)
+    G.check(G.L().b200_moe_topk_grouped(d.data_ptr(), E + pad, G.ptr(None if bias is None else G.f32(bias)), T, E, k,
+                                        int(sigmoid), groups, keep, best, int(renorm), scale, ids.data_ptr(), w.data_ptr(),
+                                        G.stream()), "moe_topk_grouped")
+    ids, w = ids.cpu().numpy(), G.host(w)
+    assert (ids[T] == -5).all() and (w[T] == -5).all()
+    return ids[:T], w[:T]
+
+
+def check(lg, k, **kw):
+    ids, w = route(lg, k, **kw)
+    kw.pop("pad", None)
+    rid, rw = moe.route_grouped(lg, k, kw.get("sigmoid", False), kw.get("bias"), kw.get("groups", 1), kw.get("keep", 1),
+                                kw.get("best", 1), kw.get("renorm", True), kw.get("scale", 1.0))
+    np.testing.assert_array_equal(ids, rid)
+    np.testing.assert_allclose(w, rw, rtol=1e-5, atol=2e-6 * kw.get("scale", 1.0))
+    return ids, w
+
+
+CASES = [(1, 1, 1, 1, 1, 1), (5, 2, 1, 1, 1, 1), (777, 8, 2, 1, 1, 1), (64, 64, 6, 1, 1, 1), (1000, 128, 8, 1, 1, 1),
+         (2049, 256, 8, 8, 4, 2), (300, 160, 6, 8, 3, 1), (301, 160, 6, 5, 2, 2), (100, 64, 8, 8, 1, 2), (100, 64, 8, 32, 4, 2),
+         (99, 96, 5, 3, 2, 2), (98, 255, 7, 17, 3, 2), (97, 252, 8, 18, 9, 1), (96, 7, 3, 7, 4, 1), (95, 30, 4, 3, 3, 2),
+         (94, 250, 8, 2, 1, 2), (93, 6, 6, 2, 2, 1), (92, 34, 2, 17, 1, 2)]
+
+
+@pytest.mark.parametrize("T,E,k,groups,keep,best", CASES)
+@pytest.mark.parametrize("sigmoid", [False, True], ids=["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True], ids=["", "bias"])
+def test_choice(T, E, k, groups, keep, best, sigmoid, biased):
+    rng = np.random.default_rng(T + E)
+    lg = (rng.standard_normal((T, E)) * 1.5).astype(F)
+    bias = (rng.standard_normal(E) * 0.05).astype(F) if biased else None
+    for renorm in (False, True):
+        check(lg, k, sigmoid=sigmoid, bias=bias, groups=groups, keep=keep, best=best, renorm=renorm,
+              scale=2.5 if renorm else 1.0, pad=E % 3)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True], ids=["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,keep,best", [(1, 1, 1), (8, 3, 1), (8, 4, 2)])
+def test_ties(sigmoid, groups, keep, best):
+    rng = np.random.default_rng(groups)
+    lg = (rng.integers(-3, 4, (400, 128)) * 0.5).astype(F)
+    lg[0] = 0
+    check(lg, 8, sigmoid=sigmoid, groups=groups, keep=keep, best=best)
+    b = (rng.integers(-2, 3, 128) * 0.25).astype(F)
+    check(lg, 8, sigmoid=sigmoid, bias=b, groups=groups, keep=keep, best=best)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True], ids=["softmax", "sigmoid"])
+def test_scores_that_fp32_cannot_tell_apart(sigmoid):
+    # logits one ulp apart, under a bias that hides the difference in fp32
+    rng = np.random.default_rng(5)
+    lg = np.full((64, 64), 0.5, F)
+    up = rng.integers(0, 20, lg.shape)
+    lg = (lg.view(np.int32) + up.astype(np.int32)).view(F)
+    bias = np.full(64, 1.0, F)
+    check(lg, 8, sigmoid=sigmoid, bias=bias, groups=8, keep=4, best=2)
+    check(lg, 8, sigmoid=sigmoid, bias=bias)
+    check(lg, 8, sigmoid=sigmoid, groups=8, keep=4, best=2)
+
+
+def test_masked_and_extreme_logits():
+    big = float(np.finfo(F).max)
+    lg = np.zeros((9, 32), F)
+    lg[0] = -np.inf  # nothing left: uniform, the lowest experts
+    lg[1] = -big
+    lg[2, :] = -np.inf
+    lg[2, 30] = 1.0  # one expert left
+    lg[3, 4] = np.inf
+    lg[4, 4], lg[4, 9] = np.inf, np.inf
+    lg[5] = np.nan
+    lg[6, 3], lg[6, 20] = np.nan, 2.0
+    lg[7] = np.linspace(-80, 80, 32)
+    lg[8, ::2] = -big
+    for sigmoid in (False, True):
+        for groups, keep, best in ((1, 1, 1), (4, 2, 1), (4, 2, 2)):
+            for renorm in (False, True):
+                check(lg, 4, sigmoid=sigmoid, groups=groups, keep=keep, best=best, renorm=renorm)
+    # sigmoids below fp32's range are renormalised in double
+    ids, w = route(np.linspace(-120, -100, 32, dtype=F)[None], 4, sigmoid=True)
+    rid, rw = moe.route_grouped(np.linspace(-120, -100, 32, dtype=F)[None], 4, True)
+    np.testing.assert_array_equal(ids, rid)
+    np.testing.assert_allclose(w, rw, rtol=1e-5)
+
+
+def test_large_biases_move_the_choice_alone():
+    rng = np.random.default_rng(6)
+    lg = rng.standard_normal((50, 64)).astype(F)
+    b = (rng.standard_normal(64) * 1000).astype(F)
+    for sigmoid in (False, True):
+        ids, w = check(lg, 6, sigmoid=sigmoid, bias=b, groups=8, keep=4, best=2, renorm=False)
+        assert (w <= 1).all()
+
+
+def test_matches_the_ungrouped_selection():
+    rng = np.random.default_rng(7)
+    lg = rng.standard_normal((500, 64)).astype(F)
+    ids, w = route(lg, 6, renorm=False, scale=1.5)
+    d = G.f32(lg)
+    i2 = torch.empty(500, 6, dtype=torch.int32, device=G.DEV)
+    w2 = torch.empty(500, 6, dtype=torch.float32, device=G.DEV)
+    G.check(G.L().b200_moe_topk(d.data_ptr(), 500, 64, 6, 0, 1.5, i2.data_ptr(), w2.data_ptr(), G.stream()))
+    np.testing.assert_array_equal(ids, i2.cpu().numpy())
+    np.testing.assert_allclose(w, G.host(w2), rtol=1e-5, atol=2e-6)
