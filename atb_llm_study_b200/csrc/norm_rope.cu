@@ -99,16 +99,27 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_quant_kernel(const __nv_
   const int64_t row = blockIdx.x;
   const int64_t nchunk = dim / 8;
   const __nv_bfloat16* xr = x + row * stride;
+  // all loads before the first store, which may be to what is still to be read
+  // for all that the compiler knows
+  uint4 xv[CH], rv[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
+    if (idx < nchunk) {
+      xv[c] = *reinterpret_cast<const uint4*>(xr + idx * 8);
+      if (residual) rv[c] = *reinterpret_cast<const uint4*>(residual + row * stride + idx * 8);
+    }
+  }
   float v[CH][8];
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
     if (idx < nchunk) {
-      unpack8(*reinterpret_cast<const uint4*>(xr + idx * 8), v[c]);
+      unpack8(xv[c], v[c]);
       if (residual) {
         float r[8];
-        unpack8(*reinterpret_cast<const uint4*>(residual + row * stride + idx * 8), r);
+        unpack8(rv[c], r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[c][i] += r[i];
         if (residual_out) *reinterpret_cast<uint4*>(residual_out + row * stride + idx * 8) = pack8(v[c]);
@@ -116,6 +127,12 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_quant_kernel(const __nv_
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
     }
+  }
+  uint4 wv[CH];  // the norm weight, loaded while the row sum is reduced
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
+    if (idx < nchunk) wv[c] = *reinterpret_cast<const uint4*>(w + idx * 8);
   }
   const float tot = block_sum<kNormThreads>(ss, red);
   const float inv = rsqrtf(tot / (float)dim + eps);
@@ -126,7 +143,7 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_quant_kernel(const __nv_
     const int64_t idx = threadIdx.x + (int64_t)c * kNormThreads;
     if (idx < nchunk) {
       float g[8], n[8];
-      unpack8(*reinterpret_cast<const uint4*>(w + idx * 8), g);
+      unpack8(wv[c], g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) n[i] = v[c][i] * inv * g[i];
       o[c] = pack8(n);

@@ -7,8 +7,6 @@ using namespace b200;
 
 namespace {
 
-constexpr int kQuantThreads = 128;
-
 struct QuantParams {
   const __nv_bfloat16* x;
   int64_t ldx;
@@ -18,39 +16,43 @@ struct QuantParams {
   int8_t* q;
   int64_t ldq;
   float* scale;
-  int64_t dim;
+  int64_t rows, dim;
   unsigned* err;
 };
 
 // The x row of output row `row`, or NULL when there is nothing to write.
-__device__ __forceinline__ const __nv_bfloat16* source_row(const QuantParams& p, int64_t row) {
+__device__ __forceinline__ const __nv_bfloat16* source_row(const QuantParams& p, int64_t row, bool leader) {
   if (p.count && row >= *p.count) return nullptr;
   int64_t sr = row;
   if (p.src) {
     sr = p.src[row];
     if (sr < 0 || sr >= p.src_rows) {
-      if (threadIdx.x == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
+      if (leader) raise_error(p.err, DEV_ERR_BAD_INDEX);
       return nullptr;
     }
   }
   return p.x + sr * p.ldx;
 }
 
-// One CTA per row; the row stays in registers between its maximum and the
-// write.  A thread owns CH chunks of 16 values (32 bytes read, 16 written).
-template <int CH>
-__global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const QuantParams p) {
-  __shared__ uint32_t red[kQuantThreads / 32];
+// W warps per row (1: the rows of a CTA's four warps are apart and nothing is
+// exchanged through shared memory).  The row stays in registers between its
+// maximum and the write; a thread owns CH chunks of 16 values (32 bytes read,
+// 16 written).
+template <int W, int CH>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) quant_rows_kernel(const QuantParams p) {
+  __shared__ uint32_t red[W];
   pdl_trigger();
   pdl_wait();
-  const int64_t row = blockIdx.x;
-  const __nv_bfloat16* xr = source_row(p, row);
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const int t = W == 1 ? threadIdx.x & 31 : threadIdx.x;
+  if (row >= p.rows) return;
+  const __nv_bfloat16* xr = source_row(p, row, t == 0);
   if (!xr) return;
   uint4 v[CH][2];
   uint32_t m = 0;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int64_t i = ((int64_t)c * kQuantThreads + threadIdx.x) * 16;
+    const int64_t i = ((int64_t)c * (W * 32) + t) * 16;
     if (i < p.dim) {
       v[c][0] = *reinterpret_cast<const uint4*>(xr + i);
       v[c][1] = *reinterpret_cast<const uint4*>(xr + i + 8);
@@ -58,14 +60,14 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const QuantPa
   }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int64_t i = ((int64_t)c * kQuantThreads + threadIdx.x) * 16;
+    const int64_t i = ((int64_t)c * (W * 32) + t) * 16;
     if (i < p.dim) m = amax_pairs(amax_pairs(m, v[c][0]), v[c][1]);
   }
-  const RowQuant r = row_quant(block_amax<kQuantThreads>(m, red));
-  if (threadIdx.x == 0) p.scale[row] = r.scale;
+  const RowQuant r = row_quant(W == 1 ? warp_amax(m) : block_amax<W * 32>(m, red));
+  if (t == 0) p.scale[row] = r.scale;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int64_t i = ((int64_t)c * kQuantThreads + threadIdx.x) * 16;
+    const int64_t i = ((int64_t)c * (W * 32) + t) * 16;
     if (i < p.dim) {
       const uint2 a = quant8(v[c][0], r), b = quant8(v[c][1], r);
       *reinterpret_cast<uint4*>(p.q + row * p.ldq + i) = make_uint4(a.x, a.y, b.x, b.y);
@@ -74,19 +76,20 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const QuantPa
 }
 
 // Rows too long for registers: the second pass reads the row again (from L2).
-__global__ void __launch_bounds__(kQuantThreads) quant_long_rows_kernel(const QuantParams p) {
-  __shared__ uint32_t red[kQuantThreads / 32];
+constexpr int kLongThreads = 512;
+__global__ void __launch_bounds__(kLongThreads) quant_long_rows_kernel(const QuantParams p) {
+  __shared__ uint32_t red[kLongThreads / 32];
   pdl_trigger();
   pdl_wait();
   const int64_t row = blockIdx.x;
-  const __nv_bfloat16* xr = source_row(p, row);
+  const __nv_bfloat16* xr = source_row(p, row, threadIdx.x == 0);
   if (!xr) return;
   uint32_t m = 0;
-  for (int64_t i = threadIdx.x * 8; i < p.dim; i += kQuantThreads * 8)
+  for (int64_t i = threadIdx.x * 8; i < p.dim; i += kLongThreads * 8)
     m = amax_pairs(m, *reinterpret_cast<const uint4*>(xr + i));
-  const RowQuant r = row_quant(block_amax<kQuantThreads>(m, red));
+  const RowQuant r = row_quant(block_amax<kLongThreads>(m, red));
   if (threadIdx.x == 0) p.scale[row] = r.scale;
-  for (int64_t i = threadIdx.x * 16; i < p.dim; i += kQuantThreads * 16) {
+  for (int64_t i = threadIdx.x * 16; i < p.dim; i += kLongThreads * 16) {
     const uint2 a = quant8(*reinterpret_cast<const uint4*>(xr + i), r);
     const uint2 b = quant8(*reinterpret_cast<const uint4*>(xr + i + 8), r);
     *reinterpret_cast<uint4*>(p.q + row * p.ldq + i) = make_uint4(a.x, a.y, b.x, b.y);
@@ -111,15 +114,19 @@ extern "C" int b200_quant_rows_int8(const void* x, int64_t ldx, int64_t src_rows
   if (rows == 0) return B200_OK;
   int dev = 0;
   cudaGetDevice(&dev);
-  const QuantParams p{static_cast<const __nv_bfloat16*>(x), ldx, row_src, src_rows, row_count, q, ldq, scale, dim,
+  const QuantParams p{static_cast<const __nv_bfloat16*>(x), ldx, row_src, src_rows, row_count, q, ldq, scale, rows, dim,
                       b200::error_word(dev)};
-  const dim3 g((unsigned)rows);
-  const int64_t per = (dim / 16 + kQuantThreads - 1) / kQuantThreads;
-  if (per <= 1) launch_kernel(quant_rows_kernel<1>, g, kQuantThreads, 0, stream, p);
-  else if (per <= 2) launch_kernel(quant_rows_kernel<2>, g, kQuantThreads, 0, stream, p);
-  else if (per <= 4) launch_kernel(quant_rows_kernel<4>, g, kQuantThreads, 0, stream, p);
-  else if (per <= 8) launch_kernel(quant_rows_kernel<8>, g, kQuantThreads, 0, stream, p);
-  else launch_kernel(quant_long_rows_kernel, g, kQuantThreads, 0, stream, p);
+  const dim3 g((unsigned)rows), g4((unsigned)((rows + 3) / 4));
+  // rows enough to fill the SMs with a warp each take that form up to 2048 values
+  const bool many = rows >= 4096;
+  if (many && dim <= 512) launch_kernel(quant_rows_kernel<1, 1>, g4, 128, 0, stream, p);
+  else if (many && dim <= 1024) launch_kernel(quant_rows_kernel<1, 2>, g4, 128, 0, stream, p);
+  else if (many && dim <= 2048) launch_kernel(quant_rows_kernel<1, 4>, g4, 128, 0, stream, p);
+  else if (dim <= 2048) launch_kernel(quant_rows_kernel<4, 1>, g, 128, 0, stream, p);
+  else if (dim <= 4096) launch_kernel(quant_rows_kernel<4, 2>, g, 128, 0, stream, p);
+  else if (dim <= 8192) launch_kernel(quant_rows_kernel<8, 2>, g, 256, 0, stream, p);
+  else if (dim <= 16384) launch_kernel(quant_rows_kernel<8, 4>, g, 256, 0, stream, p);
+  else launch_kernel(quant_long_rows_kernel, g, kLongThreads, 0, stream, p);
   B200_CHECK_LAUNCH();
   return B200_OK;
 }
