@@ -348,6 +348,38 @@ B200_DEV void cp_async_wait() {
 }
 
 // ---------------------------------------------------------------------------
+// Thread-block clusters
+// ---------------------------------------------------------------------------
+B200_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+B200_DEV uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(n));
+  return n;
+}
+// Every thread of every CTA of the cluster; shared-memory writes before it are
+// visible to the whole cluster after it.
+B200_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of CTA `rank`'s copy of a shared-memory location.
+B200_DEV uint32_t cluster_map(uint32_t smem_addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+  return a;
+}
+B200_DEV int4 cluster_load4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+// ---------------------------------------------------------------------------
 // Programmatic dependent launch.  Every kernel of this library is launched
 // with programmatic stream serialisation: it may start while its predecessor
 // on the stream is still finishing, runs its prologue (and anything that only
@@ -364,6 +396,27 @@ B200_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" :
 // prefill, whose large grids gain nothing from early launch).
 bool pdl_enabled();
 void set_pdl(bool on);
+
+// launch_kernel in clusters of `cluster` CTAs along x (1: none).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_clusters(void (*kernel)(KArgs...), unsigned cluster, dim3 grid, dim3 block, size_t smem,
+                                   cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
 
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

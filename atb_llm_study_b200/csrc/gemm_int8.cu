@@ -15,6 +15,9 @@
 //
 // Nothing is loaded before the previous kernel on the stream has finished: the
 // weights can be that kernel's output (the row quantisation makes them).
+// TMEM is allocated after that wait and the next kernel released after the
+// allocation: two kernels of which one holds TMEM the other needs never wait
+// for one another.
 #include <math.h>
 
 #include <algorithm>
@@ -49,7 +52,7 @@ struct Cfg {
 struct Params {
   int64_t rows;  // MMA M extent
   int64_t cols;  // MMA N extent
-  int tiles_m, tiles_n, kb_total;
+  int tiles_m, tiles_n, kb_total, kb_per_split;
   const float* row_scale;  // of the MMA rows / columns (tokens or features by orientation)
   const float* col_scale;
   __nv_bfloat16* C;
@@ -74,8 +77,11 @@ struct Unit {
   int64_t rs0, cs0;         // scale index of row0 / col0
 };
 
+// 0.5 x (1 + tanh(u)) = x / (1 + e^-2u), u = sqrt(2/pi) (x + 0.044715 x^3): one
+// exponential and one division where tanhf costs several times that, and no
+// cancellation for negative x.
 __device__ __forceinline__ float gelu_tanh_f(float x) {
-  return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
+  return __fdividef(x, 1.f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
 }
 __device__ __forceinline__ float silu_f(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
@@ -231,7 +237,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int units = p.tiles_m * p.tiles_n;
-  pdl_trigger();
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -247,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
+  pdl_wait();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -254,8 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
-  pdl_wait();
   if (GROUPED) {
     if (threadIdx.x == 0) {
       int prev = 0, run = 0;
@@ -381,6 +387,220 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
+// Few tokens (M <= 128): one 128-feature tile per cluster, its K range split
+// over the cluster's CTAs.
+// ---------------------------------------------------------------------------
+template <int BN>
+struct SplitCfg {
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 100 * 1024 / STAGE_BYTES;  // two CTAs per SM
+  static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ + BN * 4 /*token scales*/;
+  static constexpr uint32_t IDESC = idesc_i8_s32(BM, BN);
+  static_assert(BN * BM * 4 <= STAGES * STAGE_BYTES, "the partial tile reuses the ring");
+};
+
+__device__ __forceinline__ void add4(float v[4], const __nv_bfloat16* src) {
+  const uint2 u = *reinterpret_cast<const uint2*>(src);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  v[0] += a.x, v[1] += a.y, v[2] += b.x, v[3] += b.y;
+}
+
+// Four consecutive features f0.. of token `tok`, values already scaled, through
+// the epilogue with their bias and residual.
+template <int EPI>
+__device__ __forceinline__ void emit4(float v[4], const float bias[4], const float res[4], int64_t f0, int64_t tok,
+                                      const Params& p) {
+  if (EPI == B200_EPI_SWIGLU) {
+    *reinterpret_cast<uint32_t*>(p.C + tok * p.ldc + f0 / 2) = pack2(silu_f(v[0]) * v[1], silu_f(v[2]) * v[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] += bias[i];
+    if (EPI == B200_EPI_BIAS_GELU) v[i] = gelu_tanh_f(v[i]);
+    v[i] += res[i];
+  }
+  *reinterpret_cast<uint2*>(p.C + tok * p.ldc + f0) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+}
+
+// Tokens t0, t0 + 6, ... < last of the lane's four features: the partial sums of
+// the cluster's S <= NS CTAs added up and finished.  U tokens x NS loads are in
+// flight at once.
+template <int EPI, int U, int NS>
+__device__ __forceinline__ void finish_tokens(uint32_t base, int S, int t0, int last, const float4& fs, const float fb[4],
+                                              const float* tscale, int64_t f0, const Params& p) {
+  constexpr int kWarps = kThreads / 32;
+  for (; t0 < last; t0 += U * kWarps) {
+    int4 a[U][NS];
+    float r[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kWarps;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        a[u][s] = t < last && s < S ? cluster_load4(cluster_map(base + t * (BM * 4), s)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[u][i] = 0.f;
+      if (has_residual(EPI) && t < last) add4(r[u], p.R + (int64_t)t * p.ldr + f0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kWarps;
+      if (t >= last) continue;
+      int4 sum = a[u][0];
+#pragma unroll
+      for (int s = 1; s < NS; ++s)
+        sum.x += a[u][s].x, sum.y += a[u][s].y, sum.z += a[u][s].z, sum.w += a[u][s].w;
+      const float ts = tscale[t];
+      float v[4] = {(float)sum.x * ts * fs.x, (float)sum.y * ts * fs.y, (float)sum.z * ts * fs.z, (float)sum.w * ts * fs.w};
+      emit4<EPI>(v, fb, r[u], f0, t, p);
+    }
+  }
+}
+
+template <int BN, int EPI>
+__global__ void __launch_bounds__(kThreads, 2)
+    gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const Params p) {
+  using C = SplitCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * C::A_BYTES;
+  int* part = reinterpret_cast<int*>(smem);  // [token][128 features], once the ring is drained
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  float* tscale = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + 256);  // of the tokens
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = (int)cluster_size(), rank = (int)cluster_rank();
+  const int row0 = (int)(blockIdx.x / S) * BM;
+  const int kb0 = rank * p.kb_per_split, nkb = min(p.kb_total - kb0, p.kb_per_split);
+  const int tokens = (int)p.cols;
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  __syncthreads();
+  pdl_wait();
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < nkb; ++i) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) break;
+        mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
+        tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], (kb0 + i) * BK, row0);
+        tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], (kb0 + i) * BK, 0);
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // TMEM is allocated while the first tiles are on their way
+    if (warp == 1) {
+      tmem_alloc(tmem_slot, C::TMEM_COLS);
+      tmem_relinquish();
+      pdl_trigger();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");  // warps 1-5
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < nkb; ++i) {
+          if (!mbar_wait(&full[stage], phase, p.err)) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * C::A_BYTES);
+          const uint32_t b0 = smem_u32(sB + stage * C::B_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_i8(tmem_base, smem_desc_k128(a0 + k * 32), smem_desc_k128(b0 + k * 32), C::IDESC,
+                    (i > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        umma_commit(tfull);
+      }
+      __syncwarp();
+    } else {
+      // ---------------- partial sums to shared memory (warps 2-5) ----------------
+      const int q = warp & 3;  // TMEM lane quarter this warp may access
+      const int rit = q * 32 + lane;
+      if (rit < tokens) tscale[rit] = p.col_scale[rit];
+      const bool ok = mbar_wait(tfull, 0, p.err);
+      tc_fence_after();
+      constexpr int CW = BN < 32 ? BN : 32;
+      for (int ch = 0; ch < BN / CW && ch * CW < tokens && ok; ++ch) {
+        uint32_t r[CW];
+        const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + ch * CW;
+        if constexpr (CW == 32) tmem_ld_32x32b_x32(t, r);
+        else tmem_ld_32x32b_x16(t, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+          if (ch * CW + i < tokens) part[(ch * CW + i) * BM + rit] = (int)r[i];
+      }
+      tc_fence_before();
+      __syncwarp();
+    }
+  }
+  // This CTA finishes its share of the tokens: the cluster's partial sums
+  // (integers: their order does not matter).  A lane keeps four features, a
+  // warp takes every sixth token, and what does not depend on the sums is
+  // loaded before they are there.
+  const int share = (tokens + S - 1) / S;
+  const int first = rank * share, last = min(tokens, first + share);
+  const int64_t f0 = row0 + lane * 4;
+  const bool live = f0 < p.rows;
+  float4 fs = make_float4(0.f, 0.f, 0.f, 0.f);
+  float fb[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    fs = *reinterpret_cast<const float4*>(p.row_scale + f0);
+    if (has_bias(EPI)) add4(fb, p.bias + f0);
+  }
+  if (S > 1) cluster_sync();
+  else __syncthreads();
+  if (live) {
+    const uint32_t base = smem_u32(part) + lane * 16;
+    if (S == 1) finish_tokens<EPI, 4, 1>(base, S, first + warp, last, fs, fb, tscale, f0, p);
+    else if (S <= 4) finish_tokens<EPI, 4, 4>(base, S, first + warp, last, fs, fb, tscale, f0, p);
+    else finish_tokens<EPI, 2, 8>(base, S, first + warp, last, fs, fb, tscale, f0, p);
+  }
+  __syncwarp();
+  if (S > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(*tmem_slot, C::TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -443,15 +663,43 @@ int launch_t(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int gr
   return B200_OK;
 }
 
-template <int BN, bool SWAP>
+template <int BN>
 int launch_epi(int epi, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t st) {
   switch (epi) {
-    case B200_EPI_NONE: return launch_t<BN, B200_EPI_NONE, SWAP, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS: return launch_t<BN, B200_EPI_BIAS, SWAP, false>(a, b, p, grid, st);
-    case B200_EPI_RESIDUAL: return launch_t<BN, B200_EPI_RESIDUAL, SWAP, false>(a, b, p, grid, st);
-    case B200_EPI_SWIGLU: return launch_t<BN, B200_EPI_SWIGLU, SWAP, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS_GELU: return launch_t<BN, B200_EPI_BIAS_GELU, SWAP, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS_RESIDUAL: return launch_t<BN, B200_EPI_BIAS_RESIDUAL, SWAP, false>(a, b, p, grid, st);
+    case B200_EPI_NONE: return launch_t<BN, B200_EPI_NONE, false, false>(a, b, p, grid, st);
+    case B200_EPI_BIAS: return launch_t<BN, B200_EPI_BIAS, false, false>(a, b, p, grid, st);
+    case B200_EPI_RESIDUAL: return launch_t<BN, B200_EPI_RESIDUAL, false, false>(a, b, p, grid, st);
+    case B200_EPI_SWIGLU: return launch_t<BN, B200_EPI_SWIGLU, false, false>(a, b, p, grid, st);
+    case B200_EPI_BIAS_GELU: return launch_t<BN, B200_EPI_BIAS_GELU, false, false>(a, b, p, grid, st);
+    case B200_EPI_BIAS_RESIDUAL: return launch_t<BN, B200_EPI_BIAS_RESIDUAL, false, false>(a, b, p, grid, st);
+  }
+  return B200_ERROR_INVALID_PARAM;
+}
+
+template <int BN, int EPI>
+int launch_split_t(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int splits, cudaStream_t st) {
+  auto k = gemm_i8_split_kernel<BN, EPI>;
+  static bool attr_set[64] = {false};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<BN>::SMEM) != cudaSuccess)
+      return B200_ERROR_UNSUPPORTED;
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  launch_clusters(k, splits, dim3(p.tiles_m * splits), kThreads, SplitCfg<BN>::SMEM, st, a, b, p);
+  B200_CHECK_LAUNCH();
+  return B200_OK;
+}
+
+template <int BN>
+int launch_split(int epi, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int splits, cudaStream_t st) {
+  switch (epi) {
+    case B200_EPI_NONE: return launch_split_t<BN, B200_EPI_NONE>(a, b, p, splits, st);
+    case B200_EPI_BIAS: return launch_split_t<BN, B200_EPI_BIAS>(a, b, p, splits, st);
+    case B200_EPI_RESIDUAL: return launch_split_t<BN, B200_EPI_RESIDUAL>(a, b, p, splits, st);
+    case B200_EPI_SWIGLU: return launch_split_t<BN, B200_EPI_SWIGLU>(a, b, p, splits, st);
+    case B200_EPI_BIAS_GELU: return launch_split_t<BN, B200_EPI_BIAS_GELU>(a, b, p, splits, st);
+    case B200_EPI_BIAS_RESIDUAL: return launch_split_t<BN, B200_EPI_BIAS_RESIDUAL>(a, b, p, splits, st);
   }
   return B200_ERROR_INVALID_PARAM;
 }
@@ -463,6 +711,19 @@ int launch_grouped(int epi, const CUtensorMap& a, const CUtensorMap& b, const Pa
 }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// CTAs of a cluster that share one 128-feature tile's K range: as many as keep
+// two k-blocks each and fit one wave of clusters (256 of the 296 places: a
+// cluster needs its places within one group of SMs, and 288 CTAs of 48 tiles
+// already take two waves, 13.7 us against 9.6 at 192).  Past 4 the exchange
+// costs more than a short K gains (4096 x 4096, one token: 6.2 us at 4, 6.9 at
+// 8) and less than a long one does (12288: 12.6 at 4, 11.5 at 8).
+int plan_splits(int tiles, int kb_total) {
+  const int most = kb_total >= 64 ? 8 : 4;
+  int s = 1;
+  while (s < most && tiles * (s + 1) <= 256 && kb_total / (s + 1) >= 2) ++s;
+  return s;
+}
 
 // The checks that the plain and the grouped call share.
 bool operands_ok(const void* A, int64_t lda, const void* as, const void* B, int64_t ldb, const void* bs, const void* C,
@@ -507,15 +768,18 @@ extern "C" int b200_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale
   if (!make_tmap(&ta, swap ? B : A, p.rows, K, swap ? ldb : lda, BM) ||
       !make_tmap(&tb, swap ? A : B, p.cols, K, swap ? lda : ldb, bn))
     return B200_ERROR_UNSUPPORTED;
-  const int grid = std::min(p.tiles_m * p.tiles_n, num_sms());
-  if (!swap) {
-    return bn == 256 ? launch_epi<256, false>(epilogue, ta, tb, p, grid, stream)
-                     : launch_epi<128, false>(epilogue, ta, tb, p, grid, stream);
+  if (swap) {
+    const int splits = plan_splits(p.tiles_m, p.kb_total);
+    p.kb_per_split = (p.kb_total + splits - 1) / splits;
+    const int used = (p.kb_total + p.kb_per_split - 1) / p.kb_per_split;
+    if (bn == 16) return launch_split<16>(epilogue, ta, tb, p, used, stream);
+    if (bn == 32) return launch_split<32>(epilogue, ta, tb, p, used, stream);
+    if (bn == 64) return launch_split<64>(epilogue, ta, tb, p, used, stream);
+    return launch_split<128>(epilogue, ta, tb, p, used, stream);
   }
-  if (bn == 16) return launch_epi<16, true>(epilogue, ta, tb, p, grid, stream);
-  if (bn == 32) return launch_epi<32, true>(epilogue, ta, tb, p, grid, stream);
-  if (bn == 64) return launch_epi<64, true>(epilogue, ta, tb, p, grid, stream);
-  return launch_epi<128, true>(epilogue, ta, tb, p, grid, stream);
+  const int grid = std::min(p.tiles_m * p.tiles_n, num_sms());
+  return bn == 256 ? launch_epi<256>(epilogue, ta, tb, p, grid, stream)
+                   : launch_epi<128>(epilogue, ta, tb, p, grid, stream);
 }
 
 extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
