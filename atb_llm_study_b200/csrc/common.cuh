@@ -258,6 +258,47 @@ B200_DEV void umma_commit(uint64_t* bar) {
                : "memory");
 }
 
+// ---- CTA pairs (cta_group::2: two CTAs of a cluster run one MMA, each holding half of both operands and the 128
+// accumulator rows of its half of A) ----
+
+// Both CTAs' warps take part in the allocation and the release.
+B200_DEV void tmem_alloc_pair(uint32_t* smem_slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_slot)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+B200_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+B200_DEV void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on this mbarrier in both CTAs when all previously issued MMAs complete.
+B200_DEV void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Load into this CTA's shared memory, counted on an mbarrier (cluster address) of either CTA of the pair.
+B200_DEV void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor: K-major tile whose rows are 128 bytes, stored
 // with the 128-byte swizzle (8-row atoms of 1024 bytes).
 B200_DEV uint64_t smem_desc_k128(uint32_t smem_addr) {
@@ -363,6 +404,7 @@ B200_DEV uint32_t cluster_size() {
 // Every thread of every CTA of the cluster; shared-memory writes before it are
 // visible to the whole cluster after it.
 B200_DEV void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Address of CTA `rank`'s copy of a shared-memory location.
@@ -370,6 +412,10 @@ B200_DEV uint32_t cluster_map(uint32_t smem_addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
   return a;
+}
+// Arrive on an mbarrier of any CTA of the cluster (cluster address).
+B200_DEV void cluster_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 B200_DEV int4 cluster_load4(uint32_t addr) {
   int4 v;

@@ -2,16 +2,14 @@
 //   C[m, n] = epi(a_scale[m] * b_scale[n] * sum_k A[m, k] B[n, k])
 // with int8 operands, exact 32-bit integer sums and one rounding to bf16.
 //
-// One persistent CTA per SM, 192 threads:
-//   warp 0      TMA producer: 128 x 128-byte tile of the row operand and
-//               BN x 128-byte tile of the column operand per stage, 128-byte
-//               swizzle, a ring of shared-memory stages.
-//   warp 1      allocates TMEM; one thread issues tcgen05.mma kind::i8
-//               (M = 128, N = BN, K = 32) into one of two TMEM accumulators.
-//   warps 2-5   epilogue: tcgen05.ld, scales, bias / residual / SwiGLU / GELU,
-//               bf16 stores.
-// Few token rows run "swapped": the weights feed the 128-row side, the tokens
-// the N side, and the epilogue writes the transpose.
+// Three kernels, each with a TMA producer warp, an MMA issuer thread and
+// epilogue warps around a ring of shared-memory stages (128-byte swizzle):
+//   gemm_i8_pair_kernel   many tokens: persistent CTA pairs, 256 x 256 tiles
+//                         (cta_group::2), two TMEM accumulators; also grouped.
+//   gemm_i8_split_kernel  few tokens: weights on the 128-row MMA side, tokens on
+//                         the N side, K split over a cluster.
+//   gemm_i8_group_kernel  few tokens per expert: weights on the 128-row side,
+//                         one persistent CTA per SM over all experts' tiles.
 //
 // Nothing is loaded before the previous kernel on the stream has finished: the
 // weights can be that kernel's output (the row quantisation makes them).
@@ -32,22 +30,10 @@ namespace {
 constexpr int BM = 128;
 constexpr int BK = 128;  // bytes of K per stage: the swizzle span
 constexpr int kThreads = 192;
-constexpr int kGroupM = 16;
 constexpr int kMaxGroups = 256;                           // experts of one grouped GEMM
 constexpr int kGroupTabBytes = 2 * (kMaxGroups + 2) * 4;  // row offsets + unit prefix in shared memory
 // The largest |sum| is 128 * 128 * K (both operands may hold -128): it fits 31 bits up to here.
 constexpr int64_t kMaxK = 131056;
-
-template <int BN>
-struct Cfg {
-  static constexpr int A_BYTES = BM * BK;
-  static constexpr int B_BYTES = BN * BK;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 200 * 1024 / STAGE_BYTES;
-  static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/ + kGroupTabBytes;
-  static constexpr uint32_t IDESC = idesc_i8_s32(BM, BN);
-};
 
 struct Params {
   int64_t rows;  // MMA M extent
@@ -71,10 +57,9 @@ struct Params {
 };
 
 struct Unit {
-  int a_row, b_row;         // TMA rows of both operands
-  int64_t row0, col0;       // output origin (token / feature by orientation)
-  int64_t row_lim, col_lim;
-  int64_t rs0, cs0;         // scale index of row0 / col0
+  int tok0, wrow0;  // TMA rows of the token and the weight operand
+  int feat0;        // first output column
+  int tok_lim, feat_lim;
 };
 
 // 0.5 x (1 + tanh(u)) = x / (1 + e^-2u), u = sqrt(2/pi) (x + 0.044715 x^3): one
@@ -90,23 +75,19 @@ constexpr bool has_bias(int e) {
 }
 constexpr bool has_residual(int e) { return e == B200_EPI_RESIDUAL || e == B200_EPI_BIAS_RESIDUAL; }
 
-template <int BN, bool SWAP, bool GROUPED>
-__device__ __forceinline__ Unit get_unit(int w, const Params& p, const int* gtab) {
-  Unit u;
-  if (!GROUPED) {
-    const int group = kGroupM * p.tiles_n;
-    const int first_m = w / group * kGroupM;
-    const int gm = min(p.tiles_m - first_m, kGroupM);
-    const int r = w % group;
-    const int tm = first_m + r % gm, tn = r / gm;
-    u.a_row = tm * BM;
-    u.b_row = tn * BN;
-    u.row0 = u.rs0 = u.a_row;
-    u.col0 = u.cs0 = u.b_row;
-    u.row_lim = p.rows;
-    u.col_lim = p.cols;
-    return u;
-  }
+__device__ __forceinline__ void add4(float v[4], const __nv_bfloat16* src) {
+  const uint2 u = *reinterpret_cast<const uint2*>(src);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  v[0] += a.x, v[1] += a.y, v[2] += b.x, v[3] += b.y;
+}
+
+// Unit w of a grouped launch over tiles of TOKT tokens x FEATT features.
+// gtab[0..G] holds the groups' token row offsets and gtab[G+1..2G+1] the prefix
+// of their unit counts; within a group the token tiles of one feature tile are
+// consecutive (they share that weight tile).
+template <int TOKT, int FEATT>
+__device__ __forceinline__ Unit group_unit(int w, const Params& p, const int* gtab) {
   const int* up = gtab + p.groups + 1;
   int lo = 0, hi = p.groups;
   while (hi - lo > 1) {
@@ -114,115 +95,327 @@ __device__ __forceinline__ Unit get_unit(int w, const Params& p, const int* gtab
     if (up[mid] <= w) lo = mid;
     else hi = mid;
   }
-  const int g = lo;
-  constexpr int TOKT = SWAP ? BN : BM, FEATT = SWAP ? BM : BN;
-  const int t0 = gtab[g], t1 = gtab[g + 1];
+  const int t0 = gtab[lo], t1 = gtab[lo + 1];
   const int tt = (t1 - t0 + TOKT - 1) / TOKT;
-  const int r = w - up[g];
-  const int tok = t0 + r % tt * TOKT, feat = r / tt * FEATT;
-  const int wrow = (int)(g * p.gN) + feat;
-  if (SWAP) {
-    u.a_row = wrow;
-    u.b_row = tok;
-    u.row0 = feat;
-    u.rs0 = wrow;
-    u.row_lim = p.gN;
-    u.col0 = u.cs0 = tok;
-    u.col_lim = t1;
-  } else {
-    u.a_row = tok;
-    u.b_row = wrow;
-    u.row0 = u.rs0 = tok;
-    u.row_lim = t1;
-    u.col0 = feat;
-    u.cs0 = wrow;
-    u.col_lim = p.gN;
-  }
+  const int r = w - up[lo];
+  Unit u;
+  u.tok0 = t0 + r % tt * TOKT;
+  u.feat0 = r / tt * FEATT;
+  u.wrow0 = (int)(lo * p.gN) + u.feat0;
+  u.tok_lim = t1;
+  u.feat_lim = (int)p.gN;
   return u;
 }
 
-// Store CW accumulator columns of one MMA row with the epilogue.  Normal
-// orientation: the row is a token, the columns are features (vector stores).
-// Swapped: the row is a feature (consecutive features in consecutive lanes),
-// the columns are tokens.
-template <int EPI, bool SWAP, int CW>
-__device__ __forceinline__ void emit_chunk(const uint32_t acc[CW], int64_t row, int64_t col0, float rscale,
-                                           const float* cscale, const Unit& u, int lane, const Params& p) {
-  float v[CW];
+// One thread fills gtab from the device offsets; offsets that fall or leave
+// [0, rows] are clamped and reported.
+template <int TOKT>
+__device__ __forceinline__ void fill_group_table(int* gtab, const Params& p) {
+  int prev = 0, run = 0;
+  for (int g = 0; g <= p.groups; ++g) {
+    int v = p.goff[g];
+    if (v < prev || v > p.gRows || (g == 0 && v != 0)) {
+      raise_error(p.err, DEV_ERR_BAD_INDEX);
+      v = min(max(v, prev), (int)p.gRows);
+      if (g == 0) v = 0;
+    }
+    if (g > 0) run += ((v - prev + TOKT - 1) / TOKT) * p.gF;
+    gtab[g] = prev = v;
+    gtab[p.groups + 1 + g] = run;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many tokens: persistent CTA pairs.  CTA r of a pair loads 128 token rows and
+// 128 weight rows of each k-block; the leader (rank 0) issues M = 256, N = 256
+// MMAs that read both halves, and each CTA's epilogue drains its 128 token rows
+// from its own TMEM.  Against single CTAs with 128 x 256 tiles a pair moves a
+// third less through L2 and shared memory per product.
+// ---------------------------------------------------------------------------
+constexpr int kPairTile = 256;
+constexpr int kPairGroup = 8;  // token tiles walked per feature tile
+constexpr int kPairStages = 6;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
+constexpr int kPairStageBytes = 2 * BM * BK;  // of each CTA
+constexpr int kPairColBytes = kPairEpiWarps * 128 * 2 * 4;  // column scales and biases of each epilogue warp
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kPairColBytes + kGroupTabBytes;
+constexpr uint32_t kPairIdesc = idesc_i8_s32(256, kPairTile);
+
+// 32 accumulator columns of one token row through the epilogue; scale and bias
+// of the columns come from shared memory.
+template <int EPI>
+__device__ __forceinline__ void emit_row(const uint32_t acc[32], int64_t tok, int feat0, float rscale, const float* cscale,
+                                         const float* cbias, const Unit& u, const Params& p) {
 #pragma unroll
-  for (int i = 0; i < CW; ++i) v[i] = (float)(int)acc[i] * rscale;
-  if (!SWAP) {
-    if (row >= u.row_lim) return;
+  for (int g = 0; g < 4; ++g) {
+    const int c = feat0 + g * 8;
+    if (c >= u.feat_lim) continue;
+    float x[8];
 #pragma unroll
-    for (int g = 0; g < CW / 8; ++g) {
-      const int64_t c = col0 + g * 8;
-      if (c >= u.col_lim) continue;
-      float* x = v + 8 * g;
-      const float4 s0 = *reinterpret_cast<const float4*>(cscale + g * 8);
-      const float4 s1 = *reinterpret_cast<const float4*>(cscale + g * 8 + 4);
-      x[0] *= s0.x, x[1] *= s0.y, x[2] *= s0.z, x[3] *= s0.w;
-      x[4] *= s1.x, x[5] *= s1.y, x[6] *= s1.z, x[7] *= s1.w;
+    for (int h = 0; h < 2; ++h) {
+      const float4 s = *reinterpret_cast<const float4*>(cscale + g * 8 + h * 4);
+      x[4 * h] = (float)(int)acc[8 * g + 4 * h] * rscale * s.x;
+      x[4 * h + 1] = (float)(int)acc[8 * g + 4 * h + 1] * rscale * s.y;
+      x[4 * h + 2] = (float)(int)acc[8 * g + 4 * h + 2] * rscale * s.z;
+      x[4 * h + 3] = (float)(int)acc[8 * g + 4 * h + 3] * rscale * s.w;
       if (has_bias(EPI)) {
-        float b[8];
-        unpack8(*reinterpret_cast<const uint4*>(p.bias + c), b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += b[i];
-      }
-      if (EPI == B200_EPI_BIAS_GELU) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = gelu_tanh_f(x[i]);
-      }
-      if (has_residual(EPI)) {
-        float r[8];
-        unpack8(*reinterpret_cast<const uint4*>(p.R + row * p.ldr + c), r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += r[i];
-      }
-      if (EPI == B200_EPI_SWIGLU) {
-        uint2 o;
-        o.x = pack2(silu_f(x[0]) * x[1], silu_f(x[2]) * x[3]);
-        o.y = pack2(silu_f(x[4]) * x[5], silu_f(x[6]) * x[7]);
-        *reinterpret_cast<uint2*>(p.C + row * p.ldc + c / 2) = o;
-      } else {
-        *reinterpret_cast<uint4*>(p.C + row * p.ldc + c) = pack8(x);
+        const float4 b = *reinterpret_cast<const float4*>(cbias + g * 8 + h * 4);
+        x[4 * h] += b.x, x[4 * h + 1] += b.y, x[4 * h + 2] += b.z, x[4 * h + 3] += b.w;
       }
     }
-    return;
-  }
+    if (EPI == B200_EPI_BIAS_GELU) {
 #pragma unroll
-  for (int i = 0; i < CW; ++i) v[i] *= col0 + i < u.col_lim ? cscale[i] : 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = gelu_tanh_f(x[i]);
+    }
+    if (has_residual(EPI)) {
+      float r[8];
+      unpack8(*reinterpret_cast<const uint4*>(p.R + tok * p.ldr + c), r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += r[i];
+    }
+    if (EPI == B200_EPI_SWIGLU) {
+      uint2 o;
+      o.x = pack2(silu_f(x[0]) * x[1], silu_f(x[2]) * x[3]);
+      o.y = pack2(silu_f(x[4]) * x[5], silu_f(x[6]) * x[7]);
+      *reinterpret_cast<uint2*>(p.C + tok * p.ldc + c / 2) = o;
+    } else {
+      *reinterpret_cast<uint4*>(p.C + tok * p.ldc + c) = pack8(x);
+    }
+  }
+}
+
+template <int EPI, bool GROUPED>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kPairStages * BM * BK;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStageBytes);  // the leader's are used
+  uint64_t* empty = full + kPairStages;
+  uint64_t* tfull = empty + kPairStages;
+  uint64_t* tempty = tfull + 2;  // the leader's are used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* cols = reinterpret_cast<float*>(smem + kPairStages * kPairStageBytes + 256);
+  int* gtab = reinterpret_cast<int*>(smem + kPairStages * kPairStageBytes + 256 + kPairColBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  int units = p.tiles_m * p.tiles_n;
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kPairEpiWarps);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  pdl_wait();
+  if (GROUPED && warp == 0 && lane == 0) fill_group_table<kPairTile>(gtab, p);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 2 * kPairTile);
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers are ready, and both have their TMEM
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem_base = *tmem_slot;
+  if (GROUPED) units = gtab[2 * p.groups + 1];
+
+  auto unit_at = [&](int w) {
+    if (GROUPED) return group_unit<kPairTile, kPairTile>(w, p, gtab);
+    const int span = kPairGroup * p.tiles_n;
+    const int first = w / span * kPairGroup;
+    const int gm = min(p.tiles_m - first, kPairGroup);
+    const int r = w % span;
+    Unit u;
+    u.tok0 = (first + r % gm) * kPairTile;
+    u.feat0 = u.wrow0 = r / gm * kPairTile;
+    u.tok_lim = (int)p.rows;
+    u.feat_lim = (int)p.cols;
+    return u;
+  };
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int w = pair; w < units && !*abort_flag; w += pairs) {
+        const Unit u = unit_at(w);
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
+            *abort_flag = 1;
+            break;
+          }
+          // the leader expects both CTAs' bytes; the other's may land first
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kPairStageBytes);
+          const uint32_t bar = cluster_map(smem_u32(&full[stage]), 0);
+          tma_load_2d_pair(sA + stage * BM * BK, &tmA, bar, kb * BK, u.tok0 + rank * BM);
+          tma_load_2d_pair(sB + stage * BM * BK, &tmB, bar, kb * BK, u.wrow0 + rank * BM);
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader) ----------------
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      for (int w = pair; w < units && !*abort_flag; w += pairs, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        bool ok = true;
+        for (int kb = 0; kb < p.kb_total; ++kb) {
+          if (!mbar_wait(&full[stage], phase, p.err)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + stage * BM * BK);
+          const uint32_t b0 = smem_u32(sB + stage * BM * BK);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_i8_pair(tmem_base + acc * kPairTile, smem_desc_k128(a0 + k * 32), smem_desc_k128(b0 + k * 32),
+                         kPairIdesc, (kb > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[stage]);
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        umma_commit_pair(&tfull[acc]);
+        if (!ok) {
+          *abort_flag = 1;
+          break;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue: 32 token rows x 128 columns a warp ----------------
+    const int q = warp & 3;  // TMEM lane quarter this warp may access
+    const int half = (warp - 2) >> 2;
+    float* cscale = cols + (warp - 2) * 256;
+    float* cbias = cscale + 128;
+    int local = 0;
+    for (int w = pair; w < units && !*abort_flag; w += pairs, ++local) {
+      const Unit u = unit_at(w);
+      const int acc = local & 1;
+      const int64_t tok = u.tok0 + rank * BM + q * 32 + lane;
+      const bool live = tok < u.tok_lim;
+      const float rscale = live ? p.row_scale[tok] : 0.f;
+      const int c4 = half * 128 + lane * 4;
+      __syncwarp();
+      if (u.feat0 + c4 < u.feat_lim) {
+        *reinterpret_cast<float4*>(cscale + lane * 4) = *reinterpret_cast<const float4*>(p.col_scale + u.wrow0 + c4);
+        if (has_bias(EPI)) {
+          float b[4] = {0.f, 0.f, 0.f, 0.f};
+          add4(b, p.bias + u.feat0 + c4);
+          *reinterpret_cast<float4*>(cbias + lane * 4) = make_float4(b[0], b[1], b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (!mbar_wait(&tfull[acc], (local >> 1) & 1, p.err)) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kPairTile + half * 128;
+      uint32_t r[2][32];
+      tmem_ld_32x32b_x32(t, r[0]);
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {
+        tmem_ld_wait();
+        if (ch < 3) {
+          tmem_ld_32x32b_x32(t + (ch + 1) * 32, r[(ch + 1) & 1]);
+        } else {
+          // all read: the accumulator is free for the tile after next
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) cluster_arrive(cluster_map(smem_u32(&tempty[acc]), 0));
+        }
+        if (live)
+          emit_row<EPI>(r[ch & 1], tok, u.feat0 + half * 128 + ch * 32, rscale, cscale + ch * 32, cbias + ch * 32, u, p);
+        __syncwarp();
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync();  // neither CTA leaves while the other may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kPairTile);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens per expert: one persistent CTA per SM walks the (expert, feature
+// tile, token tile) units; the ring runs on across units and the accumulator
+// is double-buffered.
+// ---------------------------------------------------------------------------
+template <int BN>
+struct GroupCfg {
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 200 * 1024 / STAGE_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/ + kGroupTabBytes;
+  static constexpr uint32_t IDESC = idesc_i8_s32(BM, BN);
+};
+
+// 32 accumulator columns (tokens) of one feature row.
+template <int EPI>
+__device__ __forceinline__ void emit_feature(const uint32_t acc[32], int row, int tok0, float rscale, const Unit& u, int lane,
+                                             const Params& p) {
+  const int feat = u.feat0 + row;
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = (float)(int)acc[i] * rscale * (tok0 + i < u.tok_lim ? p.col_scale[tok0 + i] : 0.f);
   if (EPI == B200_EPI_SWIGLU) {
     // lanes 2j / 2j+1 hold the gate / up rows of feature j: the even lane
     // finishes the first half of the chunk's tokens, the odd lane the second
     const bool odd = lane & 1;
-    const int64_t f = row >> 1;
-    constexpr int H = CW / 2;
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[H + i], 1);
-      const int64_t tok = col0 + (odd ? H + i : i);
-      const float o = odd ? silu_f(other) * v[H + i] : silu_f(v[i]) * other;
-      if (row < u.row_lim && tok < u.col_lim) p.C[tok * p.ldc + f] = f2bf(o);
+    for (int i = 0; i < 16; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[16 + i], 1);
+      const int64_t tok = tok0 + (odd ? 16 + i : i);
+      const float o = odd ? silu_f(other) * v[16 + i] : silu_f(v[i]) * other;
+      if (feat < u.feat_lim && tok < u.tok_lim) p.C[tok * p.ldc + (feat >> 1)] = f2bf(o);
     }
-    return;
-  }
-  if (row >= u.row_lim) return;
-  const float b = has_bias(EPI) ? bf2f(p.bias[row]) : 0.f;
+  } else if (feat < u.feat_lim) {
 #pragma unroll
-  for (int i = 0; i < CW; ++i) {
-    const int64_t tok = col0 + i;
-    if (tok >= u.col_lim) continue;
-    float x = v[i] + b;
-    if (EPI == B200_EPI_BIAS_GELU) x = gelu_tanh_f(x);
-    if (has_residual(EPI)) x += bf2f(p.R[tok * p.ldr + row]);
-    p.C[tok * p.ldc + row] = f2bf(x);
+    for (int i = 0; i < 32; ++i) {
+      const int64_t tok = tok0 + i;
+      if (tok < u.tok_lim) p.C[tok * p.ldc + feat] = f2bf(v[i]);
+    }
   }
 }
 
-template <int BN, int EPI, bool SWAP, bool GROUPED>
+template <int BN, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
-  using C = Cfg<BN>;
+    gemm_i8_group_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+  using C = GroupCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -233,10 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* gtab = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE_BYTES + 512);  // grouped launches only
+  int* gtab = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE_BYTES + 512);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int units = p.tiles_m * p.tiles_n;
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -253,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmB);
   }
   pdl_wait();
+  if (warp == 0 && lane == 0) fill_group_table<BN>(gtab, p);
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -262,28 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
-  if (GROUPED) {
-    if (threadIdx.x == 0) {
-      int prev = 0, run = 0;
-      for (int g = 0; g <= p.groups; ++g) {
-        int v = p.goff[g];
-        if (v < prev || v > p.gRows || (g == 0 && v != 0)) {
-          raise_error(p.err, DEV_ERR_BAD_INDEX);
-          v = min(max(v, prev), (int)p.gRows);
-          if (g == 0) v = 0;
-        }
-        gtab[g] = prev = v;
-      }
-      constexpr int TOKT = SWAP ? BN : BM;
-      for (int g = 0; g < p.groups; ++g) {
-        gtab[p.groups + 1 + g] = run;
-        run += ((gtab[g + 1] - gtab[g] + TOKT - 1) / TOKT) * p.gF;
-      }
-      gtab[2 * p.groups + 1] = run;
-    }
-    __syncthreads();
-    units = gtab[2 * p.groups + 1];
-  }
+  const int units = gtab[2 * p.groups + 1];
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -291,15 +463,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       for (int w = blockIdx.x; w < units && !*abort_flag; w += gridDim.x) {
-        const Unit u = get_unit<BN, SWAP, GROUPED>(w, p, gtab);
+        const Unit u = group_unit<BN, BM>(w, p, gtab);
         for (int kb = 0; kb < p.kb_total; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
             *abort_flag = 1;
             break;
           }
           mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
-          tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], kb * BK, u.a_row);
-          tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], kb * BK, u.b_row);
+          tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], kb * BK, u.wrow0);
+          tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], kb * BK, u.tok0);
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1;
@@ -352,26 +524,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- epilogue (warps 2..5) ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
     const int rit = q * 32 + lane;
-    constexpr int CW = BN < 32 ? BN : 32;
     int local = 0;
     for (int w = blockIdx.x; w < units && !*abort_flag; w += gridDim.x, ++local) {
-      const Unit u = get_unit<BN, SWAP, GROUPED>(w, p, gtab);
+      const Unit u = group_unit<BN, BM>(w, p, gtab);
       const int acc = local & 1;
-      const int64_t row = u.row0 + rit;
-      const float rscale = row < u.row_lim ? p.row_scale[u.rs0 + rit] : 0.f;
+      const float rscale = u.feat0 + rit < u.feat_lim ? p.row_scale[u.wrow0 + rit] : 0.f;
       if (!mbar_wait(&tfull[acc], (local >> 1) & 1, p.err)) {
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int ch = 0; ch < BN / CW; ++ch) {
-        uint32_t r[CW];
-        const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + ch * CW;
-        if constexpr (CW == 32) tmem_ld_32x32b_x32(t, r);
-        else tmem_ld_32x32b_x16(t, r);
+      for (int ch = 0; ch < BN / 32 && u.tok0 + ch * 32 < u.tok_lim; ++ch) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + ch * 32, r);
         tmem_ld_wait();
-        emit_chunk<EPI, SWAP, CW>(r, row, u.col0 + ch * CW, rscale, p.col_scale + u.cs0 + ch * CW, u, lane, p);
+        emit_feature<EPI>(r, rit, u.tok0 + ch * 32, rscale, u, lane, p);
       }
       tc_fence_before();
       mbar_arrive(&tempty[acc]);
@@ -387,8 +555,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens (M <= 128): one 128-feature tile per cluster, its K range split
-// over the cluster's CTAs.
+// Few tokens: one tile of 128 features x BN tokens per cluster, its K range
+// split over the cluster's CTAs; two CTAs per SM, so that one's epilogue runs
+// under another's loads.
 // ---------------------------------------------------------------------------
 template <int BN>
 struct SplitCfg {
@@ -401,13 +570,6 @@ struct SplitCfg {
   static constexpr uint32_t IDESC = idesc_i8_s32(BM, BN);
   static_assert(BN * BM * 4 <= STAGES * STAGE_BYTES, "the partial tile reuses the ring");
 };
-
-__device__ __forceinline__ void add4(float v[4], const __nv_bfloat16* src) {
-  const uint2 u = *reinterpret_cast<const uint2*>(src);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-  v[0] += a.x, v[1] += a.y, v[2] += b.x, v[3] += b.y;
-}
 
 // Four consecutive features f0.. of token `tok`, values already scaled, through
 // the epilogue with their bias and residual.
@@ -427,12 +589,12 @@ __device__ __forceinline__ void emit4(float v[4], const float bias[4], const flo
   *reinterpret_cast<uint2*>(p.C + tok * p.ldc + f0) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
 }
 
-// Tokens t0, t0 + 6, ... < last of the lane's four features: the partial sums of
+// Tokens t0, t0 + 6, ... < last (of the tile that begins at tok0) of the lane's four features: the partial sums of
 // the cluster's S <= NS CTAs added up and finished.  U tokens x NS loads are in
 // flight at once.
 template <int EPI, int U, int NS>
-__device__ __forceinline__ void finish_tokens(uint32_t base, int S, int t0, int last, const float4& fs, const float fb[4],
-                                              const float* tscale, int64_t f0, const Params& p) {
+__device__ __forceinline__ void finish_tokens(uint32_t base, int S, int t0, int last, int64_t tok0, const float4& fs,
+                                              const float fb[4], const float* tscale, int64_t f0, const Params& p) {
   constexpr int kWarps = kThreads / 32;
   for (; t0 < last; t0 += U * kWarps) {
     int4 a[U][NS];
@@ -445,7 +607,7 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int S, int t0, int 
         a[u][s] = t < last && s < S ? cluster_load4(cluster_map(base + t * (BM * 4), s)) : make_int4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[u][i] = 0.f;
-      if (has_residual(EPI) && t < last) add4(r[u], p.R + (int64_t)t * p.ldr + f0);
+      if (has_residual(EPI) && t < last) add4(r[u], p.R + (tok0 + t) * p.ldr + f0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -457,7 +619,7 @@ __device__ __forceinline__ void finish_tokens(uint32_t base, int S, int t0, int 
         sum.x += a[u][s].x, sum.y += a[u][s].y, sum.z += a[u][s].z, sum.w += a[u][s].w;
       const float ts = tscale[t];
       float v[4] = {(float)sum.x * ts * fs.x, (float)sum.y * ts * fs.y, (float)sum.z * ts * fs.z, (float)sum.w * ts * fs.w};
-      emit4<EPI>(v, fb, r[u], f0, t, p);
+      emit4<EPI>(v, fb, r[u], f0, tok0 + t, p);
     }
   }
 }
@@ -480,9 +642,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = (int)cluster_size(), rank = (int)cluster_rank();
-  const int row0 = (int)(blockIdx.x / S) * BM;
+  const int tile = (int)(blockIdx.x / S);
+  const int row0 = tile % p.tiles_m * BM;
+  const int tok0 = tile / p.tiles_m * BN;
   const int kb0 = rank * p.kb_per_split, nkb = min(p.kb_total - kb0, p.kb_per_split);
-  const int tokens = (int)p.cols;
+  const int tokens = min((int)p.cols - tok0, BN);
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -506,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) break;
         mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
         tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], (kb0 + i) * BK, row0);
-        tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], (kb0 + i) * BK, 0);
+        tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], (kb0 + i) * BK, tok0);
         if (++stage == C::STAGES) {
           stage = 0;
           phase ^= 1;
@@ -552,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // ---------------- partial sums to shared memory (warps 2-5) ----------------
       const int q = warp & 3;  // TMEM lane quarter this warp may access
       const int rit = q * 32 + lane;
-      if (rit < tokens) tscale[rit] = p.col_scale[rit];
+      if (rit < tokens) tscale[rit] = p.col_scale[tok0 + rit];
       const bool ok = mbar_wait(tfull, 0, p.err);
       tc_fence_after();
       constexpr int CW = BN < 32 ? BN : 32;
@@ -588,11 +752,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   else __syncthreads();
   if (live) {
     const uint32_t base = smem_u32(part) + lane * 16;
-    if (S == 1) finish_tokens<EPI, 4, 1>(base, S, first + warp, last, fs, fb, tscale, f0, p);
-    else if (S <= 4) finish_tokens<EPI, 4, 4>(base, S, first + warp, last, fs, fb, tscale, f0, p);
-    else finish_tokens<EPI, 2, 8>(base, S, first + warp, last, fs, fb, tscale, f0, p);
+    if (S == 1) finish_tokens<EPI, 4, 1>(base, S, first + warp, last, tok0, fs, fb, tscale, f0, p);
+    else if (S <= 4) finish_tokens<EPI, 4, 4>(base, S, first + warp, last, tok0, fs, fb, tscale, f0, p);
+    else finish_tokens<EPI, 2, 8>(base, S, first + warp, last, tok0, fs, fb, tscale, f0, p);
   }
-  __syncwarp();
   if (S > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
   if (warp == 1) {
     tc_fence_after();
@@ -648,66 +811,56 @@ int num_sms() {
   return n[dev] > 0 ? n[dev] : 148;
 }
 
-template <int BN, int EPI, bool SWAP, bool GROUPED>
-int launch_t(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t st) {
-  auto k = gemm_i8_kernel<BN, EPI, SWAP, GROUPED>;
-  static bool attr_set[64] = {false};
+template <typename Kernel>
+bool allow_smem(Kernel k, int bytes, bool (&done)[64]) {
   const int dev = current_device();
-  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::SMEM) != cudaSuccess)
-      return B200_ERROR_UNSUPPORTED;
-    if (dev >= 0 && dev < 64) attr_set[dev] = true;
-  }
-  launch_kernel(k, dim3(grid), kThreads, Cfg<BN>::SMEM, st, a, b, p);
-  B200_CHECK_LAUNCH();
-  return B200_OK;
+  if (dev >= 0 && dev < 64 && done[dev]) return true;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return true;
 }
 
-template <int BN>
-int launch_epi(int epi, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t st) {
-  switch (epi) {
-    case B200_EPI_NONE: return launch_t<BN, B200_EPI_NONE, false, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS: return launch_t<BN, B200_EPI_BIAS, false, false>(a, b, p, grid, st);
-    case B200_EPI_RESIDUAL: return launch_t<BN, B200_EPI_RESIDUAL, false, false>(a, b, p, grid, st);
-    case B200_EPI_SWIGLU: return launch_t<BN, B200_EPI_SWIGLU, false, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS_GELU: return launch_t<BN, B200_EPI_BIAS_GELU, false, false>(a, b, p, grid, st);
-    case B200_EPI_BIAS_RESIDUAL: return launch_t<BN, B200_EPI_BIAS_RESIDUAL, false, false>(a, b, p, grid, st);
-  }
-  return B200_ERROR_INVALID_PARAM;
+template <int EPI, bool GROUPED>
+int launch_pair(const CUtensorMap& tok, const CUtensorMap& w, const Params& p, int64_t units, cudaStream_t st) {
+  auto k = gemm_i8_pair_kernel<EPI, GROUPED>;
+  static bool done[64] = {false};
+  if (!allow_smem(k, kPairSmem, done)) return B200_ERROR_UNSUPPORTED;
+  const int pairs = (int)std::min<int64_t>(units, num_sms() / 2);
+  launch_clusters(k, 2, dim3(2 * pairs), kPairThreads, kPairSmem, st, tok, w, p);
+  B200_CHECK_LAUNCH();
+  return B200_OK;
 }
 
 template <int BN, int EPI>
-int launch_split_t(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int splits, cudaStream_t st) {
+int launch_split(const CUtensorMap& tok, const CUtensorMap& w, const Params& p, int splits, cudaStream_t st) {
   auto k = gemm_i8_split_kernel<BN, EPI>;
-  static bool attr_set[64] = {false};
-  const int dev = current_device();
-  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SplitCfg<BN>::SMEM) != cudaSuccess)
-      return B200_ERROR_UNSUPPORTED;
-    if (dev >= 0 && dev < 64) attr_set[dev] = true;
-  }
-  launch_clusters(k, splits, dim3(p.tiles_m * splits), kThreads, SplitCfg<BN>::SMEM, st, a, b, p);
+  static bool done[64] = {false};
+  if (!allow_smem(k, SplitCfg<BN>::SMEM, done)) return B200_ERROR_UNSUPPORTED;
+  launch_clusters(k, splits, dim3(p.tiles_m * p.tiles_n * splits), kThreads, SplitCfg<BN>::SMEM, st, w, tok, p);
   B200_CHECK_LAUNCH();
   return B200_OK;
 }
 
-template <int BN>
-int launch_split(int epi, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int splits, cudaStream_t st) {
-  switch (epi) {
-    case B200_EPI_NONE: return launch_split_t<BN, B200_EPI_NONE>(a, b, p, splits, st);
-    case B200_EPI_BIAS: return launch_split_t<BN, B200_EPI_BIAS>(a, b, p, splits, st);
-    case B200_EPI_RESIDUAL: return launch_split_t<BN, B200_EPI_RESIDUAL>(a, b, p, splits, st);
-    case B200_EPI_SWIGLU: return launch_split_t<BN, B200_EPI_SWIGLU>(a, b, p, splits, st);
-    case B200_EPI_BIAS_GELU: return launch_split_t<BN, B200_EPI_BIAS_GELU>(a, b, p, splits, st);
-    case B200_EPI_BIAS_RESIDUAL: return launch_split_t<BN, B200_EPI_BIAS_RESIDUAL>(a, b, p, splits, st);
-  }
-  return B200_ERROR_INVALID_PARAM;
+template <int BN, int EPI>
+int launch_group(const CUtensorMap& tok, const CUtensorMap& w, const Params& p, int64_t units, cudaStream_t st) {
+  auto k = gemm_i8_group_kernel<BN, EPI>;
+  static bool done[64] = {false};
+  if (!allow_smem(k, GroupCfg<BN>::SMEM, done)) return B200_ERROR_UNSUPPORTED;
+  launch_kernel(k, dim3((unsigned)std::min<int64_t>(units, num_sms())), kThreads, GroupCfg<BN>::SMEM, st, w, tok, p);
+  B200_CHECK_LAUNCH();
+  return B200_OK;
 }
 
-template <int BN, bool SWAP>
-int launch_grouped(int epi, const CUtensorMap& a, const CUtensorMap& b, const Params& p, int grid, cudaStream_t st) {
-  return epi == B200_EPI_SWIGLU ? launch_t<BN, B200_EPI_SWIGLU, SWAP, true>(a, b, p, grid, st)
-                                : launch_t<BN, B200_EPI_NONE, SWAP, true>(a, b, p, grid, st);
+// bn: the token tile of the split form, 0 for CTA pairs.
+template <int EPI>
+int launch_plain(int bn, int splits, const CUtensorMap& tok, const CUtensorMap& w, const Params& p, cudaStream_t st) {
+  switch (bn) {
+    case 16: return launch_split<16, EPI>(tok, w, p, splits, st);
+    case 32: return launch_split<32, EPI>(tok, w, p, splits, st);
+    case 64: return launch_split<64, EPI>(tok, w, p, splits, st);
+    case 128: return launch_split<128, EPI>(tok, w, p, splits, st);
+    default: return launch_pair<EPI, false>(tok, w, p, (int64_t)p.tiles_m * p.tiles_n, st);
+  }
 }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -723,6 +876,11 @@ int plan_splits(int tiles, int kb_total) {
   int s = 1;
   while (s < most && tiles * (s + 1) <= 256 && kb_total / (s + 1) >= 2) ++s;
   return s;
+}
+
+// CTA pairs once their 256 x 256 tiles fill the SMs; a narrow N would waste the tile.
+bool use_pairs(int64_t M, int64_t N, int sms) {
+  return M > 128 && N > 128 && ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile) * 2 >= sms;
 }
 
 // The checks that the plain and the grouped call share.
@@ -747,39 +905,49 @@ extern "C" int b200_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale
     return B200_ERROR_INVALID_PARAM;
   if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > kMaxK) return B200_ERROR_UNSUPPORTED;
   if (M == 0 || N == 0) return B200_OK;
-  const bool swap = M <= 128;
-  const int bn = swap ? (M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128) : (N > 128 ? 256 : 128);
   Params p{};
-  p.rows = swap ? N : M;
-  p.cols = swap ? M : N;
-  p.tiles_m = (int)((p.rows + BM - 1) / BM);
-  p.tiles_n = (int)((p.cols + bn - 1) / bn);
   p.kb_total = (int)((K + BK - 1) / BK);
-  p.row_scale = swap ? b_scale : a_scale;
-  p.col_scale = swap ? a_scale : b_scale;
   p.C = static_cast<__nv_bfloat16*>(C);
   p.ldc = ldc;
   p.bias = static_cast<const __nv_bfloat16*>(bias);
   p.R = static_cast<const __nv_bfloat16*>(residual);
   p.ldr = ldr;
   p.err = b200::error_word(current_device());
-  if ((int64_t)p.tiles_m * p.tiles_n > INT32_MAX / 2) return B200_ERROR_UNSUPPORTED;
-  CUtensorMap ta, tb;
-  if (!make_tmap(&ta, swap ? B : A, p.rows, K, swap ? ldb : lda, BM) ||
-      !make_tmap(&tb, swap ? A : B, p.cols, K, swap ? lda : ldb, bn))
-    return B200_ERROR_UNSUPPORTED;
-  if (swap) {
-    const int splits = plan_splits(p.tiles_m, p.kb_total);
-    p.kb_per_split = (p.kb_total + splits - 1) / splits;
-    const int used = (p.kb_total + p.kb_per_split - 1) / p.kb_per_split;
-    if (bn == 16) return launch_split<16>(epilogue, ta, tb, p, used, stream);
-    if (bn == 32) return launch_split<32>(epilogue, ta, tb, p, used, stream);
-    if (bn == 64) return launch_split<64>(epilogue, ta, tb, p, used, stream);
-    return launch_split<128>(epilogue, ta, tb, p, used, stream);
+  const auto tiles = [](int64_t n, int64_t t) { return (n + t - 1) / t; };
+  const bool pairs = use_pairs(M, N, num_sms());
+  const int bn = pairs ? 0 : (M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128);
+  int splits = 1;
+  if (pairs) {
+    p.rows = M;
+    p.cols = N;
+    p.tiles_m = (int)tiles(M, kPairTile);
+    p.tiles_n = (int)tiles(N, kPairTile);
+    p.row_scale = a_scale;
+    p.col_scale = b_scale;
+  } else {
+    p.rows = N;
+    p.cols = M;
+    p.tiles_m = (int)tiles(N, BM);
+    p.tiles_n = (int)tiles(M, bn);
+    p.row_scale = b_scale;
+    p.col_scale = a_scale;
   }
-  const int grid = std::min(p.tiles_m * p.tiles_n, num_sms());
-  return bn == 256 ? launch_epi<256>(epilogue, ta, tb, p, grid, stream)
-                   : launch_epi<128>(epilogue, ta, tb, p, grid, stream);
+  if ((int64_t)p.tiles_m * p.tiles_n > INT32_MAX / 16) return B200_ERROR_UNSUPPORTED;
+  if (!pairs) {
+    splits = plan_splits(p.tiles_m * p.tiles_n, p.kb_total);
+    p.kb_per_split = (int)tiles(p.kb_total, splits);
+    splits = (int)tiles(p.kb_total, p.kb_per_split);
+  }
+  CUtensorMap tok, w;
+  if (!make_tmap(&tok, A, M, K, lda, pairs ? BM : bn) || !make_tmap(&w, B, N, K, ldb, BM)) return B200_ERROR_UNSUPPORTED;
+  switch (epilogue) {
+    case B200_EPI_NONE: return launch_plain<B200_EPI_NONE>(bn, splits, tok, w, p, stream);
+    case B200_EPI_BIAS: return launch_plain<B200_EPI_BIAS>(bn, splits, tok, w, p, stream);
+    case B200_EPI_RESIDUAL: return launch_plain<B200_EPI_RESIDUAL>(bn, splits, tok, w, p, stream);
+    case B200_EPI_SWIGLU: return launch_plain<B200_EPI_SWIGLU>(bn, splits, tok, w, p, stream);
+    case B200_EPI_BIAS_GELU: return launch_plain<B200_EPI_BIAS_GELU>(bn, splits, tok, w, p, stream);
+    default: return launch_plain<B200_EPI_BIAS_RESIDUAL>(bn, splits, tok, w, p, stream);
+  }
 }
 
 extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
@@ -793,14 +961,14 @@ extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float*
   if (rows > INT32_MAX / 4 || N > INT32_MAX / 4 || groups * N > INT32_MAX / 4 || K > kMaxK)
     return B200_ERROR_UNSUPPORTED;
   if (rows == 0) return B200_OK;
-  // Few tokens per group (decode): weights on the 128-row side, otherwise tokens.
-  const bool swap = rows <= 96LL * groups;
-  const int bn = swap ? 64 : (N > 128 ? 256 : 128);
-  const int feat_tile = swap ? BM : bn, tok_tile = swap ? bn : BM;
+  // Few tokens per group (decode): weights on the 128-row side, up to 64 of a
+  // group's tokens on the N side.
+  const bool few = rows <= 96LL * groups;
+  const int feat_tile = few ? BM : kPairTile, tok_tile = few ? 64 : kPairTile;
   Params p{};
   p.kb_total = (int)((K + BK - 1) / BK);
-  p.row_scale = swap ? b_scale : a_scale;
-  p.col_scale = swap ? a_scale : b_scale;
+  p.row_scale = few ? b_scale : a_scale;
+  p.col_scale = few ? a_scale : b_scale;
   p.C = static_cast<__nv_bfloat16*>(C);
   p.ldc = ldc;
   p.err = b200::error_word(current_device());
@@ -812,11 +980,12 @@ extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float*
   // host upper bound of the units: every group's partial token tile + the full ones
   const int64_t max_units = ((rows + tok_tile - 1) / tok_tile + groups) * (int64_t)p.gF;
   if (max_units > INT32_MAX / 2) return B200_ERROR_UNSUPPORTED;
-  CUtensorMap tw, tt;
-  if (!make_tmap(&tw, B, (int64_t)groups * N, K, ldb, feat_tile) || !make_tmap(&tt, A, rows, K, lda, tok_tile))
+  CUtensorMap w, tok;
+  if (!make_tmap(&w, B, (int64_t)groups * N, K, ldb, BM) || !make_tmap(&tok, A, rows, K, lda, few ? 64 : BM))
     return B200_ERROR_UNSUPPORTED;
-  const int grid = (int)std::min<int64_t>(max_units, num_sms());
-  if (swap) return launch_grouped<64, true>(epilogue, tw, tt, p, grid, stream);
-  return bn == 256 ? launch_grouped<256, false>(epilogue, tt, tw, p, grid, stream)
-                   : launch_grouped<128, false>(epilogue, tt, tw, p, grid, stream);
+  if (few)
+    return epilogue == B200_EPI_SWIGLU ? launch_group<64, B200_EPI_SWIGLU>(tok, w, p, max_units, stream)
+                                       : launch_group<64, B200_EPI_NONE>(tok, w, p, max_units, stream);
+  return epilogue == B200_EPI_SWIGLU ? launch_pair<B200_EPI_SWIGLU, true>(tok, w, p, max_units, stream)
+                                     : launch_pair<B200_EPI_NONE, true>(tok, w, p, max_units, stream);
 }

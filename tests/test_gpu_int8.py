@@ -203,7 +203,7 @@ def gemm(a, sa, b, sb, epi, bias=None, res=None, pad=0, out=None, inplace=False)
 SHAPES = [(1, 8, 16), (1, 4096, 4096), (2, 136, 144), (8, 256, 48), (15, 520, 1040), (16, 128, 128), (17, 264, 272),
           (32, 6144, 512), (33, 1032, 2064), (64, 512, 4096), (65, 2056, 128), (96, 24, 4112), (128, 640, 1408),
           (129, 128, 256), (130, 136, 272), (200, 1408, 2048), (257, 264, 1040), (300, 8, 16), (512, 4096, 1024),
-          (777, 520, 1040), (1025, 1288, 400), (2049, 2568, 144)]
+          (777, 520, 1040), (1025, 1288, 400), (2049, 2568, 144), (2300, 2312, 1040), (257, 20000, 272), (5000, 1160, 4112)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -215,7 +215,7 @@ def test_gemm_shapes(M, N, K):
 
 @pytest.mark.parametrize("epi", range(6))
 @pytest.mark.parametrize("M,N,K", [(1, 144, 272), (20, 528, 1040), (50, 272, 4112), (128, 1040, 512), (131, 144, 272),
-                                   (700, 1296, 528)])
+                                   (700, 1296, 528), (2100, 2576, 400)])
 def test_gemm_epilogues(M, N, K, epi):
     rng = np.random.default_rng(M + epi)
     a, sa, b, sb, bias, res = operands(rng, M, N, K, epi)
