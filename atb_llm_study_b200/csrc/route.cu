@@ -10,8 +10,7 @@
 //
 // The choice is that of the definition in 64 bits: it is made on fp32 scores
 // whose error is bounded, and a token with two candidates nearer to one another
-// than that bound is chosen again on scores in double.  Without a bias the
-// experts are ranked by the logits themselves, which needs no bound.
+// than that bound is chosen again on scores in double.
 #include <float.h>
 #include <math.h>
 
@@ -32,139 +31,297 @@ struct RouteParams {
   int64_t T;
   int E, k, sigmoid, G, gs, lpg_shift, keep, best, renorm;
   float scale;
+  int vec;  // the lanes' runs of logits (and biases) are whole, aligned float4s
   int32_t* ids;
   float* wts;
 };
 
-__device__ __forceinline__ float wmax(float v) { return warp_max(v); }
-__device__ __forceinline__ double wmax(double v) {
+// ---------------------------------------------------------------------------
+// One warp per token.  Lane l of group g's 2^lpg_shift lanes holds PER
+// consecutive experts, so lanes, and values within a lane, are in expert order.
+// ---------------------------------------------------------------------------
+struct Slot {
+  int g, e0, n;  // group, first expert and number of experts of this lane
+};
+
+template <int PER>
+__device__ __forceinline__ Slot slot_of(const RouteParams& p, int lane) {
+  const int l = lane & ((1 << p.lpg_shift) - 1);
+  Slot s;
+  s.g = lane >> p.lpg_shift;
+  s.e0 = s.g * p.gs + l * PER;
+  s.n = s.g < p.G ? min(max(p.gs - l * PER, 0), PER) : 0;
+  return s;
+}
+
+__device__ __forceinline__ float clamp_logit(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX); }  // NaN: -FLT_MAX
+
+template <int PER>
+__device__ __forceinline__ void load_run(float v[PER], const float* src, const Slot& s, int vec, float fill) {
+  if (PER % 4 == 0 && vec) {
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i)
+      if (s.n > 0) {
+        const float4 f = *reinterpret_cast<const float4*>(src + s.e0 + 4 * i);
+        v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+      } else {
+        v[4 * i] = v[4 * i + 1] = v[4 * i + 2] = v[4 * i + 3] = fill;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = i < s.n ? src[s.e0 + i] : fill;
+  }
+}
+
+// fp32 values as unsigned integers of the same order (0: below every value),
+// the lowest bits replaced by a tag.
+__device__ __forceinline__ uint32_t to_key(float v, uint32_t tag_bits, uint32_t tag) {
+  const uint32_t b = __float_as_uint(v);
+  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return (o & ~tag_bits) | tag;
+}
+__device__ __forceinline__ float from_key(uint32_t k, uint32_t tag_bits) {
+  k &= ~tag_bits;
+  return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
+}
+
+// Descending (Batcher's odd-even merge sort).
+template <int N>
+__device__ __forceinline__ void sort_desc(uint32_t k[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j <= N - 1 - q; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t x = k[i + j], y = k[i + j + q];
+            k[i + j] = max(x, y);
+            k[i + j + q] = min(x, y);
+          }
+}
+
+// The choice on fp32 scores; false (nothing written) when two candidates of a
+// decision are nearer than the scores' error.
+//
+// What is compared carries a tag in its low bits, so one 32-bit maximum over
+// the warp gives value and place: 4 bits among experts (the place in the lane;
+// relative error 2^-19), 5 among groups (2^-18).  Two equal values are always
+// in doubt, so ties are settled in double, by index.
+//
+// Error of a score, relative to the largest one (exp is the fast one, 2 +
+// 1.2 |x| ulp of e^x, which is at most 2 ulp of 1 for a softmax term and less
+// for a sigmoid): 2.4e-7, the sum of up to 256 terms (21 roundings and the
+// terms' own errors, 1.6e-6 where every term counts), the quotient 2.4e-7.
+// Below 2.5e-6; a difference of two 5e-6.
+template <int PER>
+__device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int lane) {
+  constexpr uint32_t kTag = 15u, kGroupTag = 31u;
+  const Slot sl = slot_of<PER>(p, lane);
+  const float* lg = p.logits + t * p.ld;
+  float c[PER];
+  load_run<PER>(c, lg, sl, p.vec, -FLT_MAX);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) c[i] = clamp_logit(c[i]);
+  const bool pair_groups = p.keep < p.G && p.best > 1;
+  const bool by_score = p.bias != nullptr;  // without a bias experts are ranked by their logits
+  float m = 0.f, inv = 1.f, top = 1.f;      // softmax: the largest logit, 1 / sum, the largest score
+  if (!p.sigmoid) {
+    m = c[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) m = fmaxf(m, c[i]);
+    m = from_key(__reduce_max_sync(0xffffffffu, to_key(m, 0u, 0u)), 0u);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += i < sl.n ? __expf(c[i] - m) : 0.f;
+    inv = __fdividef(1.f, warp_sum(sum));
+    top = inv;
+  }
+  float s[PER];  // scores, where anything is ranked by them
+  if (by_score || pair_groups) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[i])) : __expf(c[i] - m) * inv;
+  }
+  if (by_score) {
+    float b[PER];
+    load_run<PER>(b, p.bias, sl, p.vec, 0.f);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = s[i] + b[i];
+      if (!(c[i] >= -FLT_MAX)) c[i] = -FLT_MAX;
+    }
+  }
+  const float tol = by_score || pair_groups ? 5e-6f * top : 0.f;
+  bool in = true, clear = true;
+  if (p.keep < p.G) {
+    // the group's one or two largest, over its lanes
+    float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float v = i < sl.n ? (p.best > 1 && !by_score ? s[i] : c[i]) : -INFINITY;
+      b = fmaxf(b, fminf(a, v));
+      a = fmaxf(a, v);
+    }
+    for (int o = 1; o < (1 << p.lpg_shift); o <<= 1) {
+      const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+      a = fmaxf(a, oa);
+    }
+    const float score = p.best > 1 ? a + b : a;
+    // roundings of the biased sums are relative to their terms, which can cancel
+    const float size = p.best > 1 ? fabsf(a) + fabsf(b) : fabsf(a);
+    uint32_t key = sl.g < p.G ? to_key(score, kGroupTag, 31u - sl.g) : 0u;
+    uint32_t last = 0;
+    float last_size = 0.f;
+    in = false;
+    for (int j = 0; j <= p.keep; ++j) {  // one more than is kept: the best that is not
+      const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+      const bool hit = key == best;
+      const float sz = __shfl_sync(0xffffffffu, size, (31 - (int)(best & kGroupTag)) << p.lpg_shift);
+      if (j < p.keep) {
+        in |= hit;
+        key = hit ? 0u : key;
+        last = best;
+        last_size = sz;
+      } else {
+        const float x = from_key(last, kGroupTag), y = from_key(best, kGroupTag);
+        const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 1e-6f * fmaxf(sz, last_size) + 8e-6f * fabsf(x) : 0.f);
+        clear = x - y > near;
+      }
+    }
+  }
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = in && i < sl.n ? to_key(c[i], kTag, 15u - i) : 0u;
+  sort_desc<PER>(key);
+  uint32_t mine = 0, before = 0xffffffffu;
+  int from_lane = 0;
+  for (int j = 0; j <= p.k && clear; ++j) {  // one more than is chosen: the best that is not
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
+    if (j > 0) {
+      const float x = from_key(before, kTag), y = from_key(best, kTag);
+      clear = best == 0u || x - y > (by_score ? tol + 4e-6f * fabsf(x) : 0.f);
+    }
+    if (j == p.k) break;
+    const int from = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+    if (lane == j) {
+      mine = best;
+      from_lane = from;
+    }
+    if (lane == from) {
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+      key[PER - 1] = 0u;
+    }
+    before = best;
+  }
+  if (!clear) return false;
+  // lane j < k: the j-th choice and its weight, from its logit
+  int e = 0;
+  float w = 0.f;
+  if (lane < p.k) {
+    const Slot from = slot_of<PER>(p, from_lane);
+    e = from.e0 + 15 - (int)(mine & kTag);
+    const float x = clamp_logit(lg[e]);
+    w = p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - m) * inv;
+  }
+  if (p.renorm) {
+    float sum = w;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (__shfl_sync(0xffffffffu, sum, 0) < 1e-30f) return false;  // scores below fp32's range
+    w = w / sum;
+  }
+  if (lane < p.k) {
+    p.ids[t * p.k + lane] = e;
+    p.wts[t * p.k + lane] = w * p.scale;
+  }
+  return true;
+}
+
+__device__ __forceinline__ double warp_max(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <typename F>
-__device__ __forceinline__ F wsum(F v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
 
-// One warp chooses one token's experts with scores of type F.  Lane l of group
-// g's 2^lpg_shift lanes holds PER consecutive experts, so lanes, and values
-// within a lane, are in expert order.  Returns whether every decision was
-// clear of the scores' error (double: always).
-template <typename F, int PER>
-__device__ __forceinline__ bool choose(const RouteParams& p, int64_t t, int lane) {
-  constexpr bool kFloat = sizeof(F) == 4;
-  const int lpg = 1 << p.lpg_shift;
-  const int g = lane >> p.lpg_shift, l = lane & (lpg - 1);
-  const int e0 = g * p.gs + l * PER;
-  const int n = g < p.G ? min(max(p.gs - l * PER, 0), PER) : 0;  // experts in this lane
-  F s[PER], c[PER];
+// The choice on scores in double (experts without a bias by their logits).
+template <int PER>
+__device__ __noinline__ void choose_exact(const RouteParams& p, int64_t t, int lane) {
+  const Slot sl = slot_of<PER>(p, lane);
+  const double low = -INFINITY;
+  double s[PER], c[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    float x = -FLT_MAX;
-    if (i < n) x = fminf(fmaxf(p.logits[t * p.ld + e0 + i], -FLT_MAX), FLT_MAX);  // NaN gives -FLT_MAX
-    c[i] = (F)x;
-  }
+  for (int i = 0; i < PER; ++i) c[i] = i < sl.n ? clamp_logit(p.logits[t * p.ld + sl.e0 + i]) : low;
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = i < n ? F(1) / (F(1) + exp_of(-c[i])) : F(0);
+    for (int i = 0; i < PER; ++i) s[i] = 1.0 / (1.0 + exp(-c[i]));
   } else {
-    F m = F(-FLT_MAX);
+    double m = low;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) m = c[i] > m ? c[i] : m;
-    m = wmax(m);
-    F sum = F(0);
+    for (int i = 0; i < PER; ++i) m = fmax(m, c[i]);
+    m = warp_max(m);
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = i < n ? exp_of(c[i] - m) : F(0);
+      s[i] = exp(c[i] - m);
       sum += s[i];
     }
-    sum = wsum(sum);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = s[i] / sum;
-  }
-  // Bounds for fp32 scores.  expf is within 2 ulp and its argument within half
-  // an ulp of x - max (s |x - max| <= 0.37), the sum of up to 256 terms within
-  // 21 roundings (16 in the lane, 5 over the lanes), the division within half
-  // an ulp: 1.8e-6 of the largest score covers an error, twice that and the
-  // roundings of the biased sums a difference of two.
-  F tol = F(0);
-  bool clear = true;
-  if (kFloat && (p.bias || p.best > 1)) {
-    F top = F(0);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) top = s[i] > top ? s[i] : top;
-    tol = F(4e-6) * wmax(top);
+    for (int i = 0; i < PER; ++i) s[i] /= sum;
   }
-  const bool ranked_by_score = p.bias != nullptr;
-  if (ranked_by_score) {
+  if (p.bias) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const F v = i < n ? s[i] + (F)p.bias[e0 + i] : F(0);
-      c[i] = v == v ? v : F(-FLT_MAX);
+      if (i < sl.n) c[i] = s[i] + (double)p.bias[sl.e0 + i];
+      if (!(c[i] >= -DBL_MAX)) c[i] = i < sl.n ? -DBL_MAX : low;
     }
   }
-  bool in = n > 0;  // this lane's group is kept
+  bool in = sl.n > 0;
   if (p.keep < p.G) {
-    // the group's two largest scores, over its lanes
-    const F low = F(-INFINITY);
-    F a = low, b = low;
+    double a = low, b = low;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const F v = i < n ? (p.best > 1 && !ranked_by_score ? s[i] : c[i]) : low;
-      const F lo = a < v ? a : v;
-      a = a < v ? v : a;
-      b = b < lo ? lo : b;
+      const double v = i < sl.n ? (p.best > 1 && !p.bias ? s[i] : c[i]) : low;
+      b = fmax(b, fmin(a, v));
+      a = fmax(a, v);
     }
-    for (int o = 1; o < lpg; o <<= 1) {
-      const F oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-      const F lo = a < oa ? a : oa, hb = b < ob ? ob : b;
-      a = a < oa ? oa : a;
-      b = lo < hb ? hb : lo;
+    for (int o = 1; o < (1 << p.lpg_shift); o <<= 1) {
+      const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      b = fmax(fmin(a, oa), fmax(b, ob));
+      a = fmax(a, oa);
     }
-    const F score = p.best > 1 ? a + b : a;
-    const F size = (a < 0 ? -a : a) + (p.best > 1 ? (b < 0 ? -b : b) : F(0));
-    const F near = (p.best > 1 ? 2 * tol : tol) + F(3.6e-7) * size;
+    const double score = p.best > 1 ? a + b : a;
     int rank = 0;
-    bool doubt = false;
     for (int h = 0; h < p.G; ++h) {
-      const F other = __shfl_sync(0xffffffffu, score, h << p.lpg_shift);
-      rank += other > score || (other == score && h < g);
-      const F d = other > score ? other - score : score - other;
-      doubt |= h != g && d <= near;
+      const double other = __shfl_sync(0xffffffffu, score, h << p.lpg_shift);
+      rank += other > score || (other == score && h < sl.g);
     }
     in = in && rank < p.keep;
-    if (kFloat && tol > F(0)) clear = !__any_sync(0xffffffffu, doubt && g < p.G);
   }
-  int mine = 0x7fffffff;  // lane j < k: the j-th choice
-  F mine_s = F(0), sum = F(0), before = F(0);
+  int mine = 0;  // lane j < k: the j-th choice
+  double mine_s = 0.0, sum = 0.0;
   unsigned taken = 0;
-  // one round more than k, when it exists: the best that was not chosen
 #pragma unroll 1
-  for (int j = 0; j <= p.k; ++j) {
-    F bv = F(0), bs = F(0);
+  for (int j = 0; j < p.k; ++j) {
+    double bv = low, bs = 0.0;
     int bi = -1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (in && i < n && !(taken >> i & 1u) && (bi < 0 || c[i] > bv)) {
+      if (in && i < sl.n && !(taken >> i & 1u) && (bi < 0 || c[i] > bv)) {
         bv = c[i];
         bs = s[i];
         bi = i;
       }
     }
-    const unsigned have = __ballot_sync(0xffffffffu, bi >= 0);
-    if (!have) break;
-    const F top = wmax(bi >= 0 ? bv : F(-INFINITY));
+    const double top = warp_max(bv);
     const int from = __ffs(__ballot_sync(0xffffffffu, bi >= 0 && bv == top)) - 1;
-    if (kFloat && ranked_by_score && j > 0 && before - top <= tol + F(1.2e-7) * (top < 0 ? -top : top)) clear = false;
-    before = top;
-    if (j == p.k) break;
-    const int e = __shfl_sync(0xffffffffu, e0 + bi, from);
-    const F w = __shfl_sync(0xffffffffu, bs, from);
+    const int e = __shfl_sync(0xffffffffu, sl.e0 + bi, from);
+    const double w = __shfl_sync(0xffffffffu, bs, from);
     if (lane == from) taken |= 1u << bi;
     if (lane == j) {
       mine = e;
@@ -172,19 +329,11 @@ __device__ __forceinline__ bool choose(const RouteParams& p, int64_t t, int lane
     }
     sum += w;
   }
-  if (kFloat && p.renorm && sum < F(1e-30)) clear = false;  // weights below fp32's range
-  if (kFloat && !clear) return false;
   if (lane < p.k) {
     p.ids[t * p.k + lane] = mine;
-    const F w = p.renorm ? (sum > F(0) ? mine_s / sum : F(0)) : mine_s;
-    p.wts[t * p.k + lane] = (float)(w * (F)p.scale);
+    if (p.renorm) mine_s = sum > 0.0 ? mine_s / sum : 0.0;
+    p.wts[t * p.k + lane] = (float)(mine_s * (double)p.scale);
   }
-  return true;
-}
-
-template <int PER>
-__device__ __noinline__ void choose_in_double(const RouteParams& p, int64_t t, int lane) {
-  choose<double, PER>(p, t, lane);
 }
 
 template <int PER>
@@ -194,7 +343,7 @@ __global__ void __launch_bounds__(kWarps * 32) topk_grouped_kernel(const RoutePa
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= p.T) return;
-  if (!choose<float, PER>(p, t, lane)) choose_in_double<PER>(p, t, lane);
+  if (!choose_fast<PER>(p, t, lane)) choose_exact<PER>(p, t, lane);
 }
 
 }  // namespace
@@ -235,6 +384,8 @@ extern "C" int b200_moe_topk_grouped(const float* logits, int64_t ld, const floa
   p.wts = topk_weights;
   while ((p.G << (p.lpg_shift + 1)) <= 32) ++p.lpg_shift;
   const int per = (p.gs + (1 << p.lpg_shift) - 1) >> p.lpg_shift;
+  const int held = per <= 4 ? 4 : 8;
+  p.vec = p.gs == held << p.lpg_shift && ld % 4 == 0 && ((uintptr_t)logits & 15u) == 0 && ((uintptr_t)bias & 15u) == 0;
   const dim3 grid((unsigned)((T + kWarps - 1) / kWarps));
   if (per <= 1) launch_kernel(topk_grouped_kernel<1>, grid, kWarps * 32, 0, stream, p);
   else if (per <= 2) launch_kernel(topk_grouped_kernel<2>, grid, kWarps * 32, 0, stream, p);
