@@ -103,6 +103,19 @@ __device__ __forceinline__ void sort_desc(uint32_t k[N]) {
           }
 }
 
+// Without the scaling that keeps subnormal arguments and results (they are far
+// below the bounds here).
+__device__ __forceinline__ float exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The choice on fp32 scores; false (nothing written) when two candidates of a
 // decision are nearer than the scores' error.
 //
@@ -135,22 +148,21 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
     m = from_key(__reduce_max_sync(0xffffffffu, to_key(m, 0u, 0u)), 0u);
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum += i < sl.n ? __expf(c[i] - m) : 0.f;
-    inv = __fdividef(1.f, warp_sum(sum));
+    for (int i = 0; i < PER; ++i) sum += i < sl.n ? exp_fast(c[i] - m) : 0.f;
+    inv = rcp_fast(warp_sum(sum));
     top = inv;
   }
   float s[PER];  // scores, where anything is ranked by them
   if (by_score || pair_groups) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[i])) : __expf(c[i] - m) * inv;
+    for (int i = 0; i < PER; ++i) s[i] = p.sigmoid ? rcp_fast(1.f + exp_fast(-c[i])) : exp_fast(c[i] - m) * inv;
   }
   if (by_score) {
     float b[PER];
     load_run<PER>(b, p.bias, sl, p.vec, 0.f);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      c[i] = s[i] + b[i];
-      if (!(c[i] >= -FLT_MAX)) c[i] = -FLT_MAX;
+      c[i] = fmaxf(s[i] + b[i], -FLT_MAX);
     }
   }
   const float tol = by_score || pair_groups ? 5e-6f * top : 0.f;
@@ -173,38 +185,31 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
     // roundings of the biased sums are relative to their terms, which can cancel
     const float size = p.best > 1 ? fabsf(a) + fabsf(b) : fabsf(a);
     uint32_t key = sl.g < p.G ? to_key(score, kGroupTag, 31u - sl.g) : 0u;
-    uint32_t last = 0;
-    float last_size = 0.f;
+    uint32_t nth = 0;  // lane j: the j-th group's key
     in = false;
     for (int j = 0; j <= p.keep; ++j) {  // one more than is kept: the best that is not
       const uint32_t best = __reduce_max_sync(0xffffffffu, key);
-      const bool hit = key == best;
-      const float sz = __shfl_sync(0xffffffffu, size, (31 - (int)(best & kGroupTag)) << p.lpg_shift);
-      if (j < p.keep) {
-        in |= hit;
-        key = hit ? 0u : key;
-        last = best;
-        last_size = sz;
-      } else {
-        const float x = from_key(last, kGroupTag), y = from_key(best, kGroupTag);
-        const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 1e-6f * fmaxf(sz, last_size) + 8e-6f * fabsf(x) : 0.f);
-        clear = x - y > near;
+      nth = lane == j ? best : nth;
+      if (j < p.keep && key == best) {
+        in = true;
+        key = 0u;
       }
     }
+    // the last group that is kept against the best that is not
+    const float x = from_key(nth, kGroupTag);
+    const float sz = __shfl_sync(0xffffffffu, size, (31 - (int)(nth & kGroupTag)) << p.lpg_shift);
+    const float y = __shfl_down_sync(0xffffffffu, x, 1), sz1 = __shfl_down_sync(0xffffffffu, sz, 1);
+    const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 1e-6f * fmaxf(sz, sz1) + 8e-6f * fabsf(x) : 0.f);
+    clear = __shfl_sync(0xffffffffu, (int)(x - y > near), p.keep - 1) != 0;
   }
   uint32_t key[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) key[i] = in && i < sl.n ? to_key(c[i], kTag, 15u - i) : 0u;
   sort_desc<PER>(key);
-  uint32_t mine = 0, before = 0xffffffffu;
+  uint32_t mine = 0;  // lane j: the j-th choice's key, and the lane that holds it
   int from_lane = 0;
-  for (int j = 0; j <= p.k && clear; ++j) {  // one more than is chosen: the best that is not
+  for (int j = 0; j <= p.k; ++j) {  // one more than is chosen: the best that is not
     const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
-    if (j > 0) {
-      const float x = from_key(before, kTag), y = from_key(best, kTag);
-      clear = best == 0u || x - y > (by_score ? tol + 4e-6f * fabsf(x) : 0.f);
-    }
-    if (j == p.k) break;
     const int from = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
     if (lane == j) {
       mine = best;
@@ -215,7 +220,13 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
       for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
       key[PER - 1] = 0u;
     }
-    before = best;
+  }
+  {
+    // every choice against the next; a next that does not exist has key 0
+    const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1);
+    const float x = from_key(mine, kTag), y = from_key(next, kTag);
+    const bool apart = lane >= p.k || next == 0u || x - y > (by_score ? tol + 4e-6f * fabsf(x) : 0.f);
+    clear = clear && __all_sync(0xffffffffu, apart);
   }
   if (!clear) return false;
   // lane j < k: the j-th choice and its weight, from its logit
