@@ -58,6 +58,24 @@ B200_DEV uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// 32 bytes at once (32-byte aligned).
+struct alignas(32) Words8 {
+  uint32_t w[8];
+};
+B200_DEV void store_32(void* dst, const Words8& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v.w[0]), "r"(v.w[1]),
+               "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
+}
+B200_DEV Words8 load_32(const void* src) {
+  Words8 v;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]),
+                 "=r"(v.w[7])
+               : "l"(src));
+  return v;
+}
+
 B200_DEV float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -413,9 +431,12 @@ B200_DEV uint32_t cluster_map(uint32_t smem_addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
   return a;
 }
-// Arrive on an mbarrier of any CTA of the cluster (cluster address).
-B200_DEV void cluster_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrive on an mbarrier of any CTA of the cluster (cluster address), without
+// ordering this thread's memory accesses: to hand back TMEM whose reads
+// tcgen05.wait::ld has completed.  (A releasing arrive would first wait for all
+// of the thread's earlier global stores, about 2000 cycles.)
+B200_DEV void cluster_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 B200_DEV int4 cluster_load4(uint32_t addr) {
   int4 v;

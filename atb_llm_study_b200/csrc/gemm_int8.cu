@@ -60,6 +60,7 @@ struct Unit {
   int tok0, wrow0;  // TMA rows of the token and the weight operand
   int feat0;        // first output column
   int tok_lim, feat_lim;
+  int n;            // grouped pairs: tokens of this tile, rounded up to a multiple of 32
 };
 
 // 0.5 x (1 + tanh(u)) = x / (1 + e^-2u), u = sqrt(2/pi) (x + 0.044715 x^3): one
@@ -96,32 +97,119 @@ __device__ __forceinline__ Unit group_unit(int w, const Params& p, const int* gt
     else hi = mid;
   }
   const int t0 = gtab[lo], t1 = gtab[lo + 1];
-  const int tt = (t1 - t0 + TOKT - 1) / TOKT;
   const int r = w - up[lo];
+  const int tt = (t1 - t0 + TOKT - 1) / TOKT;
   Unit u;
   u.tok0 = t0 + r % tt * TOKT;
   u.feat0 = r / tt * FEATT;
   u.wrow0 = (int)(lo * p.gN) + u.feat0;
   u.tok_lim = t1;
   u.feat_lim = (int)p.gN;
+  u.n = min(TOKT, (t1 - u.tok0 + 31) & ~31);
   return u;
 }
 
-// One thread fills gtab from the device offsets; offsets that fall or leave
-// [0, rows] are clamped and reported.
+// One warp fills gtab from the device offsets, 32 groups at a time (prefix
+// maximum and prefix sum); offsets that fall or leave [0, rows] are clamped and
+// reported.
 template <int TOKT>
-__device__ __forceinline__ void fill_group_table(int* gtab, const Params& p) {
+__device__ __forceinline__ void fill_group_table(int* gtab, const Params& p, int lane) {
+  constexpr int kRounds = (kMaxGroups + 1 + 31) / 32;
+  int v[kRounds];  // all loads at once
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) v[i] = i * 32 + lane <= p.groups ? p.goff[i * 32 + lane] : 0;
   int prev = 0, run = 0;
-  for (int g = 0; g <= p.groups; ++g) {
-    int v = p.goff[g];
-    if (v < prev || v > p.gRows || (g == 0 && v != 0)) {
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    if (i * 32 > p.groups) break;
+    const int g = i * 32 + lane;
+    int x = g == 0 ? 0 : max(v[i], prev);
+    int before = __shfl_up_sync(0xffffffffu, v[i], 1);
+    if (lane == 0) before = i == 0 ? 0 : prev;
+    if (g <= p.groups && (v[i] < before || v[i] > p.gRows || v[i] < 0 || (g == 0 && v[i] != 0)))
       raise_error(p.err, DEV_ERR_BAD_INDEX);
-      v = min(max(v, prev), (int)p.gRows);
-      if (g == 0) v = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x = max(x, y);
     }
-    if (g > 0) run += ((v - prev + TOKT - 1) / TOKT) * p.gF;
-    gtab[g] = prev = v;
-    gtab[p.groups + 1 + g] = run;
+    x = min(x, (int)p.gRows);
+    int lo = __shfl_up_sync(0xffffffffu, x, 1);
+    if (lane == 0) lo = prev;
+    int sum = g > 0 && g <= p.groups ? (x - lo + TOKT - 1) / TOKT * p.gF : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    sum += run;
+    if (g <= p.groups) {
+      gtab[g] = x;
+      gtab[p.groups + 1 + g] = sum;
+    }
+    prev = __shfl_sync(0xffffffffu, x, 31);
+    run = __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
+
+// CW (16 or 32) accumulator columns, tokens tok0.., of 32 consecutive feature
+// rows (one a lane, the first at output feature feat0 of the untiled width),
+// through the epilogue and transposed among the lanes, so that a lane stores
+// four features of a token at once and a warp's store covers whole 32-byte
+// sectors.  ts: the tokens' scales; fscale: this lane's feature's.
+template <int EPI, int CW>
+__device__ __forceinline__ void emit_features(const uint32_t acc[CW], int feat0, int tok0, float fscale, const float* ts,
+                                              const Unit& u, int lane, const Params& p) {
+  float v[CW];
+#pragma unroll
+  for (int i = 0; i < CW; i += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(ts + i);
+    v[i] = (float)(int)acc[i] * fscale * s.x;
+    v[i + 1] = (float)(int)acc[i + 1] * fscale * s.y;
+    v[i + 2] = (float)(int)acc[i + 2] * fscale * s.z;
+    v[i + 3] = (float)(int)acc[i + 3] * fscale * s.w;
+  }
+  constexpr unsigned kAll = 0xffffffffu;
+  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+  if (EPI == B200_EPI_SWIGLU) {
+    // lanes 2j / 2j+1 hold gate / up of output j: the even lane finishes the
+    // first half of the tokens, the odd lane the second
+    constexpr int H = CW / 2;
+    float o[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float other = __shfl_xor_sync(kAll, b0 ? v[i] : v[H + i], 1);
+      o[i] = b0 ? silu_f(other) * v[H + i] : silu_f(v[i]) * other;
+    }
+    uint32_t a[H / 2];  // two outputs of token 2t + b1
+#pragma unroll
+    for (int t = 0; t < H / 2; ++t) {
+      const float got = __shfl_xor_sync(kAll, b1 ? o[2 * t] : o[2 * t + 1], 2);
+      a[t] = b1 ? pack2(got, o[2 * t + 1]) : pack2(o[2 * t], got);
+    }
+    const int f = feat0 / 2 + (lane >> 1 & ~3);
+#pragma unroll
+    for (int t = 0; t < H / 4; ++t) {  // four outputs of token 4t + 2 b2 + b1
+      const uint32_t got = __shfl_xor_sync(kAll, b2 ? a[2 * t] : a[2 * t + 1], 4);
+      const uint2 w = b2 ? make_uint2(got, a[2 * t + 1]) : make_uint2(a[2 * t], got);
+      const int64_t tok = tok0 + (b0 ? H : 0) + 4 * t + 2 * b2 + b1;
+      if (2 * f < u.feat_lim && tok < u.tok_lim) *reinterpret_cast<uint2*>(p.C + tok * p.ldc + f) = w;
+    }
+    return;
+  }
+  uint32_t a[CW / 2];  // two features of token 2t + b0
+#pragma unroll
+  for (int t = 0; t < CW / 2; ++t) {
+    const float got = __shfl_xor_sync(kAll, b0 ? v[2 * t] : v[2 * t + 1], 1);
+    a[t] = b0 ? pack2(got, v[2 * t + 1]) : pack2(v[2 * t], got);
+  }
+  const int f = feat0 + (lane & ~3);
+#pragma unroll
+  for (int t = 0; t < CW / 4; ++t) {  // four features of token 4t + 2 b1 + b0
+    const uint32_t got = __shfl_xor_sync(kAll, b1 ? a[2 * t] : a[2 * t + 1], 2);
+    const uint2 w = b1 ? make_uint2(got, a[2 * t + 1]) : make_uint2(a[2 * t], got);
+    const int64_t tok = tok0 + 4 * t + 2 * b1 + b0;
+    if (f < u.feat_lim && tok < u.tok_lim) *reinterpret_cast<uint2*>(p.C + tok * p.ldc + f) = w;
   }
 }
 
@@ -131,6 +219,9 @@ __device__ __forceinline__ void fill_group_table(int* gtab, const Params& p) {
 // MMAs that read both halves, and each CTA's epilogue drains its 128 token rows
 // from its own TMEM.  Against single CTAs with 128 x 256 tiles a pair moves a
 // third less through L2 and shared memory per product.
+// Grouped launches turn the operands round: 256 weight rows on the M side and
+// a group's tokens on the N side, whose extent can be any multiple of 32, so a
+// group's last tile does no product for rows it does not have.
 // ---------------------------------------------------------------------------
 constexpr int kPairTile = 256;
 constexpr int kPairGroup = 8;  // token tiles walked per feature tile
@@ -140,55 +231,84 @@ constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
 constexpr int kPairStageBytes = 2 * BM * BK;  // of each CTA
 constexpr int kPairColBytes = kPairEpiWarps * 128 * 2 * 4;  // column scales and biases of each epilogue warp
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kPairColBytes + kGroupTabBytes;
-constexpr uint32_t kPairIdesc = idesc_i8_s32(256, kPairTile);
+constexpr int kTokBox = 64;  // token rows of one TMA box of a grouped launch
 
 // 32 accumulator columns of one token row through the epilogue; scale and bias
-// of the columns come from shared memory.
+// of the columns come from shared memory.  A lane has a row of its own, so each
+// of a warp's stores (and residual loads) touches 32 lines and costs the L1 that
+// the MMA operands pass through as many cycles, whatever its width: with `wide`
+// (32-byte aligned rows) it moves 32 bytes at a time, otherwise 16 or 8.
 template <int EPI>
 __device__ __forceinline__ void emit_row(const uint32_t acc[32], int64_t tok, int feat0, float rscale, const float* cscale,
-                                         const float* cbias, const Unit& u, const Params& p) {
+                                         const float* cbias, bool wide, const Unit& u, const Params& p) {
+  constexpr bool kSwiglu = EPI == B200_EPI_SWIGLU;
+  constexpr int W = kSwiglu ? 32 : 16;  // columns behind 32 bytes of output
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int c = feat0 + g * 8;
-    if (c >= u.feat_lim) continue;
-    float x[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 s = *reinterpret_cast<const float4*>(cscale + g * 8 + h * 4);
-      x[4 * h] = (float)(int)acc[8 * g + 4 * h] * rscale * s.x;
-      x[4 * h + 1] = (float)(int)acc[8 * g + 4 * h + 1] * rscale * s.y;
-      x[4 * h + 2] = (float)(int)acc[8 * g + 4 * h + 2] * rscale * s.z;
-      x[4 * h + 3] = (float)(int)acc[8 * g + 4 * h + 3] * rscale * s.w;
-      if (has_bias(EPI)) {
-        const float4 b = *reinterpret_cast<const float4*>(cbias + g * 8 + h * 4);
-        x[4 * h] += b.x, x[4 * h + 1] += b.y, x[4 * h + 2] += b.z, x[4 * h + 3] += b.w;
+  for (int g = 0; g < 32; g += W) {
+    const int c0 = feat0 + g;
+    if (c0 >= u.feat_lim) continue;
+    const bool whole = wide && c0 + W <= u.feat_lim;
+    const __nv_bfloat16* res = has_residual(EPI) ? p.R + tok * p.ldr + c0 : nullptr;
+    Words8 r8;
+    if (has_residual(EPI)) {
+      if (whole) {
+        r8 = load_32(res);
+      } else {
+        const uint4 lo = *reinterpret_cast<const uint4*>(res);
+        const uint4 hi = c0 + 8 < u.feat_lim ? *reinterpret_cast<const uint4*>(res + 8) : make_uint4(0, 0, 0, 0);
+        r8.w[0] = lo.x, r8.w[1] = lo.y, r8.w[2] = lo.z, r8.w[3] = lo.w;
+        r8.w[4] = hi.x, r8.w[5] = hi.y, r8.w[6] = hi.z, r8.w[7] = hi.w;
       }
     }
-    if (EPI == B200_EPI_BIAS_GELU) {
+    Words8 o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = gelu_tanh_f(x[i]);
-    }
-    if (has_residual(EPI)) {
-      float r[8];
-      unpack8(*reinterpret_cast<const uint4*>(p.R + tok * p.ldr + c), r);
+    for (int h = 0; h < W; h += 4) {
+      const float4 s = *reinterpret_cast<const float4*>(cscale + g + h);
+      float x[4] = {(float)(int)acc[g + h] * rscale * s.x, (float)(int)acc[g + h + 1] * rscale * s.y,
+                    (float)(int)acc[g + h + 2] * rscale * s.z, (float)(int)acc[g + h + 3] * rscale * s.w};
+      if (has_bias(EPI)) {
+        const float4 b = *reinterpret_cast<const float4*>(cbias + g + h);
+        x[0] += b.x, x[1] += b.y, x[2] += b.z, x[3] += b.w;
+      }
+      if (EPI == B200_EPI_BIAS_GELU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] += r[i];
+        for (int i = 0; i < 4; ++i) x[i] = gelu_tanh_f(x[i]);
+      }
+      if (kSwiglu) {
+        o.w[h / 4] = pack2(silu_f(x[0]) * x[1], silu_f(x[2]) * x[3]);
+        continue;
+      }
+      if (has_residual(EPI)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 r = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r8.w[h / 2 + i]));
+          x[2 * i] += r.x, x[2 * i + 1] += r.y;
+        }
+      }
+      o.w[h / 2] = pack2(x[0], x[1]);
+      o.w[h / 2 + 1] = pack2(x[2], x[3]);
     }
-    if (EPI == B200_EPI_SWIGLU) {
-      uint2 o;
-      o.x = pack2(silu_f(x[0]) * x[1], silu_f(x[2]) * x[3]);
-      o.y = pack2(silu_f(x[4]) * x[5], silu_f(x[6]) * x[7]);
-      *reinterpret_cast<uint2*>(p.C + tok * p.ldc + c / 2) = o;
+    __nv_bfloat16* out = p.C + tok * p.ldc + (kSwiglu ? c0 / 2 : c0);
+    if (whole) {
+      store_32(out, o);
+    } else if (kSwiglu) {  // a pair of 8-byte halves for each 16 columns
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + 8 * i < u.feat_lim) *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(o.w[2 * i], o.w[2 * i + 1]);
     } else {
-      *reinterpret_cast<uint4*>(p.C + tok * p.ldc + c) = pack8(x);
+      *reinterpret_cast<uint4*>(out) = make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
+      if (c0 + 8 < u.feat_lim) *reinterpret_cast<uint4*>(out + 8) = make_uint4(o.w[4], o.w[5], o.w[6], o.w[7]);
     }
   }
 }
 
-template <int EPI, bool GROUPED>
+// MODE: kPlain, kRows (grouped, tokens on the M side) or kCols (grouped, tokens on the N side).
+constexpr int kPlain = 0, kRows = 1, kCols = 2;
+template <int EPI, int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const Params p) {
+  constexpr bool GROUPED = MODE != kPlain, COLS = MODE == kCols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -222,7 +342,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tma_prefetch_desc(&tmB);
   }
   pdl_wait();
-  if (GROUPED && warp == 0 && lane == 0) fill_group_table<kPairTile>(gtab, p);
+  if (GROUPED && warp == 0) fill_group_table<kPairTile>(gtab, p, lane);
   if (warp == 1) tmem_alloc_pair(tmem_slot, 2 * kPairTile);
   tc_fence_before();
   cluster_sync();  // both CTAs' barriers are ready, and both have their TMEM
@@ -252,16 +372,22 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       for (int w = pair; w < units && !*abort_flag; w += pairs) {
         const Unit u = unit_at(w);
+        // rows of this CTA's half of both operands
+        const int a_row = (COLS ? u.wrow0 : u.tok0) + rank * BM;
+        const int b_row = COLS ? u.tok0 + rank * (u.n / 2) : u.wrow0 + rank * BM;
+        const int boxes = COLS ? (u.n / 2 + kTokBox - 1) / kTokBox : 1;
+        constexpr int box_bytes = (COLS ? kTokBox : BM) * BK;
         for (int kb = 0; kb < p.kb_total; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
             *abort_flag = 1;
             break;
           }
           // the leader expects both CTAs' bytes; the other's may land first
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kPairStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * (BM * BK + boxes * box_bytes));
           const uint32_t bar = cluster_map(smem_u32(&full[stage]), 0);
-          tma_load_2d_pair(sA + stage * BM * BK, &tmA, bar, kb * BK, u.tok0 + rank * BM);
-          tma_load_2d_pair(sB + stage * BM * BK, &tmB, bar, kb * BK, u.wrow0 + rank * BM);
+          tma_load_2d_pair(sA + stage * BM * BK, &tmA, bar, kb * BK, a_row);
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d_pair(sB + stage * BM * BK + i * box_bytes, &tmB, bar, kb * BK, b_row + i * kTokBox);
           if (++stage == kPairStages) {
             stage = 0;
             phase ^= 1;
@@ -276,6 +402,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
+      int next_n = COLS && pair < units ? unit_at(pair).n : kPairTile;
       for (int w = pair; w < units && !*abort_flag; w += pairs, ++local) {
         const int acc = local & 1;
         if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err)) {
@@ -283,6 +410,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           break;
         }
         tc_fence_after();
+        const uint32_t idesc = idesc_i8_s32(256, next_n);
         bool ok = true;
         for (int kb = 0; kb < p.kb_total; ++kb) {
           if (!mbar_wait(&full[stage], phase, p.err)) {
@@ -295,8 +423,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
             umma_i8_pair(tmem_base + acc * kPairTile, smem_desc_k128(a0 + k * 32), smem_desc_k128(b0 + k * 32),
-                         kPairIdesc, (kb > 0 || k > 0) ? 1u : 0u);
+                         idesc, (kb > 0 || k > 0) ? 1u : 0u);
           umma_commit_pair(&empty[stage]);
+          // the next tile's extent is looked up while this one's products run
+          if (COLS && kb == 0 && w + pairs < units) next_n = unit_at(w + pairs).n;
           if (++stage == kPairStages) {
             stage = 0;
             phase ^= 1;
@@ -311,51 +441,104 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else {
-    // ---------------- epilogue: 32 token rows x 128 columns a warp ----------------
+    // ---------------- epilogue ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
     const int half = (warp - 2) >> 2;
     float* cscale = cols + (warp - 2) * 256;
     float* cbias = cscale + 128;
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.R)) & 31) == 0 &&
+                      p.ldc % 16 == 0 && (!has_residual(EPI) || p.ldr % 16 == 0);
+    // what a unit's epilogue reads besides its sums is loaded a unit ahead
+    struct Ahead {
+      Unit u;
+      float lane_scale;  // this lane's row: token (feature with COLS)
+      float4 scale, bias;  // four columns' (COLS: a token's of each of the warp's chunks)
+    };
+    const auto ahead = [&](int w) {
+      Ahead n;
+      n.u = unit_at(w);
+      n.lane_scale = 0.f;
+      n.scale = n.bias = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int r = rank * BM + q * 32 + lane;
+      if (COLS) {
+        if (n.u.feat0 + r < n.u.feat_lim) n.lane_scale = p.row_scale[n.u.wrow0 + r];
+        float* ts = &n.scale.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = n.u.tok0 + (2 * i + half) * 32 + lane;
+          if (tok < n.u.tok_lim) ts[i] = p.col_scale[tok];
+        }
+        return n;
+      }
+      if (n.u.tok0 + r < n.u.tok_lim) n.lane_scale = p.row_scale[n.u.tok0 + r];
+      const int c4 = half * 128 + lane * 4;
+      if (n.u.feat0 + c4 < n.u.feat_lim) {
+        n.scale = *reinterpret_cast<const float4*>(p.col_scale + n.u.wrow0 + c4);
+        if (has_bias(EPI)) add4(&n.bias.x, p.bias + n.u.feat0 + c4);
+      }
+      return n;
+    };
+    Ahead next;
+    if (pair < units) next = ahead(pair);
     int local = 0;
     for (int w = pair; w < units && !*abort_flag; w += pairs, ++local) {
-      const Unit u = unit_at(w);
-      const int acc = local & 1;
-      const int64_t tok = u.tok0 + rank * BM + q * 32 + lane;
-      const bool live = tok < u.tok_lim;
-      const float rscale = live ? p.row_scale[tok] : 0.f;
-      const int c4 = half * 128 + lane * 4;
+      const Unit u = next.u;
+      const float lane_scale = next.lane_scale;
       __syncwarp();
-      if (u.feat0 + c4 < u.feat_lim) {
-        *reinterpret_cast<float4*>(cscale + lane * 4) = *reinterpret_cast<const float4*>(p.col_scale + u.wrow0 + c4);
-        if (has_bias(EPI)) {
-          float b[4] = {0.f, 0.f, 0.f, 0.f};
-          add4(b, p.bias + u.feat0 + c4);
-          *reinterpret_cast<float4*>(cbias + lane * 4) = make_float4(b[0], b[1], b[2], b[3]);
-        }
+      if (COLS) {
+        cscale[lane] = next.scale.x, cscale[32 + lane] = next.scale.y;
+        cscale[64 + lane] = next.scale.z, cscale[96 + lane] = next.scale.w;
+      } else {
+        *reinterpret_cast<float4*>(cscale + lane * 4) = next.scale;
+        if (has_bias(EPI)) *reinterpret_cast<float4*>(cbias + lane * 4) = next.bias;
       }
       __syncwarp();
+      if (w + pairs < units) next = ahead(w + pairs);
+      const int acc = local & 1;
+      const uint32_t freed = cluster_map(smem_u32(&tempty[acc]), 0);
+      const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kPairTile;
       if (!mbar_wait(&tfull[acc], (local >> 1) & 1, p.err)) {
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
-      const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kPairTile + half * 128;
-      uint32_t r[2][32];
-      tmem_ld_32x32b_x32(t, r[0]);
-#pragma unroll
-      for (int ch = 0; ch < 4; ++ch) {
-        tmem_ld_wait();
-        if (ch < 3) {
-          tmem_ld_32x32b_x32(t + (ch + 1) * 32, r[(ch + 1) & 1]);
-        } else {
-          // all read: the accumulator is free for the tile after next
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) cluster_arrive(cluster_map(smem_u32(&tempty[acc]), 0));
+      if constexpr (COLS) {
+        // 32 features a warp, every second chunk of 32 tokens
+        for (int c = half; c < u.n / 32; c += 2) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(t0 + c * 32, r);
+          tmem_ld_wait();
+          if (c + 2 >= u.n / 32) {  // all read: the accumulator is free for the tile after next
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) cluster_arrive_relaxed(freed);
+          }
+          emit_features<EPI, 32>(r, u.feat0 + rank * BM + q * 32, u.tok0 + c * 32, lane_scale, cscale + (c >> 1) * 32, u,
+                                 lane, p);
         }
-        if (live)
-          emit_row<EPI>(r[ch & 1], tok, u.feat0 + half * 128 + ch * 32, rscale, cscale + ch * 32, cbias + ch * 32, u, p);
-        __syncwarp();
+        if (half >= u.n / 32 && lane == 0) cluster_arrive_relaxed(freed);  // nothing of this tile is this warp's
+      } else {
+        // 32 token rows x 128 columns a warp
+        const int64_t tok = u.tok0 + rank * BM + q * 32 + lane;
+        const bool live = tok < u.tok_lim;
+        const uint32_t t = t0 + half * 128;
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(t, r[0]);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          tmem_ld_wait();
+          if (ch < 3) {
+            tmem_ld_32x32b_x32(t + (ch + 1) * 32, r[(ch + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) cluster_arrive_relaxed(freed);
+          }
+          if (live)
+            emit_row<EPI>(r[ch & 1], tok, u.feat0 + half * 128 + ch * 32, lane_scale, cscale + ch * 32, cbias + ch * 32, wide,
+                          u, p);
+          __syncwarp();
+        }
       }
     }
   }
@@ -380,37 +563,9 @@ struct GroupCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = 200 * 1024 / STAGE_BYTES;
   static constexpr int TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/ + kGroupTabBytes;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/ + 16 * BN /*token scales*/ + kGroupTabBytes;
   static constexpr uint32_t IDESC = idesc_i8_s32(BM, BN);
 };
-
-// 32 accumulator columns (tokens) of one feature row.
-template <int EPI>
-__device__ __forceinline__ void emit_feature(const uint32_t acc[32], int row, int tok0, float rscale, const Unit& u, int lane,
-                                             const Params& p) {
-  const int feat = u.feat0 + row;
-  float v[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = (float)(int)acc[i] * rscale * (tok0 + i < u.tok_lim ? p.col_scale[tok0 + i] : 0.f);
-  if (EPI == B200_EPI_SWIGLU) {
-    // lanes 2j / 2j+1 hold the gate / up rows of feature j: the even lane
-    // finishes the first half of the chunk's tokens, the odd lane the second
-    const bool odd = lane & 1;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[16 + i], 1);
-      const int64_t tok = tok0 + (odd ? 16 + i : i);
-      const float o = odd ? silu_f(other) * v[16 + i] : silu_f(v[i]) * other;
-      if (feat < u.feat_lim && tok < u.tok_lim) p.C[tok * p.ldc + (feat >> 1)] = f2bf(o);
-    }
-  } else if (feat < u.feat_lim) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int64_t tok = tok0 + i;
-      if (tok < u.tok_lim) p.C[tok * p.ldc + feat] = f2bf(v[i]);
-    }
-  }
-}
 
 template <int BN, int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -426,7 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tempty = tfull + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* gtab = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE_BYTES + 512);
+  float* tscale = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + 512);  // of the tokens, per warp
+  int* gtab = reinterpret_cast<int*>(tscale + 4 * BN);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -445,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmB);
   }
   pdl_wait();
-  if (warp == 0 && lane == 0) fill_group_table<BN>(gtab, p);
+  if (warp == 0) fill_group_table<BN>(gtab, p, lane);
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM_COLS);
     tmem_relinquish();
@@ -523,23 +679,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------- epilogue (warps 2..5) ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const int rit = q * 32 + lane;
+    float* ts = tscale + q * BN;
     int local = 0;
     for (int w = blockIdx.x; w < units && !*abort_flag; w += gridDim.x, ++local) {
       const Unit u = group_unit<BN, BM>(w, p, gtab);
       const int acc = local & 1;
-      const float rscale = u.feat0 + rit < u.feat_lim ? p.row_scale[u.wrow0 + rit] : 0.f;
+      const float fscale = u.feat0 + q * 32 + lane < u.feat_lim ? p.row_scale[u.wrow0 + q * 32 + lane] : 0.f;
+      __syncwarp();
+      for (int i = lane; i < BN; i += 32) ts[i] = u.tok0 + i < u.tok_lim ? p.col_scale[u.tok0 + i] : 0.f;
+      __syncwarp();
       if (!mbar_wait(&tfull[acc], (local >> 1) & 1, p.err)) {
         *abort_flag = 1;
         break;
       }
       tc_fence_after();
+      constexpr int CW = BN < 32 ? BN : 32;
 #pragma unroll 1
-      for (int ch = 0; ch < BN / 32 && u.tok0 + ch * 32 < u.tok_lim; ++ch) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + ch * 32, r);
+      for (int c = 0; c < BN && u.tok0 + c < u.tok_lim; c += CW) {
+        uint32_t r[CW];
+        const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN + c;
+        if constexpr (CW == 32) tmem_ld_32x32b_x32(t, r);
+        else tmem_ld_32x32b_x16(t, r);
         tmem_ld_wait();
-        emit_feature<EPI>(r, rit, u.tok0 + ch * 32, rscale, u, lane, p);
+        emit_features<EPI, CW>(r, u.feat0 + q * 32, u.tok0 + c, fscale, ts + c, u, lane, p);
       }
       tc_fence_before();
       mbar_arrive(&tempty[acc]);
@@ -820,13 +982,13 @@ bool allow_smem(Kernel k, int bytes, bool (&done)[64]) {
   return true;
 }
 
-template <int EPI, bool GROUPED>
-int launch_pair(const CUtensorMap& tok, const CUtensorMap& w, const Params& p, int64_t units, cudaStream_t st) {
-  auto k = gemm_i8_pair_kernel<EPI, GROUPED>;
+template <int EPI, int MODE>
+int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t units, cudaStream_t st) {
+  auto k = gemm_i8_pair_kernel<EPI, MODE>;
   static bool done[64] = {false};
   if (!allow_smem(k, kPairSmem, done)) return B200_ERROR_UNSUPPORTED;
   const int pairs = (int)std::min<int64_t>(units, num_sms() / 2);
-  launch_clusters(k, 2, dim3(2 * pairs), kPairThreads, kPairSmem, st, tok, w, p);
+  launch_clusters(k, 2, dim3(2 * pairs), kPairThreads, kPairSmem, st, a, b, p);
   B200_CHECK_LAUNCH();
   return B200_OK;
 }
@@ -851,6 +1013,19 @@ int launch_group(const CUtensorMap& tok, const CUtensorMap& w, const Params& p, 
   return B200_OK;
 }
 
+// form: the token tile of the single-CTA form, or one of the pairs' two.
+constexpr int kFormCols = 0, kFormRows = 1;
+template <int EPI>
+int launch_grouped(int form, const CUtensorMap& tok, const CUtensorMap& w, const Params& p, int64_t units, cudaStream_t st) {
+  switch (form) {
+    case 16: return launch_group<16, EPI>(tok, w, p, units, st);
+    case 32: return launch_group<32, EPI>(tok, w, p, units, st);
+    case 64: return launch_group<64, EPI>(tok, w, p, units, st);
+    case kFormCols: return launch_pair<EPI, kCols>(w, tok, p, units, st);
+    default: return launch_pair<EPI, kRows>(tok, w, p, units, st);
+  }
+}
+
 // bn: the token tile of the split form, 0 for CTA pairs.
 template <int EPI>
 int launch_plain(int bn, int splits, const CUtensorMap& tok, const CUtensorMap& w, const Params& p, cudaStream_t st) {
@@ -859,7 +1034,7 @@ int launch_plain(int bn, int splits, const CUtensorMap& tok, const CUtensorMap& 
     case 32: return launch_split<32, EPI>(tok, w, p, splits, st);
     case 64: return launch_split<64, EPI>(tok, w, p, splits, st);
     case 128: return launch_split<128, EPI>(tok, w, p, splits, st);
-    default: return launch_pair<EPI, false>(tok, w, p, (int64_t)p.tiles_m * p.tiles_n, st);
+    default: return launch_pair<EPI, kPlain>(tok, w, p, (int64_t)p.tiles_m * p.tiles_n, st);
   }
 }
 
@@ -961,14 +1136,20 @@ extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float*
   if (rows > INT32_MAX / 4 || N > INT32_MAX / 4 || groups * N > INT32_MAX / 4 || K > kMaxK)
     return B200_ERROR_UNSUPPORTED;
   if (rows == 0) return B200_OK;
-  // Few tokens per group (decode): weights on the 128-row side, up to 64 of a
-  // group's tokens on the N side.
-  const bool few = rows <= 96LL * groups;
-  const int feat_tile = few ? BM : kPairTile, tok_tile = few ? 64 : kPairTile;
+  // By the average tokens of a group: up to 56, single CTAs with weights on the
+  // 128-row side and up to bn tokens on the N side (bn leaves room for a group of
+  // twice the average, past which its weights are read, from L2, again); up to
+  // 160, pairs with the tokens on the N side; beyond, pairs with the tokens on
+  // the M side, whose epilogue costs the main loop less.  64 groups of 2816 x
+  // 2048 with SwiGLU, us: at 48 tokens 65 / 72 / -, at 64 79 / 74 / 82, at 128
+  // 128 / 80 / 84, at 192 - / 88 / 87, at 768 - / 276 / 258.
+  const bool few = rows <= 56LL * groups, cols = !few && rows <= 160LL * groups;
+  const int bn = rows <= 8LL * groups ? 16 : rows <= 16LL * groups ? 32 : 64;
+  const int feat_tile = few ? BM : kPairTile, tok_tile = few ? bn : kPairTile;
   Params p{};
   p.kb_total = (int)((K + BK - 1) / BK);
-  p.row_scale = few ? b_scale : a_scale;
-  p.col_scale = few ? a_scale : b_scale;
+  p.row_scale = few || cols ? b_scale : a_scale;
+  p.col_scale = few || cols ? a_scale : b_scale;
   p.C = static_cast<__nv_bfloat16*>(C);
   p.ldc = ldc;
   p.err = b200::error_word(current_device());
@@ -981,11 +1162,10 @@ extern "C" int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float*
   const int64_t max_units = ((rows + tok_tile - 1) / tok_tile + groups) * (int64_t)p.gF;
   if (max_units > INT32_MAX / 2) return B200_ERROR_UNSUPPORTED;
   CUtensorMap w, tok;
-  if (!make_tmap(&w, B, (int64_t)groups * N, K, ldb, BM) || !make_tmap(&tok, A, rows, K, lda, few ? 64 : BM))
+  if (!make_tmap(&w, B, (int64_t)groups * N, K, ldb, BM) ||
+      !make_tmap(&tok, A, rows, K, lda, few ? bn : cols ? kTokBox : BM))
     return B200_ERROR_UNSUPPORTED;
-  if (few)
-    return epilogue == B200_EPI_SWIGLU ? launch_group<64, B200_EPI_SWIGLU>(tok, w, p, max_units, stream)
-                                       : launch_group<64, B200_EPI_NONE>(tok, w, p, max_units, stream);
-  return epilogue == B200_EPI_SWIGLU ? launch_pair<B200_EPI_SWIGLU, true>(tok, w, p, max_units, stream)
-                                     : launch_pair<B200_EPI_NONE, true>(tok, w, p, max_units, stream);
+  const int form = few ? bn : cols ? kFormCols : kFormRows;
+  return epilogue == B200_EPI_SWIGLU ? launch_grouped<B200_EPI_SWIGLU>(form, tok, w, p, max_units, stream)
+                                     : launch_grouped<B200_EPI_NONE>(form, tok, w, p, max_units, stream);
 }
