@@ -227,9 +227,12 @@ constexpr int kPairTile = 256;
 constexpr int kPairGroup = 8;  // token tiles walked per feature tile
 constexpr int kPairStages = 6;
 constexpr int kPairEpiWarps = 8;
+constexpr int kParts = kPairEpiWarps / 4;         // warps over the columns (the four TMEM lane quarters over the rows)
+constexpr int kPartCols = kPairTile / kParts;
+constexpr int kPartChunks = kPartCols / 32;
 constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
 constexpr int kPairStageBytes = 2 * BM * BK;  // of each CTA
-constexpr int kPairColBytes = kPairEpiWarps * 128 * 2 * 4;  // column scales and biases of each epilogue warp
+constexpr int kPairColBytes = kPairEpiWarps * kPartCols * 2 * 4;  // column scales and biases of each epilogue warp
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024 /*align*/ + 256 /*barriers*/ + kPairColBytes + kGroupTabBytes;
 constexpr int kTokBox = 64;  // token rows of one TMA box of a grouped launch
 
@@ -443,38 +446,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   } else {
     // ---------------- epilogue ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const int half = (warp - 2) >> 2;
-    float* cscale = cols + (warp - 2) * 256;
-    float* cbias = cscale + 128;
+    const int part = (warp - 2) >> 2;
+    float* cscale = cols + (warp - 2) * 2 * kPartCols;
+    float* cbias = cscale + kPartCols;
     const bool wide = ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.R)) & 31) == 0 &&
                       p.ldc % 16 == 0 && (!has_residual(EPI) || p.ldr % 16 == 0);
     // what a unit's epilogue reads besides its sums is loaded a unit ahead
     struct Ahead {
       Unit u;
-      float lane_scale;  // this lane's row: token (feature with COLS)
-      float4 scale, bias;  // four columns' (COLS: a token's of each of the warp's chunks)
+      float lane_scale;                              // this lane's row: token (feature with COLS)
+      float scale[kPartChunks], bias[kPartChunks];   // column 32 i + lane of the warp's
     };
     const auto ahead = [&](int w) {
       Ahead n;
       n.u = unit_at(w);
       n.lane_scale = 0.f;
-      n.scale = n.bias = make_float4(0.f, 0.f, 0.f, 0.f);
       const int r = rank * BM + q * 32 + lane;
-      if (COLS) {
-        if (n.u.feat0 + r < n.u.feat_lim) n.lane_scale = p.row_scale[n.u.wrow0 + r];
-        float* ts = &n.scale.x;
+      if (COLS ? n.u.feat0 + r < n.u.feat_lim : n.u.tok0 + r < n.u.tok_lim)
+        n.lane_scale = p.row_scale[(COLS ? n.u.wrow0 : n.u.tok0) + r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = n.u.tok0 + (2 * i + half) * 32 + lane;
-          if (tok < n.u.tok_lim) ts[i] = p.col_scale[tok];
-        }
-        return n;
-      }
-      if (n.u.tok0 + r < n.u.tok_lim) n.lane_scale = p.row_scale[n.u.tok0 + r];
-      const int c4 = half * 128 + lane * 4;
-      if (n.u.feat0 + c4 < n.u.feat_lim) {
-        n.scale = *reinterpret_cast<const float4*>(p.col_scale + n.u.wrow0 + c4);
-        if (has_bias(EPI)) add4(&n.bias.x, p.bias + n.u.feat0 + c4);
+      for (int i = 0; i < kPartChunks; ++i) {
+        // with COLS a warp takes every kParts-th chunk, so that short tiles spread over the warps
+        const int c = (COLS ? (i * kParts + part) * 32 : part * kPartCols + i * 32) + lane;
+        const bool in = COLS ? n.u.tok0 + c < n.u.tok_lim : n.u.feat0 + c < n.u.feat_lim;
+        n.scale[i] = in ? p.col_scale[(COLS ? n.u.tok0 : n.u.wrow0) + c] : 0.f;
+        n.bias[i] = has_bias(EPI) && in ? bf2f(p.bias[n.u.feat0 + c]) : 0.f;
       }
       return n;
     };
@@ -485,12 +481,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const Unit u = next.u;
       const float lane_scale = next.lane_scale;
       __syncwarp();
-      if (COLS) {
-        cscale[lane] = next.scale.x, cscale[32 + lane] = next.scale.y;
-        cscale[64 + lane] = next.scale.z, cscale[96 + lane] = next.scale.w;
-      } else {
-        *reinterpret_cast<float4*>(cscale + lane * 4) = next.scale;
-        if (has_bias(EPI)) *reinterpret_cast<float4*>(cbias + lane * 4) = next.bias;
+#pragma unroll
+      for (int i = 0; i < kPartChunks; ++i) {
+        cscale[i * 32 + lane] = next.scale[i];
+        if (has_bias(EPI)) cbias[i * 32 + lane] = next.bias[i];
       }
       __syncwarp();
       if (w + pairs < units) next = ahead(w + pairs);
@@ -503,40 +497,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_fence_after();
       if constexpr (COLS) {
-        // 32 features a warp, every second chunk of 32 tokens
-        for (int c = half; c < u.n / 32; c += 2) {
+        // 32 features a warp
+        for (int c = part; c < u.n / 32; c += kParts) {
           uint32_t r[32];
           tmem_ld_32x32b_x32(t0 + c * 32, r);
           tmem_ld_wait();
-          if (c + 2 >= u.n / 32) {  // all read: the accumulator is free for the tile after next
+          if (c + kParts >= u.n / 32) {  // all read: the accumulator is free for the tile after next
             tc_fence_before();
             __syncwarp();
             if (lane == 0) cluster_arrive_relaxed(freed);
           }
-          emit_features<EPI, 32>(r, u.feat0 + rank * BM + q * 32, u.tok0 + c * 32, lane_scale, cscale + (c >> 1) * 32, u,
+          emit_features<EPI, 32>(r, u.feat0 + rank * BM + q * 32, u.tok0 + c * 32, lane_scale, cscale + c / kParts * 32, u,
                                  lane, p);
         }
-        if (half >= u.n / 32 && lane == 0) cluster_arrive_relaxed(freed);  // nothing of this tile is this warp's
+        if (part >= u.n / 32 && lane == 0) cluster_arrive_relaxed(freed);  // nothing of this tile is this warp's
       } else {
-        // 32 token rows x 128 columns a warp
+        // 32 token rows a warp
         const int64_t tok = u.tok0 + rank * BM + q * 32 + lane;
         const bool live = tok < u.tok_lim;
-        const uint32_t t = t0 + half * 128;
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(t, r[0]);
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
+        for (int ch = 0; ch < kPartChunks; ++ch) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(t0 + part * kPartCols + ch * 32, r);
           tmem_ld_wait();
-          if (ch < 3) {
-            tmem_ld_32x32b_x32(t + (ch + 1) * 32, r[(ch + 1) & 1]);
-          } else {
+          if (ch == kPartChunks - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) cluster_arrive_relaxed(freed);
           }
           if (live)
-            emit_row<EPI>(r[ch & 1], tok, u.feat0 + half * 128 + ch * 32, lane_scale, cscale + ch * 32, cbias + ch * 32, wide,
-                          u, p);
+            emit_row<EPI>(r, tok, u.feat0 + part * kPartCols + ch * 32, lane_scale, cscale + ch * 32, cbias + ch * 32, wide, u,
+                          p);
           __syncwarp();
         }
       }
@@ -1053,9 +1044,13 @@ int plan_splits(int tiles, int kb_total) {
   return s;
 }
 
-// CTA pairs once their 256 x 256 tiles fill the SMs; a narrow N would waste the tile.
+// CTA pairs once their 256 x 256 tiles keep five eighths of them busy (a narrow
+// M or N would waste the tile), us split / pairs: 512 x 6144 x 4096 (48 tiles)
+// 18.2 / 17.3, 512 x 4096 x 4096 (32) 14.8 / 18.6, 777 x 4096 x 1024 (64) 11.7 /
+// 10.7, 2048 x 4096 x 4096 (128) 41 / 31, 1024 x 24576 x 4096 (384) 132 / 75.
 bool use_pairs(int64_t M, int64_t N, int sms) {
-  return M > 128 && N > 128 && ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile) * 2 >= sms;
+  const int64_t tiles = ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile);
+  return M > 128 && N > 128 && tiles * 8 >= sms / 2 * 5;
 }
 
 // The checks that the plain and the grouped call share.
