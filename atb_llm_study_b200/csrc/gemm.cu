@@ -861,6 +861,25 @@ int gemm_launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* Cp
   return rc;
 }
 
+int gemm_f32_launch(const void* A, int64_t lda, const void* B, int64_t ldb, float* out, int64_t M, int64_t N, int64_t K,
+                    cudaStream_t st) {
+  GemmPlan g = plan_gemm(M, N, K, B200_EPI_NONE, num_sms());
+  g.splits = 1;
+  g.kb_per_split = g.kb_total;
+  Params p = make_params(g, M, N, K, nullptr, 0, nullptr, nullptr, 0, nullptr);
+  p.ws = out;  // the one "partial" tile set is the product
+  CUtensorMap ta, tb;
+  if (!make_tmap(&ta, g.swap ? B : A, p.rows, K, g.swap ? ldb : lda, BM) ||
+      !make_tmap(&tb, g.swap ? A : B, p.cols, K, g.swap ? lda : ldb, g.bn))
+    return B200_ERROR_UNSUPPORTED;
+  const int grid = std::min(g.tiles_m * g.tiles_n, num_sms());
+  if (!g.swap)
+    return g.bn == 256 ? launch_epi<256, false, true>(B200_EPI_NONE, ta, tb, p, grid, st)
+                       : launch_epi<128, false, true>(B200_EPI_NONE, ta, tb, p, grid, st);
+  return g.bn == 128 ? launch_epi<128, true, true>(B200_EPI_NONE, ta, tb, p, grid, st)
+                     : launch_epi<64, true, true>(B200_EPI_NONE, ta, tb, p, grid, st);
+}
+
 int splitk_reduce(const float* ws, int splits, int64_t M, int64_t N, int epi, const void* bias, const void* R,
                   int64_t ldr, void* Cp, int64_t ldc, cudaStream_t st) {
   GemmPlan g;

@@ -33,6 +33,11 @@ int gemm_launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
                 cudaStream_t stream, int* splits_out, const void* prefetch = nullptr, int64_t prefetch_bytes = 0,
                 int* sk_flags = nullptr, int sk_flag_count = 0);
 
+// out[M, N] (fp32, dense) = A B^T, the whole K in one pass: logits that are
+// compared, not stored.  The caller has checked what b200_gemm_bf16 would.
+int gemm_f32_launch(const void* A, int64_t lda, const void* B, int64_t ldb, float* out, int64_t M, int64_t N, int64_t K,
+                    cudaStream_t stream);
+
 // C[M, N'] = epilogue(sum_s ws[s][M][N]).
 int splitk_reduce(const float* ws, int splits, int64_t M, int64_t N, int epilogue, const void* bias, const void* R,
                   int64_t ldr, void* C, int64_t ldc, cudaStream_t stream);

@@ -12,6 +12,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "gemm.h"
 
 using namespace b200;
 
@@ -389,6 +390,12 @@ __global__ void moe_gate_logits_kernel(const __nv_bfloat16* __restrict__ x, int6
   if (lane == 0) logits[t * E + e] = acc;
 }
 
+// Up to so many logits a warp for each gives them sooner than tensor core tiles,
+// whose few CTAs walk the whole hidden width (us, warps / tiles: 32 x 256 over
+// 7168 34 / 39, 64 x 256 60 / 40, 64 x 64 over 2048 11.6 / 15.8, 256 x 64 20 /
+// 15, 16384 x 256 3878 / 37 with the selection).
+constexpr int64_t kWarpLogits = 8192;
+
 int route_launch(const void* x, int64_t ldx, const void* wg, const float* logits_in, int64_t T, int64_t H, int E,
                  int k, int renorm, float scale, int32_t* ids, float* wts, float* logits_out, cudaStream_t st) {
   auto xb = static_cast<const __nv_bfloat16*>(x);
@@ -436,6 +443,32 @@ extern "C" int b200_moe_route(const void* x, int64_t ldx, const void* gate_weigh
   if (T == 0) return B200_OK;
   return route_launch(x, ldx, gate_weight, nullptr, T, H, num_experts, top_k, renormalize, scale, topk_ids,
                       topk_weights, logits, stream);
+}
+
+extern "C" int b200_moe_route_grouped(const void* x, int64_t ldx, const void* gate_weight, const float* bias, int64_t T,
+                                      int64_t H, int num_experts, int top_k, int scoring, int num_groups,
+                                      int topk_groups, int group_top, int renormalize, float scale,
+                                      int32_t* topk_ids, float* topk_weights, float* logits, b200_stream_t stream) {
+  if (!x || !gate_weight || !logits || T < 0 || H <= 0 || H % 8 || ldx < H || ldx % 8 || !aligned16(x) ||
+      !aligned16(gate_weight) || !aligned16(logits))
+    return B200_ERROR_INVALID_PARAM;
+  // the selection's own checks, with nothing to select
+  int rc = b200_moe_topk_grouped(logits, num_experts, bias, 0, num_experts, top_k, scoring, num_groups,
+                                 topk_groups, group_top, renormalize, scale, topk_ids, topk_weights, stream);
+  if (rc != B200_OK || T == 0) return rc;
+  if (T > INT32_MAX / kMaxExperts || H > INT32_MAX / 2) return B200_ERROR_UNSUPPORTED;
+  if (num_experts % 4 == 0 && T * num_experts > kWarpLogits) {  // (the tiles' fp32 rows are stored in fours)
+    rc = b200::gemm_f32_launch(x, ldx, gate_weight, H, logits, T, num_experts, H, stream);
+    if (rc != B200_OK) return rc;
+  } else {
+    const int64_t warps = T * num_experts;
+    launch_kernel(moe_gate_logits_kernel, dim3((unsigned)((warps * 32 + 255) / 256)), 256, 0, stream,
+                  static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(gate_weight), T, H,
+                  num_experts, logits);
+    B200_CHECK_LAUNCH();
+  }
+  return b200_moe_topk_grouped(logits, num_experts, bias, T, num_experts, top_k, scoring, num_groups, topk_groups,
+                               group_top, renormalize, scale, topk_ids, topk_weights, stream);
 }
 
 extern "C" int b200_moe_topk(const float* logits, int64_t T, int num_experts, int top_k, int renormalize, float scale,

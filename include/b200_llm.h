@@ -289,6 +289,14 @@ B200_API int b200_moe_topk_grouped(const float* logits, int64_t ld, const float*
                                    int renormalize, float scale, int32_t* topk_ids, float* topk_weights,
                                    b200_stream_t stream);
 
+/* b200_moe_topk_grouped of the logits x [T, H] (bf16, row stride ldx) .
+ * gate_weight [E, H]^T, computed in fp32 into logits [T, E] (required; 16-byte
+ * aligned, as x and gate_weight), for up to 256 experts. */
+B200_API int b200_moe_route_grouped(const void* x, int64_t ldx, const void* gate_weight, const float* bias, int64_t T,
+                                    int64_t H, int num_experts, int top_k, int scoring, int num_groups,
+                                    int topk_groups, int group_top, int renormalize, float scale,
+                                    int32_t* topk_ids, float* topk_weights, float* logits, b200_stream_t stream);
+
 /* Expert permutation of the T*top_k (token, choice) entries: entry i = t*top_k
  * + j goes to slot perm_pos[i] = expert_offsets[e] + (entries of expert e
  * before i), so each expert's slots hold its tokens in token order

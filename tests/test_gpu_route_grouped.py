@@ -128,3 +128,30 @@ def test_matches_the_ungrouped_selection():
     G.check(G.L().b200_moe_topk(d.data_ptr(), 500, 64, 6, 0, 1.5, i2.data_ptr(), w2.data_ptr(), G.stream()))
     np.testing.assert_array_equal(ids, i2.cpu().numpy())
     np.testing.assert_allclose(w, G.host(w2), rtol=1e-5, atol=2e-6)
+
+
+@pytest.mark.parametrize("T,E,H,pad", [(1, 64, 2048, 0), (5, 7, 64, 8), (200, 60, 512, 16), (130, 252, 1024, 0), (33, 256, 7168, 0),
+                                       (129, 255, 264, 0), (700, 256, 520, 8), (300, 8, 4096, 0), (3000, 160, 136, 0)])
+def test_route_from_hidden_states(T, E, H, pad):
+    """b200_moe_route_grouped: logits within fp32 accumulation of the float64 ones (H terms of two bf16 factors each,
+    2^-24 sqrt(H) of their sizes typically, 2^-24 H bounded), then the selection of those very logits."""
+    rng = np.random.default_rng(T + E)
+    x, wg = G.rounded(rng.standard_normal((T, H))), G.rounded(rng.standard_normal((E, H)) * 0.05)
+    groups = 4 if E % 4 == 0 and E >= 8 else 1
+    keep, best, k = max(1, groups // 2), 2 if groups > 1 else 1, min(6, max(1, E // 2))
+    bias = (rng.standard_normal(E) * 0.05).astype(F)
+    X = G.bf16(np.concatenate([x, np.full((T, pad), 1e30)], 1) if pad else x)
+    ids = torch.empty(T, k, dtype=torch.int32, device=G.DEV)
+    w = torch.empty(T, k, dtype=torch.float32, device=G.DEV)
+    lg = torch.full((T + 1, E), 7.0, dtype=torch.float32, device=G.DEV)
+    G.check(G.L().b200_moe_route_grouped(X.data_ptr(), H + pad, G.bf16(wg).data_ptr(), G.f32(bias).data_ptr(), T, H, E, k, 1,
+                                         groups, keep, best, 1, 2.0, ids.data_ptr(), w.data_ptr(), lg.data_ptr(), G.stream()))
+    got = G.host(lg)
+    assert (got[T] == 7).all()
+    ref = x.astype(np.float64) @ wg.astype(np.float64).T
+    size = np.abs(x.astype(np.float64)) @ np.abs(wg.astype(np.float64)).T
+    assert (np.abs(got[:T] - ref) <= 2.0**-24 * H * size + 1e-30).all()
+    rid, rw = moe.route_grouped(got[:T], k, True, bias, groups, keep, best, True, 2.0)
+    np.testing.assert_array_equal(ids.cpu().numpy(), rid)
+    np.testing.assert_allclose(G.host(w), rw, rtol=1e-5, atol=4e-6)
+    assert G.device_errors() == 0

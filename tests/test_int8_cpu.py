@@ -22,6 +22,9 @@ GROUPED = dict(A=P, lda=64, sa=P, B=P, ldb=64, sb=P, C=P, ldc=32, off=P, groups=
 TOPK = dict(logits=P, ld=64, bias=None, T=4, E=64, k=6, score=0, groups=8, keep=3, best=1, renorm=0, scale=1.0, ids=P,
             w=P, st=None)
 
+ROUTE = dict(x=P, ldx=64, gate=P, bias=None, T=4, H=64, E=64, k=6, score=0, groups=8, keep=3, best=1, renorm=0, scale=1.0,
+             ids=P, w=P, logits=P, st=None)
+
 REFUSED = [
     ("b200_quant_rows_int8", QUANT, [
         dict(x=None), dict(q=None), dict(scale=None), dict(rows=-1), dict(dim=0), dict(dim=24), dict(ldx=48), dict(ldx=65),
@@ -43,6 +46,9 @@ REFUSED = [
         dict(logits=None), dict(ids=None), dict(w=None), dict(T=-1), dict(E=0), dict(ld=63), dict(score=2), dict(score=-1),
         dict(groups=0), dict(groups=7), dict(keep=0), dict(keep=9), dict(best=0), dict(best=3), dict(groups=64, best=2),
         dict(k=0), dict(k=9), dict(keep=1, groups=16), dict(logits=P + 2), dict(bias=P + 1)]),
+    ("b200_moe_route_grouped", ROUTE, [
+        dict(x=None), dict(gate=None), dict(logits=None), dict(H=60), dict(ldx=56), dict(ldx=68), dict(x=P + 8),
+        dict(gate=P + 2), dict(logits=P + 4), dict(T=-1), dict(E=0), dict(groups=7), dict(k=9), dict(score=3)]),
 ]
 
 
@@ -63,6 +69,8 @@ def test_refused(name, base, change):
     ("b200_grouped_gemm_int8", GROUPED, dict(rows=1 << 30)),
     ("b200_moe_topk_grouped", TOPK, dict(E=264, ld=264)),
     ("b200_moe_topk_grouped", TOPK, dict(groups=64, keep=8)),
+    ("b200_moe_route_grouped", ROUTE, dict(E=264)),
+    ("b200_moe_route_grouped", ROUTE, dict(T=1 << 24)),
 ], ids=str)
 def test_unsupported(name, base, change):
     assert getattr(capi.lib(), name)(*{**base, **change}.values()) == UNSUPPORTED
@@ -72,7 +80,8 @@ def test_unsupported(name, base, change):
 @pytest.mark.parametrize("name,base,change", [
     ("b200_quant_rows_int8", QUANT, dict(rows=0)), ("b200_rmsnorm_quant_int8", NORM, dict(rows=0)),
     ("b200_gemm_int8", GEMM, dict(M=0)), ("b200_gemm_int8", GEMM, dict(N=0)),
-    ("b200_grouped_gemm_int8", GROUPED, dict(rows=0)), ("b200_moe_topk_grouped", TOPK, dict(T=0))], ids=str)
+    ("b200_grouped_gemm_int8", GROUPED, dict(rows=0)), ("b200_moe_topk_grouped", TOPK, dict(T=0)),
+    ("b200_moe_route_grouped", ROUTE, dict(T=0))], ids=str)
 def test_nothing_to_do(name, base, change):
     assert getattr(capi.lib(), name)(*{**base, **change}.values()) == 0
 
