@@ -120,18 +120,23 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // decision are nearer than the scores' error.
 //
 // What is compared carries a tag in its low bits, so one 32-bit maximum over
-// the warp gives value and place: 4 bits among experts (the place in the lane;
-// relative error 2^-19), 5 among groups (2^-18).  Two equal values are always
-// in doubt, so ties are settled in double, by index.
+// the warp gives value and place: log2(PER) bits among experts (the place in
+// the lane), 5 among groups.  Cutting b bits moves a value by less than 2^(b-23)
+// of itself.  Two equal values are always in doubt, so ties are settled in
+// double, by index.
 //
-// Error of a score, relative to the largest one (exp is the fast one, 2 +
-// 1.2 |x| ulp of e^x, which is at most 2 ulp of 1 for a softmax term and less
-// for a sigmoid): 2.4e-7, the sum of up to 256 terms (21 roundings and the
-// terms' own errors, 1.6e-6 where every term counts), the quotient 2.4e-7.
-// Below 2.5e-6; a difference of two 5e-6.
+// Error of a score (exp_fast: 2 + 1.2 |x| ulp of e^x).  Sigmoid: the quotient's
+// ulp, half an ulp of the sum 1 + e^-x, and the exponential's error times
+// s (1 - s), at most 0.6 ulp: 2.4e-7, a difference of two 5e-7.  Softmax, in
+// units of the largest score: the term's own 2 ulp of 1, the sum's 21 roundings
+// and its terms' errors (1.6e-6 where every term counts), the product: 2.5e-6, a
+// difference of two 5e-6.
 template <int PER>
 __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int lane) {
-  constexpr uint32_t kTag = 15u, kGroupTag = 31u;
+  constexpr int kTagBits = PER <= 1 ? 0 : PER <= 2 ? 1 : PER <= 4 ? 2 : PER <= 8 ? 3 : 4;
+  constexpr uint32_t kTag = (1u << kTagBits) - 1u, kGroupTag = 31u;
+  // 2^(bits - 23), and the half ulps of the two values compared
+  constexpr float kCut = (float)(1 << kTagBits) * 0x1p-23f + 1.2e-7f, kGroupCut = 0x1p-18f + 1.2e-7f;
   const Slot sl = slot_of<PER>(p, lane);
   const float* lg = p.logits + t * p.ld;
   float c[PER];
@@ -165,7 +170,7 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
       c[i] = fmaxf(s[i] + b[i], -FLT_MAX);
     }
   }
-  const float tol = by_score || pair_groups ? 5e-6f * top : 0.f;
+  const float tol = by_score || pair_groups ? (p.sigmoid ? 5e-7f : 5e-6f * top) : 0.f;
   bool in = true, clear = true;
   if (p.keep < p.G) {
     // the group's one or two largest, over its lanes
@@ -199,12 +204,12 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
     const float x = from_key(nth, kGroupTag);
     const float sz = __shfl_sync(0xffffffffu, size, (31 - (int)(nth & kGroupTag)) << p.lpg_shift);
     const float y = __shfl_down_sync(0xffffffffu, x, 1), sz1 = __shfl_down_sync(0xffffffffu, sz, 1);
-    const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 1e-6f * fmaxf(sz, sz1) + 8e-6f * fabsf(x) : 0.f);
+    const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 4e-7f * fmaxf(sz, sz1) + kGroupCut * fabsf(x) : 0.f);
     clear = __shfl_sync(0xffffffffu, (int)(x - y > near), p.keep - 1) != 0;
   }
   uint32_t key[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) key[i] = in && i < sl.n ? to_key(c[i], kTag, 15u - i) : 0u;
+  for (int i = 0; i < PER; ++i) key[i] = in && i < sl.n ? to_key(c[i], kTag, kTag - i) : 0u;
   sort_desc<PER>(key);
   uint32_t mine = 0;  // lane j: the j-th choice's key, and the lane that holds it
   int from_lane = 0;
@@ -225,7 +230,7 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
     // every choice against the next; a next that does not exist has key 0
     const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1);
     const float x = from_key(mine, kTag), y = from_key(next, kTag);
-    const bool apart = lane >= p.k || next == 0u || x - y > (by_score ? tol + 4e-6f * fabsf(x) : 0.f);
+    const bool apart = lane >= p.k || next == 0u || x - y > (by_score ? tol + kCut * fabsf(x) : 0.f);
     clear = clear && __all_sync(0xffffffffu, apart);
   }
   if (!clear) return false;
@@ -234,7 +239,7 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
   float w = 0.f;
   if (lane < p.k) {
     const Slot from = slot_of<PER>(p, from_lane);
-    e = from.e0 + 15 - (int)(mine & kTag);
+    e = from.e0 + (int)(kTag - (mine & kTag));
     const float x = clamp_logit(lg[e]);
     w = p.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - m) * inv;
   }
@@ -252,10 +257,15 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
   return true;
 }
 
-__device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+// Doubles as unsigned integers of the same order.
+__device__ __forceinline__ uint64_t to_key64(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ uint64_t warp_max64(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
 }
 
 // The choice on scores in double (experts without a bias by their logits).
@@ -270,10 +280,10 @@ __device__ __noinline__ void choose_exact(const RouteParams& p, int64_t t, int l
 #pragma unroll
     for (int i = 0; i < PER; ++i) s[i] = 1.0 / (1.0 + exp(-c[i]));
   } else {
-    double m = low;
+    float mf = -FLT_MAX;  // (logits are fp32 values)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) m = fmax(m, c[i]);
-    m = warp_max(m);
+    for (int i = 0; i < PER; ++i) mf = fmaxf(mf, (float)c[i]);
+    const double m = warp_max(mf);
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -282,8 +292,9 @@ __device__ __noinline__ void choose_exact(const RouteParams& p, int64_t t, int l
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum = 1.0 / sum;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] /= sum;
+    for (int i = 0; i < PER; ++i) s[i] *= sum;
   }
   if (p.bias) {
 #pragma unroll
@@ -314,26 +325,31 @@ __device__ __noinline__ void choose_exact(const RouteParams& p, int64_t t, int l
     }
     in = in && rank < p.keep;
   }
+  uint64_t key[PER];  // 0: not to be chosen (no value's key)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = in && i < sl.n ? to_key64(c[i]) : 0u;
   int mine = 0;  // lane j < k: the j-th choice
   double mine_s = 0.0, sum = 0.0;
-  unsigned taken = 0;
 #pragma unroll 1
   for (int j = 0; j < p.k; ++j) {
-    double bv = low, bs = 0.0;
-    int bi = -1;
+    uint64_t bk = key[0];
+    double bs = s[0];
+    int bi = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (in && i < sl.n && !(taken >> i & 1u) && (bi < 0 || c[i] > bv)) {
-        bv = c[i];
+    for (int i = 1; i < PER; ++i) {
+      if (key[i] > bk) {  // the first of equals
+        bk = key[i];
         bs = s[i];
         bi = i;
       }
     }
-    const double top = warp_max(bv);
-    const int from = __ffs(__ballot_sync(0xffffffffu, bi >= 0 && bv == top)) - 1;
+    const uint64_t top = warp_max64(bk);
+    const int from = __ffs(__ballot_sync(0xffffffffu, bk == top)) - 1;
     const int e = __shfl_sync(0xffffffffu, sl.e0 + bi, from);
     const double w = __shfl_sync(0xffffffffu, bs, from);
-    if (lane == from) taken |= 1u << bi;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane == from && i == bi) key[i] = 0u;
     if (lane == j) {
       mine = e;
       mine_s = w;
