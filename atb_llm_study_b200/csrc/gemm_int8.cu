@@ -109,6 +109,12 @@ __device__ __forceinline__ Unit group_unit(int w, const Params& p, const int* gt
   return u;
 }
 
+// A producer that gives up waits (again with a limit) for its copies in flight:
+// the last `stages` of the `issued` ones.
+__device__ __forceinline__ void drain_loads(uint64_t* full, int stages, int issued, unsigned* err) {
+  for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[i % stages], (i / stages) & 1, err);
+}
+
 // One warp fills gtab from the device offsets, 32 groups at a time (prefix
 // maximum and prefix sum); offsets that fall or leave [0, rows] are clamped and
 // reported.
@@ -320,7 +326,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* empty = full + kPairStages;
   uint64_t* tfull = empty + kPairStages;
   uint64_t* tempty = tfull + 2;  // the leader's are used
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* cols = reinterpret_cast<float*>(smem + kPairStages * kPairStageBytes + 256);
   int* gtab = reinterpret_cast<int*>(smem + kPairStages * kPairStageBytes + 256 + kPairColBytes);
@@ -339,6 +346,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 2 * kPairEpiWarps);
     }
+    mbar_init(drained, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
@@ -373,6 +381,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
+      int issued = 0;
       for (int w = pair; w < units && !*abort_flag; w += pairs) {
         const Unit u = unit_at(w);
         // rows of this CTA's half of both operands
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const int b_row = COLS ? u.tok0 + rank * (u.n / 2) : u.wrow0 + rank * BM;
         const int boxes = COLS ? (u.n / 2 + kTokBox - 1) / kTokBox : 1;
         constexpr int box_bytes = (COLS ? kTokBox : BM) * BK;
-        for (int kb = 0; kb < p.kb_total; ++kb) {
+        for (int kb = 0; kb < p.kb_total; ++kb, ++issued) {
           if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
             *abort_flag = 1;
             break;
@@ -397,6 +406,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       }
+      // the leader's barriers count both CTAs' copies; the other CTA leaves after it
+      if (*abort_flag && rank == 0) drain_loads(full, kPairStages, issued, p.err);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -440,6 +451,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           *abort_flag = 1;
           break;
         }
+      }
+      if (*abort_flag) {  // products in flight end before the operands' memory and TMEM go
+        umma_commit_pair(drained);
+        mbar_wait(drained, 0, p.err);
       }
     }
     __syncwarp();
@@ -570,7 +585,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* tscale = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + 512);  // of the tokens, per warp
   int* gtab = reinterpret_cast<int*>(tscale + 4 * BN);
@@ -586,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 128);
     }
+    mbar_init(drained, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
@@ -609,9 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
+      int issued = 0;
       for (int w = blockIdx.x; w < units && !*abort_flag; w += gridDim.x) {
         const Unit u = group_unit<BN, BM>(w, p, gtab);
-        for (int kb = 0; kb < p.kb_total; ++kb) {
+        for (int kb = 0; kb < p.kb_total; ++kb, ++issued) {
           if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
             *abort_flag = 1;
             break;
@@ -625,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (*abort_flag) drain_loads(full, C::STAGES, issued, p.err);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -664,6 +683,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           *abort_flag = 1;
           break;
         }
+      }
+      if (*abort_flag) {  // products in flight end before the operands' memory and TMEM go
+        umma_commit(drained);
+        mbar_wait(drained, 0, p.err);
       }
     }
     __syncwarp();
@@ -820,7 +843,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0; i < nkb; ++i) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) break;
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.err)) {
+          drain_loads(full, C::STAGES, i, p.err);
+          break;
+        }
         mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
         tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], (kb0 + i) * BK, row0);
         tma_load_2d(sB + stage * C::B_BYTES, &tmB, &full[stage], (kb0 + i) * BK, tok0);
@@ -862,7 +888,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             phase ^= 1;
           }
         }
-        umma_commit(tfull);
+        umma_commit(tfull);  // after a wait that ran out, too: nothing is in flight once the epilogue has seen it
       }
       __syncwarp();
     } else {
@@ -885,6 +911,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       tc_fence_before();
       __syncwarp();
+    }
+    // TMEM goes back before this CTA waits for others of its cluster: no CTA
+    // holds any while it waits for one that may still be asking for it
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
   }
   // This CTA finishes its share of the tokens: the cluster's partial sums
@@ -910,10 +943,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     else finish_tokens<EPI, 2, 8>(base, S, first + warp, last, tok0, fs, fb, tscale, f0, p);
   }
   if (S > 1) cluster_sync();  // no CTA leaves while another reads its partial sums
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(*tmem_slot, C::TMEM_COLS);
-  }
 }
 
 // ---------------------------------------------------------------------------

@@ -12,6 +12,11 @@ vanishes, and the division is within 2 ulp.  So |out - ref| <= 2^-8 |ref| +
 2e-5 (|ref| + |terms|) for all of them.
 """
 
+import os
+import subprocess
+import sys
+import textwrap
+
 import numpy as np
 import pytest
 import torch
@@ -23,6 +28,7 @@ pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
     import gpu_util as G
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 F = np.float32
 NONE, BIAS, RESIDUAL, SWIGLU, BIAS_GELU, BIAS_RESIDUAL = range(6)
 
@@ -254,9 +260,9 @@ def test_gemm_integers_are_exact(M):
 
 def test_gemm_non_finite_scales_stay_in_their_rows():
     rng = np.random.default_rng(9)
-    for M in (6, 200):
+    for M, N in ((6, 272), (200, 272), (6100, 528)):
         for epi in (NONE, SWIGLU):
-            a, sa, b, sb, _, _ = operands(rng, M, 272, 528, epi)
+            a, sa, b, sb, _, _ = operands(rng, M, N, 528, epi)
             sa[3] = np.nan
             a[3] = 0
             sa[4] = 0
@@ -265,8 +271,8 @@ def test_gemm_non_finite_scales_stay_in_their_rows():
 
 def test_gemm_swiglu_of_large_gates():
     rng = np.random.default_rng(10)
-    for M in (6, 200):
-        a, sa, b, sb, _, _ = operands(rng, M, 272, 528, SWIGLU)
+    for M, N in ((6, 272), (200, 272), (6100, 528)):
+        a, sa, b, sb, _, _ = operands(rng, M, N, 528, SWIGLU)
         out = gemm(a, sa * 200, b, sb, SWIGLU)
         assert np.isfinite(out).all()
         ref = int8.gemm(a, sa * 200, b, sb, SWIGLU)
@@ -291,6 +297,137 @@ def test_gemm_same_bits_twice_and_on_two_streams():
         torch.cuda.synchronize()
         for o in outs:
             np.testing.assert_array_equal(G.host(o), want)
+
+
+@pytest.mark.parametrize("epi", [NONE, RESIDUAL, SWIGLU, BIAS_GELU])
+def test_gemm_rows_aligned_to_16_bytes_only(epi):
+    # the widest stores want 32-byte rows: an odd start and an odd stride of 8 elements each
+    rng = np.random.default_rng(13 + epi)
+    M, N, K = 6100, 528, 272
+    a, sa, b, sb, bias, res = operands(rng, M, N, K, epi)
+    outN = N // 2 if epi == SWIGLU else N
+    ref = int8.gemm(a, sa, b, sb, epi, bias, res)
+    terms = np.abs(int8.gemm(a, sa, b, sb)).max() + 4 if epi in (RESIDUAL, BIAS_GELU) else 0.0
+    for start, pad in ((8, 0), (0, 8), (8, 24)):
+        C = torch.full((M * (outN + pad) + 16,), 7.0, dtype=torch.bfloat16, device=G.DEV)
+        R = G.bf16(np.concatenate([np.zeros(start), np.concatenate([res, np.zeros((M, pad))], 1).ravel()])) if res is not None else None
+        G.check(G.L().b200_gemm_int8(i8(a).data_ptr(), K, G.f32(sa).data_ptr(), i8(b).data_ptr(), K, G.f32(sb).data_ptr(),
+                                     C.data_ptr() + 2 * start, outN + pad, M, N, K, epi,
+                                     G.ptr(None if bias is None else G.bf16(bias)), 0 if R is None else R.data_ptr() + 2 * start,
+                                     N + pad, G.stream()))
+        torch.cuda.synchronize()
+        h = G.host(C)
+        assert (h[:start] == 7).all() and (h[start + M * (outN + pad):] == 7).all()
+        h = h[start:start + M * (outN + pad)].reshape(M, outN + pad)
+        assert (h[:, outN:] == 7).all()
+        near(h[:, :outN], ref, terms)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in x, q and C: the last rows are quantised, read and written where they belong."""
+    M, K, N = 70001, 32768, 32776
+    g = torch.Generator(device=G.DEV)
+    g.manual_seed(3)
+    last = [0, 1, 65535, 65536, M - 2, M - 1]
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=G.DEV)
+    x[last] = torch.randn(len(last), K, generator=g, device=G.DEV).bfloat16()
+    q = torch.full((M, K), 99, dtype=torch.int8, device=G.DEV)
+    s = torch.full((M,), 7.0, device=G.DEV)
+    L = G.L()
+    G.check(L.b200_quant_rows_int8(x.data_ptr(), K, M, None, None, q.data_ptr(), K, s.data_ptr(), M, K, G.stream()))
+    rq, rs = int8.quant_rows(G.host(x[last]))
+    np.testing.assert_array_equal(q[last].cpu().numpy(), rq)
+    np.testing.assert_array_equal(G.host(s[last]), rs)
+    assert int(q[2:65535].abs().max()) == 0
+    del x
+    b = torch.randint(-127, 128, (264, K), generator=g, device=G.DEV).to(torch.int8)
+    sb = torch.rand(264, generator=g, device=G.DEV) + 0.5
+    C = torch.full((M, 264), 7.0, dtype=torch.bfloat16, device=G.DEV)
+    G.check(L.b200_gemm_int8(q.data_ptr(), K, s.data_ptr(), b.data_ptr(), K, sb.data_ptr(), C.data_ptr(), 264, M, 264, K,
+                             NONE, None, None, 0, G.stream()))
+    near(G.host(C[last]), int8.gemm(rq, rs, b.cpu().numpy(), G.host(sb)))
+    assert float(C[2:65535].abs().max()) == 0
+    del C
+    b = torch.randint(-127, 128, (N, 32), generator=g, device=G.DEV).to(torch.int8)
+    sb = torch.rand(N, generator=g, device=G.DEV) + 0.5
+    q[:, :32] = torch.randint(-127, 128, (M, 32), generator=g, device=G.DEV).to(torch.int8)
+    s = torch.rand(M, generator=g, device=G.DEV) + 0.5
+    C = torch.full((M, N), 7.0, dtype=torch.bfloat16, device=G.DEV)
+    G.check(L.b200_gemm_int8(q.data_ptr(), K, s.data_ptr(), b.data_ptr(), 32, sb.data_ptr(), C.data_ptr(), N, M, N, 32,
+                             NONE, None, None, 0, G.stream()))
+    near(G.host(C[last]), int8.gemm(q[last][:, :32].cpu().numpy(), G.host(s[last]), b.cpu().numpy(), G.host(sb)))
+    assert G.device_errors() == 0
+
+
+def test_forms_side_by_side_on_streams():
+    """The pair, split and grouped forms and the bf16 GEMM running at once on four streams give what they give alone."""
+    rng = np.random.default_rng(14)
+    L = G.L()
+    jobs = []
+
+    def plain(M, N, K):
+        a, sa, b, sb, _, _ = operands(rng, M, N, K, NONE)
+        A, B, SA, SB = i8(a), i8(b), G.f32(sa), G.f32(sb)
+        return lambda st, o: G.check(L.b200_gemm_int8(A.data_ptr(), K, SA.data_ptr(), B.data_ptr(), K, SB.data_ptr(),
+                                                      o.data_ptr(), N, M, N, K, NONE, None, None, 0, st)), (M, N)
+
+    def experts(rows, n, N, K):
+        a, sa, b, sb, _, _ = operands(rng, rows, n * N, K, NONE)
+        A, B, SA, SB = i8(a), i8(b), G.f32(sa), G.f32(sb)
+        off = G.i32(np.linspace(0, rows, n + 1).astype(np.int32))
+        return lambda st, o: G.check(L.b200_grouped_gemm_int8(A.data_ptr(), K, SA.data_ptr(), B.data_ptr(), K, SB.data_ptr(),
+                                                              o.data_ptr(), N, off.data_ptr(), n, rows, N, K, NONE, st)), (rows, N)
+
+    X, W = G.bf16(rng.standard_normal((300, 1024))), G.bf16(rng.standard_normal((2048, 1024)))
+    bf = lambda st, o: G.check(L.b200_gemm_bf16(X.data_ptr(), 1024, W.data_ptr(), 1024, o.data_ptr(), 2048, 300, 2048, 1024,  # noqa: E731
+                                                NONE, None, None, 0, None, 0, st))
+    jobs = [plain(2048, 2048, 2048), plain(16, 4096, 4096), experts(900, 8, 512, 1024), (bf, (300, 2048)), plain(100, 1024, 4096),
+            experts(24, 8, 1024, 1024), experts(4000, 8, 512, 512)]
+    new = lambda shape: torch.zeros(*shape, dtype=torch.bfloat16, device=G.DEV)  # noqa: E731
+    alone = []
+    for f, shape in jobs:
+        o = new(shape)
+        f(G.stream(), o)
+        torch.cuda.synchronize()
+        alone.append(G.host(o))
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = [(i, new(shape)) for r in range(8) for i, (_, shape) in enumerate(jobs)]
+    torch.cuda.synchronize()
+    for n, (i, o) in enumerate(outs):
+        jobs[i][0](streams[(n * 3 + n // 7) % 4].cuda_stream, o)
+    torch.cuda.synchronize()
+    for i, o in outs:
+        np.testing.assert_array_equal(G.host(o), alone[i])
+    assert G.device_errors() == 0
+
+
+def test_first_calls_of_a_process_under_capture():
+    code = textwrap.dedent("""
+        import sys; sys.path[:0] = [%r, %r]
+        import torch
+        from atb_llm_study_b200 import capi
+        L = capi.lib()
+        one = lambda *s, t: torch.ones(*s, device="cuda").to(t)
+        x, w = one(8, 512, t=torch.bfloat16), one(256, 512, t=torch.int8)
+        q, s, ws = one(8, 512, t=torch.int8), one(8, t=torch.float32), one(256, t=torch.float32)
+        out, lg = one(8, 256, t=torch.bfloat16), one(8, 64, t=torch.float32)
+        ids, wt = one(8, 4, t=torch.int32), one(8, 4, t=torch.float32)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            st = torch.cuda.current_stream().cuda_stream
+            capi.check(L.b200_quant_rows_int8(x.data_ptr(), 512, 8, None, None, q.data_ptr(), 512, s.data_ptr(), 8, 512, st))
+            capi.check(L.b200_gemm_int8(q.data_ptr(), 512, s.data_ptr(), w.data_ptr(), 512, ws.data_ptr(), out.data_ptr(), 256,
+                                        8, 256, 512, 0, None, None, 0, st))
+            capi.check(L.b200_moe_topk_grouped(lg.data_ptr(), 64, None, 8, 64, 4, 0, 8, 2, 1, 1, 1.0, ids.data_ptr(),
+                                               wt.data_ptr(), st))
+        out.zero_(); ids.zero_()
+        g.replay(); torch.cuda.synchronize()
+        assert (out == 512).all(), out
+        assert ids.tolist() == [[0, 1, 2, 3]] * 8, ids
+    """ % (ROOT, os.path.join(ROOT, "tests")))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 # ------------------------------------------------------------ grouped product
