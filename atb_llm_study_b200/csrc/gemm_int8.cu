@@ -225,9 +225,18 @@ __device__ __forceinline__ void emit_features(const uint32_t acc[CW], int feat0,
 // MMAs that read both halves, and each CTA's epilogue drains its 128 token rows
 // from its own TMEM.  Against single CTAs with 128 x 256 tiles a pair moves a
 // third less through L2 and shared memory per product.
-// Grouped launches turn the operands round: 256 weight rows on the M side and
-// a group's tokens on the N side, whose extent can be any multiple of 32, so a
-// group's last tile does no product for rows it does not have.
+//
+// 16384 x 4096 x 12288 with residual: 496 us alone, 3.3 POP/s; the tensor pipe is
+// active in 90 % of the cycles that the SMs are (ncu), and a k-block takes 559
+// cycles against the MMAs' 512.  What is left of those cycles is shared memory
+// (32 KB in and as much out of it per 512 cycles) and the epilogue's use of it:
+// 611 cycles with SwiGLU at K = 4096, 560 with an epilogue that does nothing.  Run
+// back to back the power limit decides: 540 to 600 us at 1.5 GHz.
+//
+// Grouped launches come in two forms.  kRows is the plain one with a group's
+// rows past its end not stored.  kCols turns the operands round: 256 weight rows
+// on the M side and the group's tokens on the N side, whose extent can be any
+// multiple of 32, so that small groups do no products for rows they lack.
 // ---------------------------------------------------------------------------
 constexpr int kPairTile = 256;
 constexpr int kPairGroup = 8;  // token tiles walked per feature tile
@@ -560,7 +569,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // ---------------------------------------------------------------------------
 // Few tokens per expert: one persistent CTA per SM walks the (expert, feature
 // tile, token tile) units; the ring runs on across units and the accumulator
-// is double-buffered.
+// is double-buffered.  Bound by the weights' bytes: 8 experts of 28672 x 4096 at
+// 8 tokens each 146 us (6.4 TB/s, 98 % of the copy rate), 64 of 2816 x 2048 at 3
+// tokens 59 us (94 %), 64 of 2048 x 1408 34.6 us (81 %; 6.9 tiles an SM).
 // ---------------------------------------------------------------------------
 template <int BN>
 struct GroupCfg {
@@ -733,7 +744,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // Few tokens: one tile of 128 features x BN tokens per cluster, its K range
 // split over the cluster's CTAs; two CTAs per SM, so that one's epilogue runs
-// under another's loads.
+// under another's loads.  Bound by the weights' bytes and the ends of the launch:
+// 64 x 24576 x 4096 with SwiGLU 20.9 us in a chain of launches (100.7 MB, 15.4 us
+// at the copy rate: 1.3 us to the first tile, the stream done at 15 to 17, 2 for
+// the last epilogue, 2 to the next launch), 64 x 6144 x 4096 9.6 us (floor 3.8),
+// 1 x 4096 x 4096 6.2 us (2.6).  Asking for the weights' first tiles into L2 while
+// the previous kernel drains gained nothing (20.8 / 21.0 / 21.6 us with 0 / 4 / 8
+// k-blocks), and further ahead inside the loop it lost (18.5 to 22.5 us at one
+// token).
 // ---------------------------------------------------------------------------
 template <int BN>
 struct SplitCfg {

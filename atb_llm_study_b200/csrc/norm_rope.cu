@@ -84,7 +84,9 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_kernel(const __nv_bfloat
 // (out, optional, is the bf16 row it would write).  The integers come from the
 // row as rounded to bf16, so they and the scale are those of rmsnorm_kernel
 // followed by the row quantisation, bit for bit: a path can fuse the two or
-// not without changing a result.  Same thread / chunk mapping and sums.
+// not without changing a result.  Same thread / chunk mapping and sums.  Bound
+// by its bytes: 8192 x 4096 with residual in 36.5 us (235 MB, 6.4 TB/s), 64 x
+// 4096 in 4.3 us (9.0 with the loads between the stores).
 template <int CH>
 __global__ void __launch_bounds__(kNormThreads) rmsnorm_quant_kernel(const __nv_bfloat16* __restrict__ x,
                                                                      const __nv_bfloat16* residual,

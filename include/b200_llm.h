@@ -215,8 +215,8 @@ B200_API int64_t b200_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int 
  *   C[m, n] = epilogue(a_scale[m] * b_scale[n] * sum_k A[m, k] B[n, k])
  * A [M, K], B [N, K] int8 (b200_quant_rows_int8's output; any value, -128
  * included), the sum exact in 32 bits, scales fp32, one rounding to bf16.  The
- * epilogues, their operands and SwiGLU's interleaved gate / up rows are
- * b200_gemm_bf16's.  K % 16 == 0, K <= 131056; lda, ldb multiples of 16 bytes;
+ * epilogues, their operands (residual may alias C) and SwiGLU's interleaved gate
+ * / up rows are b200_gemm_bf16's.  K % 16 == 0, K <= 131056; lda, ldb multiples of 16 bytes;
  * N % 8 == 0 (SwiGLU: 16), ldc, ldr multiples of 8; every pointer 16-byte
  * aligned.  Takes no workspace, so calls on several streams need nothing of
  * their own.  Replaces LinearOp::Create(transB=true)
@@ -272,7 +272,8 @@ enum b200_router_score { B200_SCORE_SOFTMAX = 0, B200_SCORE_SIGMOID = 1 };
  * published DeepSeek-V2 / V3 gates).  Per token, with x the logits clamped to
  * the finite range (NaN counts as the lowest value):
  *   s = softmax(x) or sigmoid(x) over the E (<= 256) experts (`scoring`);
- *   c = s + bias (bias [E] fp32 or NULL; it moves the choice, not the weights);
+ *   c = s + bias (bias [E] fp32, finite, or NULL; it moves the choice, not the
+ *   weights);
  *   the experts form num_groups (<= 32) equal groups of consecutive ones, each
  *   scored by the sum of its group_top (1 or 2) largest c; only the
  *   topk_groups best groups' experts can be chosen;
