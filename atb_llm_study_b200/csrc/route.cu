@@ -61,7 +61,8 @@ __device__ __forceinline__ Slot slot_of(const RouteParams& p, int lane) {
   return s;
 }
 
-__device__ __forceinline__ float clamp_logit(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX); }  // NaN: -FLT_MAX
+// To the finite range (NaN: the lowest value), -0 to 0.
+__device__ __forceinline__ float clamp_logit(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX) + 0.f; }
 
 template <int PER>
 __device__ __forceinline__ void load_run(float v[PER], const float* src, const Slot& s, int vec, float fill) {
@@ -264,9 +265,9 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
   return true;
 }
 
-// Doubles as unsigned integers of the same order.
+// Doubles as unsigned integers of the same order (-0 as 0).
 __device__ __forceinline__ uint64_t to_key64(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
 __device__ __forceinline__ uint64_t warp_max64(uint64_t k) {
@@ -324,13 +325,16 @@ __device__ __noinline__ void choose_exact(const RouteParams& p, int64_t t, int l
       b = fmax(fmin(a, oa), fmax(b, ob));
       a = fmax(a, oa);
     }
-    const double score = p.best > 1 ? a + b : a;
-    int rank = 0;
-    for (int h = 0; h < p.G; ++h) {
-      const double other = __shfl_sync(0xffffffffu, score, h << p.lpg_shift);
-      rank += other > score || (other == score && h < sl.g);
+    uint64_t key = sl.g < p.G ? to_key64(p.best > 1 ? a + b : a) : 0u;
+    in = false;
+    for (int j = 0; j < p.keep; ++j) {
+      const uint64_t top = warp_max64(key);
+      const int from = __ffs(__ballot_sync(0xffffffffu, key == top)) - 1;  // of equals the lowest group
+      if (sl.g == from >> p.lpg_shift) {
+        in = sl.n > 0;
+        key = 0u;
+      }
     }
-    in = in && rank < p.keep;
   }
   uint64_t key[PER];  // 0: not to be chosen (no value's key)
 #pragma unroll

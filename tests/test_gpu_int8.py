@@ -455,7 +455,8 @@ GROUPS = [
     ([3, 0, 17, 64, 1, 0, 100, 7], 256, 512), ([3, 0, 17, 64, 1, 0, 100, 7], 208, 528), ([1], 128, 128), ([0, 1, 0], 24, 16),
     ([2] * 64, 176, 256), ([0, 0, 0, 40], 128, 144), ([300, 0, 513, 129], 512, 256), ([300, 0, 513, 129], 144, 272),
     ([128, 256, 1, 700], 1296, 144), ([0, 0, 900], 2816, 400), ([97] * 5, 272, 1040), ([5, 700, 3, 0, 2, 1], 544, 256),
-    ([0] * 40 + [9], 144, 272), ([1000] + [0] * 255, 48, 48)]
+    ([0] * 40 + [9], 144, 272), ([1000] + [0] * 255, 48, 48), ([700] + [1] * 63, 144, 272),
+    ([300, 0, 513, 129], 520, 272), ([100, 60, 0, 130], 520, 272)]
 
 
 @pytest.mark.parametrize("epi", [NONE, SWIGLU])

@@ -87,7 +87,7 @@ def test_scores_that_fp32_cannot_tell_apart(sigmoid):
 
 def test_masked_and_extreme_logits():
     big = float(np.finfo(F).max)
-    lg = np.zeros((9, 32), F)
+    lg = np.zeros((10, 32), F)
     lg[0] = -np.inf  # nothing left: uniform, the lowest experts
     lg[1] = -big
     lg[2, :] = -np.inf
@@ -98,6 +98,9 @@ def test_masked_and_extreme_logits():
     lg[6, 3], lg[6, 20] = np.nan, 2.0
     lg[7] = np.linspace(-80, 80, 32)
     lg[8, ::2] = -big
+    lg[6, ::2] = np.where(lg[6, ::2] == 0, -0.0, lg[6, ::2])  # zeros of both signs are equal
+    lg[9] = -1 - np.arange(32)
+    lg[9, :4] = -0.0, 0.0, -3.0, -0.0
     for sigmoid in (False, True):
         for groups, keep, best in ((1, 1, 1), (4, 2, 1), (4, 2, 2)):
             for renorm in (False, True):

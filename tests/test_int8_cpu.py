@@ -63,6 +63,7 @@ def test_refused(name, base, change):
 @pytest.mark.parametrize("name,base,change", [
     ("b200_quant_rows_int8", QUANT, dict(rows=1 << 31, src_rows=1 << 31)),
     ("b200_rmsnorm_quant_int8", NORM, dict(rows=1 << 31)),
+    ("b200_rmsnorm_quant_int8", NORM, dict(dim=8208, stride=8208, ldq=8208)),
     ("b200_gemm_int8", GEMM, dict(K=131072, lda=131072, ldb=131072)),  # 128 * 128 * K passes 31 bits
     ("b200_gemm_int8", GEMM, dict(M=1 << 31)),
     ("b200_grouped_gemm_int8", GROUPED, dict(K=131072, lda=131072, ldb=131072)),
