@@ -129,9 +129,9 @@ __device__ __forceinline__ float rcp_fast(float x) {
 //
 // What is compared carries a tag in its low bits, so one 32-bit maximum over
 // the warp gives value and place: log2(PER) bits among experts (the place in
-// the lane), 5 among groups.  Cutting b bits moves a value by less than 2^(b-23)
-// of itself.  Two equal values are always in doubt, so ties are settled in
-// double, by index.
+// the lane), 5 among groups (whose choice is then checked on the whole values).
+// Cutting b bits moves a value by less than 2^(b-23) of itself.  Two equal values
+// are always in doubt, so ties are settled in double, by index.
 //
 // Error of a score (exp_fast: 2 + 1.2 |x| ulp of e^x).  Sigmoid: the quotient's
 // ulp, half an ulp of the sum 1 + e^-x, and the exponential's error times
@@ -144,7 +144,7 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
   constexpr int kTagBits = PER <= 1 ? 0 : PER <= 2 ? 1 : PER <= 4 ? 2 : PER <= 8 ? 3 : 4;
   constexpr uint32_t kTag = (1u << kTagBits) - 1u, kGroupTag = 31u;
   // 2^(bits - 23), and the half ulps of the two values compared
-  constexpr float kCut = (float)(1 << kTagBits) * 0x1p-23f + 1.2e-7f, kGroupCut = 0x1p-18f + 1.2e-7f;
+  constexpr float kCut = (float)(1 << kTagBits) * 0x1p-23f + 1.2e-7f;
   const Slot sl = slot_of<PER>(p, lane);
   const float* lg = p.logits + t * p.ld;
   float c[PER];
@@ -195,25 +195,27 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, int64_t t, int
       a = fmaxf(a, oa);
     }
     const float score = p.best > 1 ? a + b : a;
-    // roundings of the biased sums are relative to their terms, which can cancel
-    const float size = p.best > 1 ? fabsf(a) + fabsf(b) : fabsf(a);
+    // score -+ err holds the group's score in 64 bits: the errors of its one or
+    // two scores, and where anything but logits is compared the roundings of the
+    // biased scores, of their sum and of score -+ err (half an ulp each).  Those
+    // are relative to the terms, which can cancel, so every group has a bound of
+    // its own, whatever its rank.
+    const float err = (p.best > 1 ? tol : 0.5f * tol) +
+                      (tol > 0.f ? 2.4e-7f * (p.best > 1 ? fabsf(a) + fabsf(b) : fabsf(a)) : 0.f);
     uint32_t key = sl.g < p.G ? to_key(score, kGroupTag, 31u - sl.g) : 0u;
-    uint32_t nth = 0;  // lane j: the j-th group's key
     in = false;
-    for (int j = 0; j <= p.keep; ++j) {  // one more than is kept: the best that is not
+    for (int j = 0; j < p.keep; ++j) {
       const uint32_t best = __reduce_max_sync(0xffffffffu, key);
-      nth = lane == j ? best : nth;
-      if (j < p.keep && key == best) {
+      if (key == best) {
         in = true;
         key = 0u;
       }
     }
-    // the last group that is kept against the best that is not
-    const float x = from_key(nth, kGroupTag);
-    const float sz = __shfl_sync(0xffffffffu, size, (31 - (int)(nth & kGroupTag)) << p.lpg_shift);
-    const float y = __shfl_down_sync(0xffffffffu, x, 1), sz1 = __shfl_down_sync(0xffffffffu, sz, 1);
-    const float near = (p.best > 1 ? 2.f : 1.f) * tol + (tol > 0.f ? 4e-7f * fmaxf(sz, sz1) + kGroupCut * fabsf(x) : 0.f);
-    clear = __shfl_sync(0xffffffffu, (int)(x - y > near), p.keep - 1) != 0;
+    // every group that is kept against the best that another may be (a sum below
+    // fp32's range is below -3e38, too)
+    const float most = in || sl.g >= p.G ? -INFINITY : score == -INFINITY ? -3e38f : score + err;
+    const float other = from_key(__reduce_max_sync(0xffffffffu, to_key(most, 0u, 0u)), 0u);
+    clear = __all_sync(0xffffffffu, !in || score - err > other);
   }
   uint32_t key[PER];
 #pragma unroll

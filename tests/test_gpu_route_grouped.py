@@ -158,3 +158,17 @@ def test_route_from_hidden_states(T, E, H, pad):
     np.testing.assert_array_equal(ids.cpu().numpy(), rid)
     np.testing.assert_allclose(G.host(w), rw, rtol=1e-5, atol=4e-6)
     assert G.device_errors() == 0
+
+
+@pytest.mark.parametrize("sigmoid", [False, True], ids=["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [2.0**14, 2.0**20], ids=["2^14", "2^20"])
+@pytest.mark.parametrize("groups", [(0,), (2, 7)], ids=str)
+def test_group_scores_whose_terms_cancel(sigmoid, size, groups):
+    """Groups of two experts, some biased by +size and -size: such a group's score is of the others' size, but in fp32 it
+    carries the rounding of `size` (2^-10 and 2^-4), at whatever rank it comes out and far from the cut too."""
+    rng = np.random.default_rng(17)
+    lg = rng.standard_normal((400000, 16)).astype(F)
+    bias = np.zeros(16, F)
+    for g in groups:
+        bias[2 * g:2 * g + 2] = size, -size
+    check(lg, 8, sigmoid=sigmoid, bias=bias, groups=8, keep=4, best=2)
