@@ -88,6 +88,9 @@ struct Params {
   // Stream-K (swapped SwiGLU only): one flag per tile, zero between launches;
   // ws then holds one 128 x BN fp32 partial per tile, [tile][token][row].
   int* sk_flags;
+  // The weight operand may be the previous kernel's output: no tile of it is
+  // loaded ahead of the dependency wait.
+  bool late_weights;
 };
 
 // One output tile: its MMA tile coordinates, K range, the TMA row coordinates
@@ -392,15 +395,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      // The weight operand (A when swapped, B otherwise) is constant: its
-      // tiles for the first stages are requested before waiting for the
-      // previous kernel on the stream, so the weight stream starts while that
-      // kernel drains.  Activation tiles are only loaded after the wait.
+      // The weight operand (A when swapped, B otherwise) is constant unless
+      // late_weights says otherwise: its tiles for the first stages are
+      // requested before waiting for the previous kernel on the stream, so the
+      // weight stream starts while that kernel drains.  Activation tiles are
+      // only loaded after the wait.
       // (Grouped launches already waited: their tiles depend on the offsets.)
       // The first STAGES k-blocks of the CTA's unit sequence (across unit
       // boundaries: a stream-K head piece may be short) are preloaded.
       int pre = 0;
-      if (!GROUPED) {
+      if (!GROUPED && !p.late_weights) {
         for (int w = w0; w < units && pre < C::STAGES; w += wstep) {
           const Unit u0 = unit_at(w, gtab);
           for (int kb = u0.kb0; kb < u0.kb1 && pre < C::STAGES; ++kb, ++pre) {
@@ -730,6 +734,7 @@ Params make_params(const b200::GemmPlan& g, int64_t M, int64_t N, int64_t K, voi
   p.pf = nullptr;
   p.pf_bytes = 0;
   p.sk_flags = nullptr;
+  p.late_weights = false;
   int dev = 0;
   cudaGetDevice(&dev);
   p.err = b200::error_word(dev);
@@ -868,6 +873,7 @@ int gemm_f32_launch(const void* A, int64_t lda, const void* B, int64_t ldb, floa
   g.kb_per_split = g.kb_total;
   Params p = make_params(g, M, N, K, nullptr, 0, nullptr, nullptr, 0, nullptr);
   p.ws = out;  // the one "partial" tile set is the product
+  p.late_weights = true;
   CUtensorMap ta, tb;
   if (!make_tmap(&ta, g.swap ? B : A, p.rows, K, g.swap ? ldb : lda, BM) ||
       !make_tmap(&tb, g.swap ? A : B, p.cols, K, g.swap ? lda : ldb, g.bn))

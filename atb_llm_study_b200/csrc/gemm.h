@@ -34,7 +34,8 @@ int gemm_launch(const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
                 int* sk_flags = nullptr, int sk_flag_count = 0);
 
 // out[M, N] (fp32, dense) = A B^T, the whole K in one pass: logits that are
-// compared, not stored.  The caller has checked what b200_gemm_bf16 would.
+// compared, not stored.  Both operands may be the previous kernel's output.  The
+// caller has checked what b200_gemm_bf16 would.
 int gemm_f32_launch(const void* A, int64_t lda, const void* B, int64_t ldb, float* out, int64_t M, int64_t N, int64_t K,
                     cudaStream_t stream);
 

@@ -292,7 +292,8 @@ B200_API int b200_moe_topk_grouped(const float* logits, int64_t ld, const float*
 
 /* b200_moe_topk_grouped of the logits x [T, H] (bf16, row stride ldx) .
  * gate_weight [E, H]^T, computed in fp32 into logits [T, E] (required; 16-byte
- * aligned, as x and gate_weight), for up to 256 experts. */
+ * aligned, as x and gate_weight), for up to 256 experts.  x and gate_weight may
+ * be the output of the call just before on the stream. */
 B200_API int b200_moe_route_grouped(const void* x, int64_t ldx, const void* gate_weight, const float* bias, int64_t T,
                                     int64_t H, int num_experts, int top_k, int scoring, int num_groups,
                                     int topk_groups, int group_top, int renormalize, float scale,

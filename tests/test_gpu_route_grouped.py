@@ -172,3 +172,45 @@ def test_group_scores_whose_terms_cancel(sigmoid, size, groups):
     for g in groups:
         bias[2 * g:2 * g + 2] = size, -size
     check(lg, 8, sigmoid=sigmoid, bias=bias, groups=8, keep=4, best=2)
+
+
+@pytest.mark.parametrize("T", [8, 64, 300], ids=["warps", "weights on the M side", "weights on the N side"])
+def test_gate_weights_written_right_before_the_call(T):
+    """A gate merged (base + U V^T) by a GEMM just before on the stream, in place and many times over: each call's logits
+    are those of the gate that was merged for it."""
+    rng = np.random.default_rng(T)
+    E, H, k, R = 256, 2048, 8, 64
+    L = G.L()
+    X = G.bf16(rng.standard_normal((T, H)))
+    U, V = G.bf16(rng.standard_normal((E, R)) * 0.1), G.bf16(rng.standard_normal((H, R)) * 0.1)
+    bases = [G.bf16(rng.standard_normal((E, H))) for _ in range(3)]
+    gate = torch.zeros(E, H, dtype=torch.bfloat16, device=G.DEV)
+    out = lambda: (torch.empty(T, k, dtype=torch.int32, device=G.DEV), torch.empty(T, k, device=G.DEV),  # noqa: E731
+                   torch.empty(T, E, device=G.DEV))
+
+    def merge(base):
+        G.check(L.b200_gemm_bf16(U.data_ptr(), R, V.data_ptr(), R, gate.data_ptr(), H, E, H, R, 2, None, base.data_ptr(), H,
+                                 None, 0, G.stream()))
+
+    def route_to(o):
+        G.check(L.b200_moe_route_grouped(X.data_ptr(), H, gate.data_ptr(), None, T, H, E, k, 0, 1, 1, 1, 1, 1.0,
+                                         o[0].data_ptr(), o[1].data_ptr(), o[2].data_ptr(), G.stream()))
+
+    want = []
+    for base in bases:
+        merge(base)
+        torch.cuda.synchronize()
+        want.append(out())
+        route_to(want[-1])
+        torch.cuda.synchronize()
+    assert not any(torch.equal(want[0][2], w[2]) for w in want[1:])
+    got = [out() for _ in range(60)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        merge(bases[i % 3])
+        route_to(o)
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        for a, b in zip(o, want[i % 3]):
+            assert torch.equal(a, b), i
+    assert G.device_errors() == 0
