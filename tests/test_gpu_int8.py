@@ -598,3 +598,48 @@ def test_weights_quantised_right_before_the_product():
         near(G.host(outs[i]), int8.gemm(qa, sa, qb, sb))
         for j in range(i, 30, 3):
             np.testing.assert_array_equal(G.host(outs[j]), G.host(outs[i]))
+
+
+# ------------------------------------- grouped products of many tiles a worker
+
+# Sizes of 64 groups and the form that their average takes (tokens a tile, features a tile, workers: CTAs or pairs).
+MANY_TILES = {
+    "16 tokens": ([1, 3, 9, 0, 17, 2, 15, 16], 16, 128, 148),
+    "32 tokens": ([20, 1, 33, 0, 5, 32, 7, 8], 32, 128, 148),
+    "64 tokens": ([40, 64, 65, 1, 0, 90, 30, 20], 64, 128, 148),
+    "pairs, tokens on the N side": ([1, 20, 33, 100, 200, 300, 256, 0], 256, 256, 74),
+    "pairs, tokens on the M side": ([300, 513, 1, 256, 299, 420, 0, 280], 256, 256, 74),
+}
+
+
+@pytest.mark.parametrize("K", [272, 1680], ids=["K inside the ring", "K past the ring"])
+@pytest.mark.parametrize("epi", [NONE, SWIGLU], ids=["none", "swiglu"])
+@pytest.mark.parametrize("form", MANY_TILES)
+def test_grouped_gemm_of_many_tiles_a_worker(form, epi, K):
+    """Each worker walks five tiles and more: accumulators handed back and taken again, barriers through several phases,
+    tiles of other extents and other groups one after another, with a short K the next tile's loads under this one's sums."""
+    sizes, tok, feat, workers = MANY_TILES[form]
+    rng = np.random.default_rng(tok + epi + K)
+    sizes = np.concatenate([rng.permutation(sizes) for _ in range(8)])
+    N = 1040 if "M side" in form else 1568
+    rows, n = int(sizes.sum()), len(sizes)
+    mean = (rows + 5) / n
+    assert {16: mean <= 8, 32: 8 < mean <= 16, 64: 16 < mean <= 56, 256: mean > 56}[tok]
+    assert feat == 128 or (mean <= 160) == ("N side" in form)
+    assert (-(-sizes // tok) * -(-N // feat)).sum() >= 5 * workers
+    a, sa, b, sb, _, _ = operands(rng, rows, n * N, K, epi)
+    out, off = grouped(a, sa, b, sb, sizes, N, epi, extra=5)
+    for g in range(n):
+        r, w = slice(off[g], off[g + 1]), slice(g * N, (g + 1) * N)
+        near(out[r], int8.gemm(a[r], sa[r], b[w], sb[w], epi))
+
+
+@pytest.mark.parametrize("K", [272, 1680], ids=["K inside the ring", "K past the ring"])
+@pytest.mark.parametrize("epi", [NONE, SWIGLU, BIAS_RESIDUAL], ids=["none", "swiglu", "bias, residual"])
+def test_gemm_of_many_tiles_a_pair(epi, K):
+    M, N = 3001, 8208
+    assert -(-M // 256) * -(-N // 256) >= 5 * 74
+    rng = np.random.default_rng(epi + K)
+    a, sa, b, sb, bias, res = operands(rng, M, N, K, epi)
+    terms = 0.0 if epi != BIAS_RESIDUAL else np.abs(int8.gemm(a, sa, b, sb)) + np.abs(bias) + np.abs(res)
+    near(gemm(a, sa, b, sb, epi, bias, res), int8.gemm(a, sa, b, sb, epi, bias, res), terms)
