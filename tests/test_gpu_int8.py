@@ -6,9 +6,11 @@ run through all of them.
 Tolerances.  The integer sums are exact, so a product carries: the conversion
 of the sum to fp32, two scale products, and the bias / residual additions (at
 most 6 roundings of 2^-24 of the terms), then one rounding to bf16 (2^-8 of the
-value).  GELU adds tanhf's 2 ulp.  SwiGLU's exponential is the fast one:
-(2 + 1.2 |g|) 2^-23 relative, 1.3e-5 for |g| <= 90, below which the gate
-vanishes, and the division is within 2 ulp.  So |out - ref| <= 2^-8 |ref| +
+value).  SwiGLU's and GELU's exponential is the fast one: (2 + 1.2 |w|) 2^-23
+relative for e^-w, 1.3e-5 for |w| <= 90, below which the value vanishes, and
+the division is within 2 ulp.  GELU's w = 2 sqrt(2/pi) (x + 0.044715 x^3) adds
+its own roundings, which the cases here keep small (|w| of a few units; far
+values have a test and a bound of their own).  So |out - ref| <= 2^-8 |ref| +
 2e-5 (|ref| + |terms|) for all of them.
 """
 
@@ -643,3 +645,35 @@ def test_gemm_of_many_tiles_a_pair(epi, K):
     a, sa, b, sb, bias, res = operands(rng, M, N, K, epi)
     terms = 0.0 if epi != BIAS_RESIDUAL else np.abs(int8.gemm(a, sa, b, sb)) + np.abs(bias) + np.abs(res)
     near(gemm(a, sa, b, sb, epi, bias, res), int8.gemm(a, sa, b, sb, epi, bias, res), terms)
+
+
+# ------------------------------------------------------------- GELU of far values
+
+
+@pytest.mark.parametrize("M,N", [(6, 272), (200, 272), (6100, 528)], ids=["cluster", "cluster, many tokens", "pairs"])
+def test_gemm_gelu_of_large_values(M, N):
+    """GELU as x / (1 + e^-w), w = 2 sqrt(2/pi) (x + 0.044715 x^3), with the fast exponential and division.
+
+    x carries the conversion of the sum, two scale products and the bias addition: dx <= (3 |v| + |x|) 2^-24.  The
+    result's relative error is dx / |x| (1 + 3 |w|), as w grows no faster than x^3; 8 |w| 2^-24 from w's own roundings
+    and constants; (2 + 1.2 |w|) 2^-23 from the exponential; 3 2^-23 from the sum and the division; 2^-8 from bf16.
+    Below w = -80 the value vanishes (under 1e-30)."""
+    rng = np.random.default_rng(21)
+    K = 528
+    a, sa, b, sb, bias, _ = operands(rng, M, N, K, BIAS_GELU)
+    sa = sa * np.exp2(rng.uniform(-3, 3, M)).astype(F)  # rows of all sizes: products of a few units up to hundreds
+    out = gemm(a, sa, b, sb, BIAS_GELU, bias).astype(np.float64)
+    v = int8.gemm(a, sa, b, sb)
+    x = v + bias
+    assert x.min() < -200 and x.max() > 200 and (np.abs(x) < 6).mean() > 0.01
+    w = 2 * np.sqrt(2 / np.pi) * (x + 0.044715 * x**3)
+    with np.errstate(over="ignore"):
+        ref = x / (1 + np.exp(-w))
+    assert np.isfinite(out).all()
+    seen = w > -80
+    # where w is above 20 the value is x itself, to less than the other terms
+    aw = np.minimum(np.abs(w), np.where(w > 0, 20, np.inf))
+    dx = (3 * np.abs(v) + np.abs(x)) * 2.0**-24 / np.maximum(np.abs(x), 1e-30)
+    lim = np.abs(ref) * (2.0**-8 + dx * (1 + 3 * aw) + 8 * aw * 2.0**-24 + (5 + 1.2 * aw) * 2.0**-23) + 1e-30
+    assert (np.abs(out - ref) <= lim)[seen].all(), float((np.abs(out - ref) / lim)[seen].max())
+    assert np.abs(out[~seen]).max() < 1e-30 and (~seen).any()
