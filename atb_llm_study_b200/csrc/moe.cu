@@ -391,9 +391,11 @@ __global__ void moe_gate_logits_kernel(const __nv_bfloat16* __restrict__ x, int6
 }
 
 // Up to so many logits a warp for each gives them sooner than tensor core tiles,
-// whose few CTAs walk the whole hidden width (us, warps / tiles: 32 x 256 over
-// 7168 34 / 39, 64 x 256 60 / 40, 64 x 64 over 2048 11.6 / 15.8, 256 x 64 20 /
-// 15, 16384 x 256 3878 / 37 with the selection).
+// whose few CTAs walk the whole hidden width (us, warps / tiles, the selection
+// among them: over 7168 32 x 256 34 / 39, 64 x 256 60 / 40; over 2048 64 x 64
+// 11.7 / 15.8, 256 x 64 20 / 15, 16384 x 256 3878 / 38).  The tiles are for
+// expert counts that are a multiple of 4; others take a warp a logit however
+// many there are (16384 x 62 over 2048 946, x 64 26).
 constexpr int64_t kWarpLogits = 8192;
 
 int route_launch(const void* x, int64_t ldx, const void* wg, const float* logits_in, int64_t T, int64_t H, int E,

@@ -2,7 +2,7 @@
 // the 8-bit products, made from activations (per token) and from weights (per
 // output channel) alike.  Reads 2 bytes and writes 1 byte a value, and is bound
 // by that: 16384 x 12288 in 86 us (604 MB, 7.0 TB/s), 49152 rows of 2048 gathered
-// from 8192 in 31 us, 49152 x 1408 in 33 us (207 MB, 6.3 TB/s); one row, or 64 of
+// from 8192 in 31 us (134 MB at DRAM, and 201 MB read out of L2), 49152 x 1408 in 33 us (207 MB, 6.3 TB/s); one row, or 64 of
 // 4096, in 3.2 us, the length of a launch.  (A rounding and a conversion
 // instruction a value, both on the slow conversion pipe, took 137 us for the
 // first; one FMA does both, see quant.cuh.)

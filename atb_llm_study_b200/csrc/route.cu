@@ -13,10 +13,11 @@
 // than that bound is chosen again on scores in double.
 //
 // One warp a token, four a CTA.  The bytes (4 E T read) are not what bounds it
-// but the comparisons' half-rate integer pipe and the latency of the few tokens
-// that are chosen twice: 16384 x 256, 4 of 8 groups, top-8 with a bias 20.5 us,
-// 14.7 of them the fp32 choices (17.8 MB, 2.7 us at the copy rate); 16384 x 64
-// ungrouped 9.9 us, 4099 x 160 6.2 us, 64 x 64 2.1 us.  All tokens in double take
+// but the comparisons' half-rate integer pipe, and the choice in double beside
+// them: 16384 x 256, 4 of 8 groups, top-8 with a bias 21.2 us (17.8 MB, 2.7 us at
+// the copy rate), 15.1 in a build that has no choice in double (32 registers
+// instead of 80), for the 0.12 % of tokens that take it; 16384 x 64 ungrouped 10.5
+// us (7.9 without), 4099 x 160 7.0 us, 64 x 64 2.1 us.  All tokens in double take
 // 46 us for the first, as a batch of nothing but ties does.
 #include <float.h>
 #include <math.h>

@@ -92,7 +92,8 @@ B200_API int b200_quant_rows_int8(const void* x, int64_t ldx, int64_t src_rows, 
 /* b200_rmsnorm and b200_quant_rows_int8 of its output in one pass: q, scale,
  * residual_out (optional, may alias residual) and out (optional, the bf16 row
  * itself) are what the two calls give, bit for bit.  x / residual / out /
- * residual_out have row stride `stride`, q ldq.  dim % 16 == 0, dim <= 8192.
+ * residual_out have row stride `stride`, q ldq; q and scale overlap none of the
+ * others.  dim % 16 == 0, dim <= 8192.
  * Replaces RmsNormGraph::Build (atb_cpp_llm/src/components/common/rms_norm_graph.cpp:59-84)
  * in front of 8-bit projections. */
 B200_API int b200_rmsnorm_quant_int8(const void* x, const void* residual, const void* weight, int8_t* q, int64_t ldq,
@@ -200,6 +201,10 @@ enum b200_epilogue {
  * With split-K each K slice stores its fp32 partial tile in the workspace and
  * a second kernel sums them and applies the epilogue; calls that overlap on
  * the GPU must not share a workspace.
+ * B is taken as constant: its first tiles are read while this library's calls
+ * ahead of it on the stream are still running, so none of those may write it
+ * (after a write, let the host wait for the stream before the call).
+ * The layer calls take their weights in the same way.
  * Replaces LinearOp::Create(transB=true) (atb_cpp_llm/src/ops/linear_op.cpp:7-20)
  * and the SiLU/Mul/Add ops fused into its consumers
  * (atb_cpp_llm/src/components/common/mlp_builder.cpp:12-56). */
@@ -218,8 +223,11 @@ B200_API int64_t b200_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int 
  * epilogues, their operands (residual may alias C) and SwiGLU's interleaved gate
  * / up rows are b200_gemm_bf16's.  K % 16 == 0, K <= 131056; lda, ldb multiples of 16 bytes;
  * N % 8 == 0 (SwiGLU: 16), ldc, ldr multiples of 8; every pointer 16-byte
- * aligned.  Takes no workspace, so calls on several streams need nothing of
- * their own.  Replaces LinearOp::Create(transB=true)
+ * aligned (the scales too: a part of a quantised batch starts at a multiple of
+ * four rows).  The sum is scaled in fp32 by one scale after the other, in an
+ * order that depends on the size.  Every operand may be the output of the call
+ * just before on the stream.  Takes no workspace, so calls on several streams
+ * need nothing of their own.  Replaces LinearOp::Create(transB=true)
  * (atb_cpp_llm/src/ops/linear_op.cpp:7-20) where the weights are kept in 8 bits. */
 B200_API int b200_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
                             const float* b_scale, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int epilogue,
@@ -243,7 +251,9 @@ B200_API int b200_grouped_gemm_bf16(const void* A, int64_t lda, const void* B, i
 /* b200_grouped_gemm_bf16 with 8-bit operands and b200_gemm_int8's scales:
  * a_scale [rows] of the rows of A, b_scale [groups * N] of the rows of B.
  * Rows outside [0, group_offsets[groups]) are left as they are; offsets that
- * fall or leave [0, rows] are clamped and set the device error word. */
+ * fall or leave [0, rows] are clamped and set the device error word.  The
+ * kernel is chosen by rows / groups: a `rows` far above group_offsets[groups]
+ * gives the same results more slowly. */
 B200_API int b200_grouped_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
                                     const float* b_scale, void* C, int64_t ldc, const int32_t* group_offsets,
                                     int groups, int64_t rows, int64_t N, int64_t K, int epilogue,
@@ -293,7 +303,9 @@ B200_API int b200_moe_topk_grouped(const float* logits, int64_t ld, const float*
 /* b200_moe_topk_grouped of the logits x [T, H] (bf16, row stride ldx) .
  * gate_weight [E, H]^T, computed in fp32 into logits [T, E] (required; 16-byte
  * aligned, as x and gate_weight), for up to 256 experts.  x and gate_weight may
- * be the output of the call just before on the stream. */
+ * be the output of the call just before on the stream.  Many tokens want a
+ * number of experts that is a multiple of 4 (others are 30 to 100 times slower
+ * at 16384 tokens). */
 B200_API int b200_moe_route_grouped(const void* x, int64_t ldx, const void* gate_weight, const float* bias, int64_t T,
                                     int64_t H, int num_experts, int top_k, int scoring, int num_groups,
                                     int topk_groups, int group_top, int renormalize, float scale,
