@@ -322,6 +322,7 @@ def _plain_extend(s):
     first = need.cumsum(0) - need
     missing = (need.sum() - count).clamp(min=0)
     fits = missing == 0
+    more = more * fits
     col = torch.arange(s["width"], device="cuda")
     fresh = (col >= held[:, None]) & (col < total[:, None]) & fits
     take = (count - 1 - first[:, None] - (col - held[:, None])).clamp(0, s["free"].numel() - 1)
@@ -334,7 +335,7 @@ def _plain_extend(s):
     pos = torch.where(real, cached[seq] + t - cu[seq], torch.zeros_like(t))
     block = tables[seq, (pos // bs).clamp(max=s["width"] - 1)].long()
     slots = torch.where(real, block * bs + pos % bs, torch.full_like(pos, -1))
-    ctx = torch.where(fits, cached + more, cached)
+    ctx = cached + more
     left = torch.where(fits, count - need.sum(), count)
     i32 = torch.int32
     return tables, ctx.to(i32), cu.to(i32), pos, slots, left.to(i32), missing.to(i32)
