@@ -511,7 +511,8 @@ def _own_shared(L, check, st, s):
     nq, nkv, d = c["nq"], c["nkv"], c["d"]
     check(L.b200_paged_decode_shared(s["q"].data_ptr(), nq * d, s["k"].data_ptr(), s["v"].data_ptr(),
                                      s["prefix"].data_ptr(), s["prefix_len"].data_ptr(), c["prefix"],
-                                     s["tables"].data_ptr(), s["width"], s["ctx"].data_ptr(), c["longest"], c["batch"],
+                                     s["tables"].data_ptr(), s["width"], s["ctx"].data_ptr(),
+                                     min(c["longest"], s["width"] * c["block"]), c["batch"],
                                      nq, nkv, d, c["block"], s["blocks"], 1 / math.sqrt(d), s["out"].data_ptr(), nq * d,
                                      s["ws"].data_ptr(), s["ws_bytes"], st), "paged_decode_shared")
     return s["out"]
