@@ -1,0 +1,194 @@
+// Prompt attention with a sliding window and a few first tokens that stay
+// visible: query i of a sequence sees keys j <= i with i - j < window or
+// j < sinks.
+//
+// The tensor cores bound it: 4 flops a visible pair, head and dim, and a 128-row
+// query tile touches window / 128 + 2 key tiles (the window's ends cut through
+// one each) besides the sinks'.  Tiles without a visible pair are never
+// loaded, so the time follows the window and not the prompt.  Items are walked
+// with the heads of one sequence's rows next to each other: the nq / nkv heads
+// that share keys find them in L2.
+#include <algorithm>
+
+#include "tc_items.cuh"
+
+using namespace b200;
+
+namespace {
+
+// HEADS3D: heads narrower than the 64-column box, mapped as rows of their own (tc_attention.cuh)
+template <int HDK_, int HDV_, bool HEADS3D>
+struct Window {
+  static constexpr int HDK = HDK_, HDV = HDV_;
+  using Cf = TcCfg<HDK, HDV>;
+  __nv_bfloat16* out;
+  int64_t os, ohs;
+  const int32_t* cu;
+  int nq, nkv, nseq, mblocks, total;
+  int64_t qhs, khs, vhs;
+  float scale_log2;
+  int window, sinks, out_cols;
+
+  struct Item {
+    int n;                       // key tiles
+    int h, kvh, start, len, m0;  // m0: first query position
+    int head, first;             // sink tiles, and the window's first tile
+    int window, sinks;
+  };
+
+  struct Cursor {
+    const Window& p;
+    int w;
+    B200_DEV explicit Cursor(const Window& q) : p(q), w(blockIdx.x) {}
+    B200_DEV bool next(Item& it, unsigned* err) {
+      const int per_m = p.nq * p.nseq, W = p.mblocks * per_m;
+      for (; w < W; w += gridDim.x) {
+        const int m = p.mblocks - 1 - w / per_m, r = w % per_m;
+        it.h = r % p.nq;
+        const int sq = r / p.nq;
+        it.start = p.cu[sq];
+        it.len = p.cu[sq + 1] - it.start;
+        it.m0 = m * kTile;
+        if (it.start < 0 || it.len > p.total - it.start) {  // rows outside the operands
+          raise_error(err, DEV_ERR_BAD_INDEX);
+          continue;
+        }
+        if (it.m0 >= it.len) continue;
+        it.kvh = it.h / (p.nq / p.nkv);
+        it.first = max(0, it.m0 - p.window + 1) / kTile;
+        it.head = min((p.sinks + kTile - 1) / kTile, it.first);
+        it.n = it.head + m - it.first + 1;
+        it.window = p.window;
+        it.sinks = p.sinks;
+        w += gridDim.x;
+        return true;
+      }
+      return false;
+    }
+  };
+
+  B200_DEV static int key0(const Item& it, int j) { return (j < it.head ? j : it.first + j - it.head) * kTile; }
+  B200_DEV static bool sees(const Item& it, int row, int key) {
+    const int i = it.m0 + row;
+    return key <= i && key < it.len && (i - key < it.window || key < it.sinks);
+  }
+  B200_DEV static bool whole(const Item& it, int key, int keys) {
+    return key + keys - 1 <= it.m0 && key + keys <= it.len &&
+           (it.m0 + kTile - 1 - key < it.window || key + keys <= it.sinks);
+  }
+  B200_DEV static void load_q(const Window& p, const Item& it, uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, Cf::TILE_QK);
+    if (HEADS3D) tma_load_3d(dst, map, bar, 0, it.h, it.start + it.m0);
+    else
+      for (int x = 0; x < Cf::BOXES_QK; ++x)
+        tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.h * p.qhs) + 64 * x, it.start + it.m0);
+  }
+  B200_DEV static void load_k(const Window& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar, unsigned*) {
+    mbar_arrive_expect_tx(bar, Cf::TILE_QK);
+    if (HEADS3D) tma_load_3d(dst, map, bar, 0, it.kvh, it.start + key0(it, j));
+    else
+      for (int x = 0; x < Cf::BOXES_QK; ++x)
+        tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.kvh * p.khs) + 64 * x, it.start + key0(it, j));
+  }
+  B200_DEV static void load_v(const Window& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar, unsigned*) {
+    mbar_arrive_expect_tx(bar, Cf::TILE_V);
+    if (HEADS3D) tma_load_3d(dst, map, bar, 0, it.kvh, it.start + key0(it, j));
+    else
+      for (int x = 0; x < Cf::BOXES_V; ++x)
+        tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.kvh * p.vhs) + 64 * x, it.start + key0(it, j));
+  }
+  // O / l from TMEM as bf16 rows, this thread's half of the columns
+  B200_DEV static void store(const Window& p, const Item& it, int row, int half, float, float l, uint32_t tO) {
+    const float inv = 1.f / l;  // every row sees itself
+    const bool valid = it.m0 + row < it.len;
+    __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.m0 + row : 0)) * p.os + (int64_t)it.h * p.ohs + half * (HDV / 2);
+#pragma unroll 1
+    for (int c = 0; c < HDV / 64; ++c) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tO + c * 32, r);
+      tmem_ld_wait();
+      if (valid) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (HEADS3D && half * (HDV / 2) + c * 32 + k * 8 >= p.out_cols) break;
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[8 * k + i]) * inv;
+          *reinterpret_cast<uint4*>(o + c * 32 + k * 8) = pack8(f);
+        }
+      }
+    }
+  }
+};
+
+}  // namespace
+
+extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_t q_head_stride, const void* k,
+                                         int64_t k_stride, int64_t k_head_stride, const void* v, int64_t v_stride,
+                                         int64_t v_head_stride, void* out, int64_t out_stride,
+                                         int64_t out_head_stride, const int32_t* cu_seqlens, int num_seqs,
+                                         int max_seqlen, int64_t total_tokens, int nq, int nkv, int head_dim_qk,
+                                         int head_dim_v, float scale, int window, int sinks, b200_stream_t stream) {
+  if (!q || !k || !v || !out || !cu_seqlens || num_seqs < 0 || max_seqlen < 0 || total_tokens < 0 || nq <= 0 ||
+      nkv <= 0 || nq % nkv || window <= 0 || sinks < 0 || !(scale > 0.f && scale < INFINITY))
+    return B200_ERROR_INVALID_PARAM;
+  const int hd = head_dim_qk, hdv = head_dim_v;
+  if (!((hd == hdv && (hd == 128 || hd == 64 || hd == 32 || hd == 16)) || (hd == 192 && hdv == 128)))
+    return B200_ERROR_UNSUPPORTED;
+  for (int64_t s : {q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, out_stride,
+                    out_head_stride})
+    if (s < 0 || s % 8) return B200_ERROR_INVALID_PARAM;
+  for (const void* x : {q, k, v, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(x) & 15u) return B200_ERROR_INVALID_PARAM;
+  if (reinterpret_cast<uintptr_t>(cu_seqlens) & 3u) return B200_ERROR_INVALID_PARAM;
+  const int64_t qcols = (int64_t)(nq - 1) * q_head_stride + hd, kcols = (int64_t)(nkv - 1) * k_head_stride + hd,
+                vcols = (int64_t)(nkv - 1) * v_head_stride + hdv;
+  if (q_stride < qcols || k_stride < kcols || v_stride < vcols ||
+      out_stride < (int64_t)(nq - 1) * out_head_stride + hdv)
+    return B200_ERROR_INVALID_PARAM;
+  if (num_seqs == 0 || max_seqlen == 0 || total_tokens == 0) return B200_OK;
+  const int mblocks = (int)(((int64_t)max_seqlen + kTile - 1) / kTile);
+  const int64_t items = (int64_t)mblocks * nq * num_seqs;
+  if (total_tokens > INT32_MAX - kTile || qcols > INT32_MAX || kcols > INT32_MAX || vcols > INT32_MAX ||
+      items > INT32_MAX - 4096 || max_seqlen > INT32_MAX - kTile)
+    return B200_ERROR_UNSUPPORTED;
+  // a window or sinks behind the longest prompt change nothing; kept small so that sums of positions fit
+  window = std::min(window, max_seqlen);
+  sinks = std::min(sinks, max_seqlen);
+  const int grid = (int)std::min<int64_t>(items, sm_count());
+  CUtensorMap mq, mk, mv;
+  auto run = [&](auto prob, int cols) {
+    prob.out = static_cast<__nv_bfloat16*>(out);
+    prob.os = out_stride;
+    prob.ohs = out_head_stride;
+    prob.cu = cu_seqlens;
+    prob.nq = nq;
+    prob.nkv = nkv;
+    prob.nseq = num_seqs;
+    prob.mblocks = mblocks;
+    prob.total = (int)total_tokens;
+    prob.qhs = q_head_stride;
+    prob.khs = k_head_stride;
+    prob.vhs = v_head_stride;
+    prob.scale_log2 = scale * 1.4426950408889634f;
+    prob.window = window;
+    prob.sinks = sinks;
+    prob.out_cols = cols;
+    return launch_items(mq, mk, mv, prob, grid, stream);
+  };
+  if (hd < 64) {
+    if (!make_map_heads(&mq, q, total_tokens, nq, hd, q_head_stride, q_stride) ||
+        !make_map_heads(&mk, k, total_tokens, nkv, hd, k_head_stride, k_stride) ||
+        !make_map_heads(&mv, v, total_tokens, nkv, hd, v_head_stride, v_stride))
+      return B200_ERROR_UNSUPPORTED;
+    return run(Window<64, 64, true>{}, hd);
+  }
+  if (!make_map(&mq, q, total_tokens, qcols, q_stride) || !make_map(&mk, k, total_tokens, kcols, k_stride) ||
+      !make_map(&mv, v, total_tokens, vcols, v_stride))
+    return B200_ERROR_UNSUPPORTED;
+  if (hd == 192) return run(Window<192, 128, false>{}, hdv);
+  if (hd == 128) return run(Window<128, 128, false>{}, hdv);
+  return run(Window<64, 64, false>{}, hdv);
+}

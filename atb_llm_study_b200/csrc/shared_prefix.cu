@@ -1,0 +1,212 @@
+// Single-token attention of a batch whose sequences share a long prefix, the
+// prefix computed once for all.
+//
+//   out = (2^(lse_0 - M) o_0 + sum_i 2^(lse_i - M) o_i) / (the weights' sum)
+//
+// with o_0 the attention over the sequence's own tokens, o_i over stretches of
+// the prefix and lse their log2 sums: softmax over both is the sum of the parts
+// weighted by their share of the whole sum.
+//
+// One token a sequence reads the cache once for 4 flops a byte and head, and a
+// prefix in every sequence's table is read batch times.  Taken together, the
+// batch's query heads of a kv head are the rows of a matrix product: the prefix
+// is read once, and with 64 sequences of 4 heads a kv head the operations (256
+// a byte) reach the tensor cores' rate at the time that the bytes take.  So
+// this half runs on tcgen05 (tc_items.cuh), 128 rows a tile, the items' key
+// tiles dealt evenly over the SMs, each stretch leaving a part in 32 bits; the
+// kernel for the sequences' own tokens joins them (paged_window.cu), two
+// launches in all.
+#include <algorithm>
+
+#include "shared_prefix.h"
+#include "tc_items.cuh"
+
+using namespace b200;
+
+namespace {
+
+template <int HD>
+struct Prefix {
+  static constexpr int HDK = HD, HDV = HD;
+  using Cf = TcCfg<HD, HD>;
+  PrefixParts at;
+  const int32_t* blocks;
+  int64_t num_blocks;
+  int nkv, block_size, batch;
+  float scale_log2;
+
+  struct Item {
+    int n;       // key tiles of this stretch
+    int first;   // the first of them
+    int length;  // of the prefix
+    int kvh, row_tile, slot;
+  };
+
+  struct Cursor {
+    const Prefix& p;
+    int length;
+    int64_t K, unit, end;
+    B200_DEV explicit Cursor(const Prefix& q) : p(q) {
+      length = prefix_length(p.at);
+      K = (length + kTile - 1) / kTile;
+      const PrefixDeal deal(p.at, K * p.nkv * p.at.row_tiles);
+      const bool has = blockIdx.x < deal.W;
+      unit = has ? deal.first_unit(blockIdx.x) : 0;
+      end = has ? deal.first_unit(blockIdx.x + 1) : 0;
+    }
+    B200_DEV bool next(Item& it, unsigned*) {
+      if (unit >= end) return false;
+      const int item = (int)(unit / K);
+      it.first = (int)(unit % K);
+      it.n = (int)min(end - unit, K - it.first);
+      it.length = length;
+      it.kvh = item / p.at.row_tiles;
+      it.row_tile = item % p.at.row_tiles;
+      it.slot = blockIdx.x + item;
+      unit += it.n;
+      return true;
+    }
+  };
+
+  B200_DEV static int key0(const Item& it, int j) { return (it.first + j) * kTile; }
+  B200_DEV static bool sees(const Item& it, int, int key) { return key < it.length; }
+  B200_DEV static bool whole(const Item& it, int key, int keys) { return key + keys <= it.length; }
+  // box rows are the group's heads of per_tile sequences; rows behind them are not written, and not used
+  B200_DEV static void load_q(const Prefix& p, const Item& it, uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, Cf::BOXES_QK * p.at.per_tile * p.at.group * 128);
+    for (int x = 0; x < Cf::BOXES_QK; ++x)
+      tma_load_3d(dst + x * kBoxBytes, map, bar, 64 * x, it.kvh * p.at.group, it.row_tile * p.at.per_tile);
+  }
+  // a tile is one block of 128 tokens or two of 64, of which the second may lie behind the prefix: it is not loaded,
+  // and its keys are hidden like the rest of a last block
+  B200_DEV static void load(const Prefix& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
+                            uint64_t* bar, unsigned* err) {
+    const int key = key0(it, j), per = kTile / p.block_size;
+    const int n = min(per, (it.length - key + p.block_size - 1) / p.block_size);
+    mbar_arrive_expect_tx(bar, n * Cf::BOXES_QK * p.block_size * 128);
+    for (int i = 0; i < n; ++i) {
+      int blk = p.blocks[key / p.block_size + i];
+      if (blk < 0 || blk >= p.num_blocks) {
+        raise_error(err, DEV_ERR_BAD_INDEX);
+        blk = 0;
+      }
+      const int row = (blk * p.nkv + it.kvh) * p.block_size;
+      for (int x = 0; x < Cf::BOXES_QK; ++x)
+        tma_load_2d(dst + x * kBoxBytes + i * p.block_size * 128, map, bar, 64 * x, row);
+    }
+  }
+  B200_DEV static void load_k(const Prefix& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar, unsigned* err) {
+    load(p, it, j, dst, map, bar, err);
+  }
+  B200_DEV static void load_v(const Prefix& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar, unsigned* err) {
+    load(p, it, j, dst, map, bar, err);
+  }
+  B200_DEV static void store(const Prefix& p, const Item& it, int row, int half, float m, float l, uint32_t tO) {
+    const int seqs = min(p.at.per_tile, p.batch - it.row_tile * p.at.per_tile);
+    const bool valid = row < seqs * p.at.group;
+    const float inv = 1.f / l;  // every row sees the stretch's keys
+    float* o = p.at.parts + ((int64_t)it.slot * kTile + row) * HD + half * (HD / 2);
+    if (valid && half == 0) p.at.lse[(int64_t)it.slot * kTile + row] = m + log2f(l);
+#pragma unroll 1
+    for (int c = 0; c < HD / 64; ++c) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tO + c * 32, r);
+      tmem_ld_wait();
+      if (valid) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          Words8 w;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w.w[i] = __float_as_uint(__uint_as_float(r[8 * k + i]) * inv);
+          store_32(o + c * 32 + k * 8, w);
+        }
+      }
+    }
+  }
+};
+
+struct Plan {
+  int per_tile, row_tiles, workers;
+  int64_t slots;
+};
+
+// SMs share the key tiles evenly, with no CTA left without one.
+Plan prefix_plan(int batch, int nq, int nkv, int max_prefix) {
+  Plan p;
+  p.per_tile = kTile / (nq / nkv);
+  p.row_tiles = (batch + p.per_tile - 1) / p.per_tile;
+  const int64_t items = (int64_t)nkv * p.row_tiles, units = items * ((max_prefix + (int64_t)kTile - 1) / kTile);
+  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(units, sm_count()));
+  p.slots = p.workers + items;
+  return p;
+}
+
+int64_t plan_bytes(const Plan& p, int head_dim) { return p.slots * kTile * (head_dim + 1) * (int64_t)sizeof(float); }
+
+template <int HD>
+int launch_prefix(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, int nq,
+                  const Prefix<HD>& p, int64_t rows, cudaStream_t stream) {
+  CUtensorMap mq, mk, mv;
+  if (!encode_tiled_3d(&mq, q, HD, nq, p.batch, HD * 2, q_stride * 2, 64, p.at.group, p.at.per_tile) ||
+      !encode_tiled_2d(&mk, k_cache, HD, rows, HD * 2, 64, p.block_size) ||
+      !encode_tiled_2d(&mv, v_cache, HD, rows, HD * 2, 64, p.block_size))
+    return B200_ERROR_UNSUPPORTED;
+  return launch_items(mq, mk, mv, p, p.at.workers, stream);
+}
+
+}  // namespace
+
+extern "C" int64_t b200_paged_decode_shared_workspace_bytes(int batch, int nq, int nkv, int head_dim, int max_prefix) {
+  if (batch <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > kTile || (head_dim != 64 && head_dim != 128) ||
+      max_prefix <= 0)
+    return 0;
+  return plan_bytes(prefix_plan(batch, nq, nkv, max_prefix), head_dim);
+}
+
+extern "C" int b200_paged_decode_shared(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                                        const int32_t* prefix_blocks, const int32_t* prefix_len, int max_prefix,
+                                        const int32_t* block_tables, int max_blocks_per_seq,
+                                        const int32_t* context_lens, int max_context, int batch, int nq, int nkv,
+                                        int head_dim, int block_size, int64_t num_blocks, float scale, void* out,
+                                        int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                        b200_stream_t stream) {
+  const int rc = paged_window_check(q, q_stride, k_cache, v_cache, block_tables, max_blocks_per_seq, context_lens,
+                                    batch, nq, nkv, head_dim, block_size, num_blocks, scale, out, out_stride,
+                                    max_context);
+  if (rc != B200_OK) return rc;
+  if (max_prefix < 0 || (max_prefix > 0 && (!prefix_blocks || !prefix_len)) ||
+      (reinterpret_cast<uintptr_t>(prefix_blocks) & 3u) || (reinterpret_cast<uintptr_t>(prefix_len) & 3u))
+    return B200_ERROR_INVALID_PARAM;
+  if (nq / nkv > kTile || max_prefix > INT32_MAX - 256) return B200_ERROR_UNSUPPORTED;
+  if (batch == 0) return B200_OK;
+  PrefixParts at{};
+  if (max_prefix > 0) {
+    const Plan plan = prefix_plan(batch, nq, nkv, max_prefix);
+    if (!workspace || workspace_bytes < plan_bytes(plan, head_dim) || (reinterpret_cast<uintptr_t>(workspace) & 31u))
+      return B200_ERROR_INVALID_PARAM;
+    at.parts = static_cast<float*>(workspace);
+    at.lse = at.parts + plan.slots * kTile * head_dim;
+    at.length = prefix_len;
+    at.max_length = max_prefix;
+    at.workers = plan.workers;
+    at.row_tiles = plan.row_tiles;
+    at.per_tile = plan.per_tile;
+    at.group = nq / nkv;
+    const int64_t rows = num_blocks * nkv * block_size;
+    const float sl2 = scale * 1.4426950408889634f;
+    const int r = head_dim == 128
+                      ? launch_prefix<128>(q, q_stride, k_cache, v_cache, nq,
+                                           Prefix<128>{at, prefix_blocks, num_blocks, nkv, block_size, batch, sl2},
+                                           rows, stream)
+                      : launch_prefix<64>(q, q_stride, k_cache, v_cache, nq,
+                                          Prefix<64>{at, prefix_blocks, num_blocks, nkv, block_size, batch, sl2},
+                                          rows, stream);
+    if (r != B200_OK) return r;
+  }
+  // the sequences' own tokens: a window of all of them
+  return paged_window_launch(q, q_stride, k_cache, v_cache, block_tables, max_blocks_per_seq, context_lens, batch, nq,
+                             nkv, head_dim, block_size, num_blocks, scale, INT32_MAX, 0, out, out_stride, max_context,
+                             at, stream);
+}

@@ -1,0 +1,73 @@
+// The parts of a shared prefix's attention, as the kernel that computes them
+// (shared_prefix.cu) leaves them and the one that joins them with each
+// sequence's own tokens (paged_window.cu) reads them.
+//
+// Query rows are the batch's heads of one kv head: per_tile sequences of
+// `group` heads fill a 128-row tile.  An item is a (kv head, row tile); its
+// prefix has K = ceil(length / 128) key tiles.  The items' key tiles in a row,
+// U of them, are dealt to W = min(workers, U) CTAs in equal stretches, worker c
+// taking [c U / W, (c + 1) U / W), so each has a tile at least.  Each stretch of
+// an item is a part; the part of worker c in item i lies in slot c + i: of two
+// consecutive parts the later has a larger worker or item.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200 {
+
+struct PrefixParts {
+  float* parts;  // [slots][128][head_dim] outputs over their sums
+  float* lse;    // [slots][128] log2 of the sums, with their maximum; -inf: no key
+  const int32_t* length;
+  int max_length;
+  int workers, row_tiles, per_tile, group;
+};
+
+B200_DEV int prefix_length(const PrefixParts& p) { return max(0, min(*p.length, p.max_length)); }
+
+// The stretches of U units: how many, the first unit of stretch c, the stretch of unit u.
+struct PrefixDeal {
+  int64_t U, W;
+  B200_DEV PrefixDeal(const PrefixParts& p, int64_t units) : U(units), W(min((int64_t)p.workers, units)) {}
+  B200_DEV int64_t first_unit(int64_t c) const { return c * U / W; }
+  B200_DEV int worker(int64_t u) const { return (int)(((u + 1) * W - 1) / U); }
+};
+
+// The parts of one sequence's heads [first_head, ..) of a kv head.
+struct PrefixSpan {
+  const float* parts = nullptr;
+  const float* lse_at = nullptr;
+  int count = 0;
+  B200_DEV float lse(int k, int row) const { return lse_at[k * 128 + row]; }
+  B200_DEV float out(int k, int row, int head_dim, int d) const { return parts[(k * 128 + row) * head_dim + d]; }
+};
+
+B200_DEV PrefixSpan prefix_span(const PrefixParts& p, int sequence, int kv_head, int nkv, int first_head, int head_dim) {
+  PrefixSpan s;
+  const int64_t K = (prefix_length(p) + 127) / 128;
+  if (K == 0) return s;
+  const int item = kv_head * p.row_tiles + sequence / p.per_tile;
+  const PrefixDeal deal(p, K * nkv * p.row_tiles);
+  const int w0 = deal.worker(item * K), w1 = deal.worker(item * K + K - 1);
+  const int row = (sequence % p.per_tile) * p.group + first_head;
+  s.count = w1 - w0 + 1;
+  s.parts = p.parts + ((int64_t)(w0 + item) * 128 + row) * head_dim;
+  s.lse_at = p.lse + (int64_t)(w0 + item) * 128 + row;
+  return s;
+}
+
+// Single-token attention over the sequences' own tokens (paged_window.cu), joined with a prefix's parts when there are
+// any (prefix.parts, of the kernel launched just before).  Arguments are checked by the callers.
+int paged_window_launch(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                        const int32_t* block_tables, int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                        int nq, int nkv, int head_dim, int block_size, int64_t num_blocks, float scale, int window,
+                        int sinks, void* out, int64_t out_stride, int max_context, const PrefixParts& prefix,
+                        cudaStream_t stream);
+
+// The checks that both entry points make of their common arguments (a status, B200_OK to go on).
+int paged_window_check(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                       const int32_t* block_tables, int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                       int nq, int nkv, int head_dim, int block_size, int64_t num_blocks, float scale, const void* out,
+                       int64_t out_stride, int max_context);
+
+}  // namespace b200

@@ -370,6 +370,25 @@ B200_API int b200_flash_prefill_packed(const void* q, int64_t q_stride, int64_t 
                                        int nq, int nkv, int head_dim_qk, int head_dim_v, float scale, int causal,
                                        b200_stream_t stream);
 
+/* b200_flash_prefill_packed with a sliding window and a few first tokens that
+ * stay visible (sinks): query i of a sequence sees the keys j <= i with
+ * i - j < window (>= 1) or j < sinks (>= 0).  Key tiles without a visible pair
+ * are not read, so the time follows the window.  Same operands, head widths
+ * (others are B200_ERROR_UNSUPPORTED), strides and alignment; scale > 0; all on
+ * the tcgen05 tensor cores.  Rows of out that belong to no sequence, and of a
+ * sequence behind max_seqlen, are left as they are; a sequence outside
+ * [0, total_tokens) is left out and sets the device error word.  What a row
+ * does not see does not reach it, NaN and infinities included; a row that sees
+ * a value row with one is not finite.  Extends SelfAttentionOp::Create
+ * (PA_ENCODER) (atb_cpp_llm/src/ops/self_attention_op.cpp:8-30), whose only
+ * mask is the causal one. */
+B200_API int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_t q_head_stride, const void* k,
+                                       int64_t k_stride, int64_t k_head_stride, const void* v, int64_t v_stride,
+                                       int64_t v_head_stride, void* out, int64_t out_stride, int64_t out_head_stride,
+                                       const int32_t* cu_seqlens, int num_seqs, int max_seqlen, int64_t total_tokens,
+                                       int nq, int nkv, int head_dim_qk, int head_dim_v, float scale, int window,
+                                       int sinks, b200_stream_t stream);
+
 /* ---- multi-head latent attention (DeepSeek-V2): fills the reference's stubs
  * MlaAttentionBuilder (atb_cpp_llm/src/components/common/attention_builder.h:60-69)
  * and AttnConfig.kv_lora_rank / q_lora_rank (atb_cpp_llm/include/atb_llm/layer_desc.h:47-49).
@@ -453,12 +472,99 @@ B200_API int b200_paged_decode_noalloc(const void* q, int64_t q_stride, const vo
                                        int64_t out_stride, int max_context, b200_stream_t stream);
 B200_API int64_t b200_paged_decode_noalloc_max_scratch_bytes(void);
 
+/* b200_paged_decode with a sliding window and sinks: the token of sequence b
+ * (the last of its context_lens[b]) sees the cached positions
+ * j < context_lens[b] with j >= context_lens[b] - window or j < sinks;
+ * window >= 1, sinks >= 0, scale > 0.  Only blocks with a visible position are
+ * looked up, so table entries of the others may be stale and their blocks
+ * given to other sequences; what lies in hidden positions (NaN included) does
+ * not matter.  A context of 0 gives zeros; one outside the table is clamped,
+ * and a visible entry outside [0, num_blocks) read as block 0, and both set the
+ * device error word.  head_dim 64 or 128, block_size 64 or 128, any
+ * nq % nkv == 0; q_stride a multiple of 8, q and the caches 16-byte aligned.
+ * max_context (the longest context, host) picks how many CTAs share a sequence;
+ * a longer one is still right.  Takes no workspace: calls may overlap and be
+ * captured freely.  No reference counterpart
+ * (atb_cpp_llm/include/atb_llm/kv_cache.h:23-35). */
+B200_API int b200_paged_decode_window(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                                      const int32_t* block_tables, int max_blocks_per_seq,
+                                      const int32_t* context_lens, int batch, int nq, int nkv, int head_dim,
+                                      int block_size, int64_t num_blocks, float scale, int window, int sinks,
+                                      void* out, int64_t out_stride, int max_context, b200_stream_t stream);
+
+/* Decode attention of a batch whose sequences all begin with the same
+ * *prefix_len tokens, whose K and V are read once for all of them: sequence b
+ * attends to the prefix (positions 0 .. *prefix_len - 1 through prefix_blocks,
+ * [ceil(max_prefix / block_size)]) and to its own context_lens[b] tokens behind
+ * it (through block_tables[b], position 0 being the first own token; both may
+ * be empty, and with both empty the output is zeros).  The blocks lie in the
+ * same caches; the prefix need not end with a block.  prefix_len is a device
+ * int32, clamped to [0, max_prefix] (host), so a captured call follows it.
+ * Other arguments, limits and the treatment of bad entries and hidden
+ * positions are b200_paged_decode_window's, with nq / nkv <= 128.  workspace:
+ * b200_paged_decode_shared_workspace_bytes(), 32-byte aligned, required when
+ * max_prefix > 0; calls that overlap on the GPU must not share it.  Two
+ * launches, between which no other thread may launch on the stream.  No
+ * reference counterpart (atb_cpp_llm/include/atb_llm/kv_cache.h:23-35). */
+B200_API int64_t b200_paged_decode_shared_workspace_bytes(int batch, int nq, int nkv, int head_dim, int max_prefix);
+B200_API int b200_paged_decode_shared(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                                      const int32_t* prefix_blocks, const int32_t* prefix_len, int max_prefix,
+                                      const int32_t* block_tables, int max_blocks_per_seq,
+                                      const int32_t* context_lens, int max_context, int batch, int nq, int nkv,
+                                      int head_dim, int block_size, int64_t num_blocks, float scale, void* out,
+                                      int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                      b200_stream_t stream);
+
 /* slots[t] = block_tables[seq_ids[t], positions[t] / block_size] * block_size
  *            + positions[t] % block_size   (int64, bit-exact).
  * No reference counterpart (the reference has no paged KV cache,
  * atb_cpp_llm/include/atb_llm/kv_cache.h:23-35). */
 B200_API int b200_slot_mapping(const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_ids,
                       const int64_t* positions, int64_t T, int block_size, int64_t* slots, b200_stream_t stream);
+
+/* A step's block tables and slots from its request lengths, on the GPU.
+ * Sequence i (row i of block_tables [num_seqs, max_blocks_per_seq]) holds
+ * cached_lens[i] tokens in its first ceil(cached / block_size) entries and gets
+ * new_lens[i] (0 or more) behind them.  The blocks that takes come off the top
+ * of the free list (free_blocks [num_blocks], *free_count of them free):
+ * free_blocks[count - 1] is the first block of the first sequence that needs
+ * one, and so on in sequence and then position order.  Written: the new table
+ * entries, context_lens[i] = cached + new, cu_seqlens [num_seqs + 1] (sums of
+ * new_lens), for each new token t < cu_seqlens[num_seqs] its position and cache
+ * slot (b200_qk_norm_rope's slot_mapping), for t up to `capacity` (a batch
+ * padded for a captured graph) position 0 and slot -1, and *free_left.
+ * When the free blocks do not suffice nothing is taken: *missing is the number
+ * of blocks that lack (0 otherwise), the tables stay, context_lens = cached_lens,
+ * cu_seqlens = 0, all slots -1.  The same with *missing = -1 and the device
+ * error word when a length is negative or does not fit the table, the tokens
+ * exceed `capacity` or *free_count is not in [0, num_blocks].  A block outside
+ * [0, num_blocks), free or in a table, gives slots of -1 and sets the error word.
+ * cu_seqlens, positions, slots and missing may be NULL (and with no sequences
+ * the arrays that would be empty); context_lens may be cached_lens, and
+ * free_left free_count; nothing else may overlap.
+ * num_seqs <= 8192.  Replaces KVCacheManager's allocation
+ * (atb_cpp_llm/src/core/kv_cache_manager.h:25-76), which the reference only
+ * declares. */
+B200_API int b200_block_tables_extend(const int32_t* cached_lens, const int32_t* new_lens, int num_seqs,
+                                      int block_size, int32_t* block_tables, int max_blocks_per_seq,
+                                      const int32_t* free_blocks, const int32_t* free_count, int64_t num_blocks,
+                                      int32_t* context_lens, int32_t* cu_seqlens, int64_t* positions, int64_t* slots,
+                                      int64_t capacity, int32_t* free_left, int32_t* missing, b200_stream_t stream);
+
+/* The way back: sequence i keeps its first min(cached_lens[i], keep_lens[i])
+ * tokens (0: it has ended; fewer than cached: draft tokens were rejected), and
+ * the blocks behind them go on top of the free list [free_capacity], in
+ * sequence and then position order.  Written: lens (may be cached_lens),
+ * free_blocks[*free_count ..) and *free_left (may be free_count); table entries
+ * stay, and mean nothing behind ceil(lens / block_size).  A negative or too long
+ * length, or a list that would overflow, leaves everything as it is (lens =
+ * cached_lens) and sets the device error word; so does a block outside
+ * [0, num_blocks), which is handed on.  Replaces KVCacheManager's release
+ * (atb_cpp_llm/src/core/kv_cache_manager.h:25-76). */
+B200_API int b200_block_tables_release(const int32_t* cached_lens, const int32_t* keep_lens, int num_seqs,
+                                       int block_size, const int32_t* block_tables, int max_blocks_per_seq,
+                                       int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
+                                       int64_t num_blocks, int32_t* lens, int32_t* free_left, b200_stream_t stream);
 
 /* ------------------------------------------------------------ elementwise */
 
@@ -477,6 +583,36 @@ B200_API int b200_scatter_add_rows(void* hidden, int64_t rows, int64_t dim, cons
 
 /* out[r] = argmax_j logits[r, j] (lowest index on ties), logits [rows, vocab] bf16. */
 B200_API int b200_argmax(const void* logits, int64_t rows, int64_t vocab, int64_t ld, int64_t* out, b200_stream_t stream);
+
+/* A decode step's logits [rows, ld] (bf16) made ready for the choice of a token.
+ * Per row, for token v with x = logits[v], in double:
+ *   history [rows, history_ld] (token ids, lens[row] of them, the first
+ *   prompt_lens[row] the prompt's; prompt_lens NULL: none): if v occurs,
+ *   x = x > 0 ? x / repetition : x * repetition; then, with said the times it
+ *   occurs behind the prompt, x -= frequency * said, and x -= presence if said
+ *   (each a value a row, fp32, NULL: not applied);
+ *   x += the sum of the bias_values listed for v, in the order of the list (entries
+ *   bias_offsets[row] .. bias_offsets[row + 1] of bias_ids / bias_values);
+ *   x = -inf unless bit v % 32 of word v / 32 of the row's mask is set (mask
+ *   [num_masks, mask_ld] words; the row's is mask_rows[row], -1 for none, or
+ *   its own when mask_rows is NULL).
+ * out [rows, ldo] (bf16, one rounding; may be logits; NULL: not written)
+ * receives x, next [rows] (NULL: not written) the token with the largest x
+ * before the rounding: the lowest on ties, never one at NaN or -inf, -1 when
+ * there is no other.  Tokens that neither the history, a bias nor the mask
+ * touches keep their bits.  Each of history, bias_offsets and mask may be NULL
+ * (with what belongs to it).  Ids outside [0, vocab) are passed over, lengths
+ * clamped to history_ld and rows of no mask not masked; all three set the device
+ * error word.  Any stride; rows whose pointers and strides are multiples of 16
+ * bytes are faster.  Up to 900 thousand tokens (half with both a history and
+ * biases).  Stands before b200_argmax; the reference chooses no token
+ * (atb_cpp_llm/include/atb_llm/model.h:47-50). */
+B200_API int b200_logits_process(const void* logits, int64_t ld, int64_t rows, int64_t vocab, const int32_t* history,
+                                 int64_t history_ld, const int32_t* prompt_lens, const int32_t* lens,
+                                 const float* repetition, const float* frequency, const float* presence,
+                                 const int32_t* bias_offsets, const int32_t* bias_ids, const float* bias_values,
+                                 const uint32_t* mask, int64_t mask_ld, int64_t num_masks, const int32_t* mask_rows,
+                                 void* out, int64_t ldo, int64_t* next, b200_stream_t stream);
 
 /* -------------------------------------------------------- image preprocess */
 
