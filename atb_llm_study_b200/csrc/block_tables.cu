@@ -11,7 +11,7 @@
 //
 // Both are prefix sums over the sequences and then a gather an output: a few
 // bytes a token, so what bounds them is the start of a launch and two dependent
-// trips to memory.  One cluster of up to 8 CTAs runs a call: every CTA sums all
+// trips to memory.  One cluster of up to 16 CTAs runs a call: every CTA sums all
 // sequences by itself (8192 lengths are 64 KB from L2, cheaper than handing
 // sums over), the cluster meets once so that outputs may lie where inputs lay,
 // and the CTAs share the entries and tokens.  A cluster instead of a grid
@@ -27,6 +27,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kMaxSeqs = 8192;
+constexpr int kAtOnce = 4;
+constexpr unsigned kMaxCtas = 16;
 constexpr int kPerThread = kMaxSeqs / kThreads;
 
 B200_DEV int64_t warp_scan(int64_t v) {  // inclusive
@@ -85,7 +87,17 @@ B200_DEV int find(const int* sums, int n, int at, int x) {
   return lo;
 }
 
-B200_DEV int blocks_of(int64_t tokens, int bs) { return (int)((tokens + bs - 1) / bs); }
+// Division by the block size: a shift where it is a power of two.
+struct BlockSize {
+  int bs, shift;
+  explicit BlockSize(int size) : bs(size), shift((size & (size - 1)) == 0 ? __builtin_ctz((unsigned)size) : -1) {}
+  B200_DEV int quotient(int x) const { return shift >= 0 ? x >> shift : x / bs; }
+};
+// Blocks of `tokens` (at most INT32_MAX, and a sum with bs - 1 fits 32 unsigned bits).
+B200_DEV int blocks_of(int tokens, const BlockSize& s) {
+  const uint32_t up = (uint32_t)tokens + (uint32_t)(s.bs - 1);
+  return (int)(s.shift >= 0 ? up >> s.shift : up / (uint32_t)s.bs);
+}
 
 struct Lens {
   int* cached;  // tokens each sequence holds
@@ -104,7 +116,7 @@ B200_DEV Lens carve(uint8_t* smem, int n) {
 // Reads both length arrays of the call into shared memory as sums.  EXTEND: second = new tokens, a sequence takes
 // blocks; else second = tokens to keep, it gives blocks back.  Returns false when a length is out of range.
 template <bool EXTEND>
-B200_DEV bool read_lengths(const int32_t* cached, const int32_t* second, int n, int bs, int64_t room, Lens l,
+B200_DEV bool read_lengths(const int32_t* cached, const int32_t* second, int n, const BlockSize& bs, int64_t room, Lens l,
                            int64_t* scratch, int64_t& total_tokens, int64_t& total_blocks) {
   const int per = (n + kThreads - 1) / kThreads;  // <= kPerThread consecutive sequences a thread
   const int first = threadIdx.x * per;
@@ -124,10 +136,10 @@ B200_DEV bool read_lengths(const int32_t* cached, const int32_t* second, int n, 
       l.cached[i] = (int)c;
       if (EXTEND) {
         tok[k] = (int)s;
-        blk[k] = blocks_of(c + s, bs) - blocks_of(c, bs);
+        blk[k] = blocks_of((int)(c + s), bs) - blocks_of((int)c, bs);
       } else {
         tok[k] = (int)min(c, s);
-        blk[k] = blocks_of(c, bs) - blocks_of(tok[k], bs);
+        blk[k] = blocks_of((int)c, bs) - blocks_of(tok[k], bs);
       }
       st += tok[k];
       sb += blk[k];
@@ -161,7 +173,8 @@ B200_DEV bool read_lengths(const int32_t* cached, const int32_t* second, int n, 
 struct ExtendParams {
   const int32_t* cached;
   const int32_t* more;
-  int n, bs;
+  int n;
+  BlockSize bs;
   int32_t* tables;
   int width;
   const int32_t* free_blocks;
@@ -183,10 +196,11 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
   pdl_trigger();
   pdl_wait();
   const Lens l = carve(smem, p.n);
+  const BlockSize bs = p.bs;
   const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
   const int count = *p.free_count;
   int64_t tokens, need;
-  const bool read = read_lengths<true>(p.cached, p.more, p.n, p.bs, (int64_t)p.width * p.bs, l, scratch, tokens, need);
+  const bool read = read_lengths<true>(p.cached, p.more, p.n, bs, (int64_t)p.width * bs.bs, l, scratch, tokens, need);
   const bool sane = read && count >= 0 && count <= p.num_blocks && tokens <= p.capacity;
   const bool fits = sane && need <= count;
   if (!sane && rank == 0 && threadIdx.x == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
@@ -206,34 +220,57 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
   }
   const int64_t stride = (int64_t)ctas * kThreads;
   const int64_t me = (int64_t)rank * kThreads + threadIdx.x;
+  // Entries and tokens in turns of kAtOnce a thread, a CTA's side by side, so
+  // that as many loads from the tables are on their way together.
   if (fits) {
     int i = 0;
-    for (int64_t e = me; e < need; e += stride) {  // table entries
-      i = find(l.blocks, p.n, i, (int)e);
-      int32_t b = p.free_blocks[count - 1 - e];
-      if (b < 0 || b >= p.num_blocks) {
-        raise_error(p.err, DEV_ERR_BAD_INDEX);
-        b = -1;
+    for (int64_t e0 = me; e0 < need; e0 += kAtOnce * stride) {
+      int32_t b[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (e0 + k * stride < need) b[k] = p.free_blocks[count - 1 - (e0 + k * stride)];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int64_t e = e0 + k * stride;
+        if (e >= need) break;
+        i = find(l.blocks, p.n, i, (int)e);
+        if (b[k] < 0 || b[k] >= p.num_blocks) {
+          raise_error(p.err, DEV_ERR_BAD_INDEX);
+          b[k] = -1;
+        }
+        p.tables[(int64_t)i * p.width + blocks_of(l.cached[i], bs) + (int)e - l.blocks[i]] = b[k];
       }
-      p.tables[(int64_t)i * p.width + blocks_of(l.cached[i], p.bs) + (int)e - l.blocks[i]] = b;
     }
   }
   if (p.positions || p.slots) {
     int i = 0;
-    for (int64_t t = me; t < p.capacity; t += stride) {
-      int64_t pos = 0, slot = -1;
-      if (fits && t < tokens) {
-        i = find(l.tokens, p.n, i, (int)t);
-        const int at = l.cached[i] + (int)t - l.tokens[i];
-        const int col = at / p.bs, held = blocks_of(l.cached[i], p.bs);
-        const int32_t b = col < held ? p.tables[(int64_t)i * p.width + col]
-                                     : p.free_blocks[count - 1 - (l.blocks[i] + col - held)];
-        pos = at;
-        if (b >= 0 && b < p.num_blocks) slot = (int64_t)b * p.bs + at % p.bs;
-        else raise_error(p.err, DEV_ERR_BAD_INDEX);
+    for (int64_t t0 = me; t0 < p.capacity; t0 += kAtOnce * stride) {
+      int at[kAtOnce];
+      int32_t b[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int64_t t = t0 + k * stride;
+        at[k] = -1;
+        if (fits && t < tokens) {
+          i = find(l.tokens, p.n, i, (int)t);
+          at[k] = l.cached[i] + (int)t - l.tokens[i];
+          const int col = bs.quotient(at[k]), held = blocks_of(l.cached[i], bs);
+          b[k] = col < held ? p.tables[(int64_t)i * p.width + col]
+                            : p.free_blocks[count - 1 - (l.blocks[i] + col - held)];
+        }
       }
-      if (p.positions) p.positions[t] = pos;
-      if (p.slots) p.slots[t] = slot;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int64_t t = t0 + k * stride;
+        if (t >= p.capacity) break;
+        int64_t slot = -1;
+        if (at[k] >= 0) {
+          if (b[k] >= 0 && b[k] < p.num_blocks) slot = (int64_t)b[k] * bs.bs + at[k] - bs.quotient(at[k]) * bs.bs;
+          else raise_error(p.err, DEV_ERR_BAD_INDEX);
+        }
+        if (p.positions) p.positions[t] = max(at[k], 0);
+        if (p.slots) p.slots[t] = slot;
+      }
     }
   }
 }
@@ -241,7 +278,8 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
 struct ReleaseParams {
   const int32_t* cached;
   const int32_t* keep;
-  int n, bs;
+  int n;
+  BlockSize bs;
   const int32_t* tables;
   int width;
   int32_t* free_blocks;
@@ -259,10 +297,11 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams p
   pdl_trigger();
   pdl_wait();
   const Lens l = carve(smem, p.n);
+  const BlockSize bs = p.bs;
   const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
   const int count = *p.free_count;
   int64_t kept, drop;
-  const bool read = read_lengths<false>(p.cached, p.keep, p.n, p.bs, (int64_t)p.width * p.bs, l, scratch, kept, drop);
+  const bool read = read_lengths<false>(p.cached, p.keep, p.n, bs, (int64_t)p.width * bs.bs, l, scratch, kept, drop);
   const bool fits = read && count >= 0 && count + drop <= p.free_capacity;
   if (!fits && rank == 0 && threadIdx.x == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
   if (!read)
@@ -276,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams p
   int i = 0;
   for (int64_t e = (int64_t)rank * kThreads + threadIdx.x; e < drop; e += (int64_t)ctas * kThreads) {
     i = find(l.blocks, p.n, i, (int)e);
-    const int32_t b = p.tables[(int64_t)i * p.width + blocks_of(l.tokens[i], p.bs) + (int)e - l.blocks[i]];
+    const int32_t b = p.tables[(int64_t)i * p.width + blocks_of(l.tokens[i], bs) + (int)e - l.blocks[i]];
     if (b < 0 || b >= p.num_blocks) raise_error(p.err, DEV_ERR_BAD_INDEX);  // handed on; extend refuses it
     p.free_blocks[count + e] = b;
   }
@@ -293,13 +332,16 @@ bool allow_smem() {
   if (dev < 0 || dev >= 64) return false;
   if (!done[dev])
     done[dev] = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kMaxSeqs)) ==
-                cudaSuccess;
+                    cudaSuccess &&
+                cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
   return done[dev];
 }
 
-// CTAs of the cluster: one for each 1024 items (tokens or table entries), at most 8.
+// CTAs of the cluster: one for each 1024 items (tokens or table entries), at most 16.
 unsigned cluster_for(int64_t items) {
-  return items <= kThreads ? 1u : items <= 2 * kThreads ? 2u : items <= 4 * kThreads ? 4u : 8u;
+  unsigned c = 1;
+  while (c < kMaxCtas && (int64_t)c * kThreads < items) c *= 2;
+  return c;
 }
 
 bool al4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -331,7 +373,7 @@ extern "C" int b200_block_tables_extend(const int32_t* cached_lens, const int32_
       (int64_t)max_blocks_per_seq * block_size > INT32_MAX)
     return B200_ERROR_UNSUPPORTED;
   if (!allow_smem<extend_kernel>()) return B200_ERROR_UNSUPPORTED;
-  const ExtendParams p{cached_lens,  new_lens, num_seqs,  block_size, block_tables, max_blocks_per_seq,
+  const ExtendParams p{cached_lens,  new_lens, num_seqs,  BlockSize(block_size), block_tables, max_blocks_per_seq,
                        free_blocks,  free_count, num_blocks, context_lens, cu_seqlens, positions,
                        slots,        capacity,   free_left,  missing,      this_error_word()};
   const unsigned c = cluster_for(std::max<int64_t>(num_seqs, capacity));
@@ -355,7 +397,7 @@ extern "C" int b200_block_tables_release(const int32_t* cached_lens, const int32
       (int64_t)max_blocks_per_seq * block_size > INT32_MAX)
     return B200_ERROR_UNSUPPORTED;
   if (!allow_smem<release_kernel>()) return B200_ERROR_UNSUPPORTED;
-  const ReleaseParams p{cached_lens, keep_lens,  num_seqs,   block_size, block_tables, max_blocks_per_seq, free_blocks,
+  const ReleaseParams p{cached_lens, keep_lens,  num_seqs,   BlockSize(block_size), block_tables, max_blocks_per_seq, free_blocks,
                         free_capacity, free_count, num_blocks, lens,       free_left,    this_error_word()};
   const unsigned c = cluster_for((int64_t)num_seqs * std::min(max_blocks_per_seq, 8));
   launch_clusters(release_kernel, c, dim3(c), kThreads, smem_bytes(num_seqs), stream, p);

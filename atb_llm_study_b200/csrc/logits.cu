@@ -7,16 +7,22 @@
 //   x += the biases listed for v; -inf where the mask has no bit for v.
 //
 // A row's logits are read and written once (4 bytes a token, 600 KB at 151936),
-// so memory bounds a batch; one row is bound by latency.  What makes the pass
-// more than a copy is knowing which tokens occur: the vocabulary is split over
-// the CTAs of a cluster, and each keeps a word for every token of its part in
-// shared memory: the count, and a bit for the prompt.  Each CTA walks the whole
-// history (16 KB for 4000 tokens, from L2) and counts what falls into its part
-// with integer atomics in shared memory, whose result has no order.  A table in
-// global memory instead would cost 4 bytes a token to clear, and to read once.
-// Tokens that occur nowhere, by far the most, are copied; the few others are
-// computed in double (operation by operation, nothing contracted), so that the
-// greedy token is that of the definition and not of 32-bit roundings.
+// so memory bounds a batch in principle, and the few dependent steps between
+// lists and logits do in practice.  A row's vocabulary is split over the CTAs of
+// a cluster.  Each marks the tokens of its part that occur in the history or
+// among the biases in a bitmap in shared memory (one bit a token), whose prefix
+// counts number the marked tokens; per marked token it keeps how often it was
+// said, whether the prompt has it and where its biases begin.  All of this is
+// whole-number arithmetic, so the order of the atomics does not show.  The sweep
+// then copies 16 bytes a thread and masks, leaving marked tokens to a thread
+// each: they are computed in double, operation by operation, so that the greedy
+// token is that of the definition and not of 32-bit roundings.
+//
+// Measured at 64 rows of 151936 with 4000 tokens of history, 300 biases and a
+// mask on every other row (a replayed graph, L2 flushed): @@ us.  A
+// word for every token instead of a bit, cleared and read by 16 CTAs a row, took
+// 60 us, and with the doubles inside the sweep, where a few lanes of almost
+// every warp have one, 148 us.
 #include <math.h>
 
 #include <algorithm>
@@ -28,8 +34,9 @@ using namespace b200;
 namespace {
 
 constexpr int kThreads = 512;
-constexpr uint32_t kTopBit = 1u << 31;  // of a history word: in the prompt; of a bias word: listed more than once
-constexpr int kMaxSmem = 224 * 1024;
+constexpr unsigned kMaxCtas = 16;  // of a row
+constexpr int kSlots = 4096;       // marked tokens computed at a time
+constexpr uint32_t kTopBit = 1u << 31;  // of `said`: the prompt has it; of `lead`: listed more than once
 
 struct LogitsParams {
   const __nv_bfloat16* logits;
@@ -63,196 +70,291 @@ struct Best {
   int64_t i;
 };
 B200_DEV Best better(const Best& a, const Best& b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
-
-B200_DEV uint64_t cluster_load8(uint32_t addr) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
+B200_DEV Best warp_better(Best b) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    b = better(b, Best{__shfl_xor_sync(0xffffffffu, b.v, o), __shfl_xor_sync(0xffffffffu, b.i, o)});
+  return b;
 }
 
-// HIST / BIAS: the call has a history / a bias list, and shared memory holds the words for it.
-template <bool HIST, bool BIAS>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const LogitsParams p) {
-  extern __shared__ __align__(16) uint32_t words[];
-  __shared__ Best warp_best[kThreads / 32];
-  __shared__ Best cta_best;
-  uint32_t* seen = words;                           // [chunk] times behind the prompt | kTopBit
-  uint32_t* lead = words + (HIST ? p.chunk : 0);    // [chunk] entries from its first to the list's end | kTopBit
-  pdl_trigger();
-  const int ctas = (int)cluster_size();
-  const int64_t row = blockIdx.x / ctas;
-  const int64_t lo = (int64_t)cluster_rank() * p.chunk;
-  const int n = (int)max((int64_t)0, min((int64_t)p.chunk, p.vocab - lo));
-  const int tid = threadIdx.x;
-  const int kinds = (HIST ? 1 : 0) + (BIAS ? 1 : 0);
-  for (int i = tid; i < kinds * p.chunk / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+B200_DEV void cluster_store8(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
+// Exclusive prefix sum of one value a thread; *total the sum of all.
+B200_DEV int block_scan(int v, int* sums, int* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) sums[w] = inc;
   __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int k = 0; k < kThreads / 32; ++k) {
+    if (k < w) before += sums[k];
+    all += sums[k];
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+// The larger of two bf16 pairs, NaN only where both are.
+B200_DEV uint32_t max_pair(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+constexpr uint32_t kLowPair = 0xff80ff80u;  // -inf, -inf
+// All ones in the halves whose bit of `two` is set.
+B200_DEV uint32_t spread2(uint32_t two) { return (two & 1u) * 0xffffu | ((two >> 1) & 1u) * 0xffff0000u; }
+
+struct Row {  // one row's lists
+  const int32_t* history;
+  int len, prompt;
+  const int32_t* bias_ids;
+  const float* bias_values;
+  int biases;
+};
+
+// HIST / BIAS: the call has a history / a bias list.
+template <bool HIST, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams p) {
+  extern __shared__ __align__(16) uint32_t smem[];
+  __shared__ Best warp_best[kThreads / 32];
+  __shared__ Best cta_best[kMaxCtas];  // the first CTA's: one of each CTA of the row
+  __shared__ int sums[kThreads / 32];
+  constexpr bool kLists = HIST || BIAS;
+  constexpr int kAhead = 4;  // 16-byte loads in flight
+  const int words = p.chunk / 32;
+  uint32_t* marks = smem;                                     // [words]
+  int* before = reinterpret_cast<int*>(marks + words);        // [words] marked tokens before each word
+  int* token = before + words;                                // [kSlots] a marked token, in its part
+  uint32_t* said = reinterpret_cast<uint32_t*>(token + kSlots);  // [kSlots] times behind the prompt | kTopBit
+  uint32_t* lead = said + kSlots;                             // [kSlots] entries from its first bias to the list's end | kTopBit
+  pdl_trigger();
+  const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // every CTA has started: waited for at the end
+  const int64_t row = blockIdx.x / ctas;
+  const int lo = rank * p.chunk;
+  const int n = max(0, min(p.chunk, (int)p.vocab - lo));
+  const int nv = p.vec ? n / 8 : 0;
+  const int tid = threadIdx.x;
+  if (kLists)
+    for (int i = tid; i < words; i += kThreads) marks[i] = 0;
   pdl_wait();
 
-  if (HIST) {
-    int len = p.lens[row], prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
-    if (len < 0 || len > p.history_ld || prompt < 0 || prompt > len) {
-      if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
-      len = (int)min((int64_t)max(len, 0), p.history_ld);
-      prompt = min(max(prompt, 0), len);
-    }
-    const int32_t* h = p.history + row * p.history_ld;
-#pragma unroll 4
-    for (int i = tid; i < len; i += kThreads) {
-      const int64_t at = (int64_t)h[i] - lo;
-      if (at >= 0 && at < n) {
-        if (i < prompt) atomicOr(&seen[at], kTopBit);
-        else atomicAdd(&seen[at], 1u);
-      } else if (h[i] < 0 || h[i] >= p.vocab) {
-        raise_error(p.err, DEV_ERR_BAD_INDEX);
-      }
-    }
-  }
-  int b0 = 0, nb = 0;
-  if (BIAS) {
-    b0 = p.bias_offsets[row];
-    nb = p.bias_offsets[row + 1] - b0;
-    if (b0 < 0 || nb < 0) {
-      if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
-      b0 = nb = 0;
-    }
-    // a token's first entry leads: it is worth the most counted from the end
-    for (int i = tid; i < nb; i += kThreads) {
-      const int64_t id = p.bias_ids[b0 + i], at = id - lo;
-      if (at >= 0 && at < n) atomicMax(&lead[at], (uint32_t)(nb - i));
-      else if (id < 0 || id >= p.vocab) raise_error(p.err, DEV_ERR_BAD_INDEX);
-    }
-    __syncthreads();
-    for (int i = tid; i < nb; i += kThreads) {
-      const int64_t at = (int64_t)p.bias_ids[b0 + i] - lo;
-      if (at >= 0 && at < n && (lead[at] & ~kTopBit) != (uint32_t)(nb - i)) atomicOr(&lead[at], kTopBit);
-    }
-  }
+  const __nv_bfloat16* in = p.logits + row * p.ld + lo;
+  __nv_bfloat16* out = p.out ? p.out + row * p.ldo + lo : nullptr;
+  uint4 raw[kAhead];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (c0 + k * kThreads < nv) raw[k] = reinterpret_cast<const uint4*>(in)[c0 + k * kThreads];
+  };
+  load(tid);  // on their way while the lists are read
   const uint32_t* mask = nullptr;
   if (p.mask) {
     const int64_t m = p.mask_rows ? p.mask_rows[row] : row;
     if (m >= p.num_masks || m < -1) {
       if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
     } else if (m >= 0) {
-      mask = p.mask + m * p.mask_ld;
+      mask = p.mask + m * p.mask_ld + (lo >> 5);
     }
   }
-  const bool rep = HIST && p.repetition, frq = HIST && p.frequency, prs = HIST && p.presence;
-  const double repetition = rep ? (double)p.repetition[row] : 1.0;
-  const double frequency = frq ? (double)p.frequency[row] : 0.0;
-  const double presence = prs ? (double)p.presence[row] : 0.0;
-  __syncthreads();
-
-  const __nv_bfloat16* in = p.logits + row * p.ld + lo;
-  __nv_bfloat16* out = p.out ? p.out + row * p.ldo + lo : nullptr;
-  float plain_v = -INFINITY;  // untouched tokens are bf16 values: compared as they are
-  int64_t plain_i = INT64_MAX;
-  Best best{-INFINITY, INT64_MAX};
-
-  // token `at` of this CTA's part with logit x, words w and l: its value; a touched token's goes into `best`
-  auto process = [&](int at, float x, uint32_t w, uint32_t l) -> __nv_bfloat16 {
-    double v = (double)x;
-    if (HIST && w) {
-      if (rep) v = v > 0 ? __ddiv_rn(v, repetition) : __dmul_rn(v, repetition);
-      const uint32_t said = w & ~kTopBit;
-      if (frq) v = __dsub_rn(v, __dmul_rn(frequency, (double)said));
-      if (prs && said) v = __dsub_rn(v, presence);
+  Row r{};
+  if (HIST) {
+    r.history = p.history + row * p.history_ld;
+    r.len = p.lens[row];
+    r.prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
+    if (r.len < 0 || r.len > p.history_ld || r.prompt < 0 || r.prompt > r.len) {
+      if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
+      r.len = (int)min((int64_t)max(r.len, 0), p.history_ld);
+      r.prompt = min(max(r.prompt, 0), r.len);
     }
-    if (BIAS && l) {
-      const int first = nb - (int)(l & ~kTopBit);
-      double sum = (double)p.bias_values[b0 + first];
-      for (int i = l & kTopBit ? first + 1 : nb; i < nb; ++i)  // a token listed twice: in the order of the list
-        if (p.bias_ids[b0 + i] == p.bias_ids[b0 + first]) sum = __dadd_rn(sum, (double)p.bias_values[b0 + i]);
-      v = __dadd_rn(v, sum);
+  }
+  if (BIAS) {
+    const int b0 = p.bias_offsets[row];
+    r.biases = p.bias_offsets[row + 1] - b0;
+    if (b0 < 0 || r.biases < 0) {
+      if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
+      r.biases = 0;
     }
-    if (v > best.v) best = {v, lo + at};
-    return __double2bfloat16(v);
-  };
+    r.bias_ids = p.bias_ids + b0;
+    r.bias_values = p.bias_values + b0;
+  }
 
-  if (p.vec) {
-    for (int c = tid; c < n / 8; c += kThreads) {
-      const uint4 raw = reinterpret_cast<const uint4*>(in)[c];
-      uint32_t w[8], l[8], touched = 0;
+  // ---- which tokens are touched ----
+  int marked = 0;
+  if (kLists) {
+    __syncthreads();
+    auto mark = [&](int32_t id) {
+      const uint32_t at = (uint32_t)id - (uint32_t)lo;
+      if (at < (uint32_t)n) atomicOr(&marks[at >> 5], 1u << (at & 31));
+      else if ((uint32_t)id >= (uint32_t)p.vocab) raise_error(p.err, DEV_ERR_BAD_INDEX);
+    };
+    if (HIST)
+#pragma unroll 8
+      for (int i = tid; i < r.len; i += kThreads) mark(r.history[i]);
+    if (BIAS)
+      for (int i = tid; i < r.biases; i += kThreads) mark(r.bias_ids[i]);
+    __syncthreads();
+    const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    int mine = 0;
+    for (int w = w0; w < w1; ++w) mine += __popc(marks[w]);
+    int at = block_scan(mine, sums, &marked);
+    for (int w = w0; w < w1; ++w) {
+      before[w] = at;
+      at += __popc(marks[w]);
+    }
+  }
+
+  // ---- the sweep: copies, masks, the best of the untouched (bf16 values: compared as they are) ----
+  float plain_v = -INFINITY;
+  int plain_i = -1;
+  for (int c0 = tid; c0 < nv; c0 += kAhead * kThreads) {
+    if (c0 != tid) load(c0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = l[i] = 0;
-      if (HIST) {
-        *reinterpret_cast<uint4*>(w) = reinterpret_cast<const uint4*>(seen)[2 * c];
-        *reinterpret_cast<uint4*>(w + 4) = reinterpret_cast<const uint4*>(seen)[2 * c + 1];
-      }
-      if (BIAS) {
-        *reinterpret_cast<uint4*>(l) = reinterpret_cast<const uint4*>(lead)[2 * c];
-        *reinterpret_cast<uint4*>(l + 4) = reinterpret_cast<const uint4*>(lead)[2 * c + 1];
-      }
+    for (int k = 0; k < kAhead; ++k) {
+      const int c = c0 + k * kThreads;
+      if (c >= nv) break;
+      uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+      uint32_t skip = kLists ? reinterpret_cast<const uint8_t*>(marks)[c] : 0;
+      if (mask) {
+        const uint32_t hidden = ~(mask[c >> 2] >> ((c & 3) * 8)) & 0xffu;
+        if (hidden) {
+          skip |= hidden;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) touched |= (w[i] | l[i]) ? 1u << i : 0u;
-      const uint32_t allowed = mask ? (mask[(lo >> 5) + (c >> 2)] >> ((c & 3) * 8)) & 0xffu : 0xffu;
-      float f[8];
-      unpack8(raw, f);
-      uint4 res = raw;
-      if (touched == 0 && allowed == 0xffu) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (f[i] > plain_v) {
-            plain_v = f[i];
-            plain_i = lo + c * 8 + i;
-          }
-      } else {
-        __nv_bfloat16* r = reinterpret_cast<__nv_bfloat16*>(&res);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (!((allowed >> i) & 1u)) {
-            r[i] = __float2bfloat16_rn(-INFINITY);
-          } else if ((touched >> i) & 1u) {
-            r[i] = process(c * 8 + i, f[i], w[i], l[i]);
-          } else if (f[i] > plain_v) {
-            plain_v = f[i];
-            plain_i = lo + c * 8 + i;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t h = spread2(hidden >> (2 * i));
+            w[i] = (w[i] & ~h) | (kLowPair & h);
           }
         }
       }
-      if (out) reinterpret_cast<uint4*>(out)[c] = res;
+      if (out) reinterpret_cast<uint4*>(out)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (skip) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h = spread2(skip >> (2 * i));
+          w[i] = (w[i] & ~h) | (kLowPair & h);
+        }
+      }
+      uint32_t top = max_pair(max_pair(w[0], w[1]), max_pair(w[2], w[3]));
+      const float most = fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u));
+      if (most > plain_v) {  // seldom, after the first few
+        plain_v = most;
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+          if (__uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) == most) plain_i = c * 8 + i;
+      }
     }
   }
   // rows that 16-byte accesses do not fit, and the last few tokens of those that they do
-  for (int at = (p.vec ? n & ~7 : 0) + tid; at < n; at += kThreads) {
-    __nv_bfloat16 r = in[at];
-    const float x = bf2f(r);
-    const uint32_t w = HIST ? seen[at] : 0, l = BIAS ? lead[at] : 0;
-    if (mask && !((mask[(lo + at) >> 5] >> (at & 31)) & 1u)) {
-      r = __float2bfloat16_rn(-INFINITY);
-    } else if (w | l) {
-      r = process(at, x, w, l);
-    } else if (x > plain_v) {
+  for (int at = nv * 8 + tid; at < n; at += kThreads) {
+    __nv_bfloat16 v = in[at];
+    const float x = bf2f(v);
+    if (mask && !((mask[at >> 5] >> (at & 31)) & 1u)) {
+      v = __float2bfloat16_rn(-INFINITY);
+    } else if (!(kLists && ((marks[at >> 5] >> (at & 31)) & 1u)) && x > plain_v) {
       plain_v = x;
-      plain_i = lo + at;
+      plain_i = at;
     }
-    if (out) out[at] = r;
+    if (out) out[at] = v;
   }
-  if (!p.next) return;
+  Best best{(double)plain_v, plain_i < 0 ? INT64_MAX : lo + plain_i};
 
-  best = better(best, Best{(double)plain_v, plain_i});
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)});
-  if ((tid & 31) == 0) warp_best[tid >> 5] = best;
-  __syncthreads();
-  if (tid < 32) {
-    best = tid < kThreads / 32 ? warp_best[tid] : Best{-INFINITY, INT64_MAX};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)});
-    if (tid == 0) cta_best = best;
-  }
-  cluster_sync();
-  if (cluster_rank() == 0 && tid == 0) {
-    for (int r = 1; r < ctas; ++r) {
-      const uint32_t at = cluster_map(smem_u32(&cta_best), r);
-      best = better(best, Best{__longlong_as_double((long long)cluster_load8(at)), (int64_t)cluster_load8(at + 8)});
+  // ---- the touched tokens, kSlots at a time ----
+  if (kLists && marked > 0) {
+    const bool rep = HIST && p.repetition, frq = HIST && p.frequency, prs = HIST && p.presence;
+    const double repetition = rep ? (double)p.repetition[row] : 1.0;
+    const double frequency = frq ? (double)p.frequency[row] : 0.0;
+    const double presence = prs ? (double)p.presence[row] : 0.0;
+    for (int s0 = 0; s0 < marked; s0 += kSlots) {
+      const int slots = min(kSlots, marked - s0);
+      __syncthreads();  // `before` is written; the last turn's slots are read, and the sweep's stores are done
+      for (int i = tid; i < slots; i += kThreads) said[i] = lead[i] = 0;
+      __syncthreads();
+      // the slot of a token of this part, or -1
+      auto slot_of = [&](int32_t id) -> int {
+        const uint32_t at = (uint32_t)id - (uint32_t)lo;
+        if (at >= (uint32_t)n) return -1;
+        const int s = before[at >> 5] + __popc(marks[at >> 5] & ((1u << (at & 31)) - 1)) - s0;
+        if (s < 0 || s >= slots) return -1;
+        token[s] = (int)at;
+        return s;
+      };
+      if (HIST)
+#pragma unroll 4
+        for (int i = tid; i < r.len; i += kThreads) {
+          const int s = slot_of(r.history[i]);
+          if (s < 0) continue;
+          if (i < r.prompt) atomicOr(&said[s], kTopBit);
+          else atomicAdd(&said[s], 1u);
+        }
+      if (BIAS) {
+        // a token's first entry leads: it is worth the most counted from the end
+        for (int i = tid; i < r.biases; i += kThreads) {
+          const int s = slot_of(r.bias_ids[i]);
+          if (s >= 0) atomicMax(&lead[s], (uint32_t)(r.biases - i));
+        }
+        __syncthreads();
+        for (int i = tid; i < r.biases; i += kThreads) {
+          const int s = slot_of(r.bias_ids[i]);
+          if (s >= 0 && (lead[s] & ~kTopBit) != (uint32_t)(r.biases - i)) atomicOr(&lead[s], kTopBit);
+        }
+      }
+      __syncthreads();
+      for (int s = tid; s < slots; s += kThreads) {
+        const int at = token[s];
+        if (mask && !((mask[at >> 5] >> (at & 31)) & 1u)) continue;
+        double v = (double)bf2f(in[at]);
+        const uint32_t w = HIST ? said[s] : 0, l = BIAS ? lead[s] : 0;
+        if (w) {
+          if (rep) v = v > 0 ? __ddiv_rn(v, repetition) : __dmul_rn(v, repetition);
+          const uint32_t times = w & ~kTopBit;
+          if (frq) v = __dsub_rn(v, __dmul_rn(frequency, (double)times));
+          if (prs && times) v = __dsub_rn(v, presence);
+        }
+        if (l) {
+          const int first = r.biases - (int)(l & ~kTopBit);
+          double sum = (double)r.bias_values[first];
+          for (int e = l & kTopBit ? first + 1 : r.biases; e < r.biases; ++e)  // listed twice: in the list's order
+            if (r.bias_ids[e] == r.bias_ids[first]) sum = __dadd_rn(sum, (double)r.bias_values[e]);
+          v = __dadd_rn(v, sum);
+        }
+        if (v > best.v || (v == best.v && v > -INFINITY && lo + at < best.i)) best = {v, lo + at};
+        if (out) out[at] = __double2bfloat16(v);
+      }
     }
-    p.next[row] = best.i == INT64_MAX ? -1 : best.i;
   }
-  cluster_sync();  // the parts stay until they are read
+
+  // ---- the greedy token: the CTAs' bests meet in the first one's shared memory ----
+  if (p.next) {
+    best = warp_better(best);
+    if ((tid & 31) == 0) warp_best[tid >> 5] = best;
+    __syncthreads();
+    if (tid < 32) best = warp_better(tid < kThreads / 32 ? warp_best[tid] : Best{-INFINITY, INT64_MAX});
+  }
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (p.next && tid == 0) {
+    const uint32_t at = cluster_map(smem_u32(&cta_best[rank]), 0);
+    cluster_store8(at, (uint64_t)__double_as_longlong(best.v));
+    cluster_store8(at + 8, (uint64_t)best.i);
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (p.next && rank == 0 && tid < 32) {
+    best = warp_better(tid < ctas ? cta_best[tid] : Best{-INFINITY, INT64_MAX});
+    if (tid == 0) p.next[row] = best.i == INT64_MAX ? -1 : best.i;
+  }
 }
+
+// Shared memory of a part: a bit and an eighth of a count a token, and the slots.
+int64_t part_bytes(int64_t chunk) { return chunk / 32 * 8 + kSlots * 12; }
+constexpr int64_t kMaxSmem = 224 * 1024;
 
 template <bool HIST, bool BIAS>
 int launch(const LogitsParams& p, int64_t rows, unsigned ctas, cudaStream_t stream) {
@@ -262,12 +364,13 @@ int launch(const LogitsParams& p, int64_t rows, unsigned ctas, cudaStream_t stre
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return B200_ERROR_UNSUPPORTED;
   if (!done[dev]) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess ||
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess ||
         cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return B200_ERROR_UNSUPPORTED;
     done[dev] = true;
   }
-  const size_t smem = (size_t)p.chunk * 4 * ((HIST ? 1 : 0) + (BIAS ? 1 : 0));
+  const size_t smem = HIST || BIAS ? (size_t)part_bytes(p.chunk) : 0;
   launch_clusters(k, ctas, dim3((unsigned)(rows * ctas)), kThreads, smem, stream, p);
   B200_CHECK_LAUNCH();
   return B200_OK;
@@ -297,17 +400,19 @@ extern "C" int b200_logits_process(const void* logits, int64_t ld, int64_t rows,
     if (reinterpret_cast<uintptr_t>(q) & 3u) return B200_ERROR_INVALID_PARAM;
   const uintptr_t pl = reinterpret_cast<uintptr_t>(logits), po = reinterpret_cast<uintptr_t>(out);
   if ((pl & 1u) || (po & 1u) || (reinterpret_cast<uintptr_t>(next) & 7u)) return B200_ERROR_INVALID_PARAM;
-  if (rows > INT32_MAX / 16 || vocab > INT32_MAX || history_ld > (int64_t)(kTopBit - 1)) return B200_ERROR_UNSUPPORTED;
+  if (rows > INT32_MAX / 16 || vocab > (1 << 23) || history_ld > (int64_t)(kTopBit - 1)) return B200_ERROR_UNSUPPORTED;
   if (rows == 0) return B200_OK;
 
-  // CTAs of a row: 16, or so many that each has 1024 tokens.  (A word or two a
-  // token must fit shared memory: 16 CTAs of 224 KB.)
-  unsigned ctas = 1;
-  while (ctas < 16 && (int64_t)ctas * 1024 < vocab) ctas *= 2;
-  const int64_t chunk = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
-  if (chunk * 4 * ((hist ? 1 : 0) + (bias ? 1 : 0)) > kMaxSmem) return B200_ERROR_UNSUPPORTED;
-  int dev = 0;
+  // CTAs of a row: as many as run at once (two an SM), at most 16, each with
+  // 1024 tokens or more.
+  int dev = 0, sms = 0;
   cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  unsigned ctas = 1;
+  while (ctas < kMaxCtas && (int64_t)ctas * 1024 < vocab && rows * ctas * 2 <= 2 * sms) ctas *= 2;
+  int64_t chunk = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
+  while (ctas < kMaxCtas && part_bytes(chunk) > kMaxSmem) chunk = ((vocab + (ctas *= 2) - 1) / ctas + 31) / 32 * 32;
+  if (part_bytes(chunk) > kMaxSmem) return B200_ERROR_UNSUPPORTED;
   const int vec = (pl & 15u) == 0 && ld % 8 == 0 && (!out || ((po & 15u) == 0 && ldo % 8 == 0));
   const LogitsParams p{static_cast<const __nv_bfloat16*>(logits), ld, vocab, (int)chunk, history, history_ld,
                        prompt_lens, lens, repetition, frequency, presence, bias_offsets, bias_ids, bias_values, mask,

@@ -604,8 +604,8 @@ B200_API int b200_argmax(const void* logits, int64_t rows, int64_t vocab, int64_
  * (with what belongs to it).  Ids outside [0, vocab) are passed over, lengths
  * clamped to history_ld and rows of no mask not masked; all three set the device
  * error word.  Any stride; rows whose pointers and strides are multiples of 16
- * bytes are faster.  Up to 900 thousand tokens (half with both a history and
- * biases).  Stands before b200_argmax; the reference chooses no token
+ * bytes are faster.  Vocabularies of up to 8388608 tokens.
+ * Stands before b200_argmax; the reference chooses no token
  * (atb_cpp_llm/include/atb_llm/model.h:47-50). */
 B200_API int b200_logits_process(const void* logits, int64_t ld, int64_t rows, int64_t vocab, const int32_t* history,
                                  int64_t history_ld, const int32_t* prompt_lens, const int32_t* lens,

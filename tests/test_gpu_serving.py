@@ -285,6 +285,13 @@ def test_logits_parts(use, prompts):
 def test_logits_long_history_and_many_rows():
     check_logits(logits_case(3, 2, 200, 40000, 0, 0))  # tokens that occur hundreds of times
     check_logits(logits_case(4, 300, 777, 20, 3, 1))
+    # more tokens of one CTA touched than it computes at a time (a row a CTA, thousands of different tokens)
+    c = logits_case(4, 150, 13000, 5, 2, 1)
+    rng = np.random.default_rng(4)
+    c["history"][7], c["history"][8] = rng.permutation(13000), rng.integers(0, 13000, 9000)
+    c["prompt"][7], c["prompt"][8] = 6000, 0
+    c["biases"][8] = [(int(t), np.float32(t % 7 - 3)) for t in rng.integers(0, 13000, 700)]
+    check_logits(c)
 
 
 def test_logits_tokens_listed_twice():

@@ -64,7 +64,7 @@ TOO_MUCH = [
                                          dict(width=1 << 29)]),
     ("b200_paged_decode_shared", SHARED, [dict(d=96), dict(bs=16), dict(nq=258, nkv=2, qs=258 * 64, os=258 * 64),
                                           dict(pmax=(1 << 31) - 1)]),
-    ("b200_logits_process", LOGITS, [dict(vocab=500000, ld=500000, ldo=500000, mld=15625), dict(rows=1 << 28)]),
+    ("b200_logits_process", LOGITS, [dict(vocab=(1 << 23) + 1, ld=1 << 24, ldo=1 << 24, mld=1 << 19), dict(rows=1 << 28)]),
 ]
 
 
