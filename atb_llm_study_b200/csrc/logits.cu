@@ -36,7 +36,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr unsigned kMaxCtas = 16;  // of a row
 constexpr int kSlots = 4096;       // marked tokens computed at a time
-constexpr uint32_t kTopBit = 1u << 31;  // of `said`: the prompt has it; of `lead`: listed more than once
+constexpr uint32_t kTopBit = 1u << 31;  // of `said`: the prompt has it
 
 struct LogitsParams {
   const __nv_bfloat16* logits;
@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
   int* before = reinterpret_cast<int*>(marks + words);        // [words] marked tokens before each word
   int* token = before + words;                                // [kSlots] a marked token, in its part
   uint32_t* said = reinterpret_cast<uint32_t*>(token + kSlots);  // [kSlots] times behind the prompt | kTopBit
-  uint32_t* lead = said + kSlots;                             // [kSlots] entries from its first bias to the list's end | kTopBit
+  uint32_t* lead = said + kSlots;                             // [kSlots] entries from its first bias to the list's end
+  uint32_t* listed = lead + kSlots;                           // [kSlots] its biases
   pdl_trigger();
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // every CTA has started: waited for at the end
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
     for (int s0 = 0; s0 < marked; s0 += kSlots) {
       const int slots = min(kSlots, marked - s0);
       __syncthreads();  // `before` is written; the last turn's slots are read, and the sweep's stores are done
-      for (int i = tid; i < slots; i += kThreads) said[i] = lead[i] = 0;
+      for (int i = tid; i < slots; i += kThreads) said[i] = lead[i] = listed[i] = 0;
       __syncthreads();
       // the slot of a token of this part, or -1
       auto slot_of = [&](int32_t id) -> int {
@@ -297,33 +298,46 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
         // a token's first entry leads: it is worth the most counted from the end
         for (int i = tid; i < r.biases; i += kThreads) {
           const int s = slot_of(r.bias_ids[i]);
-          if (s >= 0) atomicMax(&lead[s], (uint32_t)(r.biases - i));
-        }
-        __syncthreads();
-        for (int i = tid; i < r.biases; i += kThreads) {
-          const int s = slot_of(r.bias_ids[i]);
-          if (s >= 0 && (lead[s] & ~kTopBit) != (uint32_t)(r.biases - i)) atomicOr(&lead[s], kTopBit);
+          if (s >= 0) {
+            atomicMax(&lead[s], (uint32_t)(r.biases - i));
+            atomicAdd(&listed[s], 1u);
+          }
         }
       }
       __syncthreads();
-      for (int s = tid; s < slots; s += kThreads) {
-        const int at = token[s];
-        if (mask && !((mask[at >> 5] >> (at & 31)) & 1u)) continue;
-        double v = (double)bf2f(in[at]);
-        const uint32_t w = HIST ? said[s] : 0, l = BIAS ? lead[s] : 0;
+      for (int base = tid & ~31; base < slots; base += kThreads) {
+        const int s = base + (tid & 31);
+        const int at = s < slots ? token[s] : 0;
+        const bool mine = s < slots && !(mask && !((mask[at >> 5] >> (at & 31)) & 1u));
+        double v = mine ? (double)bf2f(in[at]) : 0;
+        const uint32_t w = HIST && mine ? said[s] : 0, l = BIAS && mine ? lead[s] : 0;
         if (w) {
           if (rep) v = v > 0 ? __ddiv_rn(v, repetition) : __dmul_rn(v, repetition);
           const uint32_t times = w & ~kTopBit;
           if (frq) v = __dsub_rn(v, __dmul_rn(frequency, (double)times));
           if (prs && times) v = __dsub_rn(v, presence);
         }
-        if (l) {
-          const int first = r.biases - (int)(l & ~kTopBit);
-          double sum = (double)r.bias_values[first];
-          for (int e = l & kTopBit ? first + 1 : r.biases; e < r.biases; ++e)  // listed twice: in the list's order
-            if (r.bias_ids[e] == r.bias_ids[first]) sum = __dadd_rn(sum, (double)r.bias_values[e]);
-          v = __dadd_rn(v, sum);
+        if (BIAS) {
+          const int first = r.biases - (int)l;
+          double sum = l ? (double)r.bias_values[first] : 0;
+          // tokens listed more than once: the warp looks through the list for one after the other, and adds in its order
+          uint32_t many = __ballot_sync(0xffffffffu, l && listed[s] > 1);
+          for (; many; many &= many - 1) {
+            const int owner = __ffs(many) - 1;
+            const int id = lo + __shfl_sync(0xffffffffu, at, owner);
+            for (int e0 = __shfl_sync(0xffffffffu, first, owner) + 1; e0 < r.biases; e0 += 32) {
+              const int e = e0 + (tid & 31);
+              const bool same = e < r.biases && r.bias_ids[e] == id;
+              const float value = same ? r.bias_values[e] : 0.f;
+              for (uint32_t hits = __ballot_sync(0xffffffffu, same); hits; hits &= hits - 1) {
+                const double add = (double)__shfl_sync(0xffffffffu, value, __ffs(hits) - 1);
+                if ((tid & 31) == owner) sum = __dadd_rn(sum, add);
+              }
+            }
+          }
+          if (l) v = __dadd_rn(v, sum);
         }
+        if (!mine) continue;
         if (v > best.v || (v == best.v && v > -INFINITY && lo + at < best.i)) best = {v, lo + at};
         if (out) out[at] = __double2bfloat16(v);
       }
@@ -353,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
 }
 
 // Shared memory of a part: a bit and an eighth of a count a token, and the slots.
-int64_t part_bytes(int64_t chunk) { return chunk / 32 * 8 + kSlots * 12; }
+int64_t part_bytes(int64_t chunk) { return chunk / 32 * 8 + kSlots * 16; }
 constexpr int64_t kMaxSmem = 224 * 1024;
 
 template <bool HIST, bool BIAS>
