@@ -5,9 +5,11 @@
 // The tensor cores bound it: 4 flops a visible pair, head and dim, and a 128-row
 // query tile touches window / 128 + 2 key tiles (the window's ends cut through
 // one each) besides the sinks'.  Tiles without a visible pair are never
-// loaded, so the time follows the window and not the prompt.  Items are walked
-// with the heads of one sequence's rows next to each other: the nq / nkv heads
-// that share keys find them in L2.
+// loaded, so the time follows the window and not the prompt.  The two sides of an
+// item (tc_items.cuh) are two heads that share their keys, or, where nq / nkv is
+// odd, two query tiles of one head next to each other.  Items are walked with
+// the heads of one sequence's rows side by side: those that share keys find them
+// in L2.
 #include <algorithm>
 
 #include "tc_items.cuh"
@@ -20,20 +22,26 @@ namespace {
 template <int HDK_, int HDV_, bool HEADS3D>
 struct Window {
   static constexpr int HDK = HDK_, HDV = HDV_;
-  using Cf = TcCfg<HDK, HDV>;
+  using Cf = ItemsCfg<Window>;
   __nv_bfloat16* out;
   int64_t os, ohs;
   const int32_t* cu;
-  int nq, nkv, nseq, mblocks, total;
+  int nq, nkv, nseq, mblocks, total, max_rows;
   int64_t qhs, khs, vhs;
   float scale_log2;
   int window, sinks, out_cols;
+  bool pair_heads;
 
   struct Item {
     int n;                       // key tiles
-    int h, kvh, start, len, m0;  // m0: first query position
+    bool both;                   // side 1 has rows
+    int h0, h1, m0, m1;          // sides' heads and first query positions
+    int kvh, start, len;         // len: the keys'
+    int rows;                    // and the queries', up to max_seqlen
     int head, first;             // sink tiles, and the window's first tile
     int window, sinks;
+    B200_DEV int at(int s) const { return s ? m1 : m0; }
+    B200_DEV int head_of(int s) const { return s ? h1 : h0; }
   };
 
   struct Cursor {
@@ -41,23 +49,30 @@ struct Window {
     int w;
     B200_DEV explicit Cursor(const Window& q) : p(q), w(blockIdx.x) {}
     B200_DEV bool next(Item& it, unsigned* err) {
-      const int per_m = p.nq * p.nseq, W = p.mblocks * per_m;
+      // an item: two heads of a query tile, or two query tiles of a head; the latest rows of a sequence first
+      const int heads = p.pair_heads ? p.nq / 2 : p.nq, rows = p.pair_heads ? kTile : 2 * kTile;
+      const int per_m = heads * p.nseq, W = p.mblocks * per_m;
       for (; w < W; w += gridDim.x) {
         const int m = p.mblocks - 1 - w / per_m, r = w % per_m;
-        it.h = r % p.nq;
-        const int sq = r / p.nq;
+        const int sq = r / heads, h = r % heads;
         it.start = p.cu[sq];
         it.len = p.cu[sq + 1] - it.start;
-        it.m0 = m * kTile;
         if (it.start < 0 || it.len > p.total - it.start) {  // rows outside the operands
           raise_error(err, DEV_ERR_BAD_INDEX);
           continue;
         }
-        if (it.m0 >= it.len) continue;
-        it.kvh = it.h / (p.nq / p.nkv);
-        it.first = max(0, it.m0 - p.window + 1) / kTile;
+        const int m0 = m * rows;
+        it.rows = min(it.len, p.max_rows);
+        if (m0 >= it.rows) continue;
+        it.h0 = p.pair_heads ? 2 * h : h;
+        it.h1 = p.pair_heads ? 2 * h + 1 : h;
+        it.m0 = m0;
+        it.m1 = p.pair_heads ? m0 : m0 + kTile;
+        it.both = it.m1 < it.rows;
+        it.kvh = it.h0 / (p.nq / p.nkv);
+        it.first = max(0, m0 - p.window + 1) / kTile;
         it.head = min((p.sinks + kTile - 1) / kTile, it.first);
-        it.n = it.head + m - it.first + 1;
+        it.n = it.head + (it.both ? it.m1 : m0) / kTile - it.first + 1;
         it.window = p.window;
         it.sinks = p.sinks;
         w += gridDim.x;
@@ -68,20 +83,26 @@ struct Window {
   };
 
   B200_DEV static int key0(const Item& it, int j) { return (j < it.head ? j : it.first + j - it.head) * kTile; }
-  B200_DEV static bool sees(const Item& it, int row, int key) {
-    const int i = it.m0 + row;
-    return key <= i && key < it.len && (i - key < it.window || key < it.sinks);
+  B200_DEV static bool whole(const Item& it, int s, int key) {
+    return key + kTile - 1 <= it.at(s) && key + kTile <= it.len &&
+           (it.at(s) + kTile - 1 - key < it.window || key + kTile <= it.sinks);
   }
-  B200_DEV static bool whole(const Item& it, int key, int keys) {
-    return key + keys - 1 <= it.m0 && key + keys <= it.len &&
-           (it.m0 + kTile - 1 - key < it.window || key + keys <= it.sinks);
+  // key <= i and key < len and (key > i - window or key < sinks), i the row's position
+  B200_DEV static void visible(const Item& it, int s, int row, int key, uint32_t bits[4]) {
+    const int i = it.at(s) + row, end = min(i + 1, it.len) - key;
+    uint32_t sink[4];
+    bit_range(i - it.window + 1 - key, end, bits);
+    bit_range(0, min(it.sinks - key, end), sink);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) bits[w] |= sink[w];
   }
-  B200_DEV static void load_q(const Window& p, const Item& it, uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+  B200_DEV static void load_q(const Window& p, const Item& it, int s, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar) {
     mbar_arrive_expect_tx(bar, Cf::TILE_QK);
-    if (HEADS3D) tma_load_3d(dst, map, bar, 0, it.h, it.start + it.m0);
+    if (HEADS3D) tma_load_3d(dst, map, bar, 0, it.head_of(s), it.start + it.at(s));
     else
       for (int x = 0; x < Cf::BOXES_QK; ++x)
-        tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.h * p.qhs) + 64 * x, it.start + it.m0);
+        tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.head_of(s) * p.qhs) + 64 * x, it.start + it.at(s));
   }
   B200_DEV static void load_k(const Window& p, const Item& it, int j, uint8_t* dst, const CUtensorMap* map,
                               uint64_t* bar, unsigned*) {
@@ -99,20 +120,20 @@ struct Window {
       for (int x = 0; x < Cf::BOXES_V; ++x)
         tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.kvh * p.vhs) + 64 * x, it.start + key0(it, j));
   }
-  // O / l from TMEM as bf16 rows, this thread's half of the columns
-  B200_DEV static void store(const Window& p, const Item& it, int row, int half, float, float l, uint32_t tO) {
+  // O / l from TMEM as bf16 rows
+  B200_DEV static void store(const Window& p, const Item& it, int s, int row, float, float l, uint32_t tO) {
     const float inv = 1.f / l;  // every row sees itself
-    const bool valid = it.m0 + row < it.len;
-    __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.m0 + row : 0)) * p.os + (int64_t)it.h * p.ohs + half * (HDV / 2);
+    const bool valid = it.at(s) + row < it.rows;
+    __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.at(s) + row : 0)) * p.os + (int64_t)it.head_of(s) * p.ohs;
 #pragma unroll 1
-    for (int c = 0; c < HDV / 64; ++c) {
+    for (int c = 0; c < HDV / 32; ++c) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tO + c * 32, r);
       tmem_ld_wait();
       if (valid) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (HEADS3D && half * (HDV / 2) + c * 32 + k * 8 >= p.out_cols) break;
+          if (HEADS3D && c * 32 + k * 8 >= p.out_cols) break;
           float f[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[8 * k + i]) * inv;
@@ -149,10 +170,12 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
       out_stride < (int64_t)(nq - 1) * out_head_stride + hdv)
     return B200_ERROR_INVALID_PARAM;
   if (num_seqs == 0 || max_seqlen == 0 || total_tokens == 0) return B200_OK;
-  const int mblocks = (int)(((int64_t)max_seqlen + kTile - 1) / kTile);
-  const int64_t items = (int64_t)mblocks * nq * num_seqs;
-  if (total_tokens > INT32_MAX - kTile || qcols > INT32_MAX || kcols > INT32_MAX || vcols > INT32_MAX ||
-      items > INT32_MAX - 4096 || max_seqlen > INT32_MAX - kTile)
+  const bool pair_heads = nq / nkv % 2 == 0;
+  const int rows = pair_heads ? kTile : 2 * kTile;
+  const int mblocks = (int)(((int64_t)max_seqlen + rows - 1) / rows);
+  const int64_t items = (int64_t)mblocks * (pair_heads ? nq / 2 : nq) * num_seqs;
+  if (total_tokens > INT32_MAX - 2 * kTile || qcols > INT32_MAX || kcols > INT32_MAX || vcols > INT32_MAX ||
+      items > INT32_MAX - 4096 || max_seqlen > INT32_MAX - 2 * kTile)
     return B200_ERROR_UNSUPPORTED;
   // a window or sinks behind the longest prompt change nothing; kept small so that sums of positions fit
   window = std::min(window, max_seqlen);
@@ -168,6 +191,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
     prob.nkv = nkv;
     prob.nseq = num_seqs;
     prob.mblocks = mblocks;
+    prob.max_rows = max_seqlen;
     prob.total = (int)total_tokens;
     prob.qhs = q_head_stride;
     prob.khs = k_head_stride;
@@ -176,6 +200,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
     prob.window = window;
     prob.sinks = sinks;
     prob.out_cols = cols;
+    prob.pair_heads = pair_heads;
     return launch_items(mq, mk, mv, prob, grid, stream);
   };
   if (hd < 64) {

@@ -28,7 +28,7 @@ namespace {
 template <int HD>
 struct Prefix {
   static constexpr int HDK = HD, HDV = HD;
-  using Cf = TcCfg<HD, HD>;
+  using Cf = ItemsCfg<Prefix>;
   PrefixParts at;
   const int32_t* blocks;
   int64_t num_blocks;
@@ -37,9 +37,10 @@ struct Prefix {
 
   struct Item {
     int n;       // key tiles of this stretch
-    int first;   // the first of them
+    bool both;   // two row tiles
+    int first;   // the first key tile
     int length;  // of the prefix
-    int kvh, row_tile, slot;
+    int kvh, row_tile, slot;  // side 0's; side 1's follow
   };
 
   struct Cursor {
@@ -49,33 +50,35 @@ struct Prefix {
     B200_DEV explicit Cursor(const Prefix& q) : p(q) {
       length = prefix_length(p.at);
       K = (length + kTile - 1) / kTile;
-      const PrefixDeal deal(p.at, K * p.nkv * p.at.row_tiles);
+      const PrefixDeal deal(p.at, K * p.nkv * prefix_pairs(p.at));
       const bool has = blockIdx.x < deal.W;
       unit = has ? deal.first_unit(blockIdx.x) : 0;
       end = has ? deal.first_unit(blockIdx.x + 1) : 0;
     }
     B200_DEV bool next(Item& it, unsigned*) {
       if (unit >= end) return false;
-      const int item = (int)(unit / K);
+      const int item = (int)(unit / K), pairs = prefix_pairs(p.at);
       it.first = (int)(unit % K);
       it.n = (int)min(end - unit, K - it.first);
       it.length = length;
-      it.kvh = item / p.at.row_tiles;
-      it.row_tile = item % p.at.row_tiles;
-      it.slot = blockIdx.x + item;
+      it.kvh = item / pairs;
+      it.row_tile = item % pairs * 2;
+      it.both = it.row_tile + 1 < p.at.row_tiles;
+      it.slot = ((int)blockIdx.x + item) * 2;
       unit += it.n;
       return true;
     }
   };
 
   B200_DEV static int key0(const Item& it, int j) { return (it.first + j) * kTile; }
-  B200_DEV static bool sees(const Item& it, int, int key) { return key < it.length; }
-  B200_DEV static bool whole(const Item& it, int key, int keys) { return key + keys <= it.length; }
+  B200_DEV static bool whole(const Item& it, int, int key) { return key + kTile <= it.length; }
+  B200_DEV static void visible(const Item& it, int, int, int key, uint32_t bits[4]) { bit_range(0, it.length - key, bits); }
   // box rows are the group's heads of per_tile sequences; rows behind them are not written, and not used
-  B200_DEV static void load_q(const Prefix& p, const Item& it, uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+  B200_DEV static void load_q(const Prefix& p, const Item& it, int s, uint8_t* dst, const CUtensorMap* map,
+                              uint64_t* bar) {
     mbar_arrive_expect_tx(bar, Cf::BOXES_QK * p.at.per_tile * p.at.group * 128);
     for (int x = 0; x < Cf::BOXES_QK; ++x)
-      tma_load_3d(dst + x * kBoxBytes, map, bar, 64 * x, it.kvh * p.at.group, it.row_tile * p.at.per_tile);
+      tma_load_3d(dst + x * kBoxBytes, map, bar, 64 * x, it.kvh * p.at.group, (it.row_tile + s) * p.at.per_tile);
   }
   // a tile is one block of 128 tokens or two of 64, of which the second may lie behind the prefix: it is not loaded,
   // and its keys are hidden like the rest of a last block
@@ -103,14 +106,14 @@ struct Prefix {
                               uint64_t* bar, unsigned* err) {
     load(p, it, j, dst, map, bar, err);
   }
-  B200_DEV static void store(const Prefix& p, const Item& it, int row, int half, float m, float l, uint32_t tO) {
-    const int seqs = min(p.at.per_tile, p.batch - it.row_tile * p.at.per_tile);
+  B200_DEV static void store(const Prefix& p, const Item& it, int s, int row, float m, float l, uint32_t tO) {
+    const int seqs = min(p.at.per_tile, p.batch - (it.row_tile + s) * p.at.per_tile);
     const bool valid = row < seqs * p.at.group;
     const float inv = 1.f / l;  // every row sees the stretch's keys
-    float* o = p.at.parts + ((int64_t)it.slot * kTile + row) * HD + half * (HD / 2);
-    if (valid && half == 0) p.at.lse[(int64_t)it.slot * kTile + row] = m + log2f(l);
+    float* o = p.at.parts + ((int64_t)(it.slot + s) * kTile + row) * HD;
+    if (valid) p.at.lse[(int64_t)(it.slot + s) * kTile + row] = m + log2f(l);
 #pragma unroll 1
-    for (int c = 0; c < HD / 64; ++c) {
+    for (int c = 0; c < HD / 32; ++c) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tO + c * 32, r);
       tmem_ld_wait();
@@ -132,14 +135,14 @@ struct Plan {
   int64_t slots;
 };
 
-// SMs share the key tiles evenly, with no CTA left without one.
+// SMs share the key tiles evenly, with no CTA left without one.  A part has two tiles of 128 rows.
 Plan prefix_plan(int batch, int nq, int nkv, int max_prefix) {
   Plan p;
   p.per_tile = kTile / (nq / nkv);
   p.row_tiles = (batch + p.per_tile - 1) / p.per_tile;
-  const int64_t items = (int64_t)nkv * p.row_tiles, units = items * ((max_prefix + (int64_t)kTile - 1) / kTile);
+  const int64_t items = (int64_t)nkv * ((p.row_tiles + 1) / 2), units = items * ((max_prefix + (int64_t)kTile - 1) / kTile);
   p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(units, sm_count()));
-  p.slots = p.workers + items;
+  p.slots = 2 * (p.workers + items);
   return p;
 }
 

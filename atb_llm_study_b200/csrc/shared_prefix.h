@@ -3,12 +3,13 @@
 // sequence's own tokens (paged_window.cu) reads them.
 //
 // Query rows are the batch's heads of one kv head: per_tile sequences of
-// `group` heads fill a 128-row tile.  An item is a (kv head, row tile); its
-// prefix has K = ceil(length / 128) key tiles.  The items' key tiles in a row,
+// `group` heads fill a 128-row tile.  An item is a kv head and two row tiles
+// (the last may be alone); its prefix has K = ceil(length / 128) key tiles.  The items' key tiles in a row,
 // U of them, are dealt to W = min(workers, U) CTAs in equal stretches, worker c
 // taking [c U / W, (c + 1) U / W), so each has a tile at least.  Each stretch of
-// an item is a part; the part of worker c in item i lies in slot c + i: of two
-// consecutive parts the later has a larger worker or item.
+// an item is a part; the part of worker c in item i lies in slots 2 (c + i) and
+// 2 (c + i) + 1, a row tile each: of two consecutive parts the later has a larger
+// worker or item.
 #pragma once
 
 #include "common.cuh"
@@ -23,6 +24,7 @@ struct PrefixParts {
   int workers, row_tiles, per_tile, group;
 };
 
+B200_DEV int prefix_pairs(const PrefixParts& p) { return (p.row_tiles + 1) / 2; }
 B200_DEV int prefix_length(const PrefixParts& p) { return max(0, min(*p.length, p.max_length)); }
 
 // The stretches of U units: how many, the first unit of stretch c, the stretch of unit u.
@@ -38,21 +40,21 @@ struct PrefixSpan {
   const float* parts = nullptr;
   const float* lse_at = nullptr;
   int count = 0;
-  B200_DEV float lse(int k, int row) const { return lse_at[k * 128 + row]; }
-  B200_DEV float out(int k, int row, int head_dim, int d) const { return parts[(k * 128 + row) * head_dim + d]; }
+  B200_DEV float lse(int k, int row) const { return lse_at[k * 256 + row]; }
+  B200_DEV float out(int k, int row, int head_dim, int d) const { return parts[(k * 256 + row) * head_dim + d]; }
 };
 
 B200_DEV PrefixSpan prefix_span(const PrefixParts& p, int sequence, int kv_head, int nkv, int first_head, int head_dim) {
   PrefixSpan s;
   const int64_t K = (prefix_length(p) + 127) / 128;
   if (K == 0) return s;
-  const int item = kv_head * p.row_tiles + sequence / p.per_tile;
-  const PrefixDeal deal(p, K * nkv * p.row_tiles);
+  const int tile = sequence / p.per_tile, item = kv_head * prefix_pairs(p) + tile / 2;
+  const PrefixDeal deal(p, K * nkv * prefix_pairs(p));
   const int w0 = deal.worker(item * K), w1 = deal.worker(item * K + K - 1);
-  const int row = (sequence % p.per_tile) * p.group + first_head;
+  const int64_t row = (int64_t)(2 * (w0 + item) + tile % 2) * 128 + (sequence % p.per_tile) * p.group + first_head;
   s.count = w1 - w0 + 1;
-  s.parts = p.parts + ((int64_t)(w0 + item) * 128 + row) * head_dim;
-  s.lse_at = p.lse + (int64_t)(w0 + item) * 128 + row;
+  s.parts = p.parts + row * head_dim;
+  s.lse_at = p.lse + row;
   return s;
 }
 

@@ -1,50 +1,71 @@
-// Attention of query tiles over lists of key tiles on the tcgen05 tensor cores:
-// the kernel of sliding-window prompts and of shared prefixes.
+// Attention of pairs of query tiles over lists of key tiles on the tcgen05
+// tensor cores: the kernel of sliding-window prompts and of shared prefixes.
 //
 //   out = sum_j p_j v_j / sum_j p_j, p_j = 2^(q.k_j scale log2(e) - m)
 //
-// One item is 128 query rows and a list of 128-key tiles; a persistent CTA per
-// SM walks its items.  The roles are those of the whole-prompt kernel
-// (flash_tc.cu): a TMA warp, a thread that issues the scores S = Q K^T into
-// three TMEM buffers, eight softmax warps with two threads a row that write P
-// over their scores, and a warp that issues O += P V.  What an item's rows and
-// keys are, which pairs see each other and where the output goes is the
-// problem's (P below).
+// An item is one or two tiles of 128 query rows ("sides") that walk one list of
+// 128-key tiles; a persistent CTA per SM walks its items.  352 threads:
+//   warp 0      TMA: each item's Q tiles, then K and V tiles through rings
+//   warp 1      one thread issues the MMAs.  Per side and key tile: O += P V of
+//               the tile whose P is ready, right behind it S = Q K^T of the
+//               next tile (the next item's first at an item's end).  Both sides
+//               use a K / V tile while it is in shared memory.
+//   warp 2      looks through V tiles for NaN and infinities (below)
+//   warps 3-6   softmax of side 0, warps 7-10 of side 1, a thread a row: the
+//               row's 128 scores from TMEM, masked, maximum, exponentials, sum,
+//               P as bf16 pairs over the scores, where the MMA reads it.
+// What a side's chain has to wait for itself (scores, softmax, P V) the other
+// side's fills: the tensor core works for one while the softmax units work for
+// the other.  At 128-wide heads a side's tile takes 1024 cycles of MMAs and as
+// many of exponentials (16 a cycle and SM), so the two halves of the SM are
+// equally loaded.  TMEM: two score tiles and two output accumulators, 4 x 128
+// columns.  S of the next tile overwrites P that the P V before it reads: MMAs of
+// one thread run in the order of their issue.
+//
+// The running maximum moves only when it grows by more than 2^8 (the rows of O
+// in TMEM are then rescaled by their threads, seldom), which changes nothing in
+// exact arithmetic and keeps P below 2^8 of its usual scale.
 //
 // Values that nobody sees must not reach anybody: P is 0 there, but 0 x NaN is
-// not.  So the P.V warp looks through the value rows of every tile that is not
-// visible as a whole (the edges: a prompt's end, its diagonal, the ends of the
-// window and the sinks, a cache block's rest) and zeroes those with a NaN or an
-// infinity.  A row that does see such a key gets NaN: the item's list of zeroed
-// keys is looked through when its rows are stored.  The search takes one warp
-// 64 loads and ballots a tile while the tile's scores are computed.
+// not.  So warp 2 looks through the value rows of every tile that a side does
+// not see as a whole (a prompt's end, its diagonal, the ends of the window and
+// the sinks, a cache block's rest) and zeroes those with a NaN or an infinity.
+// A row that does see such a key gets NaN: the item's list of zeroed keys is
+// looked through when its rows are stored.  The search is 64 loads and ballots a
+// tile, while the tile's scores are computed.
 //
-// P provides: HDK, HDV; Item with `int n` (key tiles, > 0); Cursor(p) with
-// bool next(Item&, err); load_q / load_k / load_v(p, item, [tile,] smem, map, bar, err):
-// arrive on bar expecting bytes, copy; int key0(item, tile): its first key;
-// bool whole(item, key, keys): every row sees all of [key, key + keys);
-// bool sees(item, row, key); store(p, item, row, half, m, l, tO).
+// P provides: HDK, HDV; Item with int n (key tiles, > 0), bool both (side 1 is
+// there); Cursor(p) with bool next(Item&, err); load_q(p, item, side, ..) and
+// load_k / load_v(p, item, tile, smem, map, bar, err): arrive on bar expecting
+// bytes, copy; int key0(item, tile): its first key; bool whole(item, side, key):
+// every row of the side sees the 128 keys from key on; visible(item, side, row,
+// key, bits[4]): which of them a row sees; store(p, item, side, row, m, l, tO).
 #pragma once
 
 #include "tc_attention.cuh"
 
 namespace {
 
+constexpr int kItemThreads = 352;
+constexpr int kSides = 2;
+constexpr uint32_t kSideS = 0, kSideO = 256;  // TMEM columns of side 0's scores and outputs; side 1's lie 128 further
+constexpr int kMaxEdgeTiles = 6;
+
 struct Hidden {  // zeroed value rows of one item's edge tiles
   int count;
-  int key0[6];
-  uint32_t keys[6][4];
+  int key0[kMaxEdgeTiles];
+  uint32_t keys[kMaxEdgeTiles][4];
 };
-constexpr int kMaxEdgeTiles = 6;
+constexpr int kHiddenRing = 8;
 
 // Zeroes the rows of a V tile [128 keys] that hold a NaN or an infinity; keys' bits of those in `bad`.  One warp.
 template <int BOXES>
 B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad[i] = 0;
+  for (int w = 0; w < 4; ++w) bad[w] = 0;
   // an instruction covers 4 rows, 8 lanes of 16 bytes a row; rows are 128 contiguous bytes whatever the swizzle
-#pragma unroll 1
+#pragma unroll
   for (int w = 0; w < 4; ++w) {
     uint32_t found = 0;
 #pragma unroll
@@ -58,9 +79,10 @@ B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
         t |= (v.z & 0x7f807f80u) + 0x00800080u;
         t |= (v.w & 0x7f807f80u) + 0x00800080u;
         const uint32_t lanes = __ballot_sync(0xffffffffu, (t & 0x80008000u) != 0);
+        if (lanes)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (lanes & (0xffu << (8 * r))) found |= 1u << (i * 4 + r);
+          for (int r = 0; r < 4; ++r)
+            if (lanes & (0xffu << (8 * r))) found |= 1u << (i * 4 + r);
       }
     bad[w] = found;
     if (found)
@@ -77,61 +99,75 @@ B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
   return any;
 }
 
+// Bits [a, b) of 128.
+B200_DEV void bit_range(int a, int b, uint32_t bits[4]) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const int lo = min(max(a - 32 * w, 0), 32), hi = min(max(b - 32 * w, 0), 32);
+    bits[w] = hi > lo ? (0xffffffffu >> (32 - hi + lo)) << lo : 0u;
+  }
+}
+
 template <class P>
 struct ItemsCfg {
-  using Tc = TcCfg<P::HDK, P::HDV>;
-  static constexpr int HIDDEN = Tc::SMEM - 1024;  // behind tiles, exchange and barriers
-  static constexpr int SMEM = Tc::SMEM + 2 * (int)sizeof(Hidden);
+  static constexpr int BOXES_QK = P::HDK / 64, BOXES_V = P::HDV / 64;
+  static constexpr int TILE_QK = BOXES_QK * kBoxBytes, TILE_V = BOXES_V * kBoxBytes;
+  static constexpr int K_STAGES = P::HDK > 128 ? 2 : P::HDK > 64 ? 2 : 4;
+  static constexpr int V_STAGES = P::HDK > 128 ? 1 : P::HDK > 64 ? 2 : 4;
+  static constexpr int K_AT = kSides * TILE_QK, V_AT = K_AT + K_STAGES * TILE_QK, BARS_AT = V_AT + V_STAGES * TILE_V;
+  static constexpr int HIDDEN_AT = BARS_AT + 320;
+  static constexpr int SMEM = HIDDEN_AT + kHiddenRing * (int)sizeof(Hidden) + 1024;
+  static constexpr uint32_t IDESC_O = idesc_bf16_f32(128, P::HDV) | (1u << 16);  // B operand (V) MN-major
 };
 
 template <class P>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kItemThreads, 1)
     tc_items_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const P p, unsigned* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  using Cf = TcCfg<P::HDK, P::HDV>;
-  constexpr int HDK = P::HDK, HDV = P::HDV;
-  constexpr int kTileBytes = Cf::TILE_QK, kVBytes = Cf::TILE_V, VS = Cf::V_STAGES;
-  uint8_t* sQ = smem;
-  uint8_t* sK = smem + kTileBytes;
-  uint8_t* sV = smem + 3 * kTileBytes;
-  float* sMx = reinterpret_cast<float*>(sV + VS * kVBytes);  // [tile parity][half][row]
-  float* sL = sMx + 4 * 128;                                  // [half][row]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sL + 2 * 128);
-  uint64_t* q_full = bars;        // Q of the current item landed
-  uint64_t* q_empty = bars + 1;   // the item's last scores done: Q may be replaced
-  uint64_t* k_full = bars + 2;    // [2]
-  uint64_t* k_empty = bars + 4;   // [2]
-  uint64_t* v_full = bars + 6;    // [2]
-  uint64_t* v_empty = bars + 8;   // [2]
-  uint64_t* s_full = bars + 10;   // [3] scores of the tile in buffer i ready
-  uint64_t* p_full = bars + 13;   // [3] P of the tile in buffer i written (256 arrivals)
-  uint64_t* pv_done = bars + 16;  // [3] P.V of the tile whose P sits in buffer i done
-  uint64_t* o_free = bars + 19;   // the output accumulator read out (256 arrivals)
-  uint64_t* drain = bars + 20;    // [2] MMA issuers' teardown after an abort
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  using Cf = ItemsCfg<P>;
+  constexpr int HDK = P::HDK, HDV = P::HDV, KS = Cf::K_STAGES, VS = Cf::V_STAGES;
+  uint8_t* sK = smem + Cf::K_AT;
+  uint8_t* sV = smem + Cf::V_AT;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BARS_AT);
+  uint64_t* q_full = bars;           // [side] the item's Q landed
+  uint64_t* q_empty = bars + 2;      // [side] the item's last scores are done: Q may be replaced
+  uint64_t* s_full = bars + 4;       // [side] scores of a tile ready
+  uint64_t* p_full = bars + 6;       // [side] P of a tile written (128 arrivals)
+  uint64_t* pv_done = bars + 8;      // [side] P V of a tile done, and the list of zeroed keys behind it (2 arrivals)
+  uint64_t* o_free = bars + 10;      // [side] the outputs are read out (128 arrivals)
+  uint64_t* drain = bars + 12;       // the MMAs issued before an abort
+  uint64_t* k_full = bars + 13;      // [KS]
+  uint64_t* k_empty = k_full + KS;   // [KS]
+  uint64_t* v_full = k_empty + KS;   // [VS] landed
+  uint64_t* v_ready = v_full + VS;   // [VS] and looked through
+  uint64_t* v_empty = v_ready + VS;  // [VS]
+  static_assert((13 + 2 * KS + 3 * VS) * 8 + 8 <= 320, "barriers");
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + VS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  Hidden* hidden = reinterpret_cast<Hidden*>(smem + ItemsCfg<P>::HIDDEN);  // [item parity]
+  Hidden* hidden = reinterpret_cast<Hidden*>(smem + Cf::HIDDEN_AT);  // [item % kHiddenRing]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int s = 0; s < kSides; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&pv_done[s], 2);
+      mbar_init(&o_free[s], 128);
+    }
+    mbar_init(drain, 1);
+    for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
       mbar_init(&v_full[i], 1);
+      mbar_init(&v_ready[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < kSBufs; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 256);
-      mbar_init(&pv_done[i], 2);  // the products, and the thread whose list of zeroed keys goes with them
-    }
-    mbar_init(o_free, 256);
-    mbar_init(&drain[0], 1);
-    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
@@ -158,158 +194,179 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- TMA ----------------
     if (lane == 0) {
       bool ok = true;
-      int g = 0, n = 0;  // tiles and items so far
-      for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
-        for (int j = 0; j < it.n; ++j, ++g) {
-          const int st = g & 1, vst = g % VS;
-          if (g >= 2 && !(ok = mbar_wait_idle(&k_empty[st], ((g >> 1) & 1) ^ 1, err))) break;
-          P::load_k(p, it, j, sK + st * kTileBytes, &tmK, &k_full[st], err);
-          if (j == 0) {
-            if (n > 0 && !(ok = mbar_wait_idle(q_empty, (n - 1) & 1, err))) break;
-            P::load_q(p, it, sQ, &tmQ, q_full);
-          }
-          if (g >= VS && !(ok = mbar_wait_idle(&v_empty[vst], ((g / VS) & 1) ^ 1, err))) break;
-          P::load_v(p, it, j, sV + vst * kVBytes, &tmV, &v_full[vst], err);
+      int g = 0, n[kSides] = {0, 0};  // tiles, and items of each side, so far
+      while (ok && !*abort_flag && cursor.next(it, err)) {
+        for (int j = 0; ok && j < it.n; ++j, ++g) {
+          const int ks = g % KS, vs = g % VS;
+          if (g >= KS && !(ok = mbar_wait_idle(&k_empty[ks], (g / KS - 1) & 1, err))) break;
+          P::load_k(p, it, j, sK + ks * Cf::TILE_QK, &tmK, &k_full[ks], err);
+          if (j == 0)
+#pragma unroll
+            for (int s = 0; s < kSides; ++s) {
+              if (!ok || (s == 1 && !it.both)) break;
+              if (n[s] > 0 && !(ok = mbar_wait_idle(&q_empty[s], (n[s] - 1) & 1, err))) break;
+              P::load_q(p, it, s, smem + s * Cf::TILE_QK, &tmQ, &q_full[s]);
+              ++n[s];
+            }
+          if (!ok) break;
+          if (g >= VS && !(ok = mbar_wait_idle(&v_empty[vs], (g / VS - 1) & 1, err))) break;
+          P::load_v(p, it, j, sV + vs * Cf::TILE_V, &tmV, &v_full[vs], err);
         }
       }
       if (!ok) *abort_flag = 1;
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ---------------- scores ----------------
+    // ---------------- MMAs ----------------
     if (lane == 0) {
       bool ok = true;
-      int g = 0, n = 0;
-      for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
-        if (!(ok = mbar_wait_idle(q_full, n & 1, err))) break;
-        for (int j = 0; j < it.n; ++j, ++g) {
-          const int b = g % kSBufs, u = g / kSBufs;
-          ok = mbar_wait_idle(&k_full[g & 1], (g >> 1) & 1, err) &&
-               (g < kSBufs || mbar_wait_idle(&pv_done[b], (u - 1) & 1, err));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK + (g & 1) * kTileBytes);
+      int g = 0;                       // the current item's first tile
+      int n[kSides] = {0, 0};          // items of each side whose first scores were issued
+      int t[kSides] = {0, 0};          // tiles of each side whose P V was issued
+      int o[kSides] = {0, 0};          // items of each side whose P V began
+      // S = Q K^T of tile T (K landed) of side s; `last` of its item
+      auto scores = [&](int s, int T, bool last) {
+        const uint32_t q0 = smem_u32(smem + s * Cf::TILE_QK), k0 = smem_u32(sK + (T % KS) * Cf::TILE_QK);
 #pragma unroll
-          for (int ks = 0; ks < HDK / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * kBoxBytes + (ks & 3) * 32;
-            umma_bf16(tmem + b * 128, smem_desc_k128(q0 + off), smem_desc_k128(k0 + off), kIdescS, ks > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[b]);
-          umma_commit(&k_empty[g & 1]);
-          if (j + 1 == it.n) umma_commit(q_empty);
+        for (int k = 0; k < HDK / 16; ++k) {
+          const uint32_t off = (k >> 2) * kBoxBytes + (k & 3) * 32;
+          umma_bf16(tmem + kSideS + s * 128, smem_desc_k128(q0 + off), smem_desc_k128(k0 + off), kIdescS, k > 0 ? 1u : 0u);
         }
+        umma_commit(&s_full[s]);
+        if (last) umma_commit(&q_empty[s]);
+      };
+      auto first_scores = [&](const typename P::Item& item, int s, int T) {
+        if (!mbar_wait_idle(&q_full[s], n[s] & 1, err) || !mbar_wait_idle(&k_full[T % KS], (T / KS) & 1, err)) return false;
+        ++n[s];
+        tc_fence_after();
+        scores(s, T, item.n == 1);
+        return true;
+      };
+      bool have = cursor.next(it, err);
+      if (have) {
+#pragma unroll
+        for (int s = 0; s < kSides; ++s)
+          if (ok && (s == 0 || it.both)) ok = first_scores(it, s, 0);
+        if (ok) umma_commit(&k_empty[0]);
+      }
+      while (ok && have && !*abort_flag) {
+        typename P::Item after;
+        const bool more = cursor.next(after, err);
+        for (int j = 0; ok && j < it.n; ++j) {
+          const int T = g + j, vs = T % VS;
+          const bool last = j + 1 == it.n;
+#pragma unroll
+          for (int s = 0; s < kSides; ++s) {
+            if (!ok) break;
+            if (s == 0 || it.both) {
+              // (an item without side 1 waits for the last one that had it too)
+              ok = mbar_wait_idle(&p_full[s], t[s] & 1, err) && mbar_wait_idle(&v_ready[vs], (T / VS) & 1, err) &&
+                   (j > 0 || o[s] == 0 || mbar_wait_idle(&o_free[s], (o[s] - 1) & 1, err)) &&
+                   (j > 0 || it.both || o[1] == 0 || mbar_wait_idle(&o_free[1], (o[1] - 1) & 1, err));
+              if (!ok) break;
+              if (j == 0) ++o[s];
+              ++t[s];
+              tc_fence_after();
+              const uint32_t pa = tmem + kSideS + s * 128, v0 = smem_u32(sV + vs * Cf::TILE_V);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_bf16_ts(tmem + kSideO + s * 128, pa + k * 8, smem_desc_mn128(v0 + k * 2048, kBoxBytes), Cf::IDESC_O,
+                             (j > 0 || k > 0) ? 1u : 0u);
+              umma_commit(&pv_done[s]);
+              mbar_arrive(&pv_done[s]);
+              if (!last) {
+                if (!(ok = mbar_wait_idle(&k_full[(T + 1) % KS], ((T + 1) / KS) & 1, err))) break;
+                tc_fence_after();
+                scores(s, T + 1, j + 2 == it.n);
+              }
+            }
+            if (last && more && (s == 0 || after.both)) ok = first_scores(after, s, T + 1);
+          }
+          if (!ok) break;
+          umma_commit(&v_empty[vs]);
+          if (!last || more) umma_commit(&k_empty[(T + 1) % KS]);
+        }
+        g += it.n;
+        it = after;
+        have = more;
       }
       if (!ok) {
         *abort_flag = 1;
-        umma_commit(&drain[0]);  // every MMA issued by this thread completes before TMEM is freed
-        mbar_wait(&drain[0], 0, err);
+        umma_commit(drain);  // every MMA issued completes before TMEM is freed
+        mbar_wait(drain, 0, err);
       }
     }
     __syncwarp();
-  } else if (warp == kPvWarp) {
-    // ---------------- P.V (a whole warp: it also clears edge tiles) ----------------
+  } else if (warp == 2) {
+    // ---------------- values looked through ----------------
     bool ok = true;
     int g = 0, n = 0;
     for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
-      Hidden* hd = &hidden[n & 1];  // last read before item n - 2 let the accumulator go: see the wait on o_free
+      // Free again: V of item n was loaded after the P V of item n - VS or a later one began, and before an item's P V
+      // begins all earlier items have been stored.  VS + 1 < kHiddenRing.
+      Hidden* hd = &hidden[n % kHiddenRing];
       if (lane == 0) hd->count = 0;
-      __syncwarp();
       for (int j = 0; j < it.n; ++j, ++g) {
-        const int b = g % kSBufs, vst = g % VS;
-        ok = mbar_wait_idle(&v_full[vst], (g / VS) & 1, err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (!P::whole(it, P::key0(it, j), kTile)) {
+        const int vs = g % VS;
+        ok = __all_sync(0xffffffffu, mbar_wait_idle(&v_full[vs], (g / VS) & 1, err));
+        if (!ok) break;
+        const int key = P::key0(it, j);
+        if (!P::whole(it, 0, key) || (it.both && !P::whole(it, 1, key))) {
           uint32_t bad[4];
-          if (clear_nonfinite<Cf::BOXES_V>(sV + vst * kVBytes, bad) && lane == 0 && hd->count < kMaxEdgeTiles) {
+          if (clear_nonfinite<Cf::BOXES_V>(sV + vs * Cf::TILE_V, bad) && lane == 0 && hd->count < kMaxEdgeTiles) {
             const int at = hd->count;
-            hd->key0[at] = P::key0(it, j);
+            hd->key0[at] = key;
+#pragma unroll
             for (int i = 0; i < 4; ++i) hd->keys[at][i] = bad[i];
             hd->count = at + 1;
           }
-          __syncwarp();
-        }
-        ok = mbar_wait_idle(&p_full[b], (g / kSBufs) & 1, err) &&
-             (j > 0 || n == 0 || mbar_wait_idle(o_free, (n - 1) & 1, err));
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t pa = tmem + b * 128, v0 = smem_u32(sV + vst * kVBytes);
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            umma_bf16_ts(tmem + kOCol, pa + (ks >> 2) * 64 + (ks & 3) * 8, smem_desc_mn128(v0 + ks * 2048, kBoxBytes),
-                         Cf::IDESC_O, (j > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&pv_done[b]);
-          umma_commit(&v_empty[vst]);
-          mbar_arrive(&pv_done[b]);
         }
         __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ready[vs]);
       }
     }
-    if (!ok) {
-      *abort_flag = 1;
-      if (lane == 0) {
-        umma_commit(&drain[1]);
-        mbar_wait(&drain[1], 0, err);
-      }
-    }
-    __syncwarp();
+    if (!ok) *abort_flag = 1;
   } else {
-    // ---------------- softmax (warps 2..9: two threads per query row) ----------------
-    const int quarter = warp & 3;  // TMEM lanes this warp may access
-    const int half = (warp - 2) >> 2;
-    const int row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int pair_bar = 1 + quarter;  // named barrier of warps (quarter + 2, quarter + 6)
+    // ---------------- softmax ----------------
+    const int s = (warp - 3) >> 2;                // side
+    const int row = (warp & 3) * 32 + lane;       // TMEM lanes that this warp may access: 32 (warp % 4) ..
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + kSideS + s * 128, tO = tmem + lanes + kSideO + s * 128;
     const float scale_log2 = p.scale_log2;
     bool ok = true;
-    int g = 0, n = 0;
+    int t = 0, n = 0;  // tiles of this side, and items, so far
     for (; ok && cursor.next(it, err); ++n) {
-      const uint32_t tO = tmem + lanes + kOCol + half * (HDV / 2);
+      if (s == 1 && !it.both) continue;
       float mref = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.n; ++j, ++g) {
-        const int st = g % kSBufs;
-        // the same outcome for both warps of the pair (they meet at named barriers)
-        const bool got = __all_sync(0xffffffffu, ok && !*abort_flag && mbar_wait_idle(&s_full[st], (g / kSBufs) & 1, err));
-        if (pair_or(pair_bar, !got)) {
-          ok = false;
-          break;
-        }
+      for (int j = 0; j < it.n; ++j, ++t) {
+        // warp-uniform: the TMEM loads are warp-collective
+        ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
+        if (!ok) break;
         tc_fence_after();
-        uint32_t sr[64];
-        tmem_ld_32x32b_x32(tmem + lanes + st * 128 + half * 64, sr);
-        tmem_ld_32x32b_x32(tmem + lanes + st * 128 + half * 64 + 32, sr + 32);
-        tmem_ld_wait();
-        const int key = P::key0(it, j) + half * 64;  // first key of this thread's columns
-        if (!P::whole(it, key, 64)) {
+        uint32_t sr[128];
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (!P::sees(it, row, key + c)) sr[c] = __float_as_uint(-INFINITY);
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + c * 32, sr + c * 32);
+        tmem_ld_wait();
+        const int key = P::key0(it, j);
+        if (!P::whole(it, s, key)) {
+          uint32_t bits[4];
+          P::visible(it, s, row, key, bits);
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (!(bits[c >> 5] & (1u << (c & 31)))) sr[c] = __float_as_uint(-INFINITY);
         }
-        // raw-score max of this half (scale > 0): eight independent chains of three-input maxima
+        // raw-score maximum (scale > 0): eight independent chains of three-input maxima
         float m8[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) m8[i] = fmax3(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), -INFINITY);
 #pragma unroll
-        for (int c = 8; c < 32; ++c)
+        for (int c = 8; c < 64; ++c)
           m8[c & 7] = fmax3(m8[c & 7], __uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1]));
-        float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-        sMx[((g & 1) * 2 + half) * 128 + row] = mx;
-        named_bar_sync(pair_bar, 64);
-        mx = fmaxf(mx, sMx[((g & 1) * 2 + (half ^ 1)) * 128 + row]);
-        mx *= scale_log2;
-        // the running max moves only when it grows by more than 2^kRescaleLog2
+        const float mx = scale_log2 * fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
         float alpha = 1.f;
-        bool rescale = false;
         if (mx > mref + kRescaleLog2 || (mref == -INFINITY && mx > -INFINITY)) {
-          rescale = mref != -INFINITY;
-          alpha = rescale ? ex2(mref - mx) : 0.f;
-          l *= alpha;
+          if (mref != -INFINITY) alpha = ex2(mref - mx);
+          l *= alpha;  // 0 so far where there was no maximum
           mref = mx;
         }
         const float ref = mref == -INFINITY ? 0.f : mref;
@@ -317,54 +374,50 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i) r8[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < 64; ++c) {
           const float p0 = ex2(fmaf(__uint_as_float(sr[2 * c]), scale_log2, -ref));
           const float p1 = ex2(fmaf(__uint_as_float(sr[2 * c + 1]), scale_log2, -ref));
           r8[c & 7] += p0 + p1;
-          sr[c] = pack2(p0, p1);
+          sr[c] = pack2(p0, p1);  // 16 bits for the tensor core; the sum keeps 32
         }
+        // P over the scores: 64 columns of bf16 pairs
+        tmem_st_32x32b_x32(tS, sr);
+        tmem_st_32x32b_x32(tS + 32, sr + 32);
         l += ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
-        if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-          // a failed wait is acted on at the next tile's pair vote (no exit between pair barriers)
-          if (!__all_sync(0xffffffffu, mbar_wait_idle(&pv_done[(g - 1) % kSBufs], ((g - 1) / kSBufs) & 1, err)))
-            ok = false;
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // O holds the item's tiles before j once the last of them is done
+          ok = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+          if (!ok) break;
           tc_fence_after();
-          if (ok) {
 #pragma unroll 1
-            for (int c = 0; c < HDV / 64; ++c) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(tO + c * 32, r);
-              tmem_ld_wait();
+          for (int c = 0; c < HDV / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(tO + c * 32, r);
+            tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * (rescale ? alpha : 1.f));
-              tmem_st_32x32b_x32(tO + c * 32, r);
-            }
-            tmem_st_wait();
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st_32x32b_x32(tO + c * 32, r);
           }
         }
-        tmem_st_32x32b_x32(tmem + lanes + st * 128 + half * 64, sr);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[st]);
+        mbar_arrive(&p_full[s]);
       }
-      const bool done = __all_sync(0xffffffffu, ok && !*abort_flag &&
-                                                    mbar_wait_idle(&pv_done[(g - 1) % kSBufs], ((g - 1) / kSBufs) & 1, err));
-      if (pair_or(pair_bar, !done)) {
-        ok = false;
-        break;
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+      if (!ok) break;
+      const volatile Hidden* hd = &hidden[n % kHiddenRing];
+      for (int i = 0; i < hd->count; ++i) {  // zeroed keys that this row sees
+        uint32_t bits[4];
+        P::visible(it, s, row, hd->key0[i], bits);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (bits[w] & hd->keys[i][w]) l = NAN;
       }
-      sL[half * 128 + row] = l;
-      named_bar_sync(pair_bar, 64);
-      l += sL[(half ^ 1) * 128 + row];
-      named_bar_sync(pair_bar, 64);  // sL is rewritten at the next item's end
-      const volatile Hidden* hd = &hidden[n & 1];
-      for (int i = 0; i < hd->count; ++i)  // zeroed keys that this row sees
-        for (int c = 0; c < 128; ++c)
-          if (((hd->keys[i][c >> 5] >> (c & 31)) & 1u) && P::sees(it, row, hd->key0[i] + c)) l = NAN;
       tc_fence_after();
-      P::store(p, it, row, half, mref, l, tO);
+      P::store(p, it, s, row, mref, l, tO);
       tc_fence_before();
-      mbar_arrive(o_free);
+      mbar_arrive(&o_free[s]);
     }
     if (!ok) *abort_flag = 1;
   }
@@ -391,7 +444,7 @@ int launch_items(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
       return B200_ERROR_UNSUPPORTED;
     done[dev] = true;
   }
-  launch_kernel(k, dim3((unsigned)grid), kThreads, smem, st, mq, mk, mv, p, b200::error_word(dev));
+  launch_kernel(k, dim3((unsigned)grid), kItemThreads, smem, st, mq, mk, mv, p, b200::error_word(dev));
   B200_CHECK_LAUNCH();
   return B200_OK;
 }

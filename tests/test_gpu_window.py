@@ -159,8 +159,10 @@ def test_prompt_matches_causal_kernel_without_a_window():
     tail = (cu.data_ptr(), 2, 500, 777, 8, 2, 128, 128, 128 ** -0.5)
     G.check(G.L().b200_flash_prefill_packed(*args, outs[0].data_ptr(), 1024, 128, *tail, 1, G.stream()))
     G.check(G.L().b200_flash_prefill_window(*args, outs[1].data_ptr(), 1024, 128, *tail, 777, 0, G.stream()))
-    torch.cuda.synchronize()
-    assert torch.equal(outs[0], outs[1])
+    # the same scores, weights and products; the rows' sums are added in another order (under 2^-20 relative), which can
+    # move an output across a rounding border: one step of bf16, 2^-7 relative, and almost nowhere
+    a, b = (x.double() for x in outs)
+    assert ((a - b).abs() <= 2.0 ** -7 * a.abs()).all() and (a != b).double().mean() < 0.01
 
 
 # ------------------------------------------------------------ single tokens

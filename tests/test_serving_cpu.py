@@ -86,9 +86,9 @@ def test_nothing_to_do():
     assert L.b200_logits_process(*{**LOGITS, "rows": 0}.values()) == 0
     ws = L.b200_paged_decode_shared_workspace_bytes
     assert ws(0, 4, 2, 64, 100) == ws(2, 4, 3, 64, 100) == ws(2, 4, 2, 96, 100) == ws(2, 4, 2, 64, 0) == 0
-    # 2 sequences of 2 heads: one row tile a kv head; 1 key tile each: 2 CTAs, 4 slots of 128 x (64 + 1)
-    assert ws(2, 4, 2, 64, 100) == 4 * 128 * 65 * 4
-    assert ws(64, 32, 8, 128, 16384) >= (148 + 16) * 128 * 129 * 4
+    # 2 sequences of 2 heads: one row tile a kv head; 1 key tile each: 2 CTAs, 4 slots of 2 x 128 x (64 + 1)
+    assert ws(2, 4, 2, 64, 100) == 4 * 256 * 65 * 4
+    assert ws(64, 32, 8, 128, 16384) >= (148 + 8) * 256 * 129 * 4
 
 
 @pytest.mark.parametrize("workers", [1, 2, 7, 148])
