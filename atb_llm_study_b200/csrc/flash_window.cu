@@ -82,7 +82,13 @@ struct Window {
     }
   };
 
-  B200_DEV static int key0(const Item& it, int j) { return (j < it.head ? j : it.first + j - it.head) * kTile; }
+  // The window's tiles from its second on, then its first, then the sinks': rows
+  // meet their usual maximum at once, in a tile that they see as a whole, where
+  // the few sinks or a window's first keys would give them one to outgrow.
+  B200_DEV static int key0(const Item& it, int j) {
+    const int rest = it.n - it.head - 1;
+    return (j < rest ? it.first + 1 + j : j == rest ? it.first : j - rest - 1) * kTile;
+  }
   B200_DEV static bool whole(const Item& it, int s, int key) {
     return key + kTile - 1 <= it.at(s) && key + kTile <= it.len &&
            (it.at(s) + kTile - 1 - key < it.window || key + kTile <= it.sinks);

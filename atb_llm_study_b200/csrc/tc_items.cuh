@@ -58,14 +58,13 @@ struct Hidden {  // zeroed value rows of one item's edge tiles
 };
 constexpr int kHiddenRing = 8;
 
-// Zeroes the rows of a V tile [128 keys] that hold a NaN or an infinity; keys' bits of those in `bad`.  One warp.
+// Zeroes the rows of a V tile [128 keys] that hold a NaN or an infinity; their bits in `bad` (of lane 0).  One warp.
 template <int BOXES>
 B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) bad[w] = 0;
   // an instruction covers 4 rows, 8 lanes of 16 bytes a row; rows are 128 contiguous bytes whatever the swizzle
-#pragma unroll
+  bool any = false;
+#pragma unroll 1
   for (int w = 0; w < 4; ++w) {
     uint32_t found = 0;
 #pragma unroll
@@ -84,7 +83,8 @@ B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
           for (int r = 0; r < 4; ++r)
             if (lanes & (0xffu << (8 * r))) found |= 1u << (i * 4 + r);
       }
-    bad[w] = found;
+    if (lane == 0) bad[w] = found;
+    any |= found != 0;
     if (found)
 #pragma unroll 1
       for (int r = 0; r < 32; ++r)
@@ -93,7 +93,6 @@ B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
             *reinterpret_cast<uint4*>(sV + (c >> 3) * kBoxBytes + (w * 32 + r) * 128 + (c & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
   }
-  const bool any = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
   if (any) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads the tile
   __syncwarp();
   return any;
@@ -105,6 +104,31 @@ B200_DEV void bit_range(int a, int b, uint32_t bits[4]) {
   for (int w = 0; w < 4; ++w) {
     const int lo = min(max(a - 32 * w, 0), 32), hi = min(max(b - 32 * w, 0), 32);
     bits[w] = hi > lo ? (0xffffffffu >> (32 - hi + lo)) << lo : 0u;
+  }
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t r[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// m4 = maxima of four chains over 32 more raw scores (two an instruction).
+B200_DEV void row_max(const uint32_t r[32], float m4[4]) {
+#pragma unroll
+  for (int c = 0; c < 16; ++c) m4[c & 3] = fmax3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+}
+// 32 scores to 2^(s scale - ref): 16 bf16 pairs in place (16 bits for the tensor core), the sums in 32 bits.
+B200_DEV void row_exp(uint32_t r[32], float scale_log2, float ref, float r4[4]) {
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const float p0 = ex2(fmaf(__uint_as_float(r[2 * c]), scale_log2, -ref));
+    const float p1 = ex2(fmaf(__uint_as_float(r[2 * c + 1]), scale_log2, -ref));
+    r4[c & 3] += p0 + p1;
+    r[c] = pack2(p0, p1);
   }
 }
 
@@ -219,68 +243,74 @@ __global__ void __launch_bounds__(kItemThreads, 1)
   } else if (warp == 1) {
     // ---------------- MMAs ----------------
     if (lane == 0) {
+      // The loops over sides are not unrolled, here and in the softmax: the roles'
+      // code has to fit the SM's instruction cache together (unrolled, the fetches
+      // ran at three quarters of the rate of the cache behind it, and bound the
+      // kernel).  So what is counted per side is kept as bits.
       bool ok = true;
-      int g = 0;                       // the current item's first tile
-      int n[kSides] = {0, 0};          // items of each side whose first scores were issued
-      int t[kSides] = {0, 0};          // tiles of each side whose P V was issued
-      int o[kSides] = {0, 0};          // items of each side whose P V began
-      // S = Q K^T of tile T (K landed) of side s; `last` of its item
-      auto scores = [&](int s, int T, bool last) {
+      int g = 0;                // the current item's first tile
+      uint32_t q_bits = 0;      // parity of the items of each side whose first scores were issued
+      uint32_t p_bits = 0;      // parity of the tiles of each side whose P V was issued
+      uint32_t o_bits = 0;      // parity of the items of each side whose P V began
+      uint32_t began = 0;       // sides that had an item
+      // S = Q K^T of tile T of side s, as soon as K and (of an item's first tile) Q have landed; `last` of its item
+      auto scores = [&](int s, int T, bool first, bool last) {
+        if (first) {
+          if (!mbar_wait_idle(&q_full[s], (q_bits >> s) & 1, err)) return false;
+          q_bits ^= 1u << s;
+        }
+        if (!mbar_wait_idle(&k_full[T % KS], (T / KS) & 1, err)) return false;
+        tc_fence_after();
         const uint32_t q0 = smem_u32(smem + s * Cf::TILE_QK), k0 = smem_u32(sK + (T % KS) * Cf::TILE_QK);
+        const uint64_t qd = smem_desc_k128(q0), kd = smem_desc_k128(k0);
 #pragma unroll
         for (int k = 0; k < HDK / 16; ++k) {
-          const uint32_t off = (k >> 2) * kBoxBytes + (k & 3) * 32;
-          umma_bf16(tmem + kSideS + s * 128, smem_desc_k128(q0 + off), smem_desc_k128(k0 + off), kIdescS, k > 0 ? 1u : 0u);
+          const uint64_t off = (uint64_t)(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);  // shared memory ends below 2^18
+          umma_bf16(tmem + kSideS + s * 128, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[s]);
         if (last) umma_commit(&q_empty[s]);
-      };
-      auto first_scores = [&](const typename P::Item& item, int s, int T) {
-        if (!mbar_wait_idle(&q_full[s], n[s] & 1, err) || !mbar_wait_idle(&k_full[T % KS], (T / KS) & 1, err)) return false;
-        ++n[s];
-        tc_fence_after();
-        scores(s, T, item.n == 1);
         return true;
       };
       bool have = cursor.next(it, err);
       if (have) {
-#pragma unroll
-        for (int s = 0; s < kSides; ++s)
-          if (ok && (s == 0 || it.both)) ok = first_scores(it, s, 0);
+#pragma unroll 1
+        for (int s = 0; ok && s < (it.both ? 2 : 1); ++s) ok = scores(s, 0, true, it.n == 1);
         if (ok) umma_commit(&k_empty[0]);
       }
       while (ok && have && !*abort_flag) {
         typename P::Item after;
         const bool more = cursor.next(after, err);
+#pragma unroll 1
         for (int j = 0; ok && j < it.n; ++j) {
           const int T = g + j, vs = T % VS;
           const bool last = j + 1 == it.n;
-#pragma unroll
-          for (int s = 0; s < kSides; ++s) {
-            if (!ok) break;
+#pragma unroll 1
+          for (int s = 0; ok && s < kSides; ++s) {
             if (s == 0 || it.both) {
               // (an item without side 1 waits for the last one that had it too)
-              ok = mbar_wait_idle(&p_full[s], t[s] & 1, err) && mbar_wait_idle(&v_ready[vs], (T / VS) & 1, err) &&
-                   (j > 0 || o[s] == 0 || mbar_wait_idle(&o_free[s], (o[s] - 1) & 1, err)) &&
-                   (j > 0 || it.both || o[1] == 0 || mbar_wait_idle(&o_free[1], (o[1] - 1) & 1, err));
+              ok = mbar_wait_idle(&p_full[s], (p_bits >> s) & 1, err) && mbar_wait_idle(&v_ready[vs], (T / VS) & 1, err) &&
+                   (j > 0 || !((began >> s) & 1) || mbar_wait_idle(&o_free[s], ((o_bits >> s) & 1) ^ 1, err)) &&
+                   (j > 0 || it.both || !(began & 2) || mbar_wait_idle(&o_free[1], ((o_bits >> 1) & 1) ^ 1, err));
               if (!ok) break;
-              if (j == 0) ++o[s];
-              ++t[s];
+              if (j == 0) {
+                o_bits ^= 1u << s;
+                began |= 1u << s;
+              }
+              p_bits ^= 1u << s;
               tc_fence_after();
               const uint32_t pa = tmem + kSideS + s * 128, v0 = smem_u32(sV + vs * Cf::TILE_V);
+              const uint64_t vd = smem_desc_mn128(v0, kBoxBytes);
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                umma_bf16_ts(tmem + kSideO + s * 128, pa + k * 8, smem_desc_mn128(v0 + k * 2048, kBoxBytes), Cf::IDESC_O,
+                umma_bf16_ts(tmem + kSideO + s * 128, pa + k * 8, vd + (uint64_t)(k * 2048 >> 4), Cf::IDESC_O,
                              (j > 0 || k > 0) ? 1u : 0u);
               umma_commit(&pv_done[s]);
               mbar_arrive(&pv_done[s]);
-              if (!last) {
-                if (!(ok = mbar_wait_idle(&k_full[(T + 1) % KS], ((T + 1) / KS) & 1, err))) break;
-                tc_fence_after();
-                scores(s, T + 1, j + 2 == it.n);
-              }
             }
-            if (last && more && (s == 0 || after.both)) ok = first_scores(after, s, T + 1);
+            // the side's next scores: this item's next tile, or the next item's first
+            if (last ? more && (s == 0 || after.both) : s == 0 || it.both)
+              ok = scores(s, T + 1, last, last ? after.n == 1 : j + 2 == it.n);
           }
           if (!ok) break;
           umma_commit(&v_empty[vs]);
@@ -305,20 +335,22 @@ __global__ void __launch_bounds__(kItemThreads, 1)
       // Free again: V of item n was loaded after the P V of item n - VS or a later one began, and before an item's P V
       // begins all earlier items have been stored.  VS + 1 < kHiddenRing.
       Hidden* hd = &hidden[n % kHiddenRing];
+      int edges = 0;
       if (lane == 0) hd->count = 0;
+#pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++g) {
         const int vs = g % VS;
         ok = __all_sync(0xffffffffu, mbar_wait_idle(&v_full[vs], (g / VS) & 1, err));
         if (!ok) break;
         const int key = P::key0(it, j);
         if (!P::whole(it, 0, key) || (it.both && !P::whole(it, 1, key))) {
-          uint32_t bad[4];
-          if (clear_nonfinite<Cf::BOXES_V>(sV + vs * Cf::TILE_V, bad) && lane == 0 && hd->count < kMaxEdgeTiles) {
-            const int at = hd->count;
-            hd->key0[at] = key;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) hd->keys[at][i] = bad[i];
-            hd->count = at + 1;
+          const int at = min(edges, kMaxEdgeTiles - 1);  // an item has four at most
+          if (clear_nonfinite<Cf::BOXES_V>(sV + vs * Cf::TILE_V, hd->keys[at])) {
+            ++edges;
+            if (lane == 0) {
+              hd->key0[at] = key;
+              hd->count = at + 1;
+            }
           }
         }
         __syncwarp();
@@ -343,26 +375,39 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
         if (!ok) break;
         tc_fence_after();
-        uint32_t sr[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + c * 32, sr + c * 32);
-        tmem_ld_wait();
         const int key = P::key0(it, j);
-        if (!P::whole(it, s, key)) {
+        if (!P::whole(it, s, key)) {  // hidden scores: -inf, back to where they came from
           uint32_t bits[4];
           P::visible(it, s, row, key, bits);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t mask = c == 0 ? bits[0] : c == 1 ? bits[1] : c == 2 ? bits[2] : bits[3];
+            if (__all_sync(0xffffffffu, mask == 0xffffffffu)) continue;
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(tS + c * 32, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (!(bits[c >> 5] & (1u << (c & 31)))) sr[c] = __float_as_uint(-INFINITY);
+            for (int i = 0; i < 32; ++i)
+              if (!((mask >> i) & 1u)) r[i] = __float_as_uint(-INFINITY);
+            tmem_st_32x32b_x32(tS + c * 32, r);
+          }
+          tmem_st_wait();
         }
-        // raw-score maximum (scale > 0): eight independent chains of three-input maxima
-        float m8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmax3(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]), -INFINITY);
-#pragma unroll
-        for (int c = 8; c < 64; ++c)
-          m8[c & 7] = fmax3(m8[c & 7], __uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1]));
-        const float mx = scale_log2 * fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        // The scores are read from TMEM twice, 32 columns at a time with the next
+        // 32 on their way: once for the maximum, once for the exponentials.
+        uint32_t ra[32], rb[32];
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld_32x32b_x32(tS, ra);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_wait();
+          tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
+          row_max(ra, m4);
+          tmem_ld_wait();
+          tmem_ld_32x32b_x32(tS + ((c + 2) & 3) * 32, ra);  // at the end the first again
+          row_max(rb, m4);
+        }
+        const float mx = scale_log2 * fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);  // scale > 0
         float alpha = 1.f;
         if (mx > mref + kRescaleLog2 || (mref == -INFINITY && mx > -INFINITY)) {
           if (mref != -INFINITY) alpha = ex2(mref - mx);
@@ -370,20 +415,20 @@ __global__ void __launch_bounds__(kItemThreads, 1)
           mref = mx;
         }
         const float ref = mref == -INFINITY ? 0.f : mref;
-        float r8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r8[i] = 0.f;
-#pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          const float p0 = ex2(fmaf(__uint_as_float(sr[2 * c]), scale_log2, -ref));
-          const float p1 = ex2(fmaf(__uint_as_float(sr[2 * c + 1]), scale_log2, -ref));
-          r8[c & 7] += p0 + p1;
-          sr[c] = pack2(p0, p1);  // 16 bits for the tensor core; the sum keeps 32
+        float r4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          // P of 32 scores takes 16 columns: it never reaches scores that have not been read
+          tmem_ld_wait();
+          tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
+          row_exp(ra, scale_log2, ref, r4);
+          tmem_st_32x32b_x16(tS + c * 16, ra);
+          tmem_ld_wait();
+          if (c == 0) tmem_ld_32x32b_x32(tS + 64, ra);
+          row_exp(rb, scale_log2, ref, r4);
+          tmem_st_32x32b_x16(tS + c * 16 + 16, rb);
         }
-        // P over the scores: 64 columns of bf16 pairs
-        tmem_st_32x32b_x32(tS, sr);
-        tmem_st_32x32b_x32(tS + 32, sr + 32);
-        l += ((r8[0] + r8[1]) + (r8[2] + r8[3])) + ((r8[4] + r8[5]) + (r8[6] + r8[7]));
+        l += (r4[0] + r4[1]) + (r4[2] + r4[3]);
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           // O holds the item's tiles before j once the last of them is done
           ok = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
