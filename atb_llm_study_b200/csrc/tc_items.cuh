@@ -4,23 +4,24 @@
 //   out = sum_j p_j v_j / sum_j p_j, p_j = 2^(q.k_j scale log2(e) - m)
 //
 // An item is one or two tiles of 128 query rows ("sides") that walk one list of
-// 128-key tiles; a persistent CTA per SM walks its items.  352 threads:
-//   warp 0      TMA: each item's Q tiles, then K and V tiles through rings
-//   warp 1      one thread issues the MMAs.  Per side and key tile: O += P V of
-//               the tile whose P is ready, right behind it S = Q K^T of the
-//               next tile (the next item's first at an item's end).  Both sides
-//               use a K / V tile while it is in shared memory.
-//   warp 2      looks through V tiles for NaN and infinities (below)
-//   warps 3-6   softmax of side 0, warps 7-10 of side 1, a thread a row: the
-//               row's 128 scores from TMEM, masked, maximum, exponentials, sum,
-//               P as bf16 pairs over the scores, where the MMA reads it.
+// 128-key tiles; a persistent CTA per SM walks its items.  Its warps:
+//   0       TMA: each item's Q tiles, then K and V tiles through rings
+//   1, last  each issues the MMAs of a side.  Per key tile: O += P V of
+//           the tile whose P is ready, right behind it S = Q K^T of the next tile
+//           (the next item's first at an item's end).  Both sides use a K / V tile
+//           while it is in shared memory.
+//   2       looks through V tiles for NaN and infinities (below)
+//   3-18    softmax, eight warps a side, two threads a row (192-wide heads, whose
+//           tiles fill shared memory: four warps, one thread): scores from TMEM,
+//           masked, maximum, exponentials, sum, P as bf16 pairs over the scores,
+//           where the MMA reads it.
 // What a side's chain has to wait for itself (scores, softmax, P V) the other
 // side's fills: the tensor core works for one while the softmax units work for
 // the other.  At 128-wide heads a side's tile takes 1024 cycles of MMAs and as
 // many of exponentials (16 a cycle and SM), so the two halves of the SM are
 // equally loaded.  TMEM: two score tiles and two output accumulators, 4 x 128
-// columns.  S of the next tile overwrites P that the P V before it reads: MMAs of
-// one thread run in the order of their issue.
+// columns.  S of a side's next tile overwrites P that the P V before it reads: MMAs
+// of one lane run in the order of their issue.
 //
 // The running maximum moves only when it grows by more than 2^8 (the rows of O
 // in TMEM are then rescaled by their threads, seldom), which changes nothing in
@@ -31,22 +32,21 @@
 // not see as a whole (a prompt's end, its diagonal, the ends of the window and
 // the sinks, a cache block's rest) and zeroes those with a NaN or an infinity.
 // A row that does see such a key gets NaN: the item's list of zeroed keys is
-// looked through when its rows are stored.  The search is 64 loads and ballots a
-// tile, while the tile's scores are computed.
+// looked through when its rows are stored.  The search is 64 loads a tile,
+// while its scores are computed.
 //
 // P provides: HDK, HDV; Item with int n (key tiles, > 0), bool both (side 1 is
 // there); Cursor(p) with bool next(Item&, err); load_q(p, item, side, ..) and
 // load_k / load_v(p, item, tile, smem, map, bar, err): arrive on bar expecting
 // bytes, copy; int key0(item, tile): its first key; bool whole(item, side, key):
 // every row of the side sees the 128 keys from key on; visible(item, side, row,
-// key, bits[4]): which of them a row sees; store(p, item, side, row, m, l, tO).
+// key, bits[4]): which of them a row sees; store<COLS>(p, item, side, row, first column, m, l, tO).
 #pragma once
 
 #include "tc_attention.cuh"
 
 namespace {
 
-constexpr int kItemThreads = 352;
 constexpr int kSides = 2;
 constexpr uint32_t kSideS = 0, kSideO = 256;  // TMEM columns of side 0's scores and outputs; side 1's lie 128 further
 constexpr int kMaxEdgeTiles = 6;
@@ -62,36 +62,42 @@ constexpr int kHiddenRing = 8;
 template <int BOXES>
 B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
   const int lane = threadIdx.x & 31;
-  // an instruction covers 4 rows, 8 lanes of 16 bytes a row; rows are 128 contiguous bytes whatever the swizzle
-  bool any = false;
+  // exponent bits all ones: 0x7f80 + 0x80 carries into bit 15 of its half
+  auto odd = [](const uint4& v) {
+    return ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) |
+           ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
+  };
+  // first whether there is any: 512 bytes an instruction, sixteen on their way
+  uint32_t seen = 0;
 #pragma unroll 1
-  for (int w = 0; w < 4; ++w) {
+  for (int i = 0; i < BOXES * kBoxBytes / 512; i += 16) {
+    uint4 v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = *reinterpret_cast<const uint4*>(sV + (i + k) * 512 + lane * 16);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) seen |= odd(v[k]);
+  }
+  const bool any = __any_sync(0xffffffffu, (seen & 0x80008000u) != 0);
+  // then which rows: an instruction covers 4, 8 lanes of 16 bytes a row (a row is 128 contiguous bytes of each box,
+  // whatever the swizzle)
+#pragma unroll 1
+  for (int w = 0; any && w < 4; ++w) {
     uint32_t found = 0;
-#pragma unroll
-    for (int x = 0; x < BOXES; ++x)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(sV + x * kBoxBytes + (w * 32 + i * 4) * 128 + lane * 16);
-        // exponent bits all ones: 0x7f80 + 0x80 carries into bit 15
-        uint32_t t = (v.x & 0x7f807f80u) + 0x00800080u;
-        t |= (v.y & 0x7f807f80u) + 0x00800080u;
-        t |= (v.z & 0x7f807f80u) + 0x00800080u;
-        t |= (v.w & 0x7f807f80u) + 0x00800080u;
-        const uint32_t lanes = __ballot_sync(0xffffffffu, (t & 0x80008000u) != 0);
-        if (lanes)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (lanes & (0xffu << (8 * r))) found |= 1u << (i * 4 + r);
-      }
-    if (lane == 0) bad[w] = found;
-    any |= found != 0;
-    if (found)
 #pragma unroll 1
-      for (int r = 0; r < 32; ++r)
-        if ((found >> r) & 1u)
-          for (int c = lane; c < BOXES * 8; c += 32)
-            *reinterpret_cast<uint4*>(sV + (c >> 3) * kBoxBytes + (w * 32 + r) * 128 + (c & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < BOXES * 8; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(sV + (i >> 3) * kBoxBytes + (w * 32 + (i & 7) * 4) * 128 + lane * 16);
+      const uint32_t lanes = __ballot_sync(0xffffffffu, (odd(v) & 0x80008000u) != 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (lanes & (0xffu << (8 * r))) found |= 1u << ((i & 7) * 4 + r);
+    }
+    if (lane == 0) bad[w] = found;
+#pragma unroll 1
+    for (uint32_t left = found; left; left &= left - 1) {
+      const int r = w * 32 + __ffs(left) - 1;
+      for (int c = lane; c < BOXES * 8; c += 32)
+        *reinterpret_cast<uint4*>(sV + (c >> 3) * kBoxBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
   }
   if (any) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads the tile
   __syncwarp();
@@ -140,57 +146,64 @@ struct ItemsCfg {
   static constexpr int V_STAGES = P::HDK > 128 ? 1 : P::HDK > 64 ? 2 : 4;
   static constexpr int K_AT = kSides * TILE_QK, V_AT = K_AT + K_STAGES * TILE_QK, BARS_AT = V_AT + V_STAGES * TILE_V;
   static constexpr int HIDDEN_AT = BARS_AT + 320;
-  static constexpr int SMEM = HIDDEN_AT + kHiddenRing * (int)sizeof(Hidden) + 1024;
+  // threads a row: two where shared memory has room for what they tell each other
+  static constexpr int HALVES = 1;
+  static constexpr int EXCHANGE_AT = HIDDEN_AT + kHiddenRing * (int)sizeof(Hidden);
+  static constexpr int SMEM = EXCHANGE_AT + (HALVES - 1) * kSides * 3 * 2 * 128 * 4 + 1024;
+  static constexpr int THREADS = 128 + kSides * HALVES * 128;
+  static constexpr int MMA1_WARP = 3 + kSides * HALVES * 4;  // the second side's issuer
   static constexpr uint32_t IDESC_O = idesc_bf16_f32(128, P::HDV) | (1u << 16);  // B operand (V) MN-major
 };
 
 template <class P>
-__global__ void __launch_bounds__(kItemThreads, 1)
+__global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
     tc_items_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const P p, unsigned* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Cf = ItemsCfg<P>;
-  constexpr int HDK = P::HDK, HDV = P::HDV, KS = Cf::K_STAGES, VS = Cf::V_STAGES;
+  constexpr int HDK = P::HDK, HDV = P::HDV, KS = Cf::K_STAGES, VS = Cf::V_STAGES, HALVES = Cf::HALVES;
   uint8_t* sK = smem + Cf::K_AT;
   uint8_t* sV = smem + Cf::V_AT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BARS_AT);
   uint64_t* q_full = bars;           // [side] the item's Q landed
   uint64_t* q_empty = bars + 2;      // [side] the item's last scores are done: Q may be replaced
   uint64_t* s_full = bars + 4;       // [side] scores of a tile ready
-  uint64_t* p_full = bars + 6;       // [side] P of a tile written (128 arrivals)
+  uint64_t* p_full = bars + 6;       // [side] P of a tile written (an arrival a softmax thread)
   uint64_t* pv_done = bars + 8;      // [side] P V of a tile done, and the list of zeroed keys behind it (2 arrivals)
-  uint64_t* o_free = bars + 10;      // [side] the outputs are read out (128 arrivals)
-  uint64_t* drain = bars + 12;       // the MMAs issued before an abort
-  uint64_t* k_full = bars + 13;      // [KS]
-  uint64_t* k_empty = k_full + KS;   // [KS]
+  uint64_t* o_free = bars + 10;      // [side] the outputs are read out (an arrival a softmax thread)
+  uint64_t* drain = bars + 12;       // [side] the MMAs issued before an abort
+  uint64_t* turn = bars + 14;        // [side] it may issue
+  uint64_t* k_full = bars + 16;      // [KS]
+  uint64_t* k_empty = k_full + KS;   // [KS] (an arrival a side, as v_empty)
   uint64_t* v_full = k_empty + KS;   // [VS] landed
   uint64_t* v_ready = v_full + VS;   // [VS] and looked through
   uint64_t* v_empty = v_ready + VS;  // [VS]
-  static_assert((13 + 2 * KS + 3 * VS) * 8 + 8 <= 320, "barriers");
+  static_assert((16 + 2 * KS + 3 * VS) * 8 + 8 <= 320, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + VS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Hidden* hidden = reinterpret_cast<Hidden*>(smem + Cf::HIDDEN_AT);  // [item % kHiddenRing]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // one value a warp
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSides; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s], 128 * HALVES);
       mbar_init(&pv_done[s], 2);
-      mbar_init(&o_free[s], 128);
+      mbar_init(&o_free[s], 128 * HALVES);
+      mbar_init(&drain[s], 1);
+      mbar_init(&turn[s], 1);
     }
-    mbar_init(drain, 1);
     for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
     }
     for (int i = 0; i < VS; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_ready[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -210,7 +223,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   typename P::Cursor cursor(p);
   typename P::Item it;
 
@@ -240,91 +253,102 @@ __global__ void __launch_bounds__(kItemThreads, 1)
       if (!ok) *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ---------------- MMAs ----------------
-    if (lane == 0) {
-      // The loops over sides are not unrolled, here and in the softmax: the roles'
-      // code has to fit the SM's instruction cache together (unrolled, the fetches
-      // ran at three quarters of the rate of the cache behind it, and bound the
-      // kernel).  So what is counted per side is kept as bits.
-      bool ok = true;
-      int g = 0;                // the current item's first tile
-      uint32_t q_bits = 0;      // parity of the items of each side whose first scores were issued
-      uint32_t p_bits = 0;      // parity of the tiles of each side whose P V was issued
-      uint32_t o_bits = 0;      // parity of the items of each side whose P V began
-      uint32_t began = 0;       // sides that had an item
-      // S = Q K^T of tile T of side s, as soon as K and (of an item's first tile) Q have landed; `last` of its item
-      auto scores = [&](int s, int T, bool first, bool last) {
-        if (first) {
-          if (!mbar_wait_idle(&q_full[s], (q_bits >> s) & 1, err)) return false;
-          q_bits ^= 1u << s;
+  } else if (warp == 1 || warp == Cf::MMA1_WARP) {
+    // ---------------- MMAs of a side ----------------
+    // The sides take turns, a batch (P V, next scores) each: issued side by side,
+    // both batches end together, and so both softmaxes begin together and leave
+    // the tensor core without work.  A warp a side, so that one's waits and commits
+    // pass while the other's batch runs.  A side's MMAs keep their order, which S
+    // over the P before it needs; the sides touch different columns.
+    const int s = warp == 1 ? 0 : 1;
+    bool ok = true;
+    int g = 0;           // the current item's first tile
+    uint32_t n = 0;      // items of this side whose first scores were issued
+    uint32_t t = 0;      // its tiles whose P V was issued
+    uint32_t o = 0;      // its items whose P V began
+    uint32_t o1 = 0;     // side 0: side 1's items before
+    uint32_t turns = 0;  // of this side so far
+    const uint32_t tS = tmem + kSideS + s * 128, tO = tmem + kSideO + s * 128;
+    const uint64_t qd = smem_desc_k128(smem_u32(smem + s * Cf::TILE_QK));
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_idle(bar, parity, err)); };
+    // (a thread that sleeps in a wait wakes 200 cycles later than one that polls)
+    auto spin = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); };
+    // K of tile T and (of an item's first tile) Q have landed
+    auto landed = [&](int T, bool first) {
+      return (!first || wait(&q_full[s], n++ & 1)) && wait(&k_full[T % KS], (T / KS) & 1);
+    };
+    // S = Q K^T of tile T; `last` of its item
+    auto scores = [&](int T, bool last) {
+      const uint64_t kd = smem_desc_k128(smem_u32(sK + (T % KS) * Cf::TILE_QK));
+#pragma unroll
+      for (int k = 0; k < HDK / 16; ++k) {
+        const uint64_t off = (uint64_t)(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);  // shared memory ends below 2^18
+        umma_bf16_elect(tS, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+      }
+      umma_commit_elect(&s_full[s]);
+      umma_commit_elect(&k_empty[T % KS]);
+      if (last) umma_commit_elect(&q_empty[s]);
+    };
+    // side 0 begins; then each waits until the other has issued its batch of a tile
+    auto my_turn = [&] {
+      const uint32_t k = turns++;
+      return s == 0 ? k == 0 || wait(&turn[0], (k - 1) & 1) : wait(&turn[1], k & 1);
+    };
+    bool have = cursor.next(it, err);
+    if (have) {
+      const bool mine = s == 0 || it.both;
+      ok = landed(0, mine);
+      tc_fence_after();
+      if (ok && mine) scores(0, it.n == 1);
+      else if (ok) mbar_arrive_elect(&k_empty[0]);
+    }
+    while (ok && have && !*abort_flag) {
+      typename P::Item after;
+      const bool more = cursor.next(after, err);
+      const bool mine = s == 0 || it.both;
+#pragma unroll 1
+      for (int j = 0; ok && j < it.n; ++j) {
+        const int T = g + j, vs = T % VS;
+        const bool last = j + 1 == it.n;
+        const bool next = !last || more;                          // scores of tile T + 1 are to come
+        const bool next_mine = s == 0 || (last ? after.both : it.both);  // of this side
+        // everything is waited for before the batch is issued, so that its products follow one another
+        ok = (!next || landed(T + 1, last && next_mine)) && wait(&v_ready[vs], (T / VS) & 1);
+        if (ok && mine && j == 0) {
+          // all earlier items are stored (an item without side 1 waits for the last one that had it too)
+          ok = (o == 0 || wait(&o_free[s], (o - 1) & 1)) && (it.both || o1 == 0 || wait(&o_free[1], (o1 - 1) & 1));
+          ++o;
+          o1 += it.both;
         }
-        if (!mbar_wait_idle(&k_full[T % KS], (T / KS) & 1, err)) return false;
+        ok = ok && my_turn() && (!mine || spin(&p_full[s], t++ & 1));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t q0 = smem_u32(smem + s * Cf::TILE_QK), k0 = smem_u32(sK + (T % KS) * Cf::TILE_QK);
-        const uint64_t qd = smem_desc_k128(q0), kd = smem_desc_k128(k0);
+        if (mine) {
+          const uint64_t vd = smem_desc_mn128(smem_u32(sV + vs * Cf::TILE_V), kBoxBytes);
 #pragma unroll
-        for (int k = 0; k < HDK / 16; ++k) {
-          const uint64_t off = (uint64_t)(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);  // shared memory ends below 2^18
-          umma_bf16(tmem + kSideS + s * 128, qd + off, kd + off, kIdescS, k > 0 ? 1u : 0u);
+          for (int k = 0; k < 8; ++k)
+            umma_bf16_ts_elect(tO, tS + (HALVES == 2 ? (k >> 2) * 64 + (k & 3) * 8 : k * 8),
+                               vd + (uint64_t)(k * 2048 >> 4), Cf::IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit_elect(&pv_done[s]);
         }
-        umma_commit(&s_full[s]);
-        if (last) umma_commit(&q_empty[s]);
-        return true;
-      };
-      bool have = cursor.next(it, err);
-      if (have) {
-#pragma unroll 1
-        for (int s = 0; ok && s < (it.both ? 2 : 1); ++s) ok = scores(s, 0, true, it.n == 1);
-        if (ok) umma_commit(&k_empty[0]);
-      }
-      while (ok && have && !*abort_flag) {
-        typename P::Item after;
-        const bool more = cursor.next(after, err);
-#pragma unroll 1
-        for (int j = 0; ok && j < it.n; ++j) {
-          const int T = g + j, vs = T % VS;
-          const bool last = j + 1 == it.n;
-#pragma unroll 1
-          for (int s = 0; ok && s < kSides; ++s) {
-            if (s == 0 || it.both) {
-              // (an item without side 1 waits for the last one that had it too)
-              ok = mbar_wait_idle(&p_full[s], (p_bits >> s) & 1, err) && mbar_wait_idle(&v_ready[vs], (T / VS) & 1, err) &&
-                   (j > 0 || !((began >> s) & 1) || mbar_wait_idle(&o_free[s], ((o_bits >> s) & 1) ^ 1, err)) &&
-                   (j > 0 || it.both || !(began & 2) || mbar_wait_idle(&o_free[1], ((o_bits >> 1) & 1) ^ 1, err));
-              if (!ok) break;
-              if (j == 0) {
-                o_bits ^= 1u << s;
-                began |= 1u << s;
-              }
-              p_bits ^= 1u << s;
-              tc_fence_after();
-              const uint32_t pa = tmem + kSideS + s * 128, v0 = smem_u32(sV + vs * Cf::TILE_V);
-              const uint64_t vd = smem_desc_mn128(v0, kBoxBytes);
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                umma_bf16_ts(tmem + kSideO + s * 128, pa + k * 8, vd + (uint64_t)(k * 2048 >> 4), Cf::IDESC_O,
-                             (j > 0 || k > 0) ? 1u : 0u);
-              umma_commit(&pv_done[s]);
-              mbar_arrive(&pv_done[s]);
-            }
-            // the side's next scores: this item's next tile, or the next item's first
-            if (last ? more && (s == 0 || after.both) : s == 0 || it.both)
-              ok = scores(s, T + 1, last, last ? after.n == 1 : j + 2 == it.n);
-          }
-          if (!ok) break;
-          umma_commit(&v_empty[vs]);
-          if (!last || more) umma_commit(&k_empty[(T + 1) % KS]);
+        if (next && next_mine) scores(T + 1, last ? after.n == 1 : j + 2 == it.n);
+        mbar_arrive_elect(&turn[s ^ 1]);
+        if (next && !next_mine) mbar_arrive_elect(&k_empty[(T + 1) % KS]);  // a tile that this side does not use
+        if (mine) {
+          mbar_arrive_elect(&pv_done[s]);
+          umma_commit_elect(&v_empty[vs]);
+        } else {
+          mbar_arrive_elect(&v_empty[vs]);
         }
-        g += it.n;
-        it = after;
-        have = more;
       }
-      if (!ok) {
-        *abort_flag = 1;
-        umma_commit(drain);  // every MMA issued completes before TMEM is freed
-        mbar_wait(drain, 0, err);
-      }
+      g += it.n;
+      it = after;
+      have = more;
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      umma_commit_elect(&drain[s]);  // every MMA issued completes before TMEM is freed
+      mbar_wait(&drain[s], 0, err);
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -360,28 +384,42 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     if (!ok) *abort_flag = 1;
   } else {
     // ---------------- softmax ----------------
-    const int s = (warp - 3) >> 2;                // side
-    const int row = (warp & 3) * 32 + lane;       // TMEM lanes that this warp may access: 32 (warp % 4) ..
+    // Thread (side, half, row) takes 128 / HALVES of its row's scores.  Two of a row
+    // tell each other their maxima, a tile each, so both move the running maximum
+    // alike; their sums meet at the item's end.
+    constexpr int COLS = 128 / HALVES, OCOLS = HDV / HALVES;
+    const int s = (warp - 3) / (4 * HALVES), half = (warp - 3) / 4 % HALVES;
+    const int row = (warp & 3) * 32 + lane;  // TMEM lanes that this warp may access: 32 (warp % 4) ..
+    const int pair_bar = 1 + s * 4 + (warp & 3);
+    float* ex = reinterpret_cast<float*>(smem + Cf::EXCHANGE_AT) + s * 3 * 2 * 128;  // [2 tiles' maxima, sums][half][row]
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + kSideS + s * 128, tO = tmem + lanes + kSideO + s * 128;
+    const uint32_t tS = tmem + lanes + kSideS + s * 128 + half * COLS, tO = tmem + lanes + kSideO + s * 128 + half * OCOLS;
     const float scale_log2 = p.scale_log2;
     bool ok = true;
     int t = 0, n = 0;  // tiles of this side, and items, so far
+    // the outcome of a wait, the same for the threads that meet at barriers and for TMEM's warp-wide accesses
+    auto agreed = [&](bool mine) {
+      mine = __all_sync(0xffffffffu, mine);
+      return HALVES == 1 ? mine : !pair_or(pair_bar, !mine);
+    };
+#pragma unroll 1
     for (; ok && cursor.next(it, err); ++n) {
       if (s == 1 && !it.both) continue;
       float mref = -INFINITY, l = 0.f;
+#pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++t) {
-        // warp-uniform: the TMEM loads are warp-collective
-        ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
+        ok = agreed(!*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
         if (!ok) break;
         tc_fence_after();
         const int key = P::key0(it, j);
-        if (!P::whole(it, s, key)) {  // hidden scores: -inf, back to where they came from
+        const bool edge = !P::whole(it, s, key);
+        if (edge) {  // hidden scores: -inf, back to where they came from
           uint32_t bits[4];
           P::visible(it, s, row, key, bits);
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t mask = c == 0 ? bits[0] : c == 1 ? bits[1] : c == 2 ? bits[2] : bits[3];
+          for (int c = 0; c < COLS / 32; ++c) {
+            const int w = half * (COLS / 32) + c;
+            const uint32_t mask = w == 0 ? bits[0] : w == 1 ? bits[1] : w == 2 ? bits[2] : bits[3];
             if (__all_sync(0xffffffffu, mask == 0xffffffffu)) continue;
             uint32_t r[32];
             tmem_ld_32x32b_x32(tS + c * 32, r);
@@ -393,21 +431,34 @@ __global__ void __launch_bounds__(kItemThreads, 1)
           }
           tmem_st_wait();
         }
-        // The scores are read from TMEM twice, 32 columns at a time with the next
-        // 32 on their way: once for the maximum, once for the exponentials.
         uint32_t ra[32], rb[32];
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         tmem_ld_32x32b_x32(tS, ra);
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
+        if (HALVES == 2) {
+          tmem_ld_32x32b_x32(tS + 32, rb);
           tmem_ld_wait();
-          tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
           row_max(ra, m4);
-          tmem_ld_wait();
-          tmem_ld_32x32b_x32(tS + ((c + 2) & 3) * 32, ra);  // at the end the first again
           row_max(rb, m4);
+        } else {
+          // the scores are read from TMEM twice, 32 columns at a time with the next 32 on their way: once for the
+          // maximum, once for the exponentials
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {
+            tmem_ld_wait();
+            tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
+            row_max(ra, m4);
+            tmem_ld_wait();
+            tmem_ld_32x32b_x32(tS + ((c + 2) & 3) * 32, ra);  // at the end the first again
+            row_max(rb, m4);
+          }
         }
-        const float mx = scale_log2 * fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);  // scale > 0
+        float mx = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+        if (HALVES == 2) {  // (places alternate: the other half is at most a tile behind)
+          ex[((t & 1) * 2 + half) * 128 + row] = mx;
+          named_bar_sync(pair_bar, 64);
+          mx = fmaxf(mx, ex[((t & 1) * 2 + (half ^ 1)) * 128 + row]);
+        }
+        mx *= scale_log2;  // scale > 0
         float alpha = 1.f;
         if (mx > mref + kRescaleLog2 || (mref == -INFINITY && mx > -INFINITY)) {
           if (mref != -INFINITY) alpha = ex2(mref - mx);
@@ -416,32 +467,39 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         }
         const float ref = mref == -INFINITY ? 0.f : mref;
         float r4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          // P of 32 scores takes 16 columns: it never reaches scores that have not been read
-          tmem_ld_wait();
-          tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
+        // P of 32 scores takes 16 columns, over scores that have been read
+        if (HALVES == 2) {
           row_exp(ra, scale_log2, ref, r4);
-          tmem_st_32x32b_x16(tS + c * 16, ra);
-          tmem_ld_wait();
-          if (c == 0) tmem_ld_32x32b_x32(tS + 64, ra);
+          tmem_st_32x32b_x16(tS, ra);
           row_exp(rb, scale_log2, ref, r4);
-          tmem_st_32x32b_x16(tS + c * 16 + 16, rb);
+          tmem_st_32x32b_x16(tS + 16, rb);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {
+            tmem_ld_wait();
+            tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
+            row_exp(ra, scale_log2, ref, r4);
+            tmem_st_32x32b_x16(tS + c * 16, ra);
+            tmem_ld_wait();
+            if (c == 0) tmem_ld_32x32b_x32(tS + 64, ra);
+            row_exp(rb, scale_log2, ref, r4);
+            tmem_st_32x32b_x16(tS + c * 16 + 16, rb);
+          }
         }
         l += (r4[0] + r4[1]) + (r4[2] + r4[3]);
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // O holds the item's tiles before j once the last of them is done
-          ok = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
-          if (!ok) break;
+          // O holds the item's tiles before j once the last of them is done.  (A failed wait is acted on at the next
+          // agreement: no way out between two threads' barriers.)
+          const bool done = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+          if (!done) *abort_flag = 1;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HDV / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(tO + c * 32, r);
+          for (int c = 0; c < (done ? OCOLS / 32 : 0); ++c) {
+            tmem_ld_32x32b_x32(tO + c * 32, ra);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st_32x32b_x32(tO + c * 32, r);
+            for (int i = 0; i < 32; ++i) ra[i] = __float_as_uint(__uint_as_float(ra[i]) * alpha);
+            tmem_st_32x32b_x32(tO + c * 32, ra);
           }
         }
         tmem_st_wait();
@@ -449,9 +507,15 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         mbar_arrive(&p_full[s]);
       }
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+      ok = agreed(!*abort_flag && mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
       if (!ok) break;
+      if (HALVES == 2) {  // rewritten an item later, after an agreement
+        ex[(4 + half) * 128 + row] = l;
+        named_bar_sync(pair_bar, 64);
+        l += ex[(4 + (half ^ 1)) * 128 + row];
+      }
       const volatile Hidden* hd = &hidden[n % kHiddenRing];
+#pragma unroll 1
       for (int i = 0; i < hd->count; ++i) {  // zeroed keys that this row sees
         uint32_t bits[4];
         P::visible(it, s, row, hd->key0[i], bits);
@@ -460,7 +524,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
           if (bits[w] & hd->keys[i][w]) l = NAN;
       }
       tc_fence_after();
-      P::store(p, it, s, row, mref, l, tO);
+      P::template store<OCOLS>(p, it, s, row, half * OCOLS, mref, l, tO);
       tc_fence_before();
       mbar_arrive(&o_free[s]);
     }
@@ -489,7 +553,7 @@ int launch_items(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
       return B200_ERROR_UNSUPPORTED;
     done[dev] = true;
   }
-  launch_kernel(k, dim3((unsigned)grid), kItemThreads, smem, st, mq, mk, mv, p, b200::error_word(dev));
+  launch_kernel(k, dim3((unsigned)grid), ItemsCfg<P>::THREADS, smem, st, mq, mk, mv, p, b200::error_word(dev));
   B200_CHECK_LAUNCH();
   return B200_OK;
 }
