@@ -94,13 +94,9 @@ struct Window {
            (it.at(s) + kTile - 1 - key < it.window || key + kTile <= it.sinks);
   }
   // key <= i and key < len and (key > i - window or key < sinks), i the row's position
-  B200_DEV static void visible(const Item& it, int s, int row, int key, uint32_t bits[4]) {
+  B200_DEV static uint32_t visible(const Item& it, int s, int row, int key) {
     const int i = it.at(s) + row, end = min(i + 1, it.len) - key;
-    uint32_t sink[4];
-    bit_range(i - it.window + 1 - key, end, bits);
-    bit_range(0, min(it.sinks - key, end), sink);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) bits[w] |= sink[w];
+    return bit_range(i - it.window + 1 - key, end) | bit_range(0, min(it.sinks - key, end));
   }
   B200_DEV static void load_q(const Window& p, const Item& it, int s, uint8_t* dst, const CUtensorMap* map,
                               uint64_t* bar) {

@@ -72,7 +72,7 @@ struct Prefix {
 
   B200_DEV static int key0(const Item& it, int j) { return (it.first + j) * kTile; }
   B200_DEV static bool whole(const Item& it, int, int key) { return key + kTile <= it.length; }
-  B200_DEV static void visible(const Item& it, int, int, int key, uint32_t bits[4]) { bit_range(0, it.length - key, bits); }
+  B200_DEV static uint32_t visible(const Item& it, int, int, int key) { return bit_range(0, it.length - key); }
   // box rows are the group's heads of per_tile sequences; rows behind them are not written, and not used
   B200_DEV static void load_q(const Prefix& p, const Item& it, int s, uint8_t* dst, const CUtensorMap* map,
                               uint64_t* bar) {

@@ -40,7 +40,7 @@
 // load_k / load_v(p, item, tile, smem, map, bar, err): arrive on bar expecting
 // bytes, copy; int key0(item, tile): its first key; bool whole(item, side, key):
 // every row of the side sees the 128 keys from key on; visible(item, side, row,
-// key, bits[4]): which of them a row sees; store<COLS>(p, item, side, row, first column, m, l, tO).
+// key): bits of the 32 from key on that a row sees; store<COLS>(p, item, side, row, first column, m, l, tO).
 #pragma once
 
 #include "tc_attention.cuh"
@@ -104,13 +104,11 @@ B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
   return any;
 }
 
-// Bits [a, b) of 128.
-B200_DEV void bit_range(int a, int b, uint32_t bits[4]) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int lo = min(max(a - 32 * w, 0), 32), hi = min(max(b - 32 * w, 0), 32);
-    bits[w] = hi > lo ? (0xffffffffu >> (32 - hi + lo)) << lo : 0u;
-  }
+// Bits [a, b) of 32.
+B200_DEV uint32_t bit_range(int a, int b) {
+  a = max(a, 0);
+  b = min(b, 32);
+  return b > a ? (0xffffffffu >> (32 - b + a)) << a : 0u;
 }
 
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t r[16]) {
@@ -122,18 +120,81 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       : "memory");
 }
 
-// m4 = maxima of four chains over 32 more raw scores (two an instruction).
+// max(a, b, c), NaN where one is
+B200_DEV float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// m4 = maxima of four chains over 32 more raw scores (two an instruction); NaN stays.
 B200_DEV void row_max(const uint32_t r[32], float m4[4]) {
 #pragma unroll
-  for (int c = 0; c < 16; ++c) m4[c & 3] = fmax3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+  for (int c = 0; c < 16; ++c) m4[c & 3] = fmax3_nan(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
 }
-// 32 scores to 2^(s scale - ref): 16 bf16 pairs in place (16 bits for the tensor core), the sums in 32 bits.
-B200_DEV void row_exp(uint32_t r[32], float scale_log2, float ref, float r4[4]) {
+
+// Two floats an instruction.
+B200_DEV uint64_t pair64(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+B200_DEV void unpair64(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+B200_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+B200_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values without the special-function unit: x = n + f with n the
+// nearest integer (adding 1.5 x 2^23 leaves it in the low bits) and |f| <= 1/2;
+// 2^f by the polynomial of degree 4 with the least relative error there (2.7e-6,
+// fitted; P is rounded to 2^-9 next), n added to its exponent.  x below -126
+// (hidden scores are -inf) counts as -126, and 2^-126 is taken from all results:
+// nothing to any P that matters, and it leaves those at 1e-44, 0 as bf16, so
+// that not even the largest finite value that nobody sees adds anything.
+B200_DEV void exp2_pair(uint64_t x2, float& p0, float& p1) {
+  const uint64_t magic = pair64(12582912.f, 12582912.f);
+  float x0, x1;
+  unpair64(x2, x0, x1);
+  x2 = pair64(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t n2 = add2(x2, magic);
+  const uint64_t f2 = add2(x2, add2(magic, n2 ^ 0x8000000080000000ull));
+  uint64_t y = fma2(f2, pair64(0.009570100344717503f, 0.009570100344717503f), pair64(0.05591785907745361f, 0.05591785907745361f));
+  y = fma2(y, f2, pair64(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f2, pair64(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f2, pair64(0.9999992847442627f, 0.9999992847442627f));
+  float y0, y1, n0, n1;
+  unpair64(y, y0, y1);
+  unpair64(n2, n0, n1);
+  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(n0) << 23));
+  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(n1) << 23));
+  unpair64(add2(pair64(y0, y1), pair64(-1.17549435e-38f, -1.17549435e-38f)), p0, p1);
+}
+
+// 32 scores to 2^(s scale - ref): 16 bf16 pairs in place (16 bits for the tensor
+// core), the sums in 32 bits.  kPoly of 4 pairs go without the special-function
+// unit, whose 16 results a cycle and SM would bound the kernel as the tensor core
+// does (@@).
+constexpr int kPoly = 1;
+B200_DEV void row_exp(uint32_t r[32], float scale_log2, float ref, uint64_t sums[2]) {
+  const uint64_t scale2 = pair64(scale_log2, scale_log2), ref2 = pair64(-ref, -ref);
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
-    const float p0 = ex2(fmaf(__uint_as_float(r[2 * c]), scale_log2, -ref));
-    const float p1 = ex2(fmaf(__uint_as_float(r[2 * c + 1]), scale_log2, -ref));
-    r4[c & 3] += p0 + p1;
+    const uint64_t x2 = fma2(pair64(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), scale2, ref2);
+    float p0, p1;
+    if (c % 4 >= 4 - kPoly) {
+      exp2_pair(x2, p0, p1);
+    } else {
+      unpair64(x2, p0, p1);
+      p0 = ex2(p0);
+      p1 = ex2(p1);
+    }
+    sums[c & 1] = add2(sums[c & 1], pair64(p0, p1));
     r[c] = pack2(p0, p1);
   }
 }
@@ -412,18 +473,18 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
         if (!ok) break;
         tc_fence_after();
         const int key = P::key0(it, j);
-        const bool edge = !P::whole(it, s, key);
-        if (edge) {  // hidden scores: -inf, back to where they came from
-          uint32_t bits[4];
-          P::visible(it, s, row, key, bits);
+        // Hidden scores become -inf where they lie.  (Branches around unseen columns in
+        // the passes below cost every tile a fifth of its softmax.)
+        if (!P::whole(it, s, key)) {
 #pragma unroll 1
           for (int c = 0; c < COLS / 32; ++c) {
-            const int w = half * (COLS / 32) + c;
-            const uint32_t mask = w == 0 ? bits[0] : w == 1 ? bits[1] : w == 2 ? bits[2] : bits[3];
+            const uint32_t mask = P::visible(it, s, row, key + half * COLS + c * 32);
             if (__all_sync(0xffffffffu, mask == 0xffffffffu)) continue;
             uint32_t r[32];
-            tmem_ld_32x32b_x32(tS + c * 32, r);
-            tmem_ld_wait();
+            if (!__all_sync(0xffffffffu, mask == 0)) {
+              tmem_ld_32x32b_x32(tS + c * 32, r);
+              tmem_ld_wait();
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((mask >> i) & 1u)) r[i] = __float_as_uint(-INFINITY);
@@ -452,13 +513,14 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
             row_max(rb, m4);
           }
         }
-        float mx = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]);
+        float mx = fmax3_nan(fmax3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY);
         if (HALVES == 2) {  // (places alternate: the other half is at most a tile behind)
           ex[((t & 1) * 2 + half) * 128 + row] = mx;
           named_bar_sync(pair_bar, 64);
-          mx = fmaxf(mx, ex[((t & 1) * 2 + (half ^ 1)) * 128 + row]);
+          mx = fmax3_nan(mx, ex[((t & 1) * 2 + (half ^ 1)) * 128 + row], -INFINITY);
         }
-        mx *= scale_log2;  // scale > 0
+        if (mx != mx) l = NAN;  // a visible score is: so is the row
+        mx *= scale_log2;       // scale > 0
         float alpha = 1.f;
         if (mx > mref + kRescaleLog2 || (mref == -INFINITY && mx > -INFINITY)) {
           if (mref != -INFINITY) alpha = ex2(mref - mx);
@@ -466,27 +528,29 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
           mref = mx;
         }
         const float ref = mref == -INFINITY ? 0.f : mref;
-        float r4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sums[2] = {0, 0};
         // P of 32 scores takes 16 columns, over scores that have been read
         if (HALVES == 2) {
-          row_exp(ra, scale_log2, ref, r4);
+          row_exp(ra, scale_log2, ref, sums);
           tmem_st_32x32b_x16(tS, ra);
-          row_exp(rb, scale_log2, ref, r4);
+          row_exp(rb, scale_log2, ref, sums);
           tmem_st_32x32b_x16(tS + 16, rb);
         } else {
 #pragma unroll 1
           for (int c = 0; c < 4; c += 2) {
             tmem_ld_wait();
             tmem_ld_32x32b_x32(tS + (c + 1) * 32, rb);
-            row_exp(ra, scale_log2, ref, r4);
+            row_exp(ra, scale_log2, ref, sums);
             tmem_st_32x32b_x16(tS + c * 16, ra);
             tmem_ld_wait();
             if (c == 0) tmem_ld_32x32b_x32(tS + 64, ra);
-            row_exp(rb, scale_log2, ref, r4);
+            row_exp(rb, scale_log2, ref, sums);
             tmem_st_32x32b_x16(tS + c * 16 + 16, rb);
           }
         }
-        l += (r4[0] + r4[1]) + (r4[2] + r4[3]);
+        float l0, l1;
+        unpair64(add2(sums[0], sums[1]), l0, l1);
+        l += l0 + l1;
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           // O holds the item's tiles before j once the last of them is done.  (A failed wait is acted on at the next
           // agreement: no way out between two threads' barriers.)
@@ -517,11 +581,9 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
       const volatile Hidden* hd = &hidden[n % kHiddenRing];
 #pragma unroll 1
       for (int i = 0; i < hd->count; ++i) {  // zeroed keys that this row sees
-        uint32_t bits[4];
-        P::visible(it, s, row, hd->key0[i], bits);
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < 4; ++w)
-          if (bits[w] & hd->keys[i][w]) l = NAN;
+          if (P::visible(it, s, row, hd->key0[i] + 32 * w) & hd->keys[i][w]) l = NAN;
       }
       tc_fence_after();
       P::template store<OCOLS>(p, it, s, row, half * OCOLS, mref, l, tO);

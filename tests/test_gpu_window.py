@@ -123,7 +123,7 @@ def test_prompt_sequence_outside_the_rows():
 
 @pytest.mark.parametrize("window,sinks,bad", [(40, 0, 0), (40, 4, 2), (40, 4, 5), (130, 0, 200), (130, 0, 299), (128, 130, 129),
                                               (128, 130, 131), (300, 0, 128)])
-@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("value", [np.nan, np.inf, 3e38])
 def test_prompt_hidden_values_stay_hidden(window, sinks, bad, value):
     lens = [300, 300]
     q, k, v = prompt_inputs(3, 600, 4, 2, 64, 64)
@@ -135,7 +135,8 @@ def test_prompt_hidden_values_stay_hidden(window, sinks, bad, value):
         got = prompt(q, kk, vv, lens, window, sinks)
         close(got[300:], want[300:], weight[300:])
         close(got[:300][~sees], want[:300][~sees], weight[:300][~sees])
-        assert not np.isfinite(got[:300][sees][:, :2, 7]).any()
+        if not np.isfinite(value) or kk is not k:
+            assert not np.isfinite(got[:300][sees][:, :2, 7]).any()
         if kk is k:  # the other kv head's query heads
             close(got[:300, 2:], want[:300, 2:], weight[:300, 2:])
 
@@ -170,9 +171,9 @@ def test_prompt_matches_causal_kernel_without_a_window():
 
 
 class Cache:
-    """A paged cache whose unused blocks and block rests are NaN, with tables of shuffled blocks."""
+    """A paged cache whose unused blocks and block rests are `rest`, with tables of shuffled blocks."""
 
-    def __init__(self, seed, lens, nkv, d, bs, window=None, sinks=0, spare=3, width=None):
+    def __init__(self, seed, lens, nkv, d, bs, window=None, sinks=0, spare=3, width=None, rest=np.nan):
         rng = self.rng = np.random.default_rng(seed)
         self.nkv, self.d, self.bs, self.lens = nkv, d, bs, lens
         self.width = width or max(1, -(-max([*lens, 1]) // bs))
@@ -185,7 +186,7 @@ class Cache:
             self.tables[i, cols] = order[at:at + len(cols)]
             at += len(cols)
         shape = (self.blocks, nkv, bs, d)
-        self.k, self.v = np.full(shape, np.nan, np.float32), np.full(shape, np.nan, np.float32)
+        self.k, self.v = np.full(shape, rest, np.float32), np.full(shape, rest, np.float32)
         for i, n in enumerate(lens):
             self.fill(self.tables[i], [j for j in range(n) if window is None or j >= n - window or j < sinks])
         self.order = order[at:]
@@ -223,8 +224,8 @@ def queries(seed, B, nq, d, pad=0):
     return x.reshape(B, nq, d), dev
 
 
-def check_token(lens, nq, nkv, d, bs, window, sinks, longest=None, seed=0):
-    c = Cache(seed + len(lens), lens, nkv, d, bs, window, sinks)
+def check_token(lens, nq, nkv, d, bs, window, sinks, longest=None, seed=0, rest=np.nan):
+    c = Cache(seed + len(lens), lens, nkv, d, bs, window, sinks, rest=rest)
     q, qd = queries(seed, len(lens), nq, d, pad=8)
     got = G.host(token_call(qd, c.device(), c, nq, window, sinks, longest))
     assert (got[-1] == -5).all() and (got[:, nq * d:] == -5).all()
@@ -251,6 +252,14 @@ def test_token_heads(nq, nkv, d):
 def test_token_sharing_of_a_sequence(lens, window, longest):
     # one sequence in a cluster of eight CTAs, or in one when the longest is understated; many in one CTA each
     check_token(lens, 16, 8, 128, 128, window, 4, min(longest, -(-max(lens) // 128) * 128))
+
+
+@pytest.mark.parametrize("rest", [3e38, -3e38, np.inf])
+def test_rests_of_blocks_do_not_matter(rest):
+    check_token([1, 65, 300], 8, 2, 128, 64, 70, 3, rest=rest)
+    for bs in (64, 128):
+        check_shared([5, 0, 130], 777, 8, 2, 128, bs, rest=rest)
+        check_shared([5, 0, 130], 65, 8, 2, 64, bs, rest=rest)
 
 
 def test_token_bad_entries():
@@ -345,9 +354,9 @@ def shared_call(qd, dev, c, nq, prefix, plen, pmax, ws=None, out=None, longest=N
     return out
 
 
-def check_shared(lens, plen, nq, nkv, d, bs, pmax=None, seed=0):
+def check_shared(lens, plen, nq, nkv, d, bs, pmax=None, seed=0, rest=np.nan):
     pmax = plen if pmax is None else pmax
-    c = Cache(seed + plen, lens, nkv, d, bs, spare=-(-pmax // bs) + 2)
+    c = Cache(seed + plen, lens, nkv, d, bs, spare=-(-pmax // bs) + 2, rest=rest)
     prefix = c.order[:-(-pmax // bs)]
     c.fill_fast(prefix, plen)
     q, qd = queries(seed, len(lens), nq, d, pad=8)
