@@ -108,6 +108,15 @@ B200_DEV float cluster_load_f(uint32_t addr, int rank) {
   return v;
 }
 
+B200_DEV float4 cluster_load_f4(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_map(addr, (uint32_t)rank))
+               : "memory");
+  return v;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                 const __grid_constant__ CUtensorMap tmV,
@@ -322,6 +331,7 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
     }
   }
   __syncthreads();
+  const bool alone = ctas == 1 && !p.prefix.parts;
   for (int i = threadIdx.x; i < rows * HD; i += kThreads) {
     const int row = i / HD;
     float M = -INFINITY;
@@ -335,37 +345,69 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
       L += f * sl[w * 16 + row];
       acc += f * warp_o[(w * kRows + row) * HD + i % HD];
     }
+    if (alone) {  // this CTA's part is all there is
+      p.out[(int64_t)b * p.out_stride + (int64_t)head0 * HD + i] = f2bf(L == 0.f ? 0.f : acc / L);
+      continue;
+    }
     part_o[i] = acc;
     if (i % HD == 0) {
       part_m[row] = M;
       part_l[row] = L;
     }
   }
+  if (alone) return;
   if (ctas > 1) cluster_sync();
   else __syncthreads();
 
-  // ---- the parts of the cluster, and the prefix's, joined: a share of the outputs each ----
+  // ---- the parts of the cluster, and the prefix's, joined ----
+  // The weights of a row's parts, 2^(m_i - M) over the weighted sum, a row a warp;
+  // then a share of the outputs each, four at a time.  (A prefix's parts are
+  // divided by their sums already: the weight of their log sum is all they need.)
   if (p.prefix.parts) pdl_wait();
   const PrefixSpan span = p.prefix.parts ? prefix_span(p.prefix, b, kh, p.nkv, ht * kRows, HD) : PrefixSpan{};
   const uint32_t am = smem_u32(part_m), al = smem_u32(part_l), ao = smem_u32(part_o);
-  for (int i = rank * kThreads + threadIdx.x; i < rows * HD; i += ctas * kThreads) {
-    const int row = i / HD, d = i % HD;
+  const int parts = ctas + span.count;
+  float* weight = warp_o;  // [rows][parts]: the warps' outputs are joined
+  for (int row = warp; row < rows; row += kThreads / 32) {
     float M = -INFINITY;
-    for (int r = 0; r < ctas; ++r) M = fmaxf(M, cluster_load_f(am + 4 * row, r));
-    for (int k = 0; k < span.count; ++k) M = fmaxf(M, span.lse(k, row));
+    for (int i = lane; i < parts; i += 32)
+      M = fmaxf(M, i < ctas ? cluster_load_f(am + 4 * row, i) : span.lse[(i - ctas) * 256 + row]);
+    M = warp_max(M);
     const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc = 0.f;
-    for (int r = 0; r < ctas; ++r) {
-      const float f = exp2f(cluster_load_f(am + 4 * row, r) - ref);
-      L += f * cluster_load_f(al + 4 * row, r);
-      acc += f * cluster_load_f(ao + 4 * i, r);
+    float L = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+      const float f = exp2f((i < ctas ? cluster_load_f(am + 4 * row, i) : span.lse[(i - ctas) * 256 + row]) - ref);
+      weight[row * parts + i] = f;
+      L += i < ctas ? f * cluster_load_f(al + 4 * row, i) : f;
     }
-    for (int k = 0; k < span.count; ++k) {  // normalised outputs, their weight is the sum
-      const float f = exp2f(span.lse(k, row) - ref);
-      L += f;
-      acc += f * span.out(k, row, HD, d);
+    L = warp_sum(L);
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing visible: zeros
+    for (int i = lane; i < parts; i += 32) weight[row * parts + i] *= inv;
+  }
+  __syncthreads();
+  for (int v = rank * kThreads + threadIdx.x; v < rows * HD / 4; v += ctas * kThreads) {
+    const int row = v / (HD / 4);
+    const float* w = weight + row * parts;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, const float4& o) {
+      acc.x = fmaf(f, o.x, acc.x);
+      acc.y = fmaf(f, o.y, acc.y);
+      acc.z = fmaf(f, o.z, acc.z);
+      acc.w = fmaf(f, o.w, acc.w);
+    };
+    for (int r = 0; r < ctas; ++r) add(w[r], cluster_load_f4(ao + 16 * v, r));
+    const float4* po = reinterpret_cast<const float4*>(span.parts) + v;
+#pragma unroll 8
+    for (int k = 0; k < span.count; ++k) add(w[ctas + k], __ldcg(po + (int64_t)k * 64 * HD));
+    __nv_bfloat16* o = p.out + (int64_t)b * p.out_stride + (int64_t)head0 * HD + 4 * v;
+    const uint2 packed = make_uint2(pack2(acc.x, acc.y), pack2(acc.z, acc.w));
+    if ((reinterpret_cast<uintptr_t>(o) & 7u) == 0) {
+      *reinterpret_cast<uint2*>(o) = packed;
+    } else {
+      const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&packed);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = e[i];
     }
-    p.out[(int64_t)b * p.out_stride + (int64_t)(head0 + row) * HD + d] = f2bf(L == 0.f ? 0.f : acc / L);
   }
   if (p.prefix.parts) pdl_trigger();
   if (ctas > 1) cluster_sync();  // the parts stay until they are read

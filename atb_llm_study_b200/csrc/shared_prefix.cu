@@ -46,20 +46,20 @@ struct Prefix {
   struct Cursor {
     const Prefix& p;
     int length;
-    int64_t K, unit, end;
+    int K, unit, end;
     B200_DEV explicit Cursor(const Prefix& q) : p(q) {
       length = prefix_length(p.at);
       K = (length + kTile - 1) / kTile;
       const PrefixDeal deal(p.at, K * p.nkv * prefix_pairs(p.at));
-      const bool has = blockIdx.x < deal.W;
+      const bool has = K > 0 && (int)blockIdx.x < deal.W;
       unit = has ? deal.first_unit(blockIdx.x) : 0;
       end = has ? deal.first_unit(blockIdx.x + 1) : 0;
     }
     B200_DEV bool next(Item& it, unsigned*) {
       if (unit >= end) return false;
-      const int item = (int)(unit / K), pairs = prefix_pairs(p.at);
-      it.first = (int)(unit % K);
-      it.n = (int)min(end - unit, K - it.first);
+      const int item = unit / K, pairs = prefix_pairs(p.at);
+      it.first = unit - item * K;
+      it.n = min(end - unit, K - it.first);
       it.length = length;
       it.kvh = item / pairs;
       it.row_tile = item % pairs * 2;
@@ -133,7 +133,7 @@ struct Prefix {
 
 struct Plan {
   int per_tile, row_tiles, workers;
-  int64_t slots;
+  int64_t units, slots;
 };
 
 // SMs share the key tiles evenly, with no CTA left without one.  A part has two tiles of 128 rows.
@@ -141,8 +141,9 @@ Plan prefix_plan(int batch, int nq, int nkv, int max_prefix) {
   Plan p;
   p.per_tile = kTile / (nq / nkv);
   p.row_tiles = (batch + p.per_tile - 1) / p.per_tile;
-  const int64_t items = (int64_t)nkv * ((p.row_tiles + 1) / 2), units = items * ((max_prefix + (int64_t)kTile - 1) / kTile);
-  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(units, sm_count()));
+  const int64_t items = (int64_t)nkv * ((p.row_tiles + 1) / 2);
+  p.units = items * ((max_prefix + (int64_t)kTile - 1) / kTile);
+  p.workers = (int)std::max<int64_t>(1, std::min<int64_t>(p.units, sm_count()));
   p.slots = 2 * (p.workers + items);
   return p;
 }
@@ -188,6 +189,7 @@ extern "C" int b200_paged_decode_shared(const void* q, int64_t q_stride, const v
   PrefixParts at{};
   if (max_prefix > 0) {
     const Plan plan = prefix_plan(batch, nq, nkv, max_prefix);
+    if (plan.units > INT32_MAX) return B200_ERROR_UNSUPPORTED;
     if (!workspace || workspace_bytes < plan_bytes(plan, head_dim) || (reinterpret_cast<uintptr_t>(workspace) & 31u))
       return B200_ERROR_INVALID_PARAM;
     at.parts = static_cast<float*>(workspace);

@@ -5,8 +5,8 @@
 // Query rows are the batch's heads of one kv head: per_tile sequences of
 // `group` heads fill a 128-row tile.  An item is a kv head and two row tiles
 // (the last may be alone); its prefix has K = ceil(length / 128) key tiles.  The items' key tiles in a row,
-// U of them, are dealt to W = min(workers, U) CTAs in equal stretches, worker c
-// taking [c U / W, (c + 1) U / W), so each has a tile at least.  Each stretch of
+// U of them, are dealt to W = min(workers, U) CTAs in stretches of U / W or one
+// more (the first U mod W), so each has a tile at least.  Each stretch of
 // an item is a part; the part of worker c in item i lies in slots 2 (c + i) and
 // 2 (c + i) + 1, a row tile each: of two consecutive parts the later has a larger
 // worker or item.
@@ -29,24 +29,29 @@ B200_DEV int prefix_length(const PrefixParts& p) { return max(0, min(*p.length, 
 
 // The stretches of U units: how many, the first unit of stretch c, the stretch of unit u.
 struct PrefixDeal {
-  int64_t U, W;
-  B200_DEV PrefixDeal(const PrefixParts& p, int64_t units) : U(units), W(min((int64_t)p.workers, units)) {}
-  B200_DEV int64_t first_unit(int64_t c) const { return c * U / W; }
-  B200_DEV int worker(int64_t u) const { return (int)(((u + 1) * W - 1) / U); }
+  int W, each, longer;  // the first `longer` stretches have each + 1 units
+  B200_DEV PrefixDeal(const PrefixParts& p, int units) {
+    W = max(1, min(p.workers, units));
+    each = units / W;
+    longer = units - each * W;
+  }
+  B200_DEV int first_unit(int c) const { return c * each + min(c, longer); }
+  B200_DEV int worker(int u) const {
+    const int cut = longer * (each + 1);
+    return u < cut ? u / (each + 1) : longer + (u - cut) / each;
+  }
 };
 
-// The parts of one sequence's heads [first_head, ..) of a kv head.
+// The parts of one sequence's heads [first_head, ..) of a kv head; a part's next is 256 rows on.
 struct PrefixSpan {
   const float* parts = nullptr;
-  const float* lse_at = nullptr;
+  const float* lse = nullptr;
   int count = 0;
-  B200_DEV float lse(int k, int row) const { return lse_at[k * 256 + row]; }
-  B200_DEV float out(int k, int row, int head_dim, int d) const { return parts[(k * 256 + row) * head_dim + d]; }
 };
 
 B200_DEV PrefixSpan prefix_span(const PrefixParts& p, int sequence, int kv_head, int nkv, int first_head, int head_dim) {
   PrefixSpan s;
-  const int64_t K = (prefix_length(p) + 127) / 128;
+  const int K = (prefix_length(p) + 127) / 128;
   if (K == 0) return s;
   const int tile = sequence / p.per_tile, item = kv_head * prefix_pairs(p) + tile / 2;
   const PrefixDeal deal(p, K * nkv * prefix_pairs(p));
@@ -54,7 +59,7 @@ B200_DEV PrefixSpan prefix_span(const PrefixParts& p, int sequence, int kv_head,
   const int64_t row = (int64_t)(2 * (w0 + item) + tile % 2) * 128 + (sequence % p.per_tile) * p.group + first_head;
   s.count = w1 - w0 + 1;
   s.parts = p.parts + row * head_dim;
-  s.lse_at = p.lse + row;
+  s.lse = p.lse + row;
   return s;
 }
 

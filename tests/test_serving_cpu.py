@@ -94,16 +94,17 @@ def test_nothing_to_do():
 @pytest.mark.parametrize("workers", [1, 2, 7, 148])
 @pytest.mark.parametrize("items,K", [(1, 1), (1, 300), (3, 1), (16, 9), (64, 128), (5, 77), (200, 2)])
 def test_stretches_cover_every_item_once(workers, items, K):
-    """shared_prefix.h: of W = min(workers, U), worker c takes units [c U / W, (c + 1) U / W), unit u is worker
-    ((u + 1) W - 1) / U's, and every worker from an item's first to its last has a part, in a slot of its own."""
+    """shared_prefix.h: W = min(workers, U) stretches of U / W units or, the first U mod W, one more; the formulas for a
+    stretch's first unit and a unit's stretch agree, and every stretch from an item's first to its last has a part of it, in a
+    slot of its own."""
     U = items * K
     W = min(workers, U)
-    owner = [0] * U
-    for c in range(W):
-        assert c * U // W < (c + 1) * U // W
-        for u in range(c * U // W, (c + 1) * U // W):
-            owner[u] = c
-    assert owner == [((u + 1) * W - 1) // U for u in range(U)]
+    each, longer = divmod(U, W)
+    first = [c * each + min(c, longer) for c in range(W + 1)]
+    assert first[0] == 0 and first[W] == U and all(a < b for a, b in zip(first, first[1:]))
+    owner = [c for c in range(W) for _ in range(first[c], first[c + 1])]
+    cut = longer * (each + 1)
+    assert owner == [u // (each + 1) if u < cut else longer + (u - cut) // each for u in range(U)]
     slots = set()
     for i in range(items):
         parts = sorted(set(owner[i * K:(i + 1) * K]))
