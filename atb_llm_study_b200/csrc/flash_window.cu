@@ -122,21 +122,20 @@ struct Window {
       for (int x = 0; x < Cf::BOXES_V; ++x)
         tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.kvh * p.vhs) + 64 * x, it.start + key0(it, j));
   }
-  // O / l from TMEM as bf16 rows, COLS columns from col on
-  template <int COLS>
-  B200_DEV static void store(const Window& p, const Item& it, int s, int row, int col, float, float l, uint32_t tO) {
+  // O / l from TMEM as bf16 rows
+  B200_DEV static void store(const Window& p, const Item& it, int s, int row, float, float l, uint32_t tO) {
     const float inv = 1.f / l;  // every row sees itself
     const bool valid = it.at(s) + row < it.rows;
-    __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.at(s) + row : 0)) * p.os + (int64_t)it.head_of(s) * p.ohs + col;
+    __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.at(s) + row : 0)) * p.os + (int64_t)it.head_of(s) * p.ohs;
 #pragma unroll 1
-    for (int c = 0; c < COLS / 32; ++c) {
+    for (int c = 0; c < HDV / 32; ++c) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tO + c * 32, r);
       tmem_ld_wait();
       if (valid) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (HEADS3D && col + c * 32 + k * 8 >= p.out_cols) break;
+          if (HEADS3D && c * 32 + k * 8 >= p.out_cols) break;
           float f[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[8 * k + i]) * inv;

@@ -106,15 +106,14 @@ struct Prefix {
                               uint64_t* bar, unsigned* err) {
     load(p, it, j, dst, map, bar, err);
   }
-  template <int COLS>
-  B200_DEV static void store(const Prefix& p, const Item& it, int s, int row, int col, float m, float l, uint32_t tO) {
+  B200_DEV static void store(const Prefix& p, const Item& it, int s, int row, float m, float l, uint32_t tO) {
     const int seqs = min(p.at.per_tile, p.batch - (it.row_tile + s) * p.at.per_tile);
     const bool valid = row < seqs * p.at.group;
     const float inv = 1.f / l;  // every row sees the stretch's keys
-    float* o = p.at.parts + ((int64_t)(it.slot + s) * kTile + row) * HD + col;
-    if (valid && col == 0) p.at.lse[(int64_t)(it.slot + s) * kTile + row] = m + log2f(l);
+    float* o = p.at.parts + ((int64_t)(it.slot + s) * kTile + row) * HD;
+    if (valid) p.at.lse[(int64_t)(it.slot + s) * kTile + row] = m + log2f(l);
 #pragma unroll 1
-    for (int c = 0; c < COLS / 32; ++c) {
+    for (int c = 0; c < HD / 32; ++c) {
       uint32_t r[32];
       tmem_ld_32x32b_x32(tO + c * 32, r);
       tmem_ld_wait();

@@ -6,15 +6,14 @@
 // An item is one or two tiles of 128 query rows ("sides") that walk one list of
 // 128-key tiles; a persistent CTA per SM walks its items.  Its warps:
 //   0       TMA: each item's Q tiles, then K and V tiles through rings
-//   1, last  each issues the MMAs of a side.  Per key tile: O += P V of
+//   1, 11   each issues the MMAs of a side.  Per key tile: O += P V of
 //           the tile whose P is ready, right behind it S = Q K^T of the next tile
 //           (the next item's first at an item's end).  Both sides use a K / V tile
 //           while it is in shared memory.
 //   2       looks through V tiles for NaN and infinities (below)
-//   3-18    softmax, eight warps a side, two threads a row (192-wide heads, whose
-//           tiles fill shared memory: four warps, one thread): scores from TMEM,
-//           masked, maximum, exponentials, sum, P as bf16 pairs over the scores,
-//           where the MMA reads it.
+//   3-10    softmax, four warps a side, a thread a row: scores from TMEM, masked,
+//           maximum, exponentials, sum, P as bf16 pairs over the scores, where the
+//           MMA reads it.
 // What a side's chain has to wait for itself (scores, softmax, P V) the other
 // side's fills: the tensor core works for one while the softmax units work for
 // the other.  At 128-wide heads a side's tile takes 1024 cycles of MMAs and as
@@ -28,19 +27,19 @@
 // exact arithmetic and keeps P below 2^8 of its usual scale.
 //
 // Values that nobody sees must not reach anybody: P is 0 there, but 0 x NaN is
-// not.  So warp 2 looks through the value rows of every tile that a side does
-// not see as a whole (a prompt's end, its diagonal, the ends of the window and
-// the sinks, a cache block's rest) and zeroes those with a NaN or an infinity.
+// not.  So the value rows of every tile that a side does not see as a whole (a
+// prompt's end, its diagonal, the ends of the window and the sinks, a cache
+// block's rest) are looked through, and those with a NaN or an infinity zeroed.
 // A row that does see such a key gets NaN: the item's list of zeroed keys is
-// looked through when its rows are stored.  The search is 64 loads a tile,
-// while its scores are computed.
+// looked through when its rows are stored.  (One warp takes 2000 cycles a tile,
+// as long as V arrives ahead of its use; four were no faster in all.)
 //
 // P provides: HDK, HDV; Item with int n (key tiles, > 0), bool both (side 1 is
 // there); Cursor(p) with bool next(Item&, err); load_q(p, item, side, ..) and
 // load_k / load_v(p, item, tile, smem, map, bar, err): arrive on bar expecting
 // bytes, copy; int key0(item, tile): its first key; bool whole(item, side, key):
 // every row of the side sees the 128 keys from key on; visible(item, side, row,
-// key): bits of the 32 from key on that a row sees; store<COLS>(p, item, side, row, first column, m, l, tO).
+// key): bits of the 32 from key on that a row sees; store(p, item, side, row, m, l, tO).
 #pragma once
 
 #include "tc_attention.cuh"
@@ -48,60 +47,64 @@
 namespace {
 
 constexpr int kSides = 2;
+constexpr int kItemThreads = 384, kMma1Warp = 11;  // the second side's issuer
 constexpr uint32_t kSideS = 0, kSideO = 256;  // TMEM columns of side 0's scores and outputs; side 1's lie 128 further
 constexpr int kMaxEdgeTiles = 6;
 
 struct Hidden {  // zeroed value rows of one item's edge tiles
-  int count;
+  int any, count;
   int key0[kMaxEdgeTiles];
   uint32_t keys[kMaxEdgeTiles][4];
 };
-constexpr int kHiddenRing = 8;
 
-// Zeroes the rows of a V tile [128 keys] that hold a NaN or an infinity; their bits in `bad` (of lane 0).  One warp.
+// sum += 0 x v, two bf16 values at once
+B200_DEV void add_times_0(uint32_t& sum, uint32_t v) {
+  asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(v), "r"(0u));
+}
+
+// Zeroes those of the 32 rows of a V tile from sV on that hold a NaN or an infinity; their bits.  One warp.
 template <int BOXES>
-B200_DEV bool clear_nonfinite(uint8_t* sV, uint32_t bad[4]) {
+B200_DEV uint32_t clear_nonfinite(uint8_t* sV) {
   const int lane = threadIdx.x & 31;
-  // exponent bits all ones: 0x7f80 + 0x80 carries into bit 15 of its half
-  auto odd = [](const uint4& v) {
-    return ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) |
-           ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
-  };
-  // first whether there is any: 512 bytes an instruction, sixteen on their way
-  uint32_t seen = 0;
-#pragma unroll 1
-  for (int i = 0; i < BOXES * kBoxBytes / 512; i += 16) {
-    uint4 v[16];
+  // an instruction covers 4 rows, 8 lanes of 16 bytes a row (a row is 128 contiguous bytes of each box, whatever the
+  // swizzle)
+  uint4 v[BOXES * 8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = *reinterpret_cast<const uint4*>(sV + (i + k) * 512 + lane * 16);
+  for (int i = 0; i < BOXES * 8; ++i)
+    v[i] = *reinterpret_cast<const uint4*>(sV + (i >> 3) * kBoxBytes + (i & 7) * 512 + lane * 16);
+  // the sum of all values times 0 is 0 without one, and NaN with one
+  uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < 16; ++k) seen |= odd(v[k]);
+  for (int i = 0; i < BOXES * 8; ++i) {
+    add_times_0(sum[0], v[i].x);
+    add_times_0(sum[1], v[i].y);
+    add_times_0(sum[2], v[i].z);
+    add_times_0(sum[3], v[i].w);
   }
-  const bool any = __any_sync(0xffffffffu, (seen & 0x80008000u) != 0);
-  // then which rows: an instruction covers 4, 8 lanes of 16 bytes a row (a row is 128 contiguous bytes of each box,
-  // whatever the swizzle)
+  if (!__any_sync(0xffffffffu, ((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0)) return 0;
+  uint32_t found = 0;
 #pragma unroll 1
-  for (int w = 0; any && w < 4; ++w) {
-    uint32_t found = 0;
-#pragma unroll 1
-    for (int i = 0; i < BOXES * 8; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4*>(sV + (i >> 3) * kBoxBytes + (w * 32 + (i & 7) * 4) * 128 + lane * 16);
-      const uint32_t lanes = __ballot_sync(0xffffffffu, (odd(v) & 0x80008000u) != 0);
+  for (int i = 0; i < BOXES * 8; ++i) {
+    const uint4 u = *reinterpret_cast<const uint4*>(sV + (i >> 3) * kBoxBytes + (i & 7) * 512 + lane * 16);
+    uint32_t s = 0;
+    add_times_0(s, u.x);
+    add_times_0(s, u.y);
+    add_times_0(s, u.z);
+    add_times_0(s, u.w);
+    const uint32_t lanes = __ballot_sync(0xffffffffu, (s & 0x7fff7fffu) != 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (lanes & (0xffu << (8 * r))) found |= 1u << ((i & 7) * 4 + r);
-    }
-    if (lane == 0) bad[w] = found;
-#pragma unroll 1
-    for (uint32_t left = found; left; left &= left - 1) {
-      const int r = w * 32 + __ffs(left) - 1;
-      for (int c = lane; c < BOXES * 8; c += 32)
-        *reinterpret_cast<uint4*>(sV + (c >> 3) * kBoxBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-    }
+    for (int r = 0; r < 4; ++r)
+      if (lanes & (0xffu << (8 * r))) found |= 1u << ((i & 7) * 4 + r);
   }
-  if (any) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads the tile
+#pragma unroll 1
+  for (uint32_t left = found; left; left &= left - 1) {
+    const int r = __ffs(left) - 1;
+    for (int c = lane; c < BOXES * 8; c += 32)
+      *reinterpret_cast<uint4*>(sV + (c >> 3) * kBoxBytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor core reads the tile
   __syncwarp();
-  return any;
+  return found;
 }
 
 // Bits [a, b) of 32.
@@ -207,23 +210,19 @@ struct ItemsCfg {
   static constexpr int V_STAGES = P::HDK > 128 ? 1 : P::HDK > 64 ? 2 : 4;
   static constexpr int K_AT = kSides * TILE_QK, V_AT = K_AT + K_STAGES * TILE_QK, BARS_AT = V_AT + V_STAGES * TILE_V;
   static constexpr int HIDDEN_AT = BARS_AT + 320;
-  // threads a row: two where shared memory has room for what they tell each other
-  static constexpr int HALVES = 1;
-  static constexpr int EXCHANGE_AT = HIDDEN_AT + kHiddenRing * (int)sizeof(Hidden);
-  static constexpr int SMEM = EXCHANGE_AT + (HALVES - 1) * kSides * 3 * 2 * 128 * 4 + 1024;
-  static constexpr int THREADS = 128 + kSides * HALVES * 128;
-  static constexpr int MMA1_WARP = 3 + kSides * HALVES * 4;  // the second side's issuer
+  static constexpr int RING = 4 * V_STAGES;  // of the items' records
+  static constexpr int SMEM = HIDDEN_AT + RING * (int)sizeof(Hidden) + 1024;
   static constexpr uint32_t IDESC_O = idesc_bf16_f32(128, P::HDV) | (1u << 16);  // B operand (V) MN-major
 };
 
 template <class P>
-__global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
+__global__ void __launch_bounds__(kItemThreads, 1)
     tc_items_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const P p, unsigned* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using Cf = ItemsCfg<P>;
-  constexpr int HDK = P::HDK, HDV = P::HDV, KS = Cf::K_STAGES, VS = Cf::V_STAGES, HALVES = Cf::HALVES;
+  constexpr int HDK = P::HDK, HDV = P::HDV, KS = Cf::K_STAGES, VS = Cf::V_STAGES;
   uint8_t* sK = smem + Cf::K_AT;
   uint8_t* sV = smem + Cf::V_AT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BARS_AT);
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
   static_assert((16 + 2 * KS + 3 * VS) * 8 + 8 <= 320, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + VS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  Hidden* hidden = reinterpret_cast<Hidden*>(smem + Cf::HIDDEN_AT);  // [item % kHiddenRing]
+  Hidden* hidden = reinterpret_cast<Hidden*>(smem + Cf::HIDDEN_AT);  // [item % Cf::RING]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // one value a warp
   if (threadIdx.x == 0) {
@@ -251,9 +250,9 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128 * HALVES);
+      mbar_init(&p_full[s], 128);
       mbar_init(&pv_done[s], 2);
-      mbar_init(&o_free[s], 128 * HALVES);
+      mbar_init(&o_free[s], 128);
       mbar_init(&drain[s], 1);
       mbar_init(&turn[s], 1);
     }
@@ -267,6 +266,7 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
       mbar_init(&v_empty[i], 2);
     }
     *abort_flag = 0;
+    for (int i = 0; i < Cf::RING; ++i) hidden[i].any = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
       if (!ok) *abort_flag = 1;
     }
     __syncwarp();
-  } else if (warp == 1 || warp == Cf::MMA1_WARP) {
+  } else if (warp == 1 || warp == kMma1Warp) {
     // ---------------- MMAs of a side ----------------
     // The sides take turns, a batch (P V, next scores) each: issued side by side,
     // both batches end together, and so both softmaxes begin together and leave
@@ -388,8 +388,7 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
           const uint64_t vd = smem_desc_mn128(smem_u32(sV + vs * Cf::TILE_V), kBoxBytes);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_bf16_ts_elect(tO, tS + (HALVES == 2 ? (k >> 2) * 64 + (k & 3) * 8 : k * 8),
-                               vd + (uint64_t)(k * 2048 >> 4), Cf::IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
+            umma_bf16_ts_elect(tO, tS + k * 8, vd + (uint64_t)(k * 2048 >> 4), Cf::IDESC_O, (j > 0 || k > 0) ? 1u : 0u);
           umma_commit_elect(&pv_done[s]);
         }
         if (next && next_mine) scores(T + 1, last ? after.n == 1 : j + 2 == it.n);
@@ -416,12 +415,14 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
     // ---------------- values looked through ----------------
     bool ok = true;
     int g = 0, n = 0;
+#pragma unroll 1
     for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
       // Free again: V of item n was loaded after the P V of item n - VS or a later one began, and before an item's P V
-      // begins all earlier items have been stored.  VS + 1 < kHiddenRing.
-      Hidden* hd = &hidden[n % kHiddenRing];
+      // begins all earlier items have been stored.  So records are cleared half a ring ahead.
+      Hidden* hd = &hidden[n % Cf::RING];
+      static_assert(VS + 1 <= Cf::RING / 2, "ring of records");
+      if (lane == 0) hidden[(n + Cf::RING / 2) % Cf::RING].any = 0;
       int edges = 0;
-      if (lane == 0) hd->count = 0;
 #pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++g) {
         const int vs = g % VS;
@@ -430,13 +431,19 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
         const int key = P::key0(it, j);
         if (!P::whole(it, 0, key) || (it.both && !P::whole(it, 1, key))) {
           const int at = min(edges, kMaxEdgeTiles - 1);  // an item has four at most
-          if (clear_nonfinite<Cf::BOXES_V>(sV + vs * Cf::TILE_V, hd->keys[at])) {
-            ++edges;
-            if (lane == 0) {
-              hd->key0[at] = key;
-              hd->count = at + 1;
-            }
+          uint32_t any = 0;
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t bad = clear_nonfinite<Cf::BOXES_V>(sV + vs * Cf::TILE_V + w * 32 * 128);
+            if (lane == 0) hd->keys[at][w] = bad;
+            any |= bad;
           }
+          if (lane == 0) {
+            hd->key0[at] = key;
+            hd->count = at + 1;
+            if (any) hd->any = 1;
+          }
+          ++edges;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_ready[vs]);
@@ -445,64 +452,37 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
     if (!ok) *abort_flag = 1;
   } else {
     // ---------------- softmax ----------------
-    // Thread (side, half, row) takes 128 / HALVES of its row's scores.  Two of a row
-    // tell each other their maxima, a tile each, so both move the running maximum
-    // alike; their sums meet at the item's end.
-    constexpr int COLS = 128 / HALVES, OCOLS = HDV / HALVES;
-    const int s = (warp - 3) / (4 * HALVES), half = (warp - 3) / 4 % HALVES;
+    // A thread a row, so no row's state leaves its thread.  (Two threads a row, eight
+    // warps a side, took 310 us where this takes 281 at 8 x 2048: their exchange of
+    // maxima and the twice as many waits cost more than the shorter rows gain.)
+    const int s = (warp - 3) >> 2;           // side
     const int row = (warp & 3) * 32 + lane;  // TMEM lanes that this warp may access: 32 (warp % 4) ..
-    const int pair_bar = 1 + s * 4 + (warp & 3);
-    float* ex = reinterpret_cast<float*>(smem + Cf::EXCHANGE_AT) + s * 3 * 2 * 128;  // [2 tiles' maxima, sums][half][row]
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + kSideS + s * 128 + half * COLS, tO = tmem + lanes + kSideO + s * 128 + half * OCOLS;
+    const uint32_t tS = tmem + lanes + kSideS + s * 128, tO = tmem + lanes + kSideO + s * 128;
     const float scale_log2 = p.scale_log2;
     bool ok = true;
     int t = 0, n = 0;  // tiles of this side, and items, so far
-    // the outcome of a wait, the same for the threads that meet at barriers and for TMEM's warp-wide accesses
-    auto agreed = [&](bool mine) {
-      mine = __all_sync(0xffffffffu, mine);
-      return HALVES == 1 ? mine : !pair_or(pair_bar, !mine);
-    };
 #pragma unroll 1
     for (; ok && cursor.next(it, err); ++n) {
       if (s == 1 && !it.both) continue;
       float mref = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++t) {
-        ok = agreed(!*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
+        // warp-uniform: TMEM's accesses are
+        ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&s_full[s], t & 1, err));
         if (!ok) break;
         tc_fence_after();
         const int key = P::key0(it, j);
-        // Hidden scores become -inf where they lie.  (Branches around unseen columns in
-        // the passes below cost every tile a fifth of its softmax.)
-        if (!P::whole(it, s, key)) {
-#pragma unroll 1
-          for (int c = 0; c < COLS / 32; ++c) {
-            const uint32_t mask = P::visible(it, s, row, key + half * COLS + c * 32);
-            if (__all_sync(0xffffffffu, mask == 0xffffffffu)) continue;
-            uint32_t r[32];
-            if (!__all_sync(0xffffffffu, mask == 0)) {
-              tmem_ld_32x32b_x32(tS + c * 32, r);
-              tmem_ld_wait();
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((mask >> i) & 1u)) r[i] = __float_as_uint(-INFINITY);
-            tmem_st_32x32b_x32(tS + c * 32, r);
-          }
-          tmem_st_wait();
-        }
+        const bool edge = !P::whole(it, s, key);
         uint32_t ra[32], rb[32];
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld_32x32b_x32(tS, ra);
-        if (HALVES == 2) {
-          tmem_ld_32x32b_x32(tS + 32, rb);
-          tmem_ld_wait();
-          row_max(ra, m4);
-          row_max(rb, m4);
-        } else {
-          // the scores are read from TMEM twice, 32 columns at a time with the next 32 on their way: once for the
-          // maximum, once for the exponentials
+        // The scores are read from TMEM twice, 32 columns at a time with the next 32 on
+        // their way: once for the maximum, once for the exponentials.  Held from the
+        // one to the other, they would make the code of a tile several times longer
+        // than the instruction cache likes.
+        uint32_t unseen = 0;  // edge tiles: bit c: no row of this warp sees columns 32 c ..
+        if (!edge) {
+          tmem_ld_32x32b_x32(tS, ra);
 #pragma unroll 1
           for (int c = 0; c < 4; c += 2) {
             tmem_ld_wait();
@@ -512,13 +492,28 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
             tmem_ld_32x32b_x32(tS + ((c + 2) & 3) * 32, ra);  // at the end the first again
             row_max(rb, m4);
           }
+        } else {
+          // hidden scores become -inf where they lie; columns that the warp does not see are left out
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t mask = P::visible(it, s, row, key + c * 32);
+            if (__all_sync(0xffffffffu, mask == 0)) {
+              unseen |= 1u << c;
+              continue;
+            }
+            tmem_ld_32x32b_x32(tS + c * 32, ra);
+            tmem_ld_wait();
+            if (!__all_sync(0xffffffffu, mask == 0xffffffffu)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((mask >> i) & 1u)) ra[i] = __float_as_uint(-INFINITY);
+              tmem_st_32x32b_x32(tS + c * 32, ra);
+            }
+            row_max(ra, m4);
+          }
+          tmem_st_wait();
         }
         float mx = fmax3_nan(fmax3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY);
-        if (HALVES == 2) {  // (places alternate: the other half is at most a tile behind)
-          ex[((t & 1) * 2 + half) * 128 + row] = mx;
-          named_bar_sync(pair_bar, 64);
-          mx = fmax3_nan(mx, ex[((t & 1) * 2 + (half ^ 1)) * 128 + row], -INFINITY);
-        }
         if (mx != mx) l = NAN;  // a visible score is: so is the row
         mx *= scale_log2;       // scale > 0
         float alpha = 1.f;
@@ -530,12 +525,7 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
         const float ref = mref == -INFINITY ? 0.f : mref;
         uint64_t sums[2] = {0, 0};
         // P of 32 scores takes 16 columns, over scores that have been read
-        if (HALVES == 2) {
-          row_exp(ra, scale_log2, ref, sums);
-          tmem_st_32x32b_x16(tS, ra);
-          row_exp(rb, scale_log2, ref, sums);
-          tmem_st_32x32b_x16(tS + 16, rb);
-        } else {
+        if (!edge) {
 #pragma unroll 1
           for (int c = 0; c < 4; c += 2) {
             tmem_ld_wait();
@@ -547,18 +537,30 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
             row_exp(rb, scale_log2, ref, sums);
             tmem_st_32x32b_x16(tS + c * 16 + 16, rb);
           }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            if ((unseen >> c) & 1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) ra[i] = 0;
+            } else {
+              tmem_ld_32x32b_x32(tS + c * 32, ra);
+              tmem_ld_wait();
+              row_exp(ra, scale_log2, ref, sums);
+            }
+            tmem_st_32x32b_x16(tS + c * 16, ra);
+          }
         }
         float l0, l1;
         unpair64(add2(sums[0], sums[1]), l0, l1);
         l += l0 + l1;
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // O holds the item's tiles before j once the last of them is done.  (A failed wait is acted on at the next
-          // agreement: no way out between two threads' barriers.)
-          const bool done = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
-          if (!done) *abort_flag = 1;
+          // O holds the item's tiles before j once the last of them is done
+          ok = __all_sync(0xffffffffu, mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+          if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < (done ? OCOLS / 32 : 0); ++c) {
+          for (int c = 0; c < HDV / 32; ++c) {
             tmem_ld_32x32b_x32(tO + c * 32, ra);
             tmem_ld_wait();
 #pragma unroll
@@ -571,22 +573,16 @@ __global__ void __launch_bounds__(ItemsCfg<P>::THREADS, 1)
         mbar_arrive(&p_full[s]);
       }
       if (!ok) break;
-      ok = agreed(!*abort_flag && mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
+      ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait_idle(&pv_done[s], (t - 1) & 1, err));
       if (!ok) break;
-      if (HALVES == 2) {  // rewritten an item later, after an agreement
-        ex[(4 + half) * 128 + row] = l;
-        named_bar_sync(pair_bar, 64);
-        l += ex[(4 + (half ^ 1)) * 128 + row];
-      }
-      const volatile Hidden* hd = &hidden[n % kHiddenRing];
+      const volatile Hidden* hd = &hidden[n % Cf::RING];
 #pragma unroll 1
-      for (int i = 0; i < hd->count; ++i) {  // zeroed keys that this row sees
+      for (int i = 0; i < (hd->any ? hd->count : 0); ++i)  // zeroed keys that this row sees
 #pragma unroll 1
         for (int w = 0; w < 4; ++w)
           if (P::visible(it, s, row, hd->key0[i] + 32 * w) & hd->keys[i][w]) l = NAN;
-      }
       tc_fence_after();
-      P::template store<OCOLS>(p, it, s, row, half * OCOLS, mref, l, tO);
+      P::store(p, it, s, row, mref, l, tO);
       tc_fence_before();
       mbar_arrive(&o_free[s]);
     }
@@ -615,7 +611,7 @@ int launch_items(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
       return B200_ERROR_UNSUPPORTED;
     done[dev] = true;
   }
-  launch_kernel(k, dim3((unsigned)grid), ItemsCfg<P>::THREADS, smem, st, mq, mk, mv, p, b200::error_word(dev));
+  launch_kernel(k, dim3((unsigned)grid), kItemThreads, smem, st, mq, mk, mv, p, b200::error_word(dev));
   B200_CHECK_LAUNCH();
   return B200_OK;
 }
