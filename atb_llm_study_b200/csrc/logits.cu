@@ -9,7 +9,8 @@
 // A row's logits are read and written once (4 bytes a token, 600 KB at 151936),
 // so memory bounds a batch in principle, and the few dependent steps between
 // lists and logits do in practice.  A row's vocabulary is split over the CTAs of
-// a cluster.  Each marks the tokens of its part that occur in the history or
+// a cluster in stripes of 1024 tokens, in turn (vocabularies are sorted by how
+// often their tokens occur, so a run of them would have most of the work).  Each marks the tokens of its part that occur in the history or
 // among the biases in a bitmap in shared memory (one bit a token), whose prefix
 // counts number the marked tokens; per marked token it keeps how often it was
 // said, whether the prompt has it and where its biases begin.  All of this is
@@ -36,13 +37,16 @@ namespace {
 constexpr int kThreads = 512;
 constexpr unsigned kMaxCtas = 16;  // of a row
 constexpr int kSlots = 4096;       // marked tokens computed at a time
+constexpr int kKeep = 8;           // history entries a thread keeps
+constexpr int kStripe = 1024;      // consecutive tokens of one CTA
+constexpr int kStripeBits = 10;
 constexpr uint32_t kTopBit = 1u << 31;  // of `said`: the prompt has it
 
 struct LogitsParams {
   const __nv_bfloat16* logits;
   int64_t ld;
   int64_t vocab;
-  int chunk;  // tokens a CTA, a multiple of 32
+  int chunk;  // tokens a CTA, a multiple of kStripe
   const int32_t* history;
   int64_t history_ld;
   const int32_t* prompt_lens;
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
   const int words = p.chunk / 32;
   uint32_t* marks = smem;                                     // [words]
   int* before = reinterpret_cast<int*>(marks + words);        // [words] marked tokens before each word
-  int* token = before + words;                                // [kSlots] a marked token, in its part
+  int* token = before + words;                                // [kSlots] a marked token
   uint32_t* said = reinterpret_cast<uint32_t*>(token + kSlots);  // [kSlots] times behind the prompt | kTopBit
   uint32_t* lead = said + kSlots;                             // [kSlots] entries from its first bias to the list's end
   uint32_t* listed = lead + kSlots;                           // [kSlots] its biases
@@ -139,21 +143,31 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
   const int ctas = (int)cluster_size(), rank = (int)cluster_rank();
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // every CTA has started: waited for at the end
   const int64_t row = blockIdx.x / ctas;
-  const int lo = rank * p.chunk;
-  const int n = max(0, min(p.chunk, (int)p.vocab - lo));
-  const int nv = p.vec ? n / 8 : 0;
+  const int turn = __ffs(ctas) - 1;  // ctas is a power of two
+  const int vocab = (int)p.vocab;
   const int tid = threadIdx.x;
+  // token of this CTA's `at`, and the other way (-1: not this CTA's)
+  auto token_of = [&](int at) { return ((((at >> kStripeBits) << turn) + rank) << kStripeBits) + (at & (kStripe - 1)); };
+  auto place_of = [&](int id) {
+    const int stripe = id >> kStripeBits;
+    return (uint32_t)id < (uint32_t)vocab && (stripe & (ctas - 1)) == rank
+               ? ((stripe >> turn) << kStripeBits) + (id & (kStripe - 1)) : -1;
+  };
+  const int nv = p.vec ? p.chunk / 8 : 0;  // groups of 8 tokens; some may lie behind the vocabulary
   if (kLists)
     for (int i = tid; i < words; i += kThreads) marks[i] = 0;
   pdl_wait();
 
-  const __nv_bfloat16* in = p.logits + row * p.ld + lo;
-  __nv_bfloat16* out = p.out ? p.out + row * p.ldo + lo : nullptr;
+  const __nv_bfloat16* in = p.logits + row * p.ld;
+  __nv_bfloat16* out = p.out ? p.out + row * p.ldo : nullptr;
   uint4 raw[kAhead];
   auto load = [&](int c0) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (c0 + k * kThreads < nv) raw[k] = reinterpret_cast<const uint4*>(in)[c0 + k * kThreads];
+      if (c0 + k * kThreads < nv) {
+        const int id = token_of((c0 + k * kThreads) * 8);
+        if (id + 8 <= vocab) raw[k] = *reinterpret_cast<const uint4*>(in + id);
+      }
   };
   load(tid);  // on their way while the lists are read
   const uint32_t* mask = nullptr;
@@ -162,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
     if (m >= p.num_masks || m < -1) {
       if (tid == 0) raise_error(p.err, DEV_ERR_BAD_INDEX);
     } else if (m >= 0) {
-      mask = p.mask + m * p.mask_ld + (lo >> 5);
+      mask = p.mask + m * p.mask_ld;
     }
   }
   Row r{};
@@ -188,19 +202,31 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
   }
 
   // ---- which tokens are touched ----
+  // The first entries of both lists stay in registers, all on their way at once.
+  int32_t said_id[kKeep], bias_id;
+  if (HIST)
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (tid + k * kThreads < r.len) said_id[k] = r.history[tid + k * kThreads];
+  if (BIAS && tid < r.biases) bias_id = r.bias_ids[tid];
   int marked = 0;
   if (kLists) {
     __syncthreads();
     auto mark = [&](int32_t id) {
-      const uint32_t at = (uint32_t)id - (uint32_t)lo;
-      if (at < (uint32_t)n) atomicOr(&marks[at >> 5], 1u << (at & 31));
-      else if ((uint32_t)id >= (uint32_t)p.vocab) raise_error(p.err, DEV_ERR_BAD_INDEX);
+      const int at = place_of(id);
+      if (at >= 0) atomicOr(&marks[at >> 5], 1u << (at & 31));
+      else if ((uint32_t)id >= (uint32_t)vocab) raise_error(p.err, DEV_ERR_BAD_INDEX);
     };
-    if (HIST)
-#pragma unroll 8
-      for (int i = tid; i < r.len; i += kThreads) mark(r.history[i]);
-    if (BIAS)
-      for (int i = tid; i < r.biases; i += kThreads) mark(r.bias_ids[i]);
+    if (HIST) {
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k)
+        if (tid + k * kThreads < r.len) mark(said_id[k]);
+      for (int i = tid + kKeep * kThreads; i < r.len; i += kThreads) mark(r.history[i]);
+    }
+    if (BIAS) {
+      if (tid < r.biases) mark(bias_id);
+      for (int i = tid + kThreads; i < r.biases; i += kThreads) mark(r.bias_ids[i]);
+    }
     __syncthreads();
     const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
     int mine = 0;
@@ -221,10 +247,12 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
     for (int k = 0; k < kAhead; ++k) {
       const int c = c0 + k * kThreads;
       if (c >= nv) break;
+      const int id = token_of(c * 8);
+      if (id + 8 > vocab) break;  // and all behind it
       uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
       uint32_t skip = kLists ? reinterpret_cast<const uint8_t*>(marks)[c] : 0;
       if (mask) {
-        const uint32_t hidden = ~(mask[c >> 2] >> ((c & 3) * 8)) & 0xffu;
+        const uint32_t hidden = ~(mask[id >> 5] >> (id & 31)) & 0xffu;
         if (hidden) {
           skip |= hidden;
 #pragma unroll
@@ -234,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
           }
         }
       }
-      if (out) reinterpret_cast<uint4*>(out)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (out) *reinterpret_cast<uint4*>(out + id) = make_uint4(w[0], w[1], w[2], w[3]);
       if (skip) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -248,23 +276,27 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
         plain_v = most;
 #pragma unroll
         for (int i = 7; i >= 0; --i)
-          if (__uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) == most) plain_i = c * 8 + i;
+          if (__uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) == most) plain_i = id + i;
       }
     }
   }
   // rows that 16-byte accesses do not fit, and the last few tokens of those that they do
-  for (int at = nv * 8 + tid; at < n; at += kThreads) {
-    __nv_bfloat16 v = in[at];
+  int rest = 0;
+  if (p.vec) rest = vocab % 8 != 0 && place_of(vocab & ~7) >= 0 ? place_of(vocab & ~7) : p.chunk;
+  for (int at = rest + tid; at < p.chunk; at += kThreads) {
+    const int id = token_of(at);
+    if (id >= vocab) break;
+    __nv_bfloat16 v = in[id];
     const float x = bf2f(v);
-    if (mask && !((mask[at >> 5] >> (at & 31)) & 1u)) {
+    if (mask && !((mask[id >> 5] >> (id & 31)) & 1u)) {
       v = __float2bfloat16_rn(-INFINITY);
     } else if (!(kLists && ((marks[at >> 5] >> (at & 31)) & 1u)) && x > plain_v) {
       plain_v = x;
-      plain_i = at;
+      plain_i = id;
     }
-    if (out) out[at] = v;
+    if (out) out[id] = v;
   }
-  Best best{(double)plain_v, plain_i < 0 ? INT64_MAX : lo + plain_i};
+  Best best{(double)plain_v, plain_i < 0 ? INT64_MAX : plain_i};
 
   // ---- the touched tokens, kSlots at a time ----
   if (kLists && marked > 0) {
@@ -279,37 +311,42 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
       __syncthreads();
       // the slot of a token of this part, or -1
       auto slot_of = [&](int32_t id) -> int {
-        const uint32_t at = (uint32_t)id - (uint32_t)lo;
-        if (at >= (uint32_t)n) return -1;
+        const int at = place_of(id);
+        if (at < 0) return -1;
         const int s = before[at >> 5] + __popc(marks[at >> 5] & ((1u << (at & 31)) - 1)) - s0;
         if (s < 0 || s >= slots) return -1;
-        token[s] = (int)at;
+        token[s] = id;
         return s;
       };
-      if (HIST)
-#pragma unroll 4
-        for (int i = tid; i < r.len; i += kThreads) {
-          const int s = slot_of(r.history[i]);
-          if (s < 0) continue;
-          if (i < r.prompt) atomicOr(&said[s], kTopBit);
-          else atomicAdd(&said[s], 1u);
-        }
+      auto say = [&](int i, int32_t id) {
+        const int s = slot_of(id);
+        if (s < 0) return;
+        if (i < r.prompt) atomicOr(&said[s], kTopBit);
+        else atomicAdd(&said[s], 1u);
+      };
+      // a token's first entry leads: it is worth the most counted from the end
+      auto list = [&](int i, int32_t id) {
+        const int s = slot_of(id);
+        if (s < 0) return;
+        atomicMax(&lead[s], (uint32_t)(r.biases - i));
+        atomicAdd(&listed[s], 1u);
+      };
+      if (HIST) {
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k)
+          if (tid + k * kThreads < r.len) say(tid + k * kThreads, said_id[k]);
+        for (int i = tid + kKeep * kThreads; i < r.len; i += kThreads) say(i, r.history[i]);
+      }
       if (BIAS) {
-        // a token's first entry leads: it is worth the most counted from the end
-        for (int i = tid; i < r.biases; i += kThreads) {
-          const int s = slot_of(r.bias_ids[i]);
-          if (s >= 0) {
-            atomicMax(&lead[s], (uint32_t)(r.biases - i));
-            atomicAdd(&listed[s], 1u);
-          }
-        }
+        if (tid < r.biases) list(tid, bias_id);
+        for (int i = tid + kThreads; i < r.biases; i += kThreads) list(i, r.bias_ids[i]);
       }
       __syncthreads();
       for (int base = tid & ~31; base < slots; base += kThreads) {
         const int s = base + (tid & 31);
-        const int at = s < slots ? token[s] : 0;
-        const bool mine = s < slots && !(mask && !((mask[at >> 5] >> (at & 31)) & 1u));
-        double v = mine ? (double)bf2f(in[at]) : 0;
+        const int id = s < slots ? token[s] : 0;
+        const bool mine = s < slots && !(mask && !((mask[id >> 5] >> (id & 31)) & 1u));
+        double v = mine ? (double)bf2f(in[id]) : 0;
         const uint32_t w = HIST && mine ? said[s] : 0, l = BIAS && mine ? lead[s] : 0;
         if (w) {
           if (rep) v = v > 0 ? __ddiv_rn(v, repetition) : __dmul_rn(v, repetition);
@@ -324,10 +361,10 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
           uint32_t many = __ballot_sync(0xffffffffu, l && listed[s] > 1);
           for (; many; many &= many - 1) {
             const int owner = __ffs(many) - 1;
-            const int id = lo + __shfl_sync(0xffffffffu, at, owner);
+            const int its = __shfl_sync(0xffffffffu, id, owner);
             for (int e0 = __shfl_sync(0xffffffffu, first, owner) + 1; e0 < r.biases; e0 += 32) {
               const int e = e0 + (tid & 31);
-              const bool same = e < r.biases && r.bias_ids[e] == id;
+              const bool same = e < r.biases && r.bias_ids[e] == its;
               const float value = same ? r.bias_values[e] : 0.f;
               for (uint32_t hits = __ballot_sync(0xffffffffu, same); hits; hits &= hits - 1) {
                 const double add = (double)__shfl_sync(0xffffffffu, value, __ffs(hits) - 1);
@@ -338,8 +375,8 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
           if (l) v = __dadd_rn(v, sum);
         }
         if (!mine) continue;
-        if (v > best.v || (v == best.v && v > -INFINITY && lo + at < best.i)) best = {v, lo + at};
-        if (out) out[at] = __double2bfloat16(v);
+        if (v > best.v || (v == best.v && v > -INFINITY && id < best.i)) best = {v, id};
+        if (out) out[id] = __double2bfloat16(v);
       }
     }
   }
@@ -424,8 +461,10 @@ extern "C" int b200_logits_process(const void* logits, int64_t ld, int64_t rows,
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   unsigned ctas = 1;
   while (ctas < kMaxCtas && (int64_t)ctas * 1024 < vocab && rows * ctas * 2 <= 2 * sms) ctas *= 2;
-  int64_t chunk = ((vocab + ctas - 1) / ctas + 31) / 32 * 32;
-  while (ctas < kMaxCtas && part_bytes(chunk) > kMaxSmem) chunk = ((vocab + (ctas *= 2) - 1) / ctas + 31) / 32 * 32;
+  const int64_t stripes = (vocab + kStripe - 1) / kStripe;
+  auto part = [&](unsigned c) { return (stripes + c - 1) / c * kStripe; };
+  while (ctas < kMaxCtas && part_bytes(part(ctas)) > kMaxSmem) ctas *= 2;
+  const int64_t chunk = part(ctas);
   if (part_bytes(chunk) > kMaxSmem) return B200_ERROR_UNSUPPORTED;
   const int vec = (pl & 15u) == 0 && ld % 8 == 0 && (!out || ((po & 15u) == 0 && ldo % 8 == 0));
   const LogitsParams p{static_cast<const __nv_bfloat16*>(logits), ld, vocab, (int)chunk, history, history_ld,
