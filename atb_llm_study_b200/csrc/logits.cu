@@ -160,16 +160,6 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
 
   const __nv_bfloat16* in = p.logits + row * p.ld;
   __nv_bfloat16* out = p.out ? p.out + row * p.ldo : nullptr;
-  uint4 raw[kAhead];
-  auto load = [&](int c0) {
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (c0 + k * kThreads < nv) {
-        const int id = token_of((c0 + k * kThreads) * 8);
-        if (id + 8 <= vocab) raw[k] = *reinterpret_cast<const uint4*>(in + id);
-      }
-  };
-  load(tid);  // on their way while the lists are read
   const uint32_t* mask = nullptr;
   if (p.mask) {
     const int64_t m = p.mask_rows ? p.mask_rows[row] : row;
@@ -179,6 +169,20 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
       mask = p.mask + m * p.mask_ld;
     }
   }
+  uint4 raw[kAhead];
+  uint32_t bits[kAhead];  // the mask's words
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (c0 + k * kThreads < nv) {
+        const int id = token_of((c0 + k * kThreads) * 8);
+        if (id + 8 <= vocab) {
+          raw[k] = *reinterpret_cast<const uint4*>(in + id);
+          bits[k] = mask ? mask[id >> 5] : 0xffffffffu;
+        }
+      }
+  };
+  load(tid);  // on their way while the lists are read
   Row r{};
   if (HIST) {
     r.history = p.history + row * p.history_ld;
@@ -251,15 +255,13 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitsParams 
       if (id + 8 > vocab) break;  // and all behind it
       uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
       uint32_t skip = kLists ? reinterpret_cast<const uint8_t*>(marks)[c] : 0;
-      if (mask) {
-        const uint32_t hidden = ~(mask[id >> 5] >> (id & 31)) & 0xffu;
-        if (hidden) {
-          skip |= hidden;
+      const uint32_t hidden = ~(bits[k] >> (id & 31)) & 0xffu;
+      if (hidden) {
+        skip |= hidden;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t h = spread2(hidden >> (2 * i));
-            w[i] = (w[i] & ~h) | (kLowPair & h);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t h = spread2(hidden >> (2 * i));
+          w[i] = (w[i] & ~h) | (kLowPair & h);
         }
       }
       if (out) *reinterpret_cast<uint4*>(out + id) = make_uint4(w[0], w[1], w[2], w[3]);
