@@ -26,11 +26,11 @@ struct Window {
   __nv_bfloat16* out;
   int64_t os, ohs;
   const int32_t* cu;
-  int nq, nkv, nseq, mblocks, total, max_rows;
+  int nq, nkv, nseq, items, total, max_rows;
   int64_t qhs, khs, vhs;
   float scale_log2;
   int window, sinks, out_cols;
-  bool pair_heads;
+  bool pair_heads, by_tile;
 
   struct Item {
     int n;                       // key tiles
@@ -44,26 +44,43 @@ struct Window {
     B200_DEV int head_of(int s) const { return s ? h1 : h0; }
   };
 
+  // An item: two heads of a query tile, or two query tiles of a head, in one of two
+  // orders.  By tile: the last tiles of all sequences first, which see most keys,
+  // so that the walk ends with cheap items; it walks over numbers of sequences that
+  // have no such tile.  By sequence: sequence s owns the numbers from
+  // floor(cu[s] / rows) + s on, as many as it has tiles, or one more, whatever the
+  // lengths, and the sequence of a number is found by halving.  By tile 8 x 2048
+  // takes 282 us, by sequence 306; 17 prompts of up to 900 take 50 and 43.
   struct Cursor {
     const Window& p;
     int w;
     B200_DEV explicit Cursor(const Window& q) : p(q), w(blockIdx.x) {}
     B200_DEV bool next(Item& it, unsigned* err) {
-      // an item: two heads of a query tile, or two query tiles of a head; the latest rows of a sequence first
-      const int heads = p.pair_heads ? p.nq / 2 : p.nq, rows = p.pair_heads ? kTile : 2 * kTile;
-      const int per_m = heads * p.nseq, W = p.mblocks * per_m;
-      for (; w < W; w += gridDim.x) {
-        const int m = p.mblocks - 1 - w / per_m, r = w % per_m;
-        const int sq = r / heads, h = r % heads;
-        it.start = p.cu[sq];
-        it.len = p.cu[sq + 1] - it.start;
+      const int heads = p.pair_heads ? p.nq / 2 : p.nq, shift = p.pair_heads ? 7 : 8;
+      for (; w < p.items; w += gridDim.x) {
+        const int back = w / heads, h = w - back * heads;
+        int lo = 0, m;  // sequence, tile
+        if (p.by_tile) {
+          m = p.items / heads / p.nseq - 1 - back / p.nseq;
+          lo = back % p.nseq;
+        } else {
+          const int t = p.items / heads - 1 - back;
+          for (int hi = p.nseq; hi - lo > 1;) {  // first number of lo <= t < first number of hi
+            const int mid = (lo + hi) >> 1;
+            if ((p.cu[mid] >> shift) + mid <= t) lo = mid;
+            else hi = mid;
+          }
+          m = t - lo - (p.cu[lo] >> shift);
+        }
+        it.start = p.cu[lo];
+        it.len = p.cu[lo + 1] - it.start;
         if (it.start < 0 || it.len > p.total - it.start) {  // rows outside the operands
           raise_error(err, DEV_ERR_BAD_INDEX);
           continue;
         }
-        const int m0 = m * rows;
         it.rows = min(it.len, p.max_rows);
-        if (m0 >= it.rows) continue;
+        if (m < 0 || m > (it.rows - 1) >> shift) continue;
+        const int m0 = m << shift;
         it.h0 = p.pair_heads ? 2 * h : h;
         it.h1 = p.pair_heads ? 2 * h + 1 : h;
         it.m0 = m0;
@@ -174,8 +191,10 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
   if (num_seqs == 0 || max_seqlen == 0 || total_tokens == 0) return B200_OK;
   const bool pair_heads = nq / nkv % 2 == 0;
   const int rows = pair_heads ? kTile : 2 * kTile;
-  const int mblocks = (int)(((int64_t)max_seqlen + rows - 1) / rows);
-  const int64_t items = (int64_t)mblocks * (pair_heads ? nq / 2 : nq) * num_seqs;
+  // by tile where lengths are near each other: at most a quarter of its numbers more than by sequence
+  const int64_t by_tile = ((int64_t)max_seqlen + rows - 1) / rows * num_seqs, by_sequence = total_tokens / rows + num_seqs;
+  const bool tiles = 4 * by_tile <= 5 * by_sequence;
+  const int64_t items = (tiles ? by_tile : by_sequence) * (pair_heads ? nq / 2 : nq);
   if (total_tokens > INT32_MAX - 2 * kTile || qcols > INT32_MAX || kcols > INT32_MAX || vcols > INT32_MAX ||
       items > INT32_MAX - 4096 || max_seqlen > INT32_MAX - 2 * kTile)
     return B200_ERROR_UNSUPPORTED;
@@ -192,7 +211,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
     prob.nq = nq;
     prob.nkv = nkv;
     prob.nseq = num_seqs;
-    prob.mblocks = mblocks;
+    prob.items = (int)items;
     prob.max_rows = max_seqlen;
     prob.total = (int)total_tokens;
     prob.qhs = q_head_stride;
@@ -203,6 +222,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
     prob.sinks = sinks;
     prob.out_cols = cols;
     prob.pair_heads = pair_heads;
+    prob.by_tile = tiles;
     return launch_items(mq, mk, mv, prob, grid, stream);
   };
   if (hd < 64) {

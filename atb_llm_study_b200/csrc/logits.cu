@@ -453,7 +453,7 @@ extern "C" int b200_logits_process(const void* logits, int64_t ld, int64_t rows,
     if (reinterpret_cast<uintptr_t>(q) & 3u) return B200_ERROR_INVALID_PARAM;
   const uintptr_t pl = reinterpret_cast<uintptr_t>(logits), po = reinterpret_cast<uintptr_t>(out);
   if ((pl & 1u) || (po & 1u) || (reinterpret_cast<uintptr_t>(next) & 7u)) return B200_ERROR_INVALID_PARAM;
-  if (rows > INT32_MAX / 16 || vocab > (1 << 23) || history_ld > (int64_t)(kTopBit - 1)) return B200_ERROR_UNSUPPORTED;
+  if (rows > INT32_MAX / 16 || vocab > (1 << 23) || history_ld > (1 << 30)) return B200_ERROR_UNSUPPORTED;
   if (rows == 0) return B200_OK;
 
   // CTAs of a row: as many as run at once (two an SM), at most 16, each with

@@ -97,8 +97,16 @@ def test_prompt_heads(nq, nkv, d, dv, fused):
     check_prompt([130, 300, 5], nq, nkv, d, dv, 150, 2, fused=fused, pad_rows=70)
 
 
+@pytest.mark.parametrize("nq", [4, 2])  # two heads an item, or two row tiles
+def test_prompt_many_lengths(nq):
+    rng = np.random.default_rng(nq)
+    lens = [int(n) for n in rng.choice([0, 0, 1, 3, 100, 127, 128, 129, 255, 256, 257, 400], 60)]
+    check_prompt(lens, nq, 2, 64, 64, 90, 2)
+
+
 def test_prompt_longer_limit_and_rows_behind():
     check_prompt([200, 100], 4, 2, 128, 128, 64, 4, pad_rows=300, longest=1000)
+    check_prompt([200, 100, 0], 4, 2, 128, 128, 64, 4, pad_rows=5000, longest=100000)
     q, k, v = prompt_inputs(1, 300, 2, 2, 64, 64)  # a sequence longer than max_seqlen: its first tiles, the rest as it was
     got = prompt(q, k, v, [300], 64, 0, longest=128)
     want, weight = serving.window_prompt(q, k, v, [300], 64, 0, 0.125)
