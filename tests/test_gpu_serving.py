@@ -482,3 +482,76 @@ def test_steps_of_a_captured_serving_loop(shared):
         for b in range(B):
             history[b] = (history[b] + [tokens[b]])[-399:] if h_lens[b] else []
     assert G.device_errors() == 0 and seen_short
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {root!r}); sys.path.insert(0, {tests!r})
+import numpy as np, torch
+from atb_llm_study_b200 import capi
+torch.zeros(1, device="cuda")
+import gpu_util as G, test_gpu_window as T, test_gpu_serving as S
+from oracle import serving
+kind = sys.argv[1]
+g = torch.cuda.CUDAGraph()
+if kind in ("token", "shared"):
+    c = T.Cache(1, [70, 130], 2, 64, 64, spare=4)
+    c.fill_fast(c.order[:2], 100)
+    q, qd = T.queries(1, 2, 4, 64)
+    dev, pre, plen = c.device(), G.i32(c.order[:2]), G.i32([100])
+    out = torch.zeros(2, 256, dtype=torch.bfloat16, device=G.DEV)
+    ws = torch.zeros(1 << 20, device=G.DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        T.token_call(qd, dev, c, 4, 50, 2, out=out) if kind == "token" else T.shared_call(qd, dev, c, 4, pre, plen, 100, ws=ws, out=out)
+    g.replay()
+    want = serving.window_decode(q, c.k, c.v, c.tables, c.lens, 50, 2) if kind == "token" else \\
+        serving.shared_decode(q, c.k, c.v, c.order[:2], 100, c.tables, c.lens)
+    T.close(G.host(out).reshape(2, 4, 64), *want)
+elif kind == "prompt":
+    q, k, v = T.prompt_inputs(1, 200, 4, 2, 64, 64)
+    dq, dk, dv = (G.bf16(x.reshape(200, -1)) for x in (q, k, v))
+    out, cu = torch.zeros(200, 256, dtype=torch.bfloat16, device=G.DEV), G.i32([0, 200])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        G.check(G.L().b200_flash_prefill_window(dq.data_ptr(), 256, 64, dk.data_ptr(), 128, 64, dv.data_ptr(), 128, 64, out.data_ptr(),
+                                                256, 64, cu.data_ptr(), 1, 200, 200, 4, 2, 64, 64, 0.125, 60, 3, G.stream()))
+    g.replay()
+    T.close(G.host(out).reshape(200, 4, 64), *serving.window_prompt(q, k, v, [200], 60, 3, 0.125))
+elif kind == "logits":
+    x = G.bf16(np.arange(2000)[None] % 700)
+    nxt = torch.zeros(1, dtype=torch.int64, device=G.DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        G.check(G.L().b200_logits_process(x.data_ptr(), 2000, 1, 2000, None, 0, None, None, None, None, None, None, None, None, None, 0,
+                                          0, None, None, 0, nxt.data_ptr(), G.stream()))
+    g.replay()
+    assert nxt.item() == int(G.host(x)[0].argmax())
+else:
+    lens, new, ctx = G.i32([3]), G.i32([2]), G.i32([0])
+    tables, free, count, left = G.i32([[4, -1]]), G.i32([0, 1, 2, 3, 5, 6]), G.i32([6]), G.i32([0])
+    slots = G.i64([0, 0])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        G.check(G.L().b200_block_tables_extend(lens.data_ptr(), new.data_ptr(), 1, 4, tables.data_ptr(), 2, free.data_ptr(),
+                                               count.data_ptr(), 7, ctx.data_ptr(), None, None, slots.data_ptr(), 2, left.data_ptr(),
+                                               None, G.stream()))
+        G.check(G.L().b200_block_tables_release(ctx.data_ptr(), lens.data_ptr(), 1, 4, tables.data_ptr(), 2, free.data_ptr(), 6,
+                                                left.data_ptr(), 7, ctx.data_ptr(), left.data_ptr(), G.stream()))
+    g.replay()
+    assert slots.tolist() == [19, 24] and left.item() == 6 and ctx.item() == 3 and free.tolist()[5] == 6
+torch.cuda.synchronize()
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("kind", ["prompt", "token", "shared", "logits", "tables"])
+def test_first_call_of_a_process_may_be_captured(kind):
+    import os
+    import subprocess
+    import sys
+
+    tests = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=os.path.dirname(tests), tests=tests), kind], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout[-500:] + r.stderr[-2000:]
