@@ -206,7 +206,7 @@ template <class P>
 struct ItemsCfg {
   static constexpr int BOXES_QK = P::HDK / 64, BOXES_V = P::HDV / 64;
   static constexpr int TILE_QK = BOXES_QK * kBoxBytes, TILE_V = BOXES_V * kBoxBytes;
-  static constexpr int K_STAGES = P::HDK > 128 ? 2 : P::HDK > 64 ? 2 : 4;
+  static constexpr int K_STAGES = P::HDK > 128 ? 2 : P::HDK > 64 ? 3 : 4;
   static constexpr int V_STAGES = P::HDK > 128 ? 1 : P::HDK > 64 ? 2 : 4;
   static constexpr int K_AT = kSides * TILE_QK, V_AT = K_AT + K_STAGES * TILE_QK, BARS_AT = V_AT + V_STAGES * TILE_V;
   static constexpr int HIDDEN_AT = BARS_AT + 320;
