@@ -218,21 +218,24 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
       if (p.missing) *p.missing = fits ? 0 : sane ? (int)(need - count) : -1;
     }
   }
-  const int64_t stride = (int64_t)ctas * kThreads;
-  const int64_t me = (int64_t)rank * kThreads + threadIdx.x;
-  // Entries and tokens in turns of kAtOnce a thread, a CTA's side by side, so
-  // that as many loads from the tables are on their way together.
+  // A warp takes a run of entries, and of tokens, 32 side by side and kAtOnce of
+  // those in a turn, so that as many loads from the tables are on their way
+  // together and a lane's next item is mostly of the same sequence or the next.
+  const int64_t warps = (int64_t)ctas * (kThreads / 32), warp = (int64_t)rank * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  auto run_of = [&](int64_t items) { return (items + warps * 32 - 1) / (warps * 32) * 32; };
   if (fits) {
     int i = 0;
-    for (int64_t e0 = me; e0 < need; e0 += kAtOnce * stride) {
+    const int64_t run = run_of(need), end = min((warp + 1) * run, need);
+    for (int64_t e0 = warp * run + lane; e0 < end; e0 += kAtOnce * 32) {
       int32_t b[kAtOnce];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k)
-        if (e0 + k * stride < need) b[k] = p.free_blocks[count - 1 - (e0 + k * stride)];
+        if (e0 + k * 32 < end) b[k] = p.free_blocks[count - 1 - (e0 + k * 32)];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const int64_t e = e0 + k * stride;
-        if (e >= need) break;
+        const int64_t e = e0 + k * 32;
+        if (e >= end) break;
         i = find(l.blocks, p.n, i, (int)e);
         if (b[k] < 0 || b[k] >= p.num_blocks) {
           raise_error(p.err, DEV_ERR_BAD_INDEX);
@@ -244,14 +247,15 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
   }
   if (p.positions || p.slots) {
     int i = 0;
-    for (int64_t t0 = me; t0 < p.capacity; t0 += kAtOnce * stride) {
+    const int64_t run = run_of(p.capacity), end = min((warp + 1) * run, p.capacity);
+    for (int64_t t0 = warp * run + lane; t0 < end; t0 += kAtOnce * 32) {
       int at[kAtOnce];
       int32_t b[kAtOnce];
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const int64_t t = t0 + k * stride;
+        const int64_t t = t0 + k * 32;
         at[k] = -1;
-        if (fits && t < tokens) {
+        if (fits && t < tokens && t < end) {
           i = find(l.tokens, p.n, i, (int)t);
           at[k] = l.cached[i] + (int)t - l.tokens[i];
           const int col = bs.quotient(at[k]), held = blocks_of(l.cached[i], bs);
@@ -261,8 +265,8 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ExtendParams p) 
       }
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
-        const int64_t t = t0 + k * stride;
-        if (t >= p.capacity) break;
+        const int64_t t = t0 + k * 32;
+        if (t >= end) break;
         int64_t slot = -1;
         if (at[k] >= 0) {
           if (b[k] >= 0 && b[k] < p.num_blocks) slot = (int64_t)b[k] * bs.bs + at[k] - bs.quotient(at[k]) * bs.bs;

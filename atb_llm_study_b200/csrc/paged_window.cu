@@ -54,6 +54,8 @@ struct Cfg {
   static constexpr int Q_BYTES = kRows * HD * 2;
   static constexpr int BARS = kStages * STAGE + Q_BYTES;
   static constexpr int SMEM = BARS + 64 + 1024;
+  // the parts are joined where the tiles were: four warps' outputs, their join, maxima and sums
+  static_assert((kRows * HD * 5 + 10 * kRows) * 4 <= kStages * STAGE, "room for the join");
 };
 
 struct Params {
