@@ -16,7 +16,9 @@
 // sums over), the cluster meets once so that outputs may lie where inputs lay,
 // and the CTAs share the entries and tokens.  A cluster instead of a grid
 // because of that meeting: without it a step could not update its lengths and
-// its free count in place, which a replayed graph needs.
+// its free count in place, which a replayed graph needs.  104 thousand tokens of
+// 2048 sequences take 16.4 us in a replayed graph with L2 flushed (an empty one
+// takes 6); one token at a time in 8 CTAs, strided over all of them, they took 34.8.
 #include <algorithm>
 
 #include "common.cuh"

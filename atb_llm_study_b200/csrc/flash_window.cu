@@ -10,6 +10,12 @@
 // odd, two query tiles of one head next to each other.  Items are walked with
 // the heads of one sequence's rows side by side: those that share keys find them
 // in L2.
+//
+// Measured, 32 / 8 heads of 128, alone: 8 x 2048 with a window of 1024 in 278 us
+// (743 TFLOP/s of visible pairs, 84 % of the pairs computed), 1 x 32768 with 4096
+// in 1.90 ms (1086 TFLOP/s, 66 % of the measured burst rate); back to back, under
+// the power limit, 320 us and 2.25 ms.  A tile at the window's ends costs a side
+// half as much again as a whole one.
 #include <algorithm>
 
 #include "tc_items.cuh"

@@ -25,6 +25,13 @@
 // rows of hidden tokens are zeroed in shared memory before they are used, so a
 // NaN or an infinity there (a block's unwritten rest, another sequence's data)
 // does not reach the output.
+//
+// Measured: 64 sequences of up to 32768 tokens, window 4096, 32 / 8 heads of 128:
+// 161 us for 1.055 GB, the measured copy rate.  Two stages and three CTAs an SM
+// took 229.  Contexts of a few tiles are bound by a CTA's way from its length to
+// its table, tiles and join, 5 us: 64 of 512 tokens on average take 36 us for
+// 129 MB.  (CTAs that walk many pairs, loading ahead, took 50: more registers, and
+// joins in turns to fit two of them on an SM.)
 #include <math.h>
 
 #include <algorithm>

@@ -149,6 +149,30 @@ def test_prompt_hidden_values_stay_hidden(window, sinks, bad, value):
             close(got[:300, 2:], want[:300, 2:], weight[:300, 2:])
 
 
+def test_a_query_that_is_nan_is_alone():
+    q, k, v = prompt_inputs(6, 200, 4, 2, 64, 64)
+    want, weight = serving.window_prompt(q, k, v, [200], 70, 2, 0.125)
+    q[130, 1, 5] = np.nan
+    got = prompt(q, k, v, [200], 70, 2)
+    assert np.isnan(got[130, 1]).all()
+    got[130, 1] = want[130, 1]
+    close(got, want, weight)
+    c = Cache(9, [100, 100], 2, 64, 64, spare=4)
+    c.fill_fast(c.order[:2], 100)
+    q, _ = queries(9, 2, 4, 64)
+    qn = q.reshape(2, 256).copy()
+    qn[1, 64] = np.nan
+    qd = G.bf16(np.concatenate([qn, np.zeros((2, 8), np.float32)], 1))
+    for got, (want, weight) in (
+            (token_call(qd, c.device(), c, 4, 80, 0), serving.window_decode(q, c.k, c.v, c.tables, c.lens, 80, 0)),
+            (shared_call(qd, c.device(), c, 4, G.i32(c.order[:2]), G.i32([100]), 100),
+             serving.shared_decode(q, c.k, c.v, c.order[:2], 100, c.tables, c.lens))):
+        got = G.host(got)[:2, :256].reshape(2, 4, 64)
+        assert np.isnan(got[1, 1]).all()
+        got[1, 1] = want[1, 1]
+        close(got, want, weight)
+
+
 def test_prompt_growing_and_flat_scores():
     lens = [400]
     q, k, v = prompt_inputs(4, 400, 2, 1, 128, 128, scale=0.0)
