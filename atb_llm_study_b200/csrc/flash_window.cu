@@ -185,7 +185,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
     return B200_ERROR_UNSUPPORTED;
   for (int64_t s : {q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, out_stride,
                     out_head_stride})
-    if (s < 0 || s % 8) return B200_ERROR_INVALID_PARAM;
+    if (s < 0 || s % 8 || s > INT64_MAX / nq) return B200_ERROR_INVALID_PARAM;
   for (const void* x : {q, k, v, (const void*)out})
     if (reinterpret_cast<uintptr_t>(x) & 15u) return B200_ERROR_INVALID_PARAM;
   if (reinterpret_cast<uintptr_t>(cu_seqlens) & 3u) return B200_ERROR_INVALID_PARAM;

@@ -482,7 +482,7 @@ int paged_window_check(const void* q, int64_t q_stride, const void* k_cache, con
       (reinterpret_cast<uintptr_t>(out) & 1u))
     return B200_ERROR_INVALID_PARAM;
   if ((int64_t)max_blocks_per_seq * block_size < max_context) return B200_ERROR_INVALID_PARAM;
-  if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX - 256 || num_blocks * nkv * block_size > INT32_MAX ||
+  if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX - 256 || num_blocks > INT32_MAX / block_size / nkv ||
       (int64_t)batch * nq > INT32_MAX / kMaxCluster)
     return B200_ERROR_UNSUPPORTED;
   return B200_OK;

@@ -377,7 +377,8 @@ B200_API int b200_flash_prefill_packed(const void* q, int64_t q_stride, int64_t 
  * (others are B200_ERROR_UNSUPPORTED), strides and alignment; scale > 0; all on
  * the tcgen05 tensor cores.  Rows of out that belong to no sequence, and of a
  * sequence behind max_seqlen, are left as they are; a sequence outside
- * [0, total_tokens) is left out and sets the device error word.  What a row
+ * [0, total_tokens) is left out and sets the device error word (where offsets
+ * do not ascend, sequences beside it may be left out with it).  What a row
  * does not see does not reach it, NaN and infinities included; a row that sees
  * a value row with one is not finite.  Extends SelfAttentionOp::Create
  * (PA_ENCODER) (atb_cpp_llm/src/ops/self_attention_op.cpp:8-30), whose only

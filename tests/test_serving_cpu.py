@@ -77,6 +77,21 @@ def test_refused(name, base, change, status):
 
 
 @needs_lib
+@pytest.mark.parametrize("name,base,change,status", [
+    # products that would wrap in 64 bits: 2^62 blocks x 2 heads x 64 tokens = 2^69, 3 heads x 2^62 elements
+    ("b200_paged_decode_window", TOKEN, dict(blocks=1 << 62, b=0), UNSUPPORTED),
+    ("b200_paged_decode_shared", SHARED, dict(blocks=1 << 62, b=0), UNSUPPORTED),
+    ("b200_flash_prefill_window", PROMPT, dict(qh=1 << 62), INVALID),
+    ("b200_flash_prefill_window", PROMPT, dict(oh=1 << 62), INVALID),
+    # the largest cache that 32-bit rows reach, and one block more
+    ("b200_paged_decode_window", TOKEN, dict(blocks=((1 << 31) - 1) // 128, b=0), 0),
+    ("b200_paged_decode_window", TOKEN, dict(blocks=((1 << 31) - 1) // 128 + 1, b=0), UNSUPPORTED),
+], ids=lambda x: "" if isinstance(x, dict) and len(x) > 9 else str(x))
+def test_sizes_whose_products_wrap(name, base, change, status):
+    assert getattr(capi.lib(), name)(*{**base, **change}.values()) == status
+
+
+@needs_lib
 def test_nothing_to_do():
     L = capi.lib()
     assert L.b200_flash_prefill_window(*{**PROMPT, "n": 0}.values()) == 0
