@@ -294,11 +294,13 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     if (lane == 0) {
       bool ok = true;
       int g = 0, n[kSides] = {0, 0};  // tiles, and items of each side, so far
+      int k_loads = 0, v_loads = 0;
       while (ok && !*abort_flag && cursor.next(it, err)) {
         for (int j = 0; ok && j < it.n; ++j, ++g) {
           const int ks = g % KS, vs = g % VS;
           if (g >= KS && !(ok = mbar_wait_idle(&k_empty[ks], (g / KS - 1) & 1, err))) break;
           P::load_k(p, it, j, sK + ks * Cf::TILE_QK, &tmK, &k_full[ks], err);
+          ++k_loads;
           if (j == 0)
 #pragma unroll
             for (int s = 0; s < kSides; ++s) {
@@ -310,9 +312,15 @@ __global__ void __launch_bounds__(kItemThreads, 1)
           if (!ok) break;
           if (g >= VS && !(ok = mbar_wait_idle(&v_empty[vs], (g / VS - 1) & 1, err))) break;
           P::load_v(p, it, j, sV + vs * Cf::TILE_V, &tmV, &v_full[vs], err);
+          ++v_loads;
         }
       }
       if (!ok) *abort_flag = 1;
+      // whoever gives up before using a tile: no copy is in flight when the CTA ends
+      for (int i = max(0, k_loads - KS); i < k_loads; ++i) mbar_wait_idle(&k_full[i % KS], (i / KS) & 1, err);
+      for (int i = max(0, v_loads - VS); i < v_loads; ++i) mbar_wait_idle(&v_full[i % VS], (i / VS) & 1, err);
+      for (int s = 0; s < kSides; ++s)
+        if (n[s] > 0) mbar_wait_idle(&q_full[s], (n[s] - 1) & 1, err);
     }
     __syncwarp();
   } else if (warp == 1 || warp == kMma1Warp) {
@@ -431,7 +439,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         if (!ok) break;
         const int key = P::key0(it, j);
         if (!P::whole(it, 0, key) || (it.both && !P::whole(it, 1, key))) {
-          const int at = min(edges, kMaxEdgeTiles - 1);  // an item has four at most
+          const int at = min(edges, kMaxEdgeTiles - 1);  // an item has six at most (row tiles in pairs: the window's start cuts three, the diagonal two, the sinks one)
           uint32_t any = 0;
 #pragma unroll 1
           for (int w = 0; w < 4; ++w) {
