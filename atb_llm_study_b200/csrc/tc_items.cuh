@@ -426,17 +426,19 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     int g = 0, n = 0;
 #pragma unroll 1
     for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
-      // Free again: V of item n was loaded after the P V of item n - VS or a later one began, and before an item's P V
-      // begins all earlier items have been stored.  So records are cleared half a ring ahead.
       Hidden* hd = &hidden[n % Cf::RING];
-      static_assert(VS + 1 <= Cf::RING / 2, "ring of records");
-      if (lane == 0) hidden[(n + Cf::RING / 2) % Cf::RING].any = 0;
       int edges = 0;
 #pragma unroll 1
       for (int j = 0; j < it.n; ++j, ++g) {
         const int vs = g % VS;
         ok = __all_sync(0xffffffffu, mbar_wait_idle(&v_full[vs], (g / VS) & 1, err));
         if (!ok) break;
+        // Records are cleared half a ring ahead of their use, once V of their item n has landed: it was loaded behind the
+        // P V of item n - VS or a later one, and before an item's P V begins all earlier items have been stored (o_free).
+        // So items up to n - VS - 1 are done with their records.  (Before this wait only V of item n - 1 has landed, and
+        // with one stage item n - 2, whose record this is, may still be at reading it.)
+        static_assert(VS + 1 <= Cf::RING / 2, "the record that item n clears belongs to item n - VS - 1 or an earlier one");
+        if (j == 0 && lane == 0) hidden[(n + Cf::RING / 2) % Cf::RING].any = 0;
         const int key = P::key0(it, j);
         if (!P::whole(it, 0, key) || (it.both && !P::whole(it, 1, key))) {
           const int at = min(edges, kMaxEdgeTiles - 1);  // an item has six at most (row tiles in pairs: the window's start cuts three, the diagonal two, the sinks one)

@@ -149,6 +149,54 @@ def test_prompt_hidden_values_stay_hidden(window, sinks, bad, value):
             close(got[:300, 2:], want[:300, 2:], weight[:300, 2:])
 
 
+# heads in pairs and (odd groups) row tiles in pairs; four, two and one stages of V
+@pytest.mark.parametrize("nq,nkv,d,dv", [(3, 1, 64, 64), (4, 2, 128, 128), (3, 1, 128, 128), (4, 2, 192, 128), (2, 2, 192, 128),
+                                         (2, 1, 32, 32)])
+@pytest.mark.parametrize("window,sinks,bad", [(40, 4, 2), (130, 0, 200), (128, 130, 131), (200, 3, 255), (300, 0, 128)])
+@pytest.mark.parametrize("value", [np.nan, -np.inf])
+def test_prompt_hidden_values_of_all_widths(nq, nkv, d, dv, window, sinks, bad, value):
+    lens = [400, 90]
+    q, k, v = prompt_inputs(7, 490, nq, nkv, d, dv)
+    want, weight = serving.window_prompt(q, k, v, lens, window, sinks, d ** -0.5)
+    v = v.copy()
+    v[bad, 0, dv - 1] = value
+    sees = serving.window_mask(400, window, sinks)[:, bad]
+    got = prompt(q, k, v, lens, window, sinks)
+    group = nq // nkv
+    assert not np.isfinite(got[:400][sees][:, :group, dv - 1]).any()
+    close(got[:400][~sees], want[:400][~sees], weight[:400][~sees])
+    if nkv > 1:
+        close(got[:, group:], want[:, group:], weight[:, group:])
+    close(got[400:], want[400:], weight[400:])
+
+
+@pytest.mark.parametrize("nq,nkv,d,dv,seqs", [(4, 4, 192, 128, 500), (4, 2, 192, 128, 700), (8, 4, 128, 128, 900), (16, 8, 64, 64, 900)])
+def test_prompt_records_of_many_short_items(nq, nkv, d, dv, seqs):
+    """A CTA walks a dozen items of one key tile and more, several times what the ring of zeroed values' records holds;
+    some sequences and heads have a value that is no number, the items around them do not."""
+    rng = np.random.default_rng(d + nq)
+    lens = rng.integers(1, 9, seqs).tolist()
+    total = sum(lens)
+    q, k, v = prompt_inputs(8, total, nq, nkv, d, dv)
+    want, weight = serving.window_prompt(q, k, v, lens, 6, 1, d ** -0.5)
+    v = v.copy()
+    poisoned = np.zeros((total, nq), bool)
+    at = 0
+    for n in lens:
+        for h in np.nonzero(rng.random(nkv) < 0.3)[0]:
+            bad = int(rng.integers(0, n))
+            v[at + bad, h, int(rng.integers(0, dv))] = rng.choice([np.nan, np.inf])
+            sees = serving.window_mask(n, 6, 1)[:, bad]
+            poisoned[at:at + n, h * nq // nkv:(h + 1) * nq // nkv] |= sees[:, None]
+        at += n
+    for _ in range(3):
+        got = prompt(q, k, v, lens, 6, 1)
+        finite = np.isfinite(got).all(2)
+        np.testing.assert_array_equal(finite, ~poisoned)
+        close(got[finite], want[finite], weight[finite])
+    assert G.device_errors() == 0
+
+
 def test_a_query_that_is_nan_is_alone():
     q, k, v = prompt_inputs(6, 200, 4, 2, 64, 64)
     want, weight = serving.window_prompt(q, k, v, [200], 70, 2, 0.125)
