@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
   uint64_t* p_full = bars + 6;       // [side] P of a tile written (an arrival a softmax thread)
   uint64_t* pv_done = bars + 8;      // [side] P V of a tile done, and the list of zeroed keys behind it (2 arrivals)
   uint64_t* o_free = bars + 10;      // [side] the outputs are read out (an arrival a softmax thread)
-  uint64_t* drain = bars + 12;       // [side] the MMAs issued before an abort
+  uint64_t* drain = bars + 12;       // [side] all MMAs issued, at the end
   uint64_t* turn = bars + 14;        // [side] it may issue
   uint64_t* k_full = bars + 16;      // [KS]
   uint64_t* k_empty = k_full + KS;   // [KS] (an arrival a side, as v_empty)
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
       if (ok && mine) scores(0, it.n == 1);
       else if (ok) mbar_arrive_elect(&k_empty[0]);
     }
-    while (ok && have && !*abort_flag) {
+    while (ok && have && __all_sync(0xffffffffu, !*abort_flag)) {
       typename P::Item after;
       const bool more = cursor.next(after, err);
       const bool mine = s == 0 || it.both;
@@ -414,18 +414,17 @@ __global__ void __launch_bounds__(kItemThreads, 1)
       it = after;
       have = more;
     }
-    if (!ok) {
-      *abort_flag = 1;
-      umma_commit_elect(&drain[s]);  // every MMA issued completes before TMEM is freed
-      mbar_wait(&drain[s], 0, err);
-    }
+    // Whoever gave up, this warp or another whose flag ended the loop: every MMA issued completes before TMEM is freed.
+    if (!ok) *abort_flag = 1;
+    umma_commit_elect(&drain[s]);
+    mbar_wait(&drain[s], 0, err);
     __syncwarp();
   } else if (warp == 2) {
     // ---------------- values looked through ----------------
     bool ok = true;
     int g = 0, n = 0;
 #pragma unroll 1
-    for (; ok && !*abort_flag && cursor.next(it, err); ++n) {
+    for (; ok && __all_sync(0xffffffffu, !*abort_flag) && cursor.next(it, err); ++n) {
       Hidden* hd = &hidden[n % Cf::RING];
       int edges = 0;
 #pragma unroll 1
@@ -598,6 +597,8 @@ __global__ void __launch_bounds__(kItemThreads, 1)
       mbar_arrive(&o_free[s]);
     }
     if (!ok) *abort_flag = 1;
+    tmem_ld_wait();  // nothing of a tile that was given up is on its way when TMEM is freed
+    tmem_st_wait();
   }
   tc_fence_before();
   __syncthreads();
