@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
       }
       __syncwarp();
     }
-    if (!ok && lane == 0)  // a wait ran out: the copies in flight land before their memory is used again
+    // whoever gives up before using a tile: every copy has landed before its memory is used again
+    if (lane == 0)
       for (int k = max(0, i - kStages); k < i; ++k) mbar_wait(&full[k % kStages], (k / kStages) & 1, p.err);
     __syncwarp();
   } else {
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
     }
     for (int i = 0; i < n; ++i) {
       const int s = i % kStages;
-      if (!mbar_wait(&full[s], (i / kStages) & 1, p.err)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (i / kStages) & 1, p.err))) break;  // a warp as a whole
       uint8_t* sK = smem + s * C::STAGE;
       uint8_t* sV = sK + C::TILE;
       float sc[2][4];
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
   }
 
   // ---- this CTA's part: the four warps joined, in shared memory ----
-  __syncthreads();  // every copy has landed and been used
+  __syncthreads();  // every copy has landed, and been used where no wait ran out
   float* sm = reinterpret_cast<float*>(smem);  // [4][16] maxima
   float* sl = sm + 64;                         // [4][16] sums
   float* part_m = sl + 64;                     // [16] joined maxima

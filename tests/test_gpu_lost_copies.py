@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
     import gpu_util as G
-    from test_gpu_window import close
+    from test_gpu_window import Cache, close, queries
 
 TESTS = os.path.dirname(os.path.abspath(__file__))
 WAIT_TIMEOUT = 1
@@ -70,3 +70,28 @@ def test_items_kernel_ends_when_a_copy_is_lost(items, lost, item, tile):
                     close(got[side], want[side], weight[side])
             if i % 2 == 0 and i >= item:
                 assert any((got[side] == -5).all() for side in sides)
+
+
+@pytest.fixture(scope="module")
+def token(tmp_path_factory):
+    return compiled(str(tmp_path_factory.mktemp("lost")), "lost_token_copies")
+
+
+@pytest.mark.parametrize("lens", [[100, 1], [700, 30]], ids=["two-tiles", "ring-wraps"])
+@pytest.mark.parametrize("ctas", [1, 2])
+def test_token_kernel_ends_when_copies_are_lost(token, lens, ctas):
+    c = Cache(3, lens, 2, 64, 64)
+    q, qd = queries(3, 2, 4, 64)
+    k, v, tables, ctx = c.device()
+    want, weight = serving.window_decode(q, c.k, c.v, c.tables, lens, 1 << 20, 0)
+    for box in (32, 64):
+        out = torch.full((2, 256), -5.0, dtype=torch.bfloat16, device=G.DEV)
+        err = torch.zeros(1, dtype=torch.int32, device=G.DEV)
+        assert token.lost_token_copy(address(qd), address(k), address(v), address(tables), c.width, address(ctx), 2, 4, 2, 64,
+                                     c.blocks, 1 << 20, address(out), ctas, box, address(err), ctypes.c_void_p(G.stream())) == 0
+        torch.cuda.synchronize()
+        if box == 32:
+            assert err.item() == WAIT_TIMEOUT
+        else:
+            assert err.item() == 0
+            close(G.host(out).reshape(want.shape), want, weight)
