@@ -116,9 +116,12 @@ struct Prefix {
   B200_DEV static void store(const Prefix& p, const Item& it, int s, int row, float m, float l, uint32_t tO) {
     const int seqs = min(p.at.per_tile, p.batch - (it.row_tile + s) * p.at.per_tile);
     const bool valid = row < seqs * p.at.group;
-    const float inv = 1.f / l;  // every row sees the stretch's keys
+    // Every row sees the stretch's keys, but where all its scores are -inf they have no weight beside other parts': the
+    // part is zeros with a log sum of -inf.  (l is then what the polynomial leaves of 2^-126, or NaN where a score is.)
+    const bool none = m == -INFINITY && l == l;
+    const float inv = none ? 0.f : 1.f / l;
     float* o = p.at.parts + ((int64_t)(it.slot + s) * kTile + row) * HD;
-    if (valid) p.at.lse[(int64_t)(it.slot + s) * kTile + row] = m + log2f(l);
+    if (valid) p.at.lse[(int64_t)(it.slot + s) * kTile + row] = none ? -INFINITY : m + log2f(l);
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
       uint32_t r[32];

@@ -18,7 +18,7 @@ namespace b200 {
 
 struct PrefixParts {
   float* parts;  // [slots][128][head_dim] outputs over their sums
-  float* lse;    // [slots][128] log2 of the sums, with their maximum; -inf: no key
+  float* lse;    // [slots][128] log2 of the sums, with their maximum; -inf: no key has weight
   const int32_t* length;
   int max_length;
   int workers, row_tiles, per_tile, group;

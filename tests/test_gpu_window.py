@@ -502,6 +502,29 @@ def test_shared_visible_nan_is_not_lost():
         assert np.isnan(got[:, 2:, 3]).all() and np.isfinite(got[:, :2]).all()
 
 
+def far_below(c, table, positions):
+    """Keys of -inf in the first dim: with queries above zero there, scores of -inf."""
+    for j in positions:
+        c.k[table[j // c.bs], :, j % c.bs, 0] = -np.inf
+
+
+@pytest.mark.parametrize("plen,positions", [(1, [0]), (128, range(128)), (129, [128]), (300, range(128, 256)), (1000, range(1000)),
+                                            (1000, range(5, 1000))], ids=["1", "128", "last", "tile", "1000", "but-5"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_shared_prefix_without_weight(plen, positions, d):
+    # stretches of the prefix whose every score is -inf weigh nothing beside the rest
+    lens = [70, 1, 30]
+    c = Cache(10, lens, 2, d, 64, spare=20)
+    prefix = c.order[:-(-plen // 64)]
+    c.fill_fast(prefix, plen)
+    far_below(c, prefix, positions)
+    q = G.rounded(np.random.default_rng(10).standard_normal((3, 8 * d)) * 2)
+    q[:, ::d] = np.abs(q[:, ::d]) + 1
+    want, weight = serving.shared_decode(q.reshape(3, 8, d), c.k, c.v, prefix, plen, c.tables, lens)
+    got = G.host(shared_call(G.bf16(q), c.device(), c, 8, G.i32(prefix), G.i32([plen]), plen))[:3, :8 * d]
+    close(got.reshape(want.shape), want, weight)
+
+
 def test_shared_captured_calls_with_workspaces_of_their_own():
     c = Cache(8, [200] * 9, 4, 128, 64, spare=20)
     prefix = c.order[:16]
