@@ -146,8 +146,8 @@ struct Window {
         tma_load_2d(dst + x * kBoxBytes, map, bar, (int)(it.kvh * p.vhs) + 64 * x, it.start + key0(it, j));
   }
   // O / l from TMEM as bf16 rows
-  B200_DEV static void store(const Window& p, const Item& it, int s, int row, float, float l, uint32_t tO) {
-    const float inv = 1.f / l;  // every row sees itself
+  B200_DEV static void store(const Window& p, const Item& it, int s, int row, float m, float l, uint32_t tO) {
+    const float inv = m == -INFINITY ? NAN : 1.f / l;  // every row sees itself: scores of -inf alone are 0 / 0
     const bool valid = it.at(s) + row < it.rows;
     __nv_bfloat16* o = p.out + (int64_t)(it.start + (valid ? it.at(s) + row : 0)) * p.os + (int64_t)it.head_of(s) * p.ohs;
 #pragma unroll 1

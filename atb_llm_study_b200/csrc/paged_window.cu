@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
       acc += f * warp_o[(w * kRows + row) * HD + i % HD];
     }
     if (alone) {  // this CTA's part is all there is
-      p.out[(int64_t)b * p.out_stride + (int64_t)head0 * HD + i] = f2bf(L == 0.f ? 0.f : acc / L);
+      // an empty context gives zeros; where it is not empty, scores of -inf alone are 0 / 0
+      p.out[(int64_t)b * p.out_stride + (int64_t)head0 * HD + i] = f2bf(context == 0 ? 0.f : acc / L);
       continue;
     }
     part_o[i] = acc;
@@ -391,7 +392,8 @@ __global__ void __launch_bounds__(kThreads) paged_window_kernel(const __grid_con
       L += i < ctas ? f * cluster_load_f(al + 4 * row, i) : f;
     }
     L = warp_sum(L);
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing visible: zeros
+    // nothing visible: zeros; scores of -inf alone: 0 / 0
+    const float inv = L > 0.f ? 1.f / L : context == 0 && span.count == 0 ? 0.f : NAN;
     for (int i = lane; i < parts; i += 32) weight[row * parts + i] *= inv;
   }
   __syncthreads();

@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
           tmem_st_wait();
         }
         float mx = fmax3_nan(fmax3_nan(m4[0], m4[1], m4[2]), m4[3], -INFINITY);
-        if (mx != mx) l = NAN;  // a visible score is: so is the row
+        if (!(mx < INFINITY)) l = NAN;  // a visible score is NaN or +inf (inf / inf): so is the row
         mx *= scale_log2;       // scale > 0
         float alpha = 1.f;
         if (mx > mref + kRescaleLog2 || (mref == -INFINITY && mx > -INFINITY)) {

@@ -380,7 +380,8 @@ B200_API int b200_flash_prefill_packed(const void* q, int64_t q_stride, int64_t 
  * [0, total_tokens) is left out and sets the device error word (where offsets
  * do not ascend, sequences beside it may be left out with it).  What a row
  * does not see does not reach it, NaN and infinities included; a row that sees
- * a value row with one is not finite.  Extends SelfAttentionOp::Create
+ * a value row with one is not finite, and one whose scores are all -inf, or
+ * one of them +inf, is NaN.  Extends SelfAttentionOp::Create
  * (PA_ENCODER) (atb_cpp_llm/src/ops/self_attention_op.cpp:8-30), whose only
  * mask is the causal one. */
 B200_API int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_t q_head_stride, const void* k,
@@ -479,7 +480,8 @@ B200_API int64_t b200_paged_decode_noalloc_max_scratch_bytes(void);
  * window >= 1, sinks >= 0, scale > 0.  Only blocks with a visible position are
  * looked up, so table entries of the others may be stale and their blocks
  * given to other sequences; what lies in hidden positions (NaN included) does
- * not matter.  A context of 0 gives zeros; one outside the table is clamped,
+ * not matter.  A context of 0 gives zeros (scores that are all -inf, or one of
+ * them +inf, give NaN); one outside the table is clamped,
  * and a visible entry outside [0, num_blocks) read as block 0, and both set the
  * device error word.  head_dim 64 or 128, block_size 64 or 128, any
  * nq % nkv == 0; q_stride a multiple of 8, q and the caches 16-byte aligned.

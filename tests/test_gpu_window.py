@@ -221,6 +221,69 @@ def test_a_query_that_is_nan_is_alone():
         close(got, want, weight)
 
 
+@pytest.mark.parametrize("nq,nkv,d,dv", [(4, 2, 64, 64), (3, 1, 128, 128), (2, 2, 192, 128), (2, 2, 16, 16)])
+def test_prompt_infinite_scores(nq, nkv, d, dv):
+    """Scores of -inf alone are 0 / 0, and one of +inf is inf / inf; one of -inf beside finite ones has no weight."""
+    q, k, v = prompt_inputs(11, 300, nq, nkv, d, dv)
+    k[:, :, 0] = G.rounded(np.abs(k[:, :, 0]) + 0.5)  # the values that the kernel sees
+    q[:, :, 0] = G.rounded(np.abs(q[:, :, 0]) + 0.5)
+    for bad, value in ((170, -np.inf), (170, np.inf), (0, -np.inf), (299, np.inf)):
+        qq = q.copy()
+        qq[bad, 0, 0] = value  # all scores of one query's head
+        want, weight = serving.window_prompt(q, k, v, [300], 140, 2, d ** -0.5)
+        got = prompt(qq, k, v, [300], 140, 2)
+        assert np.isnan(got[bad, 0]).all()
+        got[bad, 0] = want[bad, 0]
+        close(got, want, weight)
+    for bad in (1, 100, 200):
+        kk = k.copy()
+        kk[bad, :, 0] = -np.inf
+        want, weight = serving.window_prompt(q, kk, v, [300], 140, 2, d ** -0.5)
+        close(prompt(q, kk, v, [300], 140, 2), want, weight)
+        kk[bad, :, 0] = np.inf
+        sees = serving.window_mask(300, 140, 2)[:, bad]
+        got = prompt(q, kk, v, [300], 140, 2)
+        assert np.isnan(got[sees]).all()
+        close(got[~sees], want[~sees], weight[~sees])
+
+
+@pytest.mark.parametrize("lens", [[100, 0, 100], [2000, 0, 2000]], ids=["short", "long"])  # one CTA a pair, and a cluster
+@pytest.mark.parametrize("d", [64, 128])
+def test_token_infinite_scores(lens, d):
+    c = Cache(12, lens, 2, d, 64, spare=2)
+    c.k[..., 0] = G.rounded(np.abs(c.k[..., 0]) + 0.5)
+    q, _ = queries(12, 3, 4, d)
+    want, weight = serving.window_decode(q, c.k, c.v, c.tables, lens, 5000, 0)
+    for value in (-np.inf, np.inf):
+        qq = q.copy()
+        qq[:2, 1, 0] = value  # one head of the first sequence, and of the empty one
+        for longest in (1, max(lens)):
+            got = G.host(token_call(G.bf16(qq.reshape(3, -1)), c.device(), c, 4, 5000, 0, longest))[:3, :4 * d].reshape(3, 4, d)
+            assert np.isnan(got[0, 1]).all() and (got[1] == 0).all()
+            got[0, 1] = want[0, 1]
+            close(got, want, weight)
+
+
+@pytest.mark.parametrize("plen", [0, 1, 300])
+def test_shared_infinite_scores(plen):
+    lens = [100, 0, 100]
+    c = Cache(13, lens, 2, 64, 64, spare=6)
+    prefix = c.order[:5]
+    c.fill_fast(prefix, plen)
+    c.k[..., 0] = G.rounded(np.abs(c.k[..., 0]) + 0.5)
+    q, _ = queries(13, 3, 4, 64)
+    want, weight = serving.shared_decode(q, c.k, c.v, prefix, plen, c.tables, lens)
+    for value in (-np.inf, np.inf):
+        qq = q.copy()
+        qq[:2, 1, 0] = value
+        got = G.host(shared_call(G.bf16(qq.reshape(3, -1)), c.device(), c, 4, G.i32(prefix), G.i32([plen]), 320))[:3, :256]
+        got = got.reshape(3, 4, 64)
+        assert np.isnan(got[0, 1]).all()
+        assert np.isnan(got[1, 1]).all() if plen else (got[1] == 0).all()
+        got[:2, 1] = want[:2, 1]
+        close(got, want, weight)
+
+
 def test_prompt_growing_and_flat_scores():
     lens = [400]
     q, k, v = prompt_inputs(4, 400, 2, 1, 128, 128, scale=0.0)
@@ -519,7 +582,7 @@ def test_shared_prefix_without_weight(plen, positions, d):
     c.fill_fast(prefix, plen)
     far_below(c, prefix, positions)
     q = G.rounded(np.random.default_rng(10).standard_normal((3, 8 * d)) * 2)
-    q[:, ::d] = np.abs(q[:, ::d]) + 1
+    q[:, ::d] = G.rounded(np.abs(q[:, ::d]) + 1)
     want, weight = serving.shared_decode(q.reshape(3, 8, d), c.k, c.v, prefix, plen, c.tables, lens)
     got = G.host(shared_call(G.bf16(q), c.device(), c, 8, G.i32(prefix), G.i32([plen]), plen))[:3, :8 * d]
     close(got.reshape(want.shape), want, weight)
