@@ -382,6 +382,29 @@ def test_logits_equal_argmax_without_changes():
     assert nxt[:7].tolist() == want.tolist() and (out == c["x"]).all()
 
 
+def test_logits_of_the_largest_vocabulary():
+    check_logits(logits_case(12, 2, 1 << 23, 300, 40, 1))
+
+
+def test_logits_offsets_past_32_bits():
+    rows, ld, vocab = 1100, 1 << 21, 1000  # 2.3e9 elements
+    rng = np.random.default_rng(13)
+    x = torch.full((rows, ld), 7.0, dtype=torch.bfloat16, device=G.DEV)
+    values = G.rounded(rng.standard_normal((rows, vocab)))
+    x[:, :vocab] = G.bf16(values)
+    history = G.i32(values.argmax(1)[:, None])
+    one, rep, nxt = G.i32([1] * rows), G.f32([1.5] * rows), torch.zeros(rows, dtype=torch.int64, device=G.DEV)
+    G.check(G.L().b200_logits_process(x.data_ptr(), ld, rows, vocab, history.data_ptr(), 1, None, one.data_ptr(), rep.data_ptr(), None,
+                                      None, None, None, None, None, 0, 0, None, x.data_ptr(), ld, nxt.data_ptr(), G.stream()))
+    want = [serving.logits(r, [], [int(r.argmax())], np.float32(1.5)) for r in values]
+    assert nxt.tolist() == [t for _, t in want]
+    np.testing.assert_allclose(G.host(x[:, :vocab]), np.stack([w for w, _ in want]), rtol=2.0 ** -8)
+    x[:, :vocab] = 7
+    assert bool((x == 7).all()) and G.device_errors() == 0
+    del x
+    torch.cuda.empty_cache()
+
+
 # --------------------------------------------------------- a step of it all
 
 

@@ -617,3 +617,69 @@ def test_shared_captured_calls_with_workspaces_of_their_own():
         want, weight = serving.shared_decode(q, c.k, c.v, prefix, n, c.tables, [own] * 9)
         for _, out, _, _ in calls:
             close(G.host(out).reshape(want.shape), want, weight)
+
+
+# ------------------------------------------------- many tiles, far offsets
+
+
+@pytest.mark.parametrize("nq,nkv,d,dv,window,sinks", [(4, 2, 128, 128, 4600, 5), (3, 1, 128, 128, 6000, 0), (2, 2, 192, 128, 3000, 200),
+                                                      (4, 2, 64, 64, 2500, 1), (4, 4, 32, 32, 5000, 4)])
+def test_prompt_items_of_many_tiles(nq, nkv, d, dv, window, sinks):
+    lens = [5777, 1500]
+    q, k, v = prompt_inputs(14, sum(lens), nq, nkv, d, dv)
+    got = prompt(q, k, v, lens, window, sinks)
+    rng, at = np.random.default_rng(14), 0
+    for n in lens:
+        rows = np.unique(np.concatenate([rng.integers(0, n, 60), [0, n - 1, min(n - 1, window), min(n - 1, window + 127)]]))
+        j = np.arange(n)[None]
+        sees = (j <= rows[:, None]) & ((rows[:, None] - j < window) | (j < sinks))
+        for h in range(nq):
+            kv = h * nkv // nq
+            want, weight = serving.attend(q[at + rows, h], k[at:at + n, kv], v[at:at + n, kv], sees, d ** -0.5)
+            close(got[at + rows, h], want, weight)
+        at += n
+    assert np.isfinite(got).all() and G.device_errors() == 0
+
+
+@pytest.mark.parametrize("nq,nkv,d,bs", [(8, 2, 128, 128), (8, 2, 64, 64)])
+def test_shared_prefix_of_many_tiles(nq, nkv, d, bs):
+    check_shared([300, 0, 1, 2000, 77], 20011, nq, nkv, d, bs)
+
+
+def test_prompt_offsets_past_32_bits():
+    rows, stride, n, nq, nkv, d = 33000, 70000, 300, 4, 2, 64  # 2.3e9 elements in inputs and outputs
+    q, k, v = prompt_inputs(15, n, nq, nkv, d, d)
+    x = torch.zeros(rows, stride, dtype=torch.bfloat16, device=G.DEV)
+    out = torch.full((rows, stride), -5.0, dtype=torch.bfloat16, device=G.DEV)
+    cols = (0, 40000, 69800)
+    for y, c in zip((q, k, v), cols):
+        x[rows - n:, c:c + y.shape[1] * d] = G.bf16(y.reshape(n, -1))
+    cu = G.i32([rows - n, rows])
+    at = [x.data_ptr() + 2 * c for c in cols]
+    G.check(G.L().b200_flash_prefill_window(at[0], stride, d, at[1], stride, d, at[2], stride, d, out.data_ptr() + 2 * 60000, stride,
+                                            d, cu.data_ptr(), 1, n, rows, nq, nkv, d, d, d ** -0.5, 130, 3, G.stream()))
+    want, weight = serving.window_prompt(q, k, v, [n], 130, 3, d ** -0.5)
+    close(G.host(out[rows - n:, 60000:60000 + nq * d]).reshape(want.shape), want, weight)
+    out[rows - n:, 60000:60000 + nq * d] = -5
+    assert bool((out == -5).all()) and G.device_errors() == 0
+    del x, out
+    torch.cuda.empty_cache()
+
+
+def test_shared_offsets_past_32_bits():
+    nkv, d, bs, plen, lens = 8, 128, 128, 500, [300, 0]
+    blocks = (1 << 31) // (nkv * bs * d) + 40  # more than 2^31 elements in each half
+    k, v = (torch.zeros(blocks, nkv, bs, d, dtype=torch.bfloat16, device=G.DEV) for _ in range(2))
+    c = Cache(16, lens, nkv, d, bs, spare=5)
+    c.fill_fast(c.order[:4], plen)
+    used = np.concatenate([c.tables[0], c.order[:4]])
+    high = torch.from_numpy(blocks - 1 - np.arange(len(used))).to(G.DEV)
+    k[high], v[high] = G.bf16(np.nan_to_num(c.k[used])), G.bf16(np.nan_to_num(c.v[used]))
+    q, qd = queries(16, 2, 16, d)
+    want, weight = serving.shared_decode(q, c.k, c.v, c.order[:4], plen, c.tables, lens)
+    c.blocks = blocks
+    tables = torch.stack([high[:3], high[:3]]).to(torch.int32)
+    got = G.host(shared_call(qd, (k, v, tables, G.i32(lens)), c, 16, high[3:].to(torch.int32), G.i32([plen]), plen))
+    close(got[:2, :2048].reshape(want.shape), want, weight)
+    del k, v
+    torch.cuda.empty_cache()

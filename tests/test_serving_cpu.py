@@ -129,6 +129,85 @@ def test_stretches_cover_every_item_once(workers, items, K):
             slots.add(c + i)
 
 
+STRETCHES = """
+#include <stdint.h>
+#include <stdio.h>
+#include <algorithm>
+#define B200_DEV inline
+typedef void* cudaStream_t;
+using std::max;
+using std::min;
+"""
+STRETCHES_MAIN = """
+#include "shared_prefix.h"
+// length max_length workers row_tiles per_tile group batch nkv -> stretches, then the slots that each sequence's head 0 reads
+int main() {
+  int length, batch, nkv;
+  b200::PrefixParts p{};
+  while (scanf("%d %d %d %d %d %d %d %d", &length, &p.max_length, &p.workers, &p.row_tiles, &p.per_tile, &p.group, &batch, &nkv) == 8) {
+    p.length = &length;
+    const int K = (b200::prefix_length(p) + 127) / 128, units = K * nkv * b200::prefix_pairs(p);
+    const b200::PrefixDeal deal(p, units);
+    printf("%d %d", K, units ? deal.W : 0);
+    for (int c = 0; units && c <= deal.W; ++c) printf(" %d", deal.first_unit(c));
+    printf("\\n");
+    for (int b = 0; b < batch; ++b)
+      for (int kh = 0; kh < nkv; ++kh) {
+        const b200::PrefixSpan s = b200::prefix_span(p, b, kh, nkv, 0, 64);
+        printf("%d %lld ", s.count, s.count ? (long long)(s.lse - p.lse) : -1);
+        if (s.count && (s.parts - p.parts) != (s.lse - p.lse) * 64) return 1;
+      }
+    printf("\\n");
+  }
+  return 0;
+}
+"""
+
+
+def test_stretches_and_parts_of_the_header(tmp_path):
+    """shared_prefix.h itself, compiled for the host: the stretches cover all units in order, every part that a stretch
+    leaves lies in a slot of its own inside the workspace, and a sequence reads the parts that hold its rows, no others."""
+    import shutil
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.abspath(capi.__file__)), "csrc")
+    shutil.copy(os.path.join(csrc, "shared_prefix.h"), tmp_path)
+    (tmp_path / "common.cuh").write_text("#pragma once\n" + STRETCHES)
+    (tmp_path / "main.cpp").write_text(STRETCHES_MAIN)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-o", tmp_path / "main", tmp_path / "main.cpp"], check=True)
+    cases = []
+    for batch, group, nkv in ((1, 1, 1), (5, 4, 8), (64, 4, 8), (65, 4, 2), (9, 17, 1), (256, 8, 1), (3, 128, 2), (140, 1, 8)):
+        for length, most in ((0, 100), (1, 1), (128, 128), (129, 1000), (1001, 1001), (16384, 16384), (500, 300), (-3, 10)):
+            per = 128 // group
+            tiles = -(-batch // per)
+            items = nkv * -(-tiles // 2)
+            workers = max(1, min(items * -(-most // 128), 148))
+            cases.append((length, most, workers, tiles, per, group, batch, nkv))
+    out = subprocess.run([tmp_path / "main"], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True,
+                         check=True).stdout.splitlines()
+    assert len(out) == 2 * len(cases)
+    for (length, most, workers, tiles, per, group, batch, nkv), head, spans in zip(cases, out[::2], out[1::2]):
+        K, W, *first = map(int, head.split())
+        items = nkv * -(-tiles // 2)
+        assert K == -(-max(0, min(length, most)) // 128) and W == min(workers, K * items)
+        spans = np.array(spans.split(), np.int64).reshape(batch, nkv, 2)
+        if K == 0:
+            assert (spans[..., 0] == 0).all()
+            continue
+        assert first[0] == 0 and first[W] == K * items and (np.diff(first) > 0).all()
+        parts = {}  # item -> the slots of its parts, as the kernel numbers them
+        for c in range(W):
+            for item in range(first[c] // K, (first[c + 1] - 1) // K + 1):
+                parts.setdefault(item, []).append(2 * (c + item))
+        slots = [s for ss in parts.values() for s in ss]
+        assert len(set(slots)) == len(slots) and max(slots) + 1 < 2 * (workers + items)
+        for b in range(batch):
+            for kh in range(nkv):
+                mine = parts[kh * -(-tiles // 2) + b // per // 2]
+                assert mine == list(range(mine[0], mine[0] + 2 * len(mine), 2))
+                assert spans[b, kh].tolist() == [len(mine), (mine[0] + b // per % 2) * 128 + b % per * group]
+
+
 def test_window_without_an_end_is_causal_attention():
     rng = np.random.default_rng(0)
     q, k, v = (rng.standard_normal((9, h, 16)).astype(np.float32) for h in (4, 2, 2))
