@@ -11,11 +11,13 @@
 // the heads of one sequence's rows side by side: those that share keys find them
 // in L2.
 //
-// Measured, 32 / 8 heads of 128, alone: 8 x 2048 with a window of 1024 in 278 us
-// (743 TFLOP/s of visible pairs, 84 % of the pairs computed), 1 x 32768 with 4096
-// in 1.90 ms (1086 TFLOP/s, 66 % of the measured burst rate); back to back, under
-// the power limit, 320 us and 2.25 ms.  A tile at the window's ends costs a side
-// half as much again as a whole one.
+// Measured, 32 / 8 heads of 128, replayed with pauses: 8 x 2048 with a window of
+// 1024 in 281 us (736 TFLOP/s of visible pairs, 84 % of the pairs computed), 1 x
+// 32768 with 4096 in 1.93 ms (1070 TFLOP/s, 65 % of the measured burst rate); back
+// to back, under the power limit, 318 us and 2.23 ms.  A tile at the window's ends
+// costs a side half as much again as a whole one.  The first of them with 16 / 8
+// heads: 145 us, and 123 at 64, 119 at 32, 116 at 16 (narrow heads take the copies
+// and products of 64-wide ones); 16 / 16 heads of 192 / 128 take 232 (556 TFLOP/s).
 #include <algorithm>
 
 #include "tc_items.cuh"
@@ -55,8 +57,12 @@ struct Window {
   // so that the walk ends with cheap items; it walks over numbers of sequences that
   // have no such tile.  By sequence: sequence s owns the numbers from
   // floor(cu[s] / rows) + s on, as many as it has tiles, or one more, whatever the
-  // lengths, and the sequence of a number is found by halving.  By tile 8 x 2048
-  // takes 282 us, by sequence 306; 17 prompts of up to 900 take 50 and 43.
+  // lengths, and the sequence of a number is found by halving.  By tile and by
+  // sequence (us), at so many times the numbers of the other order: 8 x 2048 at 0.94
+  // 271 and 294, at 1.12 246 and 239, at 1.24 222 and 218, at 1.39 198 and 182; 16 x
+  // 1024 under a window of 256 at 1.22 139 and 142, at 1.62 109 and 104; 16 x 2048
+  // with 8 / 8 heads at 1.08 120 and 127, at 1.22 115 and 114, at 1.62 95 and 82; 64
+  // x 900 with 12 / 4 heads of 64 at 1.16 154 and 161, at 1.47 119 and 120.
   struct Cursor {
     const Window& p;
     int w;
@@ -197,7 +203,7 @@ extern "C" int b200_flash_prefill_window(const void* q, int64_t q_stride, int64_
   if (num_seqs == 0 || max_seqlen == 0 || total_tokens == 0) return B200_OK;
   const bool pair_heads = nq / nkv % 2 == 0;
   const int rows = pair_heads ? kTile : 2 * kTile;
-  // by tile where lengths are near each other: at most a quarter of its numbers more than by sequence
+  // by tile where lengths are near each other: at most a quarter more numbers than by sequence, where they are level
   const int64_t by_tile = ((int64_t)max_seqlen + rows - 1) / rows * num_seqs, by_sequence = total_tokens / rows + num_seqs;
   const bool tiles = 4 * by_tile <= 5 * by_sequence;
   const int64_t items = (tiles ? by_tile : by_sequence) * (pair_heads ? nq / 2 : nq);

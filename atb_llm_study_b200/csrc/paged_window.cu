@@ -1,15 +1,18 @@
 // Single-token attention over a paged KV cache with a sliding window and a few
 // first tokens that stay visible (sinks), and, for the batch whose sequences
 // share a prefix, the part of each sequence's own tokens, joined with the
-// prefix's (prefix_attention in shared_prefix.h).
+// prefix's parts (PrefixParts in shared_prefix.h).
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(q.k_j scale log2(e) - m),
 //   over j < context with j >= context - window or j < sinks,
 // in parts that each keep (m, sum, unnormalised output) and are joined by
 //   m = max m_i, sum = sum_i 2^(m_i - m) sum_i, and the outputs alike.
 //
-// Every visible token's K and V are read once for the G = nq / nkv query heads
-// that share them, 4 flops for each byte read and head: memory bounds it.
+// Every visible token's K and V are read once for up to 16 query heads that
+// share them, 4 flops for each byte read and head: memory bounds it.  (Groups of
+// more heads take a CTA for each 16, which mostly find the tiles in L2: 64
+// sequences that show 4100 tokens of one 128-wide kv head take 34 us for 16 heads,
+// 41 for 17 and for 32, 59 for 40 and for 64; the copy rate's floor is 20.)
 // One CTA takes a stretch of the visible 64-token tiles of one (sequence, kv
 // head); when there are too few pairs to fill the GPU, up to 8 CTAs of a
 // cluster share a pair's tiles and join their parts through distributed shared
@@ -27,8 +30,8 @@
 // does not reach the output.
 //
 // Measured: 64 sequences of up to 32768 tokens, window 4096, 32 / 8 heads of 128:
-// 161 us for 1.055 GB, the measured copy rate.  Two stages and three CTAs an SM
-// took 229.  Contexts of a few tiles are bound by a CTA's way from its length to
+// 161 to 168 us for 1.055 GB, 96 % of the measured copy rate and more; heads of 64
+// 82 us for half of that.  Two stages and three CTAs an SM took 229.  Contexts of a few tiles are bound by a CTA's way from its length to
 // its table, tiles and join, 5 us: 64 of 512 tokens on average take 36 us for
 // 129 MB.  (CTAs that walk many pairs, loading ahead, took 50: more registers, and
 // joins in turns to fit two of them on an SM.)
@@ -433,7 +436,11 @@ bool make_cache_map(CUtensorMap* m, const void* ptr, int64_t rows) {
 
 // CTAs that share a (sequence, kv head, head tile): none but one when these
 // fill the GPU with two CTAs an SM by themselves, else so many that they do, at
-// most 8 and never more than the tiles that a sequence can show.
+// most 8 and never more than the tiles that a sequence can show.  Eight kv heads
+// of 128, 1028 tokens shown, with 1, 2, 4 and 8 CTAs a pair: one sequence 16.6,
+// 12.7, 10.4 and 9.5 us; eight (two CTAs an SM with 4) 18.1, 15.8, 14.3 and 23.2;
+// sixteen (with 2) 21.5, 19.6, 28.0 and 44.2.  At 8196 tokens one takes 84, 46, 27
+// and 18.5; at 300 tokens the number hardly matters (6.7 to 7.2).
 unsigned cluster_for(int64_t pairs, int max_tiles) {
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
