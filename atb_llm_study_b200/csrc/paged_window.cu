@@ -31,10 +31,11 @@
 //
 // Measured: 64 sequences of up to 32768 tokens, window 4096, 32 / 8 heads of 128:
 // 161 to 168 us for 1.055 GB, 96 % of the measured copy rate and more; heads of 64
-// 82 us for half of that.  Two stages and three CTAs an SM took 229.  Contexts of a few tiles are bound by a CTA's way from its length to
-// its table, tiles and join, 5 us: 64 of 512 tokens on average take 36 us for
-// 129 MB.  (CTAs that walk many pairs, loading ahead, took 50: more registers, and
-// joins in turns to fit two of them on an SM.)
+// 82 us for half of that.  Two stages and three CTAs an SM took 229.  Contexts of
+// a few tiles are bound by a CTA's way from its length to its table, tiles and
+// join, 5 us: 64 of 512 tokens on average take 36 us for 129 MB.  (CTAs that walk
+// many pairs, loading ahead, took 50: more registers, and joins in turns to fit
+// two of them on an SM.)
 #include <math.h>
 
 #include <algorithm>

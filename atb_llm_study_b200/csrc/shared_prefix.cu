@@ -18,11 +18,11 @@
 // launches in all.
 //
 // Measured, 64 sequences behind 16384 tokens with up to 1024 of their own, 32 / 8
-// heads of 128: 67 us (floor 30, of which 20 for the own tokens); of 64: 45 (15).  The prefix's
-// share is 25: 5 until the first scores (cold lengths, tables and tiles one after
-// the other), 7 key tiles of two row tiles at 4200 cycles, and 2 a side for 64 KB of
-// outputs.  Fewer CTAs, to let the other kernel run beside this one, gained nothing:
-// its CTAs wait for these parts in their places.
+// heads of 128: 67 us (floor 30, of which 20 for the own tokens); of 64: 45 (15).
+// The prefix's share of the 67 is 25: 5 until the first scores (cold lengths, tables
+// and tiles one after the other), 7 key tiles of two row tiles at 4200 cycles, and 2 a
+// side for 64 KB of outputs.  Fewer CTAs, to let the other kernel run beside this one,
+// gained nothing: its CTAs wait for these parts in their places.
 #include <algorithm>
 
 #include "shared_prefix.h"

@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         // Records are cleared half a ring ahead of their use, once V of their item n has landed: it was loaded behind the
         // P V of item n - VS or a later one, and before an item's P V begins all earlier items have been stored (o_free).
         // So items up to n - VS - 1 are done with their records.  (Before this wait only V of item n - 1 has landed, and
-        // with one stage item n - 2, whose record this is, may still be at reading it.)
+        // with one stage the record, then of item n - 2, may still be read.)
         static_assert(VS + 1 <= Cf::RING / 2, "the record that item n clears belongs to item n - VS - 1 or an earlier one");
         if (j == 0 && lane == 0) hidden[(n + Cf::RING / 2) % Cf::RING].any = 0;
         const int key = P::key0(it, j);
